@@ -604,6 +604,174 @@ CITLALI_EXPORT int citlali_hip_embed_at(const uint16_t* table, const int32_t* to
     return CITLALI_OK;
 }
 
+// ---------------------------------------------------------------- paged 4-bit cache
+namespace {
+int check_kv4(const char* who, const citlali_hip_kv4_cache* c, Kv4View* v) {
+    REQUIRE(c && c->pages, "%s received a null cache", who);
+    REQUIRE(c->num_pages > 0 && c->kv_heads > 0, "%s: num_pages (%d) and kv_heads (%d) must be positive", who,
+            c->num_pages, c->kv_heads);
+    if (!kv4_shape_ok(c->page_size, c->head_dim))
+        return fail(CITLALI_ERR_UNSUPPORTED,
+                    "%s: a cache of page_size %d and head_dim %d is not built (page_size 16, 32, 64, 128 or 256, "
+                    "head_dim 64 or 128)",
+                    who, c->page_size, c->head_dim);
+    REQUIRE((long long)c->num_pages * c->page_size <= INT_MAX, "%s: %d pages of %d tokens exceed the slot range", who,
+            c->num_pages, c->page_size);
+    REQUIRE(aligned(c->pages, 16), "%s: pages must be 16-byte aligned", who);
+    *v = Kv4View{c->pages, c->num_pages, __builtin_ctz((unsigned)c->page_size), c->kv_heads, c->head_dim};
+    return CITLALI_OK;
+}
+
+// heads per kv head the attention kernels have, and counts the grids hold
+constexpr int kKv4MaxGroup = 16;
+constexpr int kKv4MaxHeads = 4096;
+constexpr long long kKv4MaxRows = 1ll << 28;   // head rows of one append or read: 2^32 threads
+
+int check_kv4_attention(const char* who, int max_context, int max_query, int nseq, int tokens, int heads,
+                        int kv_heads) {
+    REQUIRE(nseq >= 0 && tokens >= 0, "%s: nseq (%d) and tokens (%d) must not be negative", who, nseq, tokens);
+    REQUIRE(max_query > 0 && max_context > 0, "%s: max_query (%d) and max_context (%d) must be positive", who,
+            max_query, max_context);
+    REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "%s: heads (%d) must be a multiple of kv_heads (%d)",
+            who, heads, kv_heads);
+    REQUIRE(nseq <= 65535 && heads <= kKv4MaxHeads, "%s: at most 65535 sequences and %d heads", who, kKv4MaxHeads);
+    if (heads / kv_heads > kKv4MaxGroup)
+        return fail(CITLALI_ERR_UNSUPPORTED, "%s: %d query heads per kv head are not built (1..%d)", who,
+                    heads / kv_heads, kKv4MaxGroup);
+    return CITLALI_OK;
+}
+}  // namespace
+
+CITLALI_EXPORT size_t citlali_hip_kv4_page_bytes(int page_size, int kv_heads, int head_dim) {
+    if (kv_heads <= 0 || !kv4_shape_ok(page_size, head_dim)) return 0;
+    return (size_t)kv_heads * page_size * head_dim * 5 / 4;
+}
+
+CITLALI_EXPORT int citlali_hip_rope_table(float* table, int positions, int head_dim, float theta) {
+    REQUIRE(table, "rope_table received a null buffer");
+    REQUIRE(positions > 0 && head_dim > 0 && head_dim % 2 == 0 && head_dim <= 2048,
+            "rope_table: bad positions (%d) or head_dim (%d)", positions, head_dim);
+    REQUIRE((long long)positions * (head_dim / 2) < 1ll << 32, "rope_table: %d positions are too many", positions);
+    REQUIRE(theta > 0.f, "rope_table: theta must be positive");
+    REQUIRE(aligned(table, 8), "rope_table: table must be 8-byte aligned");
+    HIP_TRY(launch_rope_table(table, positions, head_dim, theta, g_stream));
+    return CITLALI_OK;
+}
+
+CITLALI_EXPORT int citlali_hip_kv4_append(const citlali_hip_kv4_cache* cache, const uint16_t* q, const uint16_t* k,
+                                          const uint16_t* v, long long q_stride, long long kv_stride,
+                                          const uint16_t* q_norm, const uint16_t* k_norm, float eps,
+                                          const float* rope, int rope_positions, const int32_t* positions,
+                                          const int32_t* slots, int tokens, int heads, uint16_t* q_out,
+                                          long long q_out_stride) {
+    Kv4View c{};
+    const int st = check_kv4("kv4_append", cache, &c);
+    if (st) return st;
+    REQUIRE(tokens >= 0 && heads >= 0 && heads <= kKv4MaxHeads, "kv4_append: bad tokens (%d) or heads (%d)", tokens,
+            heads);
+    REQUIRE(k && v && rope && positions && slots, "kv4_append received a null buffer");
+    REQUIRE((heads > 0) == (q != nullptr) && (heads > 0) == (q_out != nullptr),
+            "kv4_append: q and q_out go with heads > 0");
+    REQUIRE(rope_positions > 0, "kv4_append: rope_positions must be positive");
+    const long long q_row = (long long)heads * c.head_dim, kv_row = (long long)c.kv_heads * c.head_dim;
+    REQUIRE(kv_stride >= kv_row && (heads == 0 || (q_stride >= q_row && q_out_stride >= q_row)),
+            "kv4_append: a stride is shorter than its row");
+    REQUIRE(kv_stride % 8 == 0 && (heads == 0 || (q_stride % 8 == 0 && q_out_stride % 8 == 0)),
+            "kv4_append: strides must be multiples of 8");
+    REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(q_out, 16) && aligned(q_norm, 16) &&
+                aligned(k_norm, 16) && aligned(rope, 8),
+            "kv4_append: q, k, v, q_out and the norms must be 16-byte aligned, rope 8-byte");
+    REQUIRE((long long)tokens * (heads + 2ll * c.kv_heads) <= kKv4MaxRows, "kv4_append: %d tokens are too many", tokens);
+    REQUIRE(heads == 0 || q != q_out || q_stride == q_out_stride || tokens <= 1,
+            "kv4_append: q_out is q with another stride");
+    if (tokens == 0) return CITLALI_OK;
+    const Kv4Append a{q,    k,    v,         q_stride, kv_stride, q_norm, k_norm, eps,
+                      rope, rope_positions, positions, slots,     tokens, heads,  q_out, q_out_stride};
+    HIP_TRY(launch_kv4_append(c, a, g_stream));
+    return CITLALI_OK;
+}
+
+CITLALI_EXPORT int citlali_hip_kv4_read(const citlali_hip_kv4_cache* cache, const int32_t* slots, int count,
+                                        uint16_t* k_out, uint16_t* v_out) {
+    Kv4View c{};
+    const int st = check_kv4("kv4_read", cache, &c);
+    if (st) return st;
+    REQUIRE(count >= 0, "kv4_read: negative count");
+    REQUIRE(slots && k_out && v_out, "kv4_read received a null buffer");
+    REQUIRE(aligned(k_out, 16) && aligned(v_out, 16), "kv4_read: outputs must be 16-byte aligned");
+    REQUIRE(count * 2ll * c.kv_heads <= kKv4MaxRows, "kv4_read: %d slots are too many", count);
+    if (count == 0) return CITLALI_OK;
+    HIP_TRY(launch_kv4_read(c, slots, count, k_out, v_out, g_stream));
+    return CITLALI_OK;
+}
+
+CITLALI_EXPORT size_t citlali_hip_kv4_attention_workspace_bytes(int max_context, int max_query, int nseq, int tokens,
+                                                                int heads, int kv_heads, int head_dim) {
+    if (check_kv4_attention("kv4_attention", max_context, max_query, nseq, tokens, heads, kv_heads) ||
+        !kv4_shape_ok(16, head_dim) || nseq == 0 || tokens == 0)
+        return 0;
+    return kv4_attention_workspace(max_context, max_query, nseq, tokens, heads, kv_heads, head_dim);
+}
+
+CITLALI_EXPORT int citlali_hip_kv4_attention(const citlali_hip_kv4_cache* cache, const uint16_t* q,
+                                             long long q_stride, const int32_t* query_start,
+                                             const int32_t* context_lens, const int32_t* page_table,
+                                             int pages_per_seq, int nseq, int tokens, int max_query, int max_context,
+                                             int heads, void* workspace, size_t workspace_bytes, uint16_t* out,
+                                             long long out_stride) {
+    Kv4View c{};
+    int st = check_kv4("kv4_attention", cache, &c);
+    if (st) return st;
+    st = check_kv4_attention("kv4_attention", max_context, max_query, nseq, tokens, heads, c.kv_heads);
+    if (st) return st;
+    REQUIRE(q && context_lens && page_table && out, "kv4_attention received a null buffer");
+    REQUIRE(query_start || tokens == nseq, "kv4_attention: without query_start tokens (%d) must be nseq (%d)", tokens,
+            nseq);
+    REQUIRE(pages_per_seq > 0 && max_context <= (long long)pages_per_seq << c.page_shift,
+            "kv4_attention: max_context (%d) exceeds %d pages of %d", max_context, pages_per_seq, 1 << c.page_shift);
+    const long long row = (long long)heads * c.head_dim;
+    REQUIRE(q_stride >= row && out_stride >= row, "kv4_attention: a stride is shorter than its row");
+    REQUIRE(q_stride % 8 == 0 && out_stride % 8 == 0, "kv4_attention: strides must be multiples of 8");
+    REQUIRE(aligned(q, 16) && aligned(out, 16), "kv4_attention: q and out must be 16-byte aligned");
+    if (nseq == 0 || tokens == 0) return CITLALI_OK;
+    const size_t need = kv4_attention_workspace(max_context, max_query, nseq, tokens, heads, c.kv_heads, c.head_dim);
+    REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned(workspace, 16))),
+            "kv4_attention: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    const Kv4Attention a{q,      q_stride,  query_start, context_lens, page_table, pages_per_seq, nseq,
+                         tokens, max_query, max_context, heads,        static_cast<float*>(workspace), out, out_stride};
+    HIP_TRY(launch_kv4_attention(c, a, g_stream));
+    return CITLALI_OK;
+}
+
+// ---------------------------------------------------------------- log probabilities
+CITLALI_EXPORT size_t citlali_hip_token_logprobs_workspace_bytes(int rows, int vocab, int top_k) {
+    if (rows <= 0 || vocab <= 0 || top_k < 0 || top_k > CITLALI_MAX_TOP_LOGPROBS) return 0;
+    return logprobs_workspace(rows, vocab, top_k);
+}
+
+CITLALI_EXPORT int citlali_hip_token_logprobs(const void* logits, int gguf_type, long long row_stride, int rows,
+                                              int vocab, const int32_t* tokens, float* logprobs, int32_t* ranks,
+                                              float* entropies, int top_k, int32_t* top_ids, float* top_logprobs,
+                                              void* workspace, size_t workspace_bytes) {
+    REQUIRE(gguf_type == 0 || gguf_type == 1, "token_logprobs: GGUF type %d is not F32 or F16", gguf_type);
+    REQUIRE(rows >= 0 && vocab > 0, "token_logprobs: bad rows (%d) or vocab (%d)", rows, vocab);
+    REQUIRE(logits, "token_logprobs received a null buffer");
+    REQUIRE(row_stride >= vocab, "token_logprobs: row_stride (%lld) is shorter than vocab (%d)", row_stride, vocab);
+    REQUIRE(aligned(logits, gguf_type == 0 ? 4 : 2), "token_logprobs: logits are not aligned to their type");
+    REQUIRE(tokens || (!logprobs && !ranks), "token_logprobs: logprobs and ranks need tokens");
+    REQUIRE(top_k >= 0 && top_k <= CITLALI_MAX_TOP_LOGPROBS, "token_logprobs: top_k (%d) is not in 0..%d", top_k,
+            CITLALI_MAX_TOP_LOGPROBS);
+    REQUIRE(top_k == 0 || (top_ids && top_logprobs), "token_logprobs: top_k needs top_ids and top_logprobs");
+    if (rows == 0) return CITLALI_OK;
+    const size_t need = logprobs_workspace(rows, vocab, top_k);
+    REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned(workspace, 16))),
+            "token_logprobs: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    const Logprobs a{logits, gguf_type == 1, row_stride, rows,    vocab,        tokens,   logprobs,
+                     ranks,  entropies,      top_k,      top_ids, top_logprobs, workspace};
+    HIP_TRY(launch_token_logprobs(a, g_stream));
+    return CITLALI_OK;
+}
+
 CITLALI_EXPORT int citlali_hip_stream_read(const void* buf, size_t bytes, void* sink) {
     REQUIRE(buf && sink && aligned(buf, 16) && aligned(sink, 4), "stream_read: bad arguments");
     HIP_TRY(launch_stream_read(buf, bytes, static_cast<uint32_t*>(sink), g_stream));

@@ -200,6 +200,62 @@ hipError_t launch_matvec_gate_up_swiglu(int kind, const uint8_t* wg, const uint8
 // kind 4 / 6 / 1 GEMV with the input prologue; K a matvec_fused_length
 hipError_t launch_matvec_norm(int kind, const uint8_t* w, const uint16_t* x, const NormIn& norm, void* y,
                               bool f32_out, int K, int N, hipStream_t s);
+
+// ---- paged cache of 4-bit keys and values (kv4_cache.hip, kv4_attention.hip) ----
+struct Kv4View {
+    uint8_t* pages;
+    int num_pages;
+    int page_shift;   // page_size = 1 << page_shift
+    int kv_heads, head_dim;
+};
+bool kv4_shape_ok(int page_size, int head_dim);
+hipError_t launch_rope_table(float* table, int positions, int head_dim, float theta, hipStream_t s);
+struct Kv4Append {
+    const uint16_t *q, *k, *v;
+    long long q_stride, kv_stride;
+    const uint16_t *q_norm, *k_norm;
+    float eps;
+    const float* rope;   // [rope_positions][head_dim / 2][cos, sin]
+    int rope_positions;
+    const int32_t *positions, *slots;
+    int tokens, heads;
+    uint16_t* q_out;
+    long long q_out_stride;
+};
+hipError_t launch_kv4_append(const Kv4View& c, const Kv4Append& a, hipStream_t s);
+hipError_t launch_kv4_read(const Kv4View& c, const int32_t* slots, int count, uint16_t* k_out, uint16_t* v_out,
+                           hipStream_t s);
+struct Kv4Attention {
+    const uint16_t* q;
+    long long q_stride;
+    const int32_t *query_start, *context_lens, *page_table;
+    int pages_per_seq, nseq, tokens, max_query, max_context, heads;
+    float* workspace;
+    uint16_t* out;
+    long long out_stride;
+};
+size_t kv4_attention_workspace(int max_context, int max_query, int nseq, int tokens, int heads, int kv_heads,
+                               int head_dim);
+hipError_t launch_kv4_attention(const Kv4View& c, const Kv4Attention& a, hipStream_t s);
+
+// ---- log probabilities (logprobs.hip) ----
+struct Logprobs {
+    const void* logits;
+    bool half;
+    long long row_stride;
+    int rows, vocab;
+    const int32_t* tokens;
+    float* logprobs;
+    int32_t* ranks;
+    float* entropies;
+    int top_k;
+    int32_t* top_ids;
+    float* top_logprobs;
+    void* workspace;
+};
+size_t logprobs_workspace(int rows, int vocab, int top_k);
+hipError_t launch_token_logprobs(const Logprobs& a, hipStream_t s);
+
 hipError_t launch_fill_zero(void* p, size_t bytes, hipStream_t s);
 hipError_t launch_stream_read(const void* buf, size_t bytes, uint32_t* sink, hipStream_t s);
 

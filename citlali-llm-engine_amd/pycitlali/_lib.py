@@ -33,6 +33,12 @@ class Norm(ctypes.Structure):
     _fields_ = [("delta", c_void_p), ("weight", c_void_p), ("sum_out", c_void_p), ("eps", c_float)]
 
 
+class Kv4Cache(ctypes.Structure):
+    """citlali_hip_kv4_cache: a paged cache of 4-bit keys and values."""
+    _fields_ = [("pages", c_void_p), ("num_pages", c_int), ("page_size", c_int), ("kv_heads", c_int),
+                ("head_dim", c_int)]
+
+
 SIGNATURES = [
     ("citlali_hip_last_error", c_char_p, []),
     ("citlali_hip_abi_version", c_int, []),
@@ -98,6 +104,17 @@ SIGNATURES = [
                                               POINTER(c_void_p), POINTER(c_int), c_int]),
     ("citlali_hip_matvec_gate_up_swiglu_norm", c_int, [c_int, _P, _P, _P, POINTER(Norm), _P, c_int, c_int]),
     ("citlali_hip_matvec_norm", c_int, [c_int, _P, _P, POINTER(Norm), _P, c_int, c_int, c_int]),
+    ("citlali_hip_kv4_page_bytes", c_size_t, [c_int, c_int, c_int]),
+    ("citlali_hip_rope_table", c_int, [_P, c_int, c_int, c_float]),
+    ("citlali_hip_kv4_append", c_int, [POINTER(Kv4Cache), _P, _P, _P, c_longlong, c_longlong, _P, _P, c_float, _P,
+                                       c_int, _P, _P, c_int, c_int, _P, c_longlong]),
+    ("citlali_hip_kv4_read", c_int, [POINTER(Kv4Cache), _P, c_int, _P, _P]),
+    ("citlali_hip_kv4_attention", c_int, [POINTER(Kv4Cache), _P, c_longlong, _P, _P, _P, c_int, c_int, c_int, c_int,
+                                          c_int, c_int, _P, c_size_t, _P, c_longlong]),
+    ("citlali_hip_kv4_attention_workspace_bytes", c_size_t, [c_int] * 7),
+    ("citlali_hip_token_logprobs", c_int, [_P, c_int, c_longlong, c_int, c_int, _P, _P, _P, _P, c_int, _P, _P, _P,
+                                           c_size_t]),
+    ("citlali_hip_token_logprobs_workspace_bytes", c_size_t, [c_int, c_int, c_int]),
     ("citlali_hip_set_kernel_timing", c_int, [_P, _P]),
     ("citlali_hip_set_dispatch_timing", c_int, [POINTER(c_void_p), POINTER(c_void_p), c_int]),
     ("citlali_hip_dispatch_timing_count", c_int, [POINTER(c_int)]),

@@ -415,3 +415,68 @@ def matvec_norm(kind, w, x, delta, weight, sum_out, eps, y, in_features: int, ou
     _lib.call("citlali_hip_matvec_norm", _GGUF_TYPE[kind], _vp(w), _vp(x), ctypes.byref(nrm), _vp(y),
               1 if f32_out else 0, int(in_features), int(out_features))
 
+
+# ---- paged cache of 4-bit keys and values -----------------------------------
+def _at(x):
+    """A buffer argument of the calls below: a DeviceArray, an address or None."""
+    return x.ptr if isinstance(x, DeviceArray) else x
+
+
+def kv4_page_bytes(page_size: int, kv_heads: int, head_dim: int) -> int:
+    return int(_lib.load().citlali_hip_kv4_page_bytes(page_size, kv_heads, head_dim))
+
+
+def kv4_cache(pages, num_pages: int, page_size: int, kv_heads: int, head_dim: int) -> _lib.Kv4Cache:
+    """The cache kept in `pages` (num_pages * kv4_page_bytes(...) bytes), which
+    the caller keeps alive."""
+    return _lib.Kv4Cache(_at(pages), num_pages, page_size, kv_heads, head_dim)
+
+
+def rope_table(table, positions: int, head_dim: int, theta: float) -> None:
+    _lib.call("citlali_hip_rope_table", _at(table), positions, head_dim, theta)
+
+
+def kv4_append(cache, q, k, v, q_stride: int, kv_stride: int, q_norm, k_norm, eps: float, rope, rope_positions: int,
+               positions, slots, tokens: int, heads: int, q_out, q_out_stride: int) -> None:
+    """Norms and rotates the tokens' query and key heads, stores keys and values
+    in the cache's slots; see citlali_hip_kv4_append."""
+    _lib.call("citlali_hip_kv4_append", cache, _at(q), _at(k), _at(v), q_stride, kv_stride, _at(q_norm), _at(k_norm),
+              eps, _at(rope), rope_positions, _at(positions), _at(slots), tokens, heads, _at(q_out), q_out_stride)
+
+
+def kv4_read(cache, slots, count: int, k_out, v_out) -> None:
+    """The values that `count` slots hold, fp16 [count][kv_heads][head_dim]."""
+    _lib.call("citlali_hip_kv4_read", cache, _at(slots), count, _at(k_out), _at(v_out))
+
+
+def kv4_attention_workspace_bytes(max_context: int, max_query: int, nseq: int, tokens: int, heads: int,
+                                  kv_heads: int, head_dim: int) -> int:
+    return int(_lib.load().citlali_hip_kv4_attention_workspace_bytes(max_context, max_query, nseq, tokens, heads,
+                                                                     kv_heads, head_dim))
+
+
+def kv4_attention(cache, q, q_stride: int, query_start, context_lens, page_table, pages_per_seq: int, nseq: int,
+                  tokens: int, max_query: int, max_context: int, heads: int, workspace, workspace_bytes: int, out,
+                  out_stride: int) -> None:
+    """Causal attention of each sequence's queries over its pages; `query_start`
+    None means one query per sequence.  See citlali_hip_kv4_attention."""
+    _lib.call("citlali_hip_kv4_attention", cache, _at(q), q_stride, _at(query_start), _at(context_lens),
+              _at(page_table), pages_per_seq, nseq, tokens, max_query, max_context, heads, _at(workspace),
+              workspace_bytes, _at(out), out_stride)
+
+
+# ---- log probabilities --------------------------------------------------------
+_LOGIT_TYPE = {"fp32": 0, "fp16": 1}
+
+
+def token_logprobs_workspace_bytes(rows: int, vocab: int, top_k: int) -> int:
+    return int(_lib.load().citlali_hip_token_logprobs_workspace_bytes(rows, vocab, top_k))
+
+
+def token_logprobs(logits, kind: str, row_stride: int, rows: int, vocab: int, tokens, logprobs, ranks, entropies,
+                   top_k: int, top_ids, top_logprobs, workspace, workspace_bytes: int) -> None:
+    """kind in {"fp32", "fp16"}; outputs that are None are not computed.  See
+    citlali_hip_token_logprobs."""
+    _lib.call("citlali_hip_token_logprobs", _at(logits), _LOGIT_TYPE[kind], row_stride, rows, vocab, _at(tokens),
+              _at(logprobs), _at(ranks), _at(entropies), top_k, _at(top_ids), _at(top_logprobs), _at(workspace),
+              workspace_bytes)

@@ -325,6 +325,119 @@ int citlali_hip_matvec_gate_up_swiglu_norm(int gguf_type, const uint8_t* w_gate,
 int citlali_hip_matvec_norm(int gguf_type, const uint8_t* w, const uint16_t* x, const citlali_hip_norm* norm,
                             void* y, int f32_out, int in_features, int out_features);
 
+/* ---- paged cache of 4-bit keys and values (no reference counterpart) ------ *
+ * A cache that many sequences share page by page, each with a table of the
+ * pages it holds.  A page keeps page_size tokens of every kv head at 5 bits a
+ * value: head_dim * 5 / 4 bytes for a token's K and V of one head, where the
+ * fp16 cache takes head_dim * 4.
+ *
+ * 32 dims of one token share two fp16 numbers, m = fp16(min) and
+ * d = fp16((max - m) * fp32(1 / 15)); a dim's code is clamp(round((y - m) / d), 0, 15)
+ * (ties to even; 0 where d is 0) and stands for fp16(d * code + m).  Values
+ * saturate at +-61440 first; a NaN makes its 32 dims NaN.
+ *
+ * A slot is page * page_size + row.  One kv head's part of a page
+ * (page_bytes / kv_heads, heads in order):
+ *   K codes  [page_size][head_dim / 2] bytes: 4 bytes hold 8 dims, in order
+ *            (low bits first) dims 0 2 4 6 1 3 5 7
+ *   K params [page_size][head_dim / 32] fp16 pairs d, m
+ *   V codes  [page_size / 4][head_dim / 4][4 tokens] 16-bit words of 4 dims
+ *   V params [page_size / 4][head_dim / 32] fp16 d of 4 tokens, then m
+ * page_size 16, 32, 64, 128 or 256; head_dim 64 or 128; pages 16-byte
+ * aligned; num_pages * page_size at most INT_MAX. */
+typedef struct citlali_hip_kv4_cache {
+    uint8_t* pages; /* [num_pages][kv_heads][page_bytes / kv_heads] */
+    int num_pages;
+    int page_size;
+    int kv_heads;
+    int head_dim;
+} citlali_hip_kv4_cache;
+/* Bytes of one page; 0 for a shape the cache does not have. */
+size_t citlali_hip_kv4_page_bytes(int page_size, int kv_heads, int head_dim);
+
+/* cos and sin of position * theta^(-2i / head_dim), angles in 64 bits, for
+ * citlali_hip_kv4_append: table [positions][head_dim / 2][cos, sin] floats.
+ * Any other table of that shape (a scaled rotation, say) serves as well. */
+int citlali_hip_rope_table(float* table, int positions, int head_dim, float theta);
+
+/* Appends `tokens` tokens of any sequences in one launch.  Token t's query
+ * heads (q + t * q_stride, [heads][head_dim]) and key heads (k + t *
+ * kv_stride, [kv_heads][head_dim]) get their RMSNorm (skipped for a NULL
+ * weight) and the rotation of row positions[t] of `rope` (pairs i,
+ * i + head_dim / 2); the queries go to q_out + t * q_out_stride, rounded to
+ * fp16 once, the keys and v + t * kv_stride to slot slots[t] of the cache.
+ * Keys are normed and rotated in 64 bits, so a code is the one its definition
+ * gives.  A position outside [0, rope_positions) writes nothing for its token,
+ * a slot outside the cache stores nothing: rows of a padded batch carry -1.
+ * Two tokens of one call must not name one slot: the slot then holds parts of
+ * both.  q may be NULL with heads 0 (keys and values only); q_out may be q
+ * when the strides agree.  q, k, v and q_out 16-byte aligned, strides multiples
+ * of 8 (elements); q_norm, k_norm 16-byte, rope 8-byte aligned.
+ * tokens 0 launches nothing. */
+int citlali_hip_kv4_append(const citlali_hip_kv4_cache* cache, const uint16_t* q, const uint16_t* k,
+                           const uint16_t* v, long long q_stride, long long kv_stride, const uint16_t* q_norm,
+                           const uint16_t* k_norm, float eps, const float* rope, int rope_positions,
+                           const int32_t* positions, const int32_t* slots, int tokens, int heads, uint16_t* q_out,
+                           long long q_out_stride);
+/* The values that `count` slots hold, as fp16 rows [count][kv_heads][head_dim]
+ * (16-byte aligned); a slot outside the cache reads as zeros.  count 0 launches
+ * nothing. */
+int citlali_hip_kv4_read(const citlali_hip_kv4_cache* cache, const int32_t* slots, int count, uint16_t* k_out,
+                         uint16_t* v_out);
+
+/* Causal attention over the cache: softmax(q . K / sqrt(head_dim)) V for the
+ * queries of nseq sequences, which are each sequence's last positions.
+ *  - Queries of sequence s are rows query_start[s] .. query_start[s + 1] - 1
+ *    of q (row r at q + r * q_stride, [heads][head_dim]) and out; query_start
+ *    has nseq + 1 entries and does not decrease.  NULL: one query each, row s
+ *    (tokens == nseq).  Rows past the last sequence's are left as they were.
+ *  - context_lens[s] positions are cached, the queries' own among them: with n
+ *    queries, query i sees positions 0 .. context_lens[s] - n + i.  A query
+ *    that sees none gives zeros.
+ *  - position p of sequence s is row p % page_size of page page_table[s *
+ *    pages_per_seq + p / page_size]; a page outside the cache counts as not
+ *    there (its positions take no part).
+ *  - max_query and max_context bound the queries and the positions of a
+ *    sequence: the launch is planned for them.  Queries past max_query are
+ *    left as they were; positions past max_context are not read.
+ *    max_context is at most pages_per_seq * page_size.
+ * Slots past a sequence's positions may hold anything.  Weights are kept as
+ * fp16 times 2^14 against the largest of their pass, sums in fp32.  heads /
+ * kv_heads between 1 and 16.  Workspace:
+ * citlali_hip_kv4_attention_workspace_bytes() of the same bounds, 16-byte
+ * aligned (may be NULL if that is 0); calls that overlap need one each.  q, out 16-byte aligned, strides
+ * multiples of 8.  nseq 0 or tokens 0 launches nothing. */
+int citlali_hip_kv4_attention(const citlali_hip_kv4_cache* cache, const uint16_t* q, long long q_stride,
+                              const int32_t* query_start, const int32_t* context_lens, const int32_t* page_table,
+                              int pages_per_seq, int nseq, int tokens, int max_query, int max_context, int heads,
+                              void* workspace, size_t workspace_bytes, uint16_t* out, long long out_stride);
+size_t citlali_hip_kv4_attention_workspace_bytes(int max_context, int max_query, int nseq, int tokens, int heads,
+                                                 int kv_heads, int head_dim);
+
+/* ---- log probabilities (no reference counterpart) -------------------------- *
+ * For each of `rows` rows of logits (row r at element r * row_stride; gguf_type
+ * 0 = F32 or 1 = F16), with natural logarithms and fp32 sums:
+ *  - logprobs[r] = log softmax at tokens[r], and ranks[r], the number of tokens
+ *    before it (larger logit, or equal and a lower id); a token outside
+ *    [0, vocab) -- a row without one -- gives 0 and -1;
+ *  - entropies[r] of the row's distribution;
+ *  - top_ids / top_logprobs [rows][top_k]: the top_k most likely tokens, equal
+ *    logits by the lower id first.
+ * A logit of -inf is a token that cannot come (it adds nothing to the entropy).
+ * A row with a NaN, +inf or nothing above -inf has no distribution: its log
+ * probabilities and entropy are NaN (the ids stay ordered by logit; a NaN logit
+ * is never among them and before no token).  Fewer than top_k tokens to list:
+ * id -1, log probability -inf.  Outputs may be NULL: logprobs and ranks (tokens
+ * may then be NULL too), entropies, and top_ids with top_logprobs when top_k is
+ * 0.  top_k at most CITLALI_MAX_TOP_LOGPROBS.  Workspace:
+ * citlali_hip_token_logprobs_workspace_bytes(), 16-byte aligned (may be NULL if
+ * that is 0); calls that overlap need one each.  rows 0 launches nothing. */
+#define CITLALI_MAX_TOP_LOGPROBS 64
+int citlali_hip_token_logprobs(const void* logits, int gguf_type, long long row_stride, int rows, int vocab,
+                               const int32_t* tokens, float* logprobs, int32_t* ranks, float* entropies, int top_k,
+                               int32_t* top_ids, float* top_logprobs, void* workspace, size_t workspace_bytes);
+size_t citlali_hip_token_logprobs_workspace_bytes(int rows, int vocab, int top_k);
+
 /* Kernel timing (no reference counterpart; for benchmarks): while armed with
  * two events of citlali_hip_event_create, the first kernel the calling thread
  * launches records `start` when it begins and every kernel records `stop`

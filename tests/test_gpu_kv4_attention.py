@@ -1,0 +1,217 @@
+"""Causal attention over the paged cache of 4-bit keys and values, against
+numpy in 64 bits over the values the codes stand for.  Bar: kv4_ref.tolerance."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import kv4_ref
+
+pytestmark = pytest.mark.gpu
+
+
+class Batch:
+    def __init__(self, hip, seed, heads, kv, hd, page, lens, asked=None, spare=2, big=1.0, behind=0):
+        rng = np.random.default_rng(seed)
+        self.hip, self.heads, self.kv, self.hd, self.page = hip, heads, kv, hd, page
+        self.lens = np.array(lens, np.int32)
+        need = [max(0, -(-int(n) // page)) for n in lens]
+        self.cache = kv4_ref.Cache(sum(need) + spare, page, kv, hd).fill_random(rng, big)
+        order = rng.permutation(self.cache.num_pages)
+        self.wide = max(need + [1]) + 1
+        self.table = np.full((len(lens), self.wide), -7, np.int32)      # entries no position uses
+        at = 0
+        for s, n in enumerate(need):
+            self.table[s, :n] = order[at:at + n]
+            at += n
+        self.single = asked is None
+        self.start = np.concatenate(([0], np.cumsum(asked if asked is not None else [1] * len(lens)))).astype(np.int32)
+        self.tokens = int(self.start[-1]) + behind
+        self.max_query = max([1] + list(asked or []))
+        self.max_context = max(1, int(self.lens.max()))
+        self.q = rng.standard_normal((self.tokens, heads, hd)).astype(np.float16)
+
+    def upload(self):
+        up = self.hip.DeviceArray.from_numpy
+        self.d_raw, self.d_lens, self.d_table, self.d_start = (up(x) for x in (self.cache.raw, self.lens, self.table,
+                                                                              self.start))
+        row = self.heads * self.hd
+        self.q_stride, self.o_stride = row + 8, row + 24
+        q = np.zeros((max(1, self.tokens), self.q_stride), np.float16)
+        q[:self.tokens, :row] = self.q.reshape(self.tokens, row)
+        self.d_q = up(q)
+        self.d_out = up(np.full((max(1, self.tokens), self.o_stride), 7, np.float16))
+        self.view = self.hip.device.kv4_cache(self.d_raw, self.cache.num_pages, self.page, self.kv, self.hd)
+        self.bytes = self.hip.device.kv4_attention_workspace_bytes(self.max_context, self.max_query, len(self.lens),
+                                                                   self.tokens, self.heads, self.kv, self.hd)
+        self.d_ws = up(np.full(max(16, self.bytes), 0xFF, np.uint8))     # NaN where it is read before it is written
+        return self
+
+    def launch(self, workspace=None):
+        self.hip.device.kv4_attention(self.view, self.d_q, self.q_stride, None if self.single else self.d_start,
+                                      self.d_lens, self.d_table, self.wide, len(self.lens), self.tokens,
+                                      self.max_query, self.max_context, self.heads,
+                                      self.d_ws if workspace is None else workspace, self.bytes, self.d_out,
+                                      self.o_stride)
+        return self
+
+    def result(self):
+        row = self.heads * self.hd
+        out = self.d_out.download(np.float16, self.tokens * self.o_stride).reshape(self.tokens, self.o_stride)
+        assert (out[:, row:] == 7).all()
+        return out[:, :row].reshape(self.tokens, self.heads, self.hd)
+
+    def check(self):
+        got = self.result()
+        want, spread, reach = kv4_ref.attention(self.cache, self.q, self.start, self.lens, self.table,
+                                                self.max_context, self.max_query)
+        asked = ~np.isnan(want[:, 0, 0])
+        assert (got[~asked] == 7).all()                                   # rows nobody asks for
+        got, want = got[asked].astype(np.float64), want[asked]
+        off = np.abs(got - want) - kv4_ref.tolerance(want, spread[asked], reach[asked])
+        assert np.isfinite(got).all() and (off <= 0).all(), (np.isfinite(got).all(), off.max())
+        return got
+
+
+@pytest.mark.parametrize("page", [16, 32, 256])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("heads,kv", [(2, 2), (4, 2), (16, 2)])
+def test_decode(hip, heads, kv, hd, page):
+    lens = [1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 127, 129, 200, 511, 700]
+    Batch(hip, 1, heads, kv, hd, page, lens).upload().launch().check()
+
+
+@pytest.mark.parametrize("group", range(1, 17))
+def test_every_group(hip, group):
+    Batch(hip, group, group * 2, 2, 128 if group % 2 else 64, 16, [77, 5]).upload().launch().check()
+
+
+@pytest.mark.parametrize("lens", [[5000], [9000, 40, 1], [2049] * 3])
+def test_long_contexts(hip, lens):
+    Batch(hip, len(lens), 8, 2, 128, 64, lens).upload().launch().check()
+
+
+def test_a_large_weight_beside_small_ones(hip):
+    """Scores far apart: weights over the whole range of the exponential."""
+    Batch(hip, 9, 8, 2, 128, 16, [300, 1500], big=12.0).upload().launch().check()
+
+
+@pytest.mark.parametrize("heads,kv,hd,page,lens,asked", [
+    (8, 2, 128, 16, [40, 17, 300], [3, 2, 4]),                # a few queries each
+    (10, 2, 128, 16, [40, 700], [4, 1]),
+    (8, 8, 64, 32, [130, 64, 90], [16, 9, 1]),
+    (8, 2, 128, 16, [100], [100]),                            # whole prompts
+    (4, 1, 64, 16, [257, 33, 1], [257, 33, 1]),
+    (16, 2, 128, 64, [300, 129], [129, 65]),                  # chunks behind a prefix
+    (6, 2, 128, 128, [513], [200]),
+    (32, 2, 64, 16, [90, 20], [31, 20]),
+    (5, 5, 128, 16, [70, 300], [70, 40])])
+def test_several_queries(hip, heads, kv, hd, page, lens, asked):
+    Batch(hip, sum(lens), heads, kv, hd, page, lens, asked, behind=3).upload().launch().check()
+
+
+def test_sequences_without_positions_or_queries(hip):
+    b = Batch(hip, 3, 8, 2, 128, 16, [0, 5, 33], asked=None).upload().launch()
+    got = b.check()
+    assert not got[0].any()
+    Batch(hip, 4, 8, 2, 128, 16, [40, 40, 0, 40], asked=[0, 7, 0, 20]).upload().launch().check()
+
+
+def test_queries_before_the_first_position(hip):
+    """More queries than positions: the first ones see nothing."""
+    got = Batch(hip, 5, 4, 2, 64, 16, [3, 30], asked=[9, 30]).upload().launch().check()
+    assert not got[:6].any() and got[6:].any()
+    got = Batch(hip, 6, 4, 2, 128, 16, [2, 0], asked=[3, 2]).upload().launch().check()
+    assert not got[0].any() and got[1:3].any() and not got[3:].any()
+
+
+@pytest.mark.parametrize("asked", [None, [1, 6, 40]])
+def test_slots_past_the_end_may_hold_anything(hip, asked):
+    """NaN scales and codes behind every sequence's last position."""
+    b = Batch(hip, 7, 8, 2, 128, 32, [1, 37, 95], asked)
+    clean = b.upload().launch().check()
+    live = np.zeros((b.cache.num_pages, b.page), bool)
+    for s, n in enumerate(b.lens):
+        for p in range(n):
+            live[b.table[s, p // b.page], p % b.page] = True
+    _, kp, _, vp, _ = kv4_ref.head_layout(b.page, b.hd)
+    for page, o in np.argwhere(~live):
+        g = b.hd // 32
+        b.cache.raw[page, :, kp + o * g * 4:kp + (o + 1) * g * 4] = 0xFF
+        for j in range(g):
+            at = vp + (o // 4 * g + j) * 16 + o % 4 * 2
+            b.cache.raw[page, :, at:at + 2] = 0xFF
+            b.cache.raw[page, :, at + 8:at + 10] = 0xFF
+    assert np.array_equal(b.upload().launch().check(), clean)
+
+
+@pytest.mark.parametrize("asked", [None, [1, 6, 70]])
+def test_pages_that_are_not_there(hip, asked):
+    b = Batch(hip, 8, 8, 2, 128, 16, [20, 50, 90], asked)
+    b.table[0, 0] = -1
+    b.table[1, 1] = b.cache.num_pages
+    b.table[2, :] = 1 << 30
+    got = b.upload().launch().check()
+    assert not got[-1].any() and got[0].any()
+
+
+def test_bounds_of_the_plan(hip):
+    """Positions past max_context and queries past max_query are not touched."""
+    b = Batch(hip, 9, 8, 2, 128, 16, [300, 40])
+    b.max_context = 100
+    b.upload().launch().check()
+    b = Batch(hip, 10, 8, 2, 64, 16, [60, 40], asked=[30, 4])
+    b.max_query = 21
+    b.upload().launch().check()
+    b = Batch(hip, 11, 8, 2, 64, 16, [60, 40], asked=[3, 2])
+    b.max_query = 2
+    b.upload().launch().check()
+
+
+def test_prefixes_share_pages(hip):
+    b = Batch(hip, 12, 8, 2, 128, 16, [64, 64, 80])
+    b.table[1, :3] = b.table[0, :3]
+    b.table[2, :4] = b.table[0, :4]
+    b.upload().launch().check()
+
+
+def test_two_graphs_and_eager_calls(hip):
+    """Two captured calls with a workspace each, replayed in turn with eager
+    calls between, give the eager results every time."""
+    stream = hip.device.Stream()
+    hip.device.set_stream(stream)
+    try:
+        batches = [Batch(hip, 13, 8, 2, 128, 16, [900, 20, 333]).upload(),
+                   Batch(hip, 14, 8, 2, 64, 32, [600, 100], asked=[40, 3]).upload()]
+        want = [b.launch().check() for b in batches]
+        graphs = [hip.device.Graph.capture(b.launch) for b in batches]
+        for _ in range(3):
+            for b in batches:
+                b.d_out.zero()
+                b.d_out.upload(np.full((b.tokens, b.o_stride), 7, np.float16))
+            for g in graphs:
+                g.launch()
+            for b, w in zip(batches, want):
+                assert np.array_equal(b.check(), w)
+            batches[0].launch()
+            assert np.array_equal(batches[0].check(), want[0])
+        for g in graphs:
+            g.close()
+        hip.synchronize()
+    finally:
+        hip.device.set_stream(None)
+        stream.close()
+
+
+def test_pages_past_four_gigabytes(hip):
+    page, kv, hd = 256, 8, 128
+    b = Batch(hip, 15, 16, kv, hd, page, [300], spare=0).upload()
+    size = hip.device.kv4_page_bytes(page, kv, hd)
+    num = (1 << 32) // size + 9
+    pages = hip.DeviceArray(num * size)
+    for i in range(b.cache.num_pages):
+        pages.upload(b.cache.raw[i], (num - 1 - i) * size)
+    want = b.launch().check()
+    b.view = hip.device.kv4_cache(pages, num, page, kv, hd)
+    b.d_table = hip.DeviceArray.from_numpy(np.where(b.table >= 0, num - 1 - b.table, -1).astype(np.int32))
+    assert np.array_equal(b.launch().check(), want)
