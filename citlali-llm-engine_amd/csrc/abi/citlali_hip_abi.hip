@@ -625,6 +625,7 @@ int check_kv4(const char* who, const citlali_hip_kv4_cache* c, Kv4View* v) {
 // heads per kv head the attention kernels have, and counts the grids hold
 constexpr int kKv4MaxGroup = 16;
 constexpr int kKv4MaxHeads = 4096;
+constexpr long long kKv4MaxQueryHeads = 1ll << 25;   // a wave each in the merge: 2^31 threads
 constexpr long long kKv4MaxRows = 1ll << 28;   // head rows of one append or read: 2^32 threads
 
 int check_kv4_attention(const char* who, int max_context, int max_query, int nseq, int tokens, int heads,
@@ -635,6 +636,8 @@ int check_kv4_attention(const char* who, int max_context, int max_query, int nse
     REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "%s: heads (%d) must be a multiple of kv_heads (%d)",
             who, heads, kv_heads);
     REQUIRE(nseq <= 65535 && heads <= kKv4MaxHeads, "%s: at most 65535 sequences and %d heads", who, kKv4MaxHeads);
+    REQUIRE((long long)max_query * heads <= kKv4MaxQueryHeads, "%s: max_query (%d) times heads (%d) exceeds %lld", who,
+            max_query, heads, kKv4MaxQueryHeads);
     if (heads / kv_heads > kKv4MaxGroup)
         return fail(CITLALI_ERR_UNSUPPORTED, "%s: %d query heads per kv head are not built (1..%d)", who,
                     heads / kv_heads, kKv4MaxGroup);

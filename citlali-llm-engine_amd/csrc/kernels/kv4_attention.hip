@@ -298,7 +298,8 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : 2) void kv4_decode_kernel(Kv
 // Log-sum-exp merge of the chunks of one (query, head) by one wave, HD / 64
 // dims a lane.
 template <int HD>
-__global__ __launch_bounds__(kBlk) void kv4_merge_kernel(Kv4Attention a, int chunk, int n_splits) {
+__global__ __launch_bounds__(kBlk) void kv4_merge_kernel(Kv4Attention a, int group, int tile_rows, int chunk,
+                                                         int n_splits) {
     constexpr int kPer = HD / kWave;
     const int seq = blockIdx.y, lane = threadIdx.x & (kWave - 1);
     const Kv4Seq s = kv4_seq(a, seq);
@@ -306,7 +307,9 @@ __global__ __launch_bounds__(kBlk) void kv4_merge_kernel(Kv4Attention a, int chu
     const int unit = blockIdx.x * kWaves + threadIdx.x / kWave;
     const int i = unit / a.heads, head = unit - i * a.heads;
     if (i >= asked) return;
-    const int most = s.see(asked - 1);
+    // the positions that the rows of its workgroups saw
+    const int tile = (i * group + head % group) / tile_rows;
+    const int most = s.see((int)(min((long long)asked * group, (tile + 1ll) * tile_rows) - 1) / group);
     if (most <= chunk) return;   // written by the chunk itself
     const int n = (most + chunk - 1) / chunk;
     const size_t at = ((size_t)(s.start + i) * a.heads + head) * n_splits;
@@ -337,86 +340,321 @@ __global__ __launch_bounds__(kBlk) void kv4_merge_kernel(Kv4Attention a, int chu
     for (int e = 0; e < kPer; ++e) out[e] = f2h_rne(acc[e] * inv);
 }
 
-// One wave per (query, sequence, head): lane = position for the scores, lane =
-// dims for the values.
+// ---------------------------------------------------------------------------
+// Many rows (prompts): one workgroup per (chunk of positions, 128 rows, kv
+// head, sequence), 32 rows a wave, tiles of 64 positions.  Bound by the matrix
+// products and what goes on beside them:
+//  * the workgroup turns a tile's codes into fp16 once, for all its rows: each
+//    wave takes 16 positions' K and V (one page), loaded two tiles ahead, into
+//    one of two LDS buffers while the other is used; one barrier a tile.
+//  * K in LDS as [8 dims][position][8] and V as [16 positions][half][dim][8
+//    positions]: the A operands of v_mfma_f32_32x32x16_f16 are 16-byte reads
+//    of consecutive lanes, without bank conflicts.
+//  * S^T = K Q^T: column = row of Q = lane & 31, so the softmax of a row is one
+//    lane's 32 scores and its partner's 32 lanes away, and the weights are the
+//    B operand of O^T = V^T P^T as they stand: lane half h has the positions
+//    8 a + 4 h + b of 32 (a, b = 0..3), the order V is laid in.
+//  * V's dim HD/16 c + n lies at 16 n + c, so that the 16 lanes that write one n
+//    use different banks.
+//  * the maximum a row's weights refer to moves only when it is exceeded by
+//    kSlack (base 2), which spares O its rescaling in most tiles.
+// ---------------------------------------------------------------------------
+constexpr int kRowTile = 128, kTile = 64;   // rows of a workgroup; positions of a step
+constexpr float kSlack = 4.f;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
 template <int HD>
-__global__ __launch_bounds__(kWave) void kv4_attention_rows_kernel(Kv4View c, Kv4Attention a, float scale) {
+__global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Attention a, int chunk, int n_splits,
+                                                             float scale_log2) {
     using L = Kv4Layout<HD>;
-    const int i = blockIdx.x, seq = blockIdx.y, head = blockIdx.z, lane = threadIdx.x;
+    using Vec = std::conditional_t<HD == 128, u32x4, u32x2>;
+    constexpr int kWords = HD / 32;                    // words of codes a thread has of a position (K) or of 4 (V)
+    constexpr int kHalves = HD * kTile;                // of K (or V) in a buffer
+    extern __shared__ __align__(16) float lds[];
+    uint16_t* const buf = reinterpret_cast<uint16_t*>(lds);              // [2][K, V][kHalves]
+    int* const there_at = reinterpret_cast<int*>(buf + 4 * kHalves);     // [2][4 waves]: the 16 positions have a page
+
+    // kv heads side by side, so that the workgroups of one meet in an XCD's L2
+    // where there are eight of them; row tiles with the most positions first
+    const int kvh = blockIdx.x % c.kv_heads, seq = blockIdx.y, rest = blockIdx.x / c.kv_heads;
+    const int split = rest % n_splits, tile = gridDim.x / (c.kv_heads * n_splits) - 1 - rest / n_splits;
     const Kv4Seq s = kv4_seq(a, seq);
-    if (i >= s.n) return;
-    const int see = s.see(i), kvh = head / (a.heads / c.kv_heads), P = 1 << c.page_shift;
-    __shared__ float qs[HD], ps[kWave];
-    __shared__ const uint8_t* bases[kWave];
-    for (int d = lane; d < HD; d += kWave)
-        qs[d] = h2f(a.q[(size_t)(s.start + i) * a.q_stride + (size_t)head * HD + d]) * scale;
+    const int group = a.heads / c.kv_heads, rows = min(s.n, a.max_query) * group;
+    const int row0 = tile * kRowTile;
+    if (row0 >= rows) return;
+    const int most = max(0, s.see((min(rows, row0 + kRowTile) - 1) / group));
+    const int c0 = split * chunk, c1 = min(most, c0 + chunk);
+    if (c0 >= most && split > 0) return;
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int col = lane & 31, half = lane >> 5;
+
+    // this lane's row of Q
+    const int r = row0 + 32 * wave + col;
+    const bool real = r < rows;
+    const int i = real ? r / group : 0;
+    const size_t head = (size_t)kvh * group + (real ? r - i * group : 0);
+    const int see = real ? min(s.see(i), c1) : 0;
+    half8 q[HD / 16];
+    {
+        const uint16_t* qr = a.q + (size_t)(s.start + i) * a.q_stride + head * HD + 8 * half;
+#pragma unroll
+        for (int t = 0; t < HD / 16; ++t) {
+            u32x4 v = *reinterpret_cast<const u32x4*>(qr + 16 * t);
+            if (!real) v = u32x4{0u, 0u, 0u, 0u};
+            q[t] = __builtin_bit_cast(half8, v);
+        }
+    }
+    // positions that every / any row of the wave sees
+    const int r_last = min(rows - 1, row0 + 32 * wave + 31);
+    const int wave_least = r_last < row0 + 32 * wave + 31 ? 0 : min(s.see((row0 + 32 * wave) / group), c1);
+    const int wave_most = row0 + 32 * wave >= rows ? 0 : min(s.see(r_last / group), c1);
+
+    // ---- the wave's 16 positions of a tile: pages, loads, dequantisation ----
+    const int P = 1 << c.page_shift;
+    const int last_page = (max(c1, 1) - 1) >> c.page_shift;
+    const int32_t* table = a.page_table + (size_t)seq * a.pages_per_seq;
+    int window = c0 >> c.page_shift;   // lane j has page window + j of the table, then of the 64 after them
+    auto pages_from = [&](int first) { return table[min(first + lane, last_page)]; };
+    int pages = pages_from(window), pages_next = pages_from(window + kWave);
+    const int t16 = lane & 15, g = lane >> 4;            // K: position, quarter of the dims
+    const int vb = ((g & 1) << 1) | (g >> 1);            // V: block of 4 positions, dims HD/16 t16 ..
+    Vec xk, xv;
+    uint32_t xkp;
+    u32x4 xvp;
+    int x_there = 0, x_pos = 0;
+    auto load = [&](int t) {
+        const int p = t + 16 * wave, at = min(p >> c.page_shift, last_page);
+        if (at >= window + kWave) {   // uniform
+            window += kWave;
+            pages = pages_next;
+            pages_next = pages_from(window + kWave);
+        }
+        const int page = __builtin_amdgcn_readlane(pages, at - window);
+        x_there = p < c1 && page >= 0 && page < c.num_pages;
+        x_pos = p;
+        const uint8_t* base = kv4_head<HD>(c, x_there ? page : 0, kvh);
+        const int o = p & (P - 1);
+        xk = *reinterpret_cast<const Vec*>(base + (o + t16) * L::kCodes + g * (HD / 8));
+        xkp = *reinterpret_cast<const uint32_t*>(base + L::k_params(P) + (o + t16) * L::kParams +
+                                                 (HD == 128 ? g : g >> 1) * 4);
+        xv = *reinterpret_cast<const Vec*>(base + L::v_codes(P) + ((o >> 2) + vb) * (4 * L::kCodes) + t16 * (HD / 8));
+        xvp = *reinterpret_cast<const u32x4*>(base + L::v_params(P) + ((o >> 2) + vb) * (4 * L::kParams) +
+                                              t16 / (512 / HD) * 16);
+    };
+    auto store = [&](int b) {
+        uint16_t* kb = buf + b * 2 * kHalves;
+        uint16_t* vbuf = kb + kHalves;
+        const f16x2 dm = as_h2(xkp);
+        const f16x2 d{dm.x, dm.x}, m{dm.y, dm.y};
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) {
+            f16x2 e[4];
+            kv4_pairs(xk[w], d, m, e);
+            *reinterpret_cast<half8*>(kb + ((g * kWords + w) * kTile + 16 * wave + t16) * 8) =
+                __builtin_bit_cast(half8, e);
+        }
+        // positions past the chunk or without a page: V counts as 0, whatever it holds
+        const int left = x_there ? c1 - (x_pos + 4 * vb) : 0;
+        const uint32_t lo = left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
+        const uint32_t hi = left >= 4 ? 0xffffffffu : left == 3 ? 0xffffu : 0u;
+        xvp &= u32x4{lo, hi, lo, hi};
+#pragma unroll
+        for (int h = 0; h < kWords / 2; ++h) {
+            f16x2 e[2][4];
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+                kv4_pairs(xv[2 * h + y], as_h2(xvp[y]), as_h2(xvp[2 + y]), e[y]);
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+                *reinterpret_cast<u32x2*>(vbuf + (((2 * wave + (vb & 1)) * HD) + (4 * h + n) * 16 + t16) * 8 +
+                                          (vb >> 1) * 4) =
+                    u32x2{__builtin_bit_cast(uint32_t, e[0][n]), __builtin_bit_cast(uint32_t, e[1][n])};
+        }
+        if (lane == 0) there_at[b * 4 + wave] = x_there;
+    };
+
+    f32x16 o[HD / 32];
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+    float m_run = -INFINITY, l_run = 0.f;
+
+    auto process = [&](int t, int b) {
+        const uint16_t* kb = buf + b * 2 * kHalves;
+        const uint16_t* vbuf = kb + kHalves;
+        if (t >= wave_most) return;   // uniform: no row of the wave sees the tile
+        int there = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) there |= (there_at[b * 4 + w] != 0) << w;
+        there = __builtin_amdgcn_readfirstlane(there);
+        const bool whole = there == 15 && t + kTile <= wave_least;
+        f32x16 sc[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sc[u][e] = 0.f;
+#pragma unroll
+            for (int st = 0; st < HD / 16; ++st) {
+                const half8 k = *reinterpret_cast<const half8*>(kb + ((2 * st + half) * kTile + 32 * u + col) * 8);
+                sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[st], sc[u], 0, 0, 0);
+            }
+        }
+        if (!whole) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int p = 32 * u + 8 * (e / 4) + 4 * half + e % 4;
+                    const bool seen = t + p < see && ((there >> (p >> 4)) & 1);
+                    sc[u][e] = seen ? sc[u][e] : -INFINITY;
+                }
+        }
+        float mt = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mt = fmaxf(mt, sc[u][e]);
+        mt = max32(mt) * scale_log2;
+        if (__builtin_amdgcn_ballot_w64(mt > m_run + kSlack || (m_run == -INFINITY && mt > m_run)) != 0) {
+            const float m_new = fmaxf(m_run, mt);
+            const float f = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
+            m_run = m_new;
+            l_run *= f;
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d) o[d] *= f;
+        }
+        const float off = kShift - kSlack - (m_run == -INFINITY ? 0.f : m_run);
+        half8 pw[4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float w = __builtin_amdgcn_exp2f(fmaf(sc[u][e], scale_log2, off));
+                l_run += w;
+                pw[2 * u + e / 8][e % 8] = (_Float16)w;
+            }
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d) {
+                const half8 v = *reinterpret_cast<const half8*>(vbuf + ((2 * st + half) * HD + 32 * d + col) * 8);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pw[st], o[d], 0, 0, 0);
+            }
+    };
+
+    load(c0);
+    store(0);
+    load(c0 + kTile);
     __syncthreads();
-    float m_run = -INFINITY, l_run = 0.f, acc[HD / kWave] = {};
-    for (int p0 = 0; p0 < see; p0 += kWave) {
-        const int p = p0 + lane, o = p & (P - 1);
-        int page = -1;
-        if (p < see) page = a.page_table[(size_t)seq * a.pages_per_seq + (p >> c.page_shift)];
-        if (page >= c.num_pages) page = -1;
-        float x = -INFINITY;
-        const uint8_t* base = page >= 0 ? kv4_head<HD>(c, page, kvh) : nullptr;
-        if (page >= 0) {
-            x = 0.f;
-            for (int w8 = 0; w8 < HD / 8; ++w8) {
-                const f16x2 dm =
-                    as_h2(*reinterpret_cast<const uint32_t*>(base + L::k_params(P) + o * L::kParams + w8 / 4 * 4));
-                f16x2 v[4];
-                kv4_pairs(*reinterpret_cast<const uint32_t*>(base + o * L::kCodes + 4 * w8), f16x2{dm.x, dm.x},
-                          f16x2{dm.y, dm.y}, v);
-                for (int e = 0; e < 4; ++e)
-                    x += (float)v[e].x * qs[8 * w8 + 2 * e] + (float)v[e].y * qs[8 * w8 + 2 * e + 1];
-            }
-        }
-        const float m = fmaxf(m_run, wave_max(x));
-        const float w = m == -INFINITY ? 0.f : expf(x - m), f = m == -INFINITY ? 1.f : expf(m_run - m);
-        l_run = l_run * f + wave_sum(w);
-        m_run = m;
-        ps[lane] = w;
-        bases[lane] = base;
-        __syncthreads();
-        for (int e = 0; e < HD / kWave; ++e) {
-            const int d = lane + e * kWave;
-            acc[e] *= f;
-            for (int j = 0; j < kWave; ++j) {
-                const uint8_t* b = bases[j];
-                if (b == nullptr) continue;
-                const int oj = (p0 + j) & (P - 1);
-                const uint32_t word =
-                    reinterpret_cast<const uint16_t*>(b + L::v_codes(P))[((oj >> 2) * (HD / 4) + d / 4) * 4 + (oj & 3)];
-                const _Float16* vp = reinterpret_cast<const _Float16*>(b + L::v_params(P)) +
-                                     ((oj >> 2) * (HD / kKv4Group) + d / kKv4Group) * 8 + (oj & 3);
-                const _Float16 v = __builtin_fmaf16((_Float16)(float)((word >> (4 * (d & 3))) & 15u), vp[0], vp[4]);
-                acc[e] += ps[j] * (float)v;
-            }
-        }
+    for (int t = c0, b = 0; t < c1; t += kTile, b ^= 1) {
+        store(b ^ 1);              // the next tile
+        load(t + 2 * kTile);
+        process(t, b);
         __syncthreads();
     }
-    for (int e = 0; e < HD / kWave; ++e)
-        a.out[(size_t)(s.start + i) * a.out_stride + (size_t)head * HD + lane + e * kWave] =
-            f2h_rne(l_run > 0.f ? acc[e] / l_run : 0.f);
+
+    // ---- out: O^T's rows back in dim order through LDS, a wave's rows at a time ----
+    const float l = sum32(l_run);
+    const bool alone = most <= chunk;
+    if (alone) {
+        constexpr int kPitch = HD + 8;
+        uint16_t* rowbuf = buf + wave * 32 * kPitch;
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int slot = 32 * d + 8 * (e / 4) + 4 * half + e % 4;
+                rowbuf[col * kPitch + slot % 16 * (HD / 16) + slot / 16] = f2h_rne(o[d][e] * inv);
+            }
+        wave_lds_sync();
+        for (int idx = lane; idx < 32 * (HD / 8); idx += kWave) {
+            const int rr = idx / (HD / 8), r1 = row0 + 32 * wave + rr, piece = idx % (HD / 8);
+            if (r1 >= rows) break;
+            const int i1 = r1 / group;
+            *reinterpret_cast<u32x4*>(a.out + (size_t)(s.start + i1) * a.out_stride +
+                                      ((size_t)kvh * group + (r1 - i1 * group)) * HD + 8 * piece) =
+                *reinterpret_cast<const u32x4*>(rowbuf + rr * kPitch + 8 * piece);
+        }
+        return;
+    }
+    if (!real) return;
+    const size_t at = ((size_t)(s.start + i) * a.heads + head) * n_splits + split;
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int slot = 32 * d + 8 * (e / 4) + 4 * half + e % 4;
+            a.workspace[at * HD + slot % 16 * (HD / 16) + slot / 16] = o[d][e];
+        }
+    if (half == 0) {
+        float* ml = a.workspace + (size_t)a.tokens * a.heads * n_splits * HD + 2 * at;
+        ml[0] = m_run;
+        ml[1] = l;
+    }
 }
 
-
-// Positions a workgroup takes: whole turns of its four waves, few enough for a
-// lane per page, and about eight workgroups per CU where the bound allows.
-constexpr int kChunkStep = 32 * kWaves, kChunkMost = 1024, kTargetBlocks = 2048;
+// The few-row kernel takes up to 32 rows.  Its workgroups take whole turns of
+// their four waves, at most 1024 positions (a lane per page), about eight
+// workgroups per CU where the bound allows.  The prompt kernel splits the
+// positions only where its row tiles leave CUs without work.
+constexpr int kFewRows = 32, kChunkStep = 32 * kWaves, kChunkMost = 1024, kFewBlocks = 2048;
+constexpr int kPromptBlocks = 512, kPromptChunk = 512;
 struct Kv4Plan {
-    bool few;   // the few-row kernel, else one wave per row
-    int cols, chunk, n_splits;
+    bool few;
+    int cols, tiles, chunk, n_splits;
 };
 Kv4Plan kv4_plan(int max_context, int max_query, int nseq, int heads, int kv_heads) {
     Kv4Plan p{};
     const long long rows = (long long)max_query * (heads / kv_heads);
-    p.few = rows <= 32;
+    p.few = rows <= kFewRows;
     p.cols = rows <= 16 ? 1 : 2;
-    const long long want = ((long long)max_context * nseq * kv_heads + kTargetBlocks - 1) / kTargetBlocks;
-    p.chunk = (int)std::min<long long>(kChunkMost, std::max<long long>(1, (want + kChunkStep - 1) / kChunkStep) * kChunkStep);
+    p.tiles = (int)((rows + kRowTile - 1) / kRowTile);
+    if (p.few) {
+        const long long want = ((long long)max_context * nseq * kv_heads + kFewBlocks - 1) / kFewBlocks;
+        p.chunk = (int)std::min<long long>(kChunkMost, std::max<long long>(1, (want + kChunkStep - 1) / kChunkStep) * kChunkStep);
+    } else {
+        const long long blocks = (long long)p.tiles * kv_heads * nseq;
+        const long long splits = std::max<long long>(1, std::min<long long>(kPromptBlocks / blocks, max_context / kPromptChunk));
+        p.chunk = (int)((max_context + splits - 1) / splits);
+        p.chunk = (p.chunk + kTile - 1) / kTile * kTile;
+    }
     p.n_splits = (max_context + p.chunk - 1) / p.chunk;
     return p;
+}
+
+template <int HD>
+hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
+    const Kv4Plan p = kv4_plan(a.max_context, a.max_query, a.nseq, a.heads, c.kv_heads);
+    const float scale_log2 = 1.44269504088896340736f / sqrtf((float)HD);
+    const int group = a.heads / c.kv_heads;
+    const bool last = p.n_splits == 1;
+    if (!p.few) {
+        const int lds = 4 * HD * kTile * (int)sizeof(uint16_t) + 8 * (int)sizeof(int);
+        const hipError_t e = allow_lds<kv4_prompt_kernel<HD>>(lds);
+        if (e != hipSuccess) return e;
+        launch_kernel_in_call(last, kv4_prompt_kernel<HD>, dim3(c.kv_heads * p.tiles * p.n_splits, a.nseq), dim3(kBlk), lds, s,
+                              c, a, p.chunk, p.n_splits, scale_log2);
+    } else {
+        const dim3 grid(p.n_splits, c.kv_heads, a.nseq);
+        const int lds = kWaves * a.max_query * group * (HD + 4) * (int)sizeof(float);
+        if (p.cols == 1) {
+            launch_kernel_in_call(last, kv4_decode_kernel<HD, 1>, grid, dim3(kBlk), lds, s, c, a, p.chunk, p.n_splits,
+                                  scale_log2);
+        } else {
+            const hipError_t e = allow_lds<kv4_decode_kernel<HD, 2>>(lds);
+            if (e != hipSuccess) return e;
+            launch_kernel_in_call(last, kv4_decode_kernel<HD, 2>, grid, dim3(kBlk), lds, s, c, a, p.chunk, p.n_splits,
+                                  scale_log2);
+        }
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || last) return e;
+    const long long units = (long long)a.max_query * a.heads;
+    launch_kernel(kv4_merge_kernel<HD>, dim3((unsigned)((units + kWaves - 1) / kWaves), a.nseq), dim3(kBlk), 0, s, a,
+                  group, p.few ? kFewRows : kRowTile, p.chunk, p.n_splits);
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -424,37 +662,9 @@ Kv4Plan kv4_plan(int max_context, int max_query, int nseq, int heads, int kv_hea
 size_t kv4_attention_workspace(int max_context, int max_query, int nseq, int tokens, int heads, int kv_heads,
                                int head_dim) {
     const Kv4Plan p = kv4_plan(max_context, max_query, nseq, heads, kv_heads);
-    if (!p.few || p.n_splits == 1) return 0;
+    if (p.n_splits == 1) return 0;
     return (size_t)tokens * heads * p.n_splits * (head_dim + 2) * sizeof(float);
 }
-
-namespace {
-template <int HD>
-hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
-    const Kv4Plan p = kv4_plan(a.max_context, a.max_query, a.nseq, a.heads, c.kv_heads);
-    const float scale = 1.f / sqrtf((float)HD);
-    if (!p.few) {
-        launch_kernel(kv4_attention_rows_kernel<HD>, dim3(a.max_query, a.nseq, a.heads), dim3(kWave), 0, s, c, a, scale);
-        return hipGetLastError();
-    }
-    const float scale_log2 = scale * 1.44269504088896340736f;
-    const dim3 grid(p.n_splits, c.kv_heads, a.nseq);
-    const size_t lds = (size_t)kWaves * a.max_query * (a.heads / c.kv_heads) * (HD + 4) * sizeof(float);
-    if (p.cols == 1) {
-        launch_kernel_in_call(p.n_splits == 1, kv4_decode_kernel<HD, 1>, grid, dim3(kBlk), lds, s, c, a, p.chunk,
-                              p.n_splits, scale_log2);
-    } else {
-        const hipError_t e = allow_lds<kv4_decode_kernel<HD, 2>>((int)lds);
-        if (e != hipSuccess) return e;
-        launch_kernel_in_call(p.n_splits == 1, kv4_decode_kernel<HD, 2>, grid, dim3(kBlk), lds, s, c, a, p.chunk,
-                              p.n_splits, scale_log2);
-    }
-    if (p.n_splits > 1)
-        launch_kernel(kv4_merge_kernel<HD>, dim3((a.max_query * a.heads + kWaves - 1) / kWaves, a.nseq), dim3(kBlk), 0,
-                      s, a, p.chunk, p.n_splits);
-    return hipGetLastError();
-}
-}  // namespace
 
 hipError_t launch_kv4_attention(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
     return c.head_dim == 128 ? launch_for<128>(c, a, s) : launch_for<64>(c, a, s);

@@ -78,7 +78,7 @@ def test_read(change):
 @pytest.mark.parametrize("change,status", [
     (dict(nseq=-1), INVALID), (dict(tokens=-1), INVALID), (dict(max_query=0), INVALID), (dict(max_context=0), INVALID),
     (dict(heads=0), INVALID), (dict(heads=9), INVALID), (dict(heads=34), UNSUPPORTED), (dict(nseq=1 << 16), INVALID),
-    (dict(q=None), INVALID), (dict(context_lens=None), INVALID), (dict(page_table=None), INVALID),
+    (dict(max_query=1 << 24), INVALID), (dict(q=None), INVALID), (dict(context_lens=None), INVALID), (dict(page_table=None), INVALID),
     (dict(out=None), INVALID), (dict(tokens=3), INVALID), (dict(pages_per_seq=0), INVALID),
     (dict(max_context=65), INVALID), (dict(q_stride=1016), INVALID), (dict(out_stride=8), INVALID),
     (dict(q_stride=1025), INVALID), (dict(out_stride=1028), INVALID), (dict(q=A + 4), INVALID),
