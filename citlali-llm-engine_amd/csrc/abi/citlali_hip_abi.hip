@@ -758,6 +758,7 @@ CITLALI_EXPORT int citlali_hip_token_logprobs(const void* logits, int gguf_type,
                                               void* workspace, size_t workspace_bytes) {
     REQUIRE(gguf_type == 0 || gguf_type == 1, "token_logprobs: GGUF type %d is not F32 or F16", gguf_type);
     REQUIRE(rows >= 0 && vocab > 0, "token_logprobs: bad rows (%d) or vocab (%d)", rows, vocab);
+    REQUIRE(rows <= 1 << 23, "token_logprobs: %d rows are too many", rows);
     REQUIRE(logits, "token_logprobs received a null buffer");
     REQUIRE(row_stride >= vocab, "token_logprobs: row_stride (%lld) is shorter than vocab (%d)", row_stride, vocab);
     REQUIRE(aligned(logits, gguf_type == 0 ? 4 : 2), "token_logprobs: logits are not aligned to their type");

@@ -102,7 +102,7 @@ def test_attention_workspace():
 
 
 @pytest.mark.parametrize("change", [
-    dict(rows=-1), dict(vocab=0), dict(logits=None), dict(row_stride=999), dict(logits=A + 2),
+    dict(rows=-1), dict(rows=(1 << 23) + 1), dict(vocab=0), dict(logits=None), dict(row_stride=999), dict(logits=A + 2),
     dict(kind="fp16", logits=A + 1), dict(tokens=None), dict(tokens=None, logprobs=None), dict(top_k=-1),
     dict(top_k=65), dict(top_ids=None), dict(top_logprobs=None)])
 def test_logprobs(change):
