@@ -34,19 +34,24 @@ __device__ __forceinline__ uint8_t* kv4_head(const Kv4View& c, int page, int kv_
 // neighbouring dims; OR-ed into the mantissa of 1024 (or, a nibble higher, as
 // 16 q) a pair becomes fp16 in one instruction, 1024 comes off exactly, and one
 // packed fma rounds d q + m once.  d and m: the pair's scales, one per half.
-__device__ __forceinline__ f16x2 kv4_low(uint32_t w) {   // nibbles 0 and 4
-    return __builtin_bit_cast(f16x2, (w & 0x000F000Fu) | 0x64006400u) - f16x2{(_Float16)1024.f, (_Float16)1024.f};
-}
-__device__ __forceinline__ f16x2 kv4_high(uint32_t w) {   // nibbles 1 and 5
-    const f16x2 h = __builtin_bit_cast(f16x2, (w & 0x00F000F0u) | 0x64006400u);
-    return __builtin_elementwise_fma(h, f16x2{(_Float16)0.0625f, (_Float16)0.0625f},
-                                     f16x2{(_Float16)-64.f, (_Float16)-64.f});
+// The mask lies in an SGPR and 1024 in a VGPR (an operand may not be a literal
+// there); from C++ the compiler makes two instructions of it.
+__device__ __forceinline__ uint32_t kv4_and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(mask), "v"(bits));
+    return r;
 }
 __device__ __forceinline__ void kv4_pairs(uint32_t w, f16x2 d, f16x2 m, f16x2 (&out)[4]) {
-    out[0] = __builtin_elementwise_fma(kv4_low(w), d, m);
-    out[1] = __builtin_elementwise_fma(kv4_high(w), d, m);
-    out[2] = __builtin_elementwise_fma(kv4_low(w >> 8), d, m);
-    out[3] = __builtin_elementwise_fma(kv4_high(w >> 8), d, m);
+    constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u, k1024 = 0x64006400u;
+    const f16x2 off{(_Float16)1024.f, (_Float16)1024.f};
+    const f16x2 sixteenth{(_Float16)0.0625f, (_Float16)0.0625f}, off16{(_Float16)-64.f, (_Float16)-64.f};
+    const uint32_t v = w >> 8;
+    out[0] = as_h2(kv4_and_or(w, kLow, k1024)) - off;
+    out[1] = __builtin_elementwise_fma(as_h2(kv4_and_or(w, kHigh, k1024)), sixteenth, off16);
+    out[2] = as_h2(kv4_and_or(v, kLow, k1024)) - off;
+    out[3] = __builtin_elementwise_fma(as_h2(kv4_and_or(v, kHigh, k1024)), sixteenth, off16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = __builtin_elementwise_fma(out[i], d, m);
 }
 
 }  // namespace citlali::hip

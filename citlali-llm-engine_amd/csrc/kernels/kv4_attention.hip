@@ -10,6 +10,14 @@
 namespace citlali::hip {
 namespace {
 
+// The largest of three, as one instruction (fmaxf first makes a quiet NaN of
+// each operand that a matrix instruction wrote).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
 // The queries of sequence `seq`: rows start .. start + n - 1 of q, the cached
 // positions that exist, and how many of them query i sees (see()).
 struct Kv4Seq {
@@ -74,7 +82,7 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : 2) void kv4_decode_kernel(Kv
     const int most = max(0, s.see(asked - 1));   // positions any row sees
     const int c0 = split * chunk, c1 = min(most, c0 + chunk);
     if (c0 >= most && split > 0) return;
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int col = lane & 15, grp = lane >> 4;
 
     // page of 16 .. positions j of the chunk's pages: lane j (a chunk has at most 64)
@@ -117,25 +125,25 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : 2) void kv4_decode_kernel(Kv
     Vec xk[2], xv[2];
     uint32_t xkp[2];
     u32x4 xvp[2];
+    // uniform addresses plus a lane's own offsets
+    const uint32_t at_k = col * L::kCodes + grp * (HD / 8), at_kp = col * L::kParams + (HD == 128 ? grp : grp >> 1) * 4;
+    const uint32_t at_v = grp * (4 * L::kCodes) + col * (HD / 8), at_vp = grp * (4 * L::kParams) + col / (512 / HD) * 16;
+    const uint8_t* at_head[2];
     auto load_k = [&](int t) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const uint8_t* base = head_at(t + 16 * u);
             const int o = (t + 16 * u) & (P - 1) & ~15;
-            xk[u] = *reinterpret_cast<const Vec*>(base + (o + col) * L::kCodes + grp * (HD / 8));
-            xkp[u] = *reinterpret_cast<const uint32_t*>(base + L::k_params(P) + (o + col) * L::kParams +
-                                                        (HD == 128 ? grp : grp >> 1) * 4);
+            at_head[u] = head_at(t + 16 * u);
+            xk[u] = *reinterpret_cast<const Vec*>(at_head[u] + o * L::kCodes + at_k);
+            xkp[u] = *reinterpret_cast<const uint32_t*>(at_head[u] + L::k_params(P) + o * L::kParams + at_kp);
         }
     };
-    auto load_v = [&](int t) {
+    auto load_v = [&](int t) {   // of the positions that load_k took last
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const uint8_t* base = head_at(t + 16 * u);
             const int o = (t + 16 * u) & (P - 1) & ~15;
-            xv[u] = *reinterpret_cast<const Vec*>(base + L::v_codes(P) + ((o >> 2) + grp) * (4 * L::kCodes) +
-                                                  col * (HD / 8));
-            xvp[u] = *reinterpret_cast<const u32x4*>(base + L::v_params(P) + ((o >> 2) + grp) * (4 * L::kParams) +
-                                                     col / (512 / HD) * 16);
+            xv[u] = *reinterpret_cast<const Vec*>(at_head[u] + L::v_codes(P) + o * L::kCodes + at_v);
+            xvp[u] = *reinterpret_cast<const u32x4*>(at_head[u] + L::v_params(P) + o * L::kParams + at_vp);
         }
     };
 
@@ -179,6 +187,7 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : 2) void kv4_decode_kernel(Kv
 #pragma unroll
         for (int n = 0; n < kCols; ++n) {
             if (!whole) {
+                asm volatile("");   // a branch: most tiles skip it
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -187,8 +196,8 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : 2) void kv4_decode_kernel(Kv
                         sc[n][u][i] = seen ? sc[n][u][i] : -INFINITY;
                     }
             }
-            float mt = fmaxf(fmaxf(fmaxf(sc[n][0][0], sc[n][0][1]), fmaxf(sc[n][0][2], sc[n][0][3])),
-                             fmaxf(fmaxf(sc[n][1][0], sc[n][1][1]), fmaxf(sc[n][1][2], sc[n][1][3])));
+            float mt = max3(max3(sc[n][0][0], sc[n][0][1], sc[n][0][2]), sc[n][0][3], sc[n][1][0]);
+            mt = max3(mt, sc[n][1][1], max3(sc[n][1][2], sc[n][1][3], sc[n][1][3]));
             mt = max32(max16(mt)) * scale_log2;
             if (__builtin_amdgcn_ballot_w64(mt > m_run[n]) != 0) {
                 const float m_new = fmaxf(m_run[n], mt);
@@ -346,7 +355,8 @@ __global__ __launch_bounds__(kBlk) void kv4_merge_kernel(Kv4Attention a, int gro
 // products and what goes on beside them:
 //  * the workgroup turns a tile's codes into fp16 once, for all its rows: each
 //    wave takes 16 positions' K and V (one page), loaded two tiles ahead, into
-//    one of two LDS buffers while the other is used; one barrier a tile.
+//    one of two LDS buffers while the other is used; one barrier a tile.  That
+//    work is set between the score products, which do not depend on it.
 //  * K in LDS as [8 dims][position][8] and V as [16 positions][half][dim][8
 //    positions]: the A operands of v_mfma_f32_32x32x16_f16 are 16-byte reads
 //    of consecutive lanes, without bank conflicts.
@@ -385,7 +395,7 @@ __global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Atten
     const int most = max(0, s.see((min(rows, row0 + kRowTile) - 1) / group));
     const int c0 = split * chunk, c1 = min(most, c0 + chunk);
     if (c0 >= most && split > 0) return;
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int col = lane & 31, half = lane >> 5;
 
     // this lane's row of Q
@@ -421,6 +431,8 @@ __global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Atten
     Vec xk, xv;
     uint32_t xkp;
     u32x4 xvp;
+    const uint32_t at_k = t16 * L::kCodes + g * (HD / 8), at_kp = t16 * L::kParams + (HD == 128 ? g : g >> 1) * 4;
+    const uint32_t at_v = vb * (4 * L::kCodes) + t16 * (HD / 8), at_vp = vb * (4 * L::kParams) + t16 / (512 / HD) * 16;
     int x_there = 0, x_pos = 0;
     auto load = [&](int t) {
         const int p = t + 16 * wave, at = min(p >> c.page_shift, last_page);
@@ -434,12 +446,10 @@ __global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Atten
         x_pos = p;
         const uint8_t* base = kv4_head<HD>(c, x_there ? page : 0, kvh);
         const int o = p & (P - 1);
-        xk = *reinterpret_cast<const Vec*>(base + (o + t16) * L::kCodes + g * (HD / 8));
-        xkp = *reinterpret_cast<const uint32_t*>(base + L::k_params(P) + (o + t16) * L::kParams +
-                                                 (HD == 128 ? g : g >> 1) * 4);
-        xv = *reinterpret_cast<const Vec*>(base + L::v_codes(P) + ((o >> 2) + vb) * (4 * L::kCodes) + t16 * (HD / 8));
-        xvp = *reinterpret_cast<const u32x4*>(base + L::v_params(P) + ((o >> 2) + vb) * (4 * L::kParams) +
-                                              t16 / (512 / HD) * 16);
+        xk = *reinterpret_cast<const Vec*>(base + o * L::kCodes + at_k);
+        xkp = *reinterpret_cast<const uint32_t*>(base + L::k_params(P) + o * L::kParams + at_kp);
+        xv = *reinterpret_cast<const Vec*>(base + L::v_codes(P) + o * L::kCodes + at_v);
+        xvp = *reinterpret_cast<const u32x4*>(base + L::v_params(P) + o * L::kParams + at_vp);
     };
     auto store = [&](int b) {
         uint16_t* kb = buf + b * 2 * kHalves;
@@ -481,14 +491,18 @@ __global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Atten
     float m_run = -INFINITY, l_run = 0.f;
 
     auto process = [&](int t, int b) {
+        if (t >= wave_most) {   // uniform: no row of the wave sees the tile
+            store(b ^ 1);
+            return;
+        }
         const uint16_t* kb = buf + b * 2 * kHalves;
         const uint16_t* vbuf = kb + kHalves;
-        if (t >= wave_most) return;   // uniform: no row of the wave sees the tile
         int there = 0;
 #pragma unroll
         for (int w = 0; w < 4; ++w) there |= (there_at[b * 4 + w] != 0) << w;
         there = __builtin_amdgcn_readfirstlane(there);
         const bool whole = there == 15 && t + kTile <= wave_least;
+        __builtin_amdgcn_sched_barrier(0);
         f32x16 sc[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -500,6 +514,15 @@ __global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Atten
                 sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[st], sc[u], 0, 0, 0);
             }
         }
+        store(b ^ 1);   // the next tile's codes beside this one's products
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n) {   // an LDS read, a product, 8 vector instructions and a write at a time
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);
+            __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
         if (!whole) {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
@@ -514,7 +537,7 @@ __global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Atten
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) mt = fmaxf(mt, sc[u][e]);
+            for (int e = 0; e < 16; e += 2) mt = max3(mt, sc[u][e], sc[u][e + 1]);
         mt = max32(mt) * scale_log2;
         if (__builtin_amdgcn_ballot_w64(mt > m_run + kSlack || (m_run == -INFINITY && mt > m_run)) != 0) {
             const float m_new = fmaxf(m_run, mt);
@@ -548,9 +571,8 @@ __global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Atten
     load(c0 + kTile);
     __syncthreads();
     for (int t = c0, b = 0; t < c1; t += kTile, b ^= 1) {
-        store(b ^ 1);              // the next tile
-        load(t + 2 * kTile);
         process(t, b);
+        load(t + 2 * kTile);
         __syncthreads();
     }
 

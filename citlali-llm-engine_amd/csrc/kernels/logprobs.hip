@@ -201,7 +201,7 @@ __global__ __launch_bounds__(kBlk) void logprobs_kernel(Logprobs a, int splits, 
     __shared__ uint64_t room[kWaves][kWave];
     __shared__ Part parts[kWaves];
     const int r = blockIdx.x / splits, split = blockIdx.x - r * splits;
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const char* row = static_cast<const char*>(a.logits) + (size_t)r * a.row_stride * (kHalf ? 2 : 4);
     const int lead = (int)((16 - ((uintptr_t)row & 15)) & 15) / (kHalf ? 2 : 4);
     const int head = min(lead, a.vocab);                   // logits before the aligned ones
