@@ -75,23 +75,20 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : 2) void kv4_decode_kernel(Kv
     const int rows_most = a.max_query * (a.heads / c.kv_heads);
 
     const int split = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int col = lane & 15, grp = lane >> 4;
+    // the chunk's pages, one a lane (a chunk has at most 64), with the lengths
+    // still on their way
+    const int c0 = split * chunk, first_page = c0 >> c.page_shift;
+    int my_page = a.page_table[(size_t)seq * a.pages_per_seq + min(first_page + lane, a.pages_per_seq - 1)];
     const Kv4Seq s = kv4_seq(a, seq);
     const int asked = min(s.n, a.max_query);
     if (asked <= 0) return;
     const int group = a.heads / c.kv_heads, rows = asked * group;
     const int most = max(0, s.see(asked - 1));   // positions any row sees
-    const int c0 = split * chunk, c1 = min(most, c0 + chunk);
+    const int c1 = min(most, c0 + chunk);
     if (c0 >= most && split > 0) return;
-    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int col = lane & 15, grp = lane >> 4;
-
-    // page of 16 .. positions j of the chunk's pages: lane j (a chunk has at most 64)
-    const int first_page = c0 >> c.page_shift;
-    int my_page = -1;
-    if (((first_page + lane) << c.page_shift) < c1) {
-        my_page = a.page_table[(size_t)seq * a.pages_per_seq + first_page + lane];
-        if (my_page >= c.num_pages) my_page = -1;
-    }
+    if (((first_page + lane) << c.page_shift) >= c1 || my_page >= c.num_pages) my_page = -1;
     half8 q[kCols][kSteps];
     int see[kCols];
 #pragma unroll
@@ -304,49 +301,79 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : 2) void kv4_decode_kernel(Kv
     }
 }
 
-// Log-sum-exp merge of the chunks of one (query, head) by one wave, HD / 64
-// dims a lane.
-template <int HD>
+// Log-sum-exp merge of the chunks of one (query, head) by kTeam waves: HD / 4
+// lanes read a chunk's sums 16 bytes each, the teams of a wave (and the waves)
+// take different chunks, kBatch at once.  The first batch is read before the
+// number of chunks is known (all lie in the workspace), so that the kernel is
+// one round trip behind the lengths.
+template <int HD, int kTeam>
 __global__ __launch_bounds__(kBlk) void kv4_merge_kernel(Kv4Attention a, int group, int tile_rows, int chunk,
                                                          int n_splits) {
-    constexpr int kPer = HD / kWave;
+    constexpr int kLanes = HD / 4, kTeams = kTeam * kWave / kLanes, kBatch = 4;
+    __shared__ __align__(16) float lds[kTeam > 1 ? kTeam : 1][HD];
     const int seq = blockIdx.y, lane = threadIdx.x & (kWave - 1);
-    const Kv4Seq s = kv4_seq(a, seq);
-    const int asked = min(s.n, a.max_query);
-    const int unit = blockIdx.x * kWaves + threadIdx.x / kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int unit = kTeam > 1 ? blockIdx.x : blockIdx.x * kWaves + wave;
     const int i = unit / a.heads, head = unit - i * a.heads;
+    if (i >= a.max_query) return;
+    const Kv4Seq s = kv4_seq(a, seq);
+    const size_t token = min(s.start + i, a.tokens - 1);   // i may be past the sequence's queries
+    const size_t at = (token * a.heads + head) * n_splits;
+    const int team = (kTeam > 1 ? wave * (kWave / kLanes) : 0) + lane / kLanes, d = lane % kLanes * 4;
+    const float* part = a.workspace + at * HD + d;
+    const f32x2* ml = reinterpret_cast<const f32x2*>(a.workspace + (size_t)a.tokens * a.heads * n_splits * HD) + at;
+    f32x4 v[kBatch];
+    f32x2 w[kBatch];
+    auto load = [&](int j0) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int j = min(j0 + u * kTeams + team, n_splits - 1);
+            v[u] = *reinterpret_cast<const f32x4*>(part + (size_t)j * HD);
+            w[u] = ml[j];
+        }
+    };
+    load(0);
+    f32x2 mine = ml[min(lane, n_splits - 1)];
+    const int asked = min(s.n, a.max_query);
     if (i >= asked) return;
     // the positions that the rows of its workgroups saw
     const int tile = (i * group + head % group) / tile_rows;
     const int most = s.see((int)(min((long long)asked * group, (tile + 1ll) * tile_rows) - 1) / group);
     if (most <= chunk) return;   // written by the chunk itself
     const int n = (most + chunk - 1) / chunk;
-    const size_t at = ((size_t)(s.start + i) * a.heads + head) * n_splits;
-    const float* part = a.workspace + at * HD + lane * kPer;
-    const f32x2* ml = reinterpret_cast<const f32x2*>(a.workspace + (size_t)a.tokens * a.heads * n_splits * HD) + at;
-    float M = -INFINITY;
-    for (int j = lane; j < n; j += kWave) M = fmaxf(M, ml[j].x);
+    float M = lane < n ? mine.x : -INFINITY;
+    for (int j = lane + kWave; j < n; j += kWave) M = fmaxf(M, ml[j].x);
     M = wave_max(M);
-    float l = 0.f, acc[kPer] = {};
-    for (int j0 = 0; j0 < n; j0 += kWave) {
-        float f = 0.f;
-        if (j0 + lane < n) {
-            const f32x2 v = ml[j0 + lane];
-            f = v.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - M);
-            l += v.y * f;
-        }
-        const int here = min(kWave, n - j0);
-        for (int j = 0; j < here; ++j) {
-            const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), j));
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) acc[e] = fmaf(part[(size_t)(j0 + j) * HD + e], w, acc[e]);
-        }
-    }
+    auto factor = [&](float m) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M); };
+    float l = lane < n ? mine.y * factor(mine.x) : 0.f;
+    for (int j = lane + kWave; j < n; j += kWave) l += ml[j].y * factor(ml[j].x);
     l = wave_sum(l);
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    uint16_t* out = a.out + (size_t)(s.start + i) * a.out_stride + (size_t)head * HD + lane * kPer;
+    f32x4 acc{0.f, 0.f, 0.f, 0.f};
+    for (int j0 = 0; j0 < n; j0 += kBatch * kTeams) {
+        if (j0 > 0) load(j0);
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) out[e] = f2h_rne(acc[e] * inv);
+        for (int u = 0; u < kBatch; ++u)
+            if (j0 + u * kTeams + team < n) acc += v[u] * factor(w[u].x);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if constexpr (kLanes == 16) acc[e] = sum16(acc[e]);
+        acc[e] = sum32(acc[e]);
+    }
+    if constexpr (kTeam > 1) {
+        if (lane < kLanes) *reinterpret_cast<f32x4*>(&lds[wave][d]) = acc;
+        __syncthreads();
+        if (wave != 0) return;
+        acc = *reinterpret_cast<const f32x4*>(&lds[0][d]);
+#pragma unroll
+        for (int o = 1; o < kTeam; ++o) acc += *reinterpret_cast<const f32x4*>(&lds[o][d]);
+    }
+    if (lane >= kLanes) return;
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    u32x2 out;
+    out.x = f2h_rne(acc.x * inv) | ((uint32_t)f2h_rne(acc.y * inv) << 16);
+    out.y = f2h_rne(acc.z * inv) | ((uint32_t)f2h_rne(acc.w * inv) << 16);
+    *reinterpret_cast<u32x2*>(a.out + (size_t)(s.start + i) * a.out_stride + (size_t)head * HD + d) = out;
 }
 
 // ---------------------------------------------------------------------------
@@ -673,9 +700,15 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || last) return e;
+    // one wave covers 4 chunks a lane group at once; with more of them four waves share a head
     const long long units = (long long)a.max_query * a.heads;
-    launch_kernel(kv4_merge_kernel<HD>, dim3((unsigned)((units + kWaves - 1) / kWaves), a.nseq), dim3(kBlk), 0, s, a,
-                  group, p.few ? kFewRows : kRowTile, p.chunk, p.n_splits);
+    const int tile_rows = p.few ? kFewRows : kRowTile;
+    if (p.n_splits <= 4 * kWave / (HD / 4))
+        launch_kernel(kv4_merge_kernel<HD, 1>, dim3((unsigned)((units + kWaves - 1) / kWaves), a.nseq), dim3(kBlk), 0, s, a,
+                      group, tile_rows, p.chunk, p.n_splits);
+    else
+        launch_kernel(kv4_merge_kernel<HD, kWaves>, dim3((unsigned)units, a.nseq), dim3(kBlk), 0, s, a, group, tile_rows,
+                      p.chunk, p.n_splits);
     return hipGetLastError();
 }
 
