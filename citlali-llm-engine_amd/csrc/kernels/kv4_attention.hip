@@ -74,7 +74,9 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : 2) void kv4_decode_kernel(Kv
     extern __shared__ __align__(16) float lds[];
     const int rows_most = a.max_query * (a.heads / c.kv_heads);
 
-    const int split = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
+    // every sequence's first chunks before the second ones: the chunks that
+    // short sequences lack then leave all XCDs alike
+    const int kvh = blockIdx.x % c.kv_heads, seq = blockIdx.x / c.kv_heads, split = blockIdx.y;
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int col = lane & 15, grp = lane >> 4;
     // the chunk's pages, one a lane (a chunk has at most 64), with the lengths
@@ -131,16 +133,16 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : 2) void kv4_decode_kernel(Kv
         for (int u = 0; u < 2; ++u) {
             const int o = (t + 16 * u) & (P - 1) & ~15;
             at_head[u] = head_at(t + 16 * u);
-            xk[u] = *reinterpret_cast<const Vec*>(at_head[u] + o * L::kCodes + at_k);
-            xkp[u] = *reinterpret_cast<const uint32_t*>(at_head[u] + L::k_params(P) + o * L::kParams + at_kp);
+            xk[u] = __builtin_nontemporal_load(reinterpret_cast<const Vec*>(at_head[u] + o * L::kCodes + at_k));
+            xkp[u] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(at_head[u] + L::k_params(P) + o * L::kParams + at_kp));
         }
     };
     auto load_v = [&](int t) {   // of the positions that load_k took last
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int o = (t + 16 * u) & (P - 1) & ~15;
-            xv[u] = *reinterpret_cast<const Vec*>(at_head[u] + L::v_codes(P) + o * L::kCodes + at_v);
-            xvp[u] = *reinterpret_cast<const u32x4*>(at_head[u] + L::v_params(P) + o * L::kParams + at_vp);
+            xv[u] = __builtin_nontemporal_load(reinterpret_cast<const Vec*>(at_head[u] + L::v_codes(P) + o * L::kCodes + at_v));
+            xvp[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at_head[u] + L::v_params(P) + o * L::kParams + at_vp));
         }
     };
 
@@ -686,7 +688,7 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
         launch_kernel_in_call(last, kv4_prompt_kernel<HD>, dim3(c.kv_heads * p.tiles * p.n_splits, a.nseq), dim3(kBlk), lds, s,
                               c, a, p.chunk, p.n_splits, scale_log2);
     } else {
-        const dim3 grid(p.n_splits, c.kv_heads, a.nseq);
+        const dim3 grid(c.kv_heads * a.nseq, p.n_splits);
         const int lds = kWaves * a.max_query * group * (HD + 4) * (int)sizeof(float);
         if (p.cols == 1) {
             launch_kernel_in_call(last, kv4_decode_kernel<HD, 1>, grid, dim3(kBlk), lds, s, c, a, p.chunk, p.n_splits,
