@@ -650,7 +650,7 @@ __global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Atten
 // their four waves, at most 1024 positions (a lane per page), about eight
 // workgroups per CU where the bound allows.  The prompt kernel splits the
 // positions only where its row tiles leave CUs without work.
-constexpr int kFewRows = 32, kChunkStep = 32 * kWaves, kChunkMost = 1024, kFewBlocks = 2048;
+constexpr int kFewRows = 32, kChunkStep = 32 * kWaves, kChunkMost = 1024, kFewBlocks = 1024;
 constexpr int kPromptBlocks = 512, kPromptChunk = 512;
 struct Kv4Plan {
     bool few;
