@@ -9,6 +9,7 @@ namespace citlali::hip {
 namespace {
 
 constexpr int kBlk = 256;
+constexpr long long kEnoughWaves = 4096;
 
 __global__ void rope_table_kernel(float2* __restrict__ table, size_t n, int half, double log_theta) {
     const size_t i = (size_t)blockIdx.x * kBlk + threadIdx.x;
@@ -19,157 +20,246 @@ __global__ void rope_table_kernel(float2* __restrict__ table, size_t n, int half
     table[i] = make_float2((float)cs, (float)sn);
 }
 
-template <typename T>
-__device__ __forceinline__ T add_lanes(T v, int lanes) {   // over aligned groups of `lanes` lanes
-    for (int o = 1; o < lanes; o <<= 1) v += __shfl_xor(v, o, kWave);
-    return v;
-}
 __device__ __forceinline__ _Float16 half_at(u32x4 v, int i) {
     return __builtin_bit_cast(_Float16, (uint16_t)(v[i / 2] >> (16 * (i & 1))));
 }
 
-// The eight normed and rotated values of a lane in T.  Lane l of the LR that
-// share a head row holds dims 8 l .. 8 l + 7; its rotation partner, LR / 2
-// lanes away, holds the dims head_dim / 2 away.
+// Sum over the LR lanes that share a head row (LR = 8 or 16).
+template <int LR>
+__device__ __forceinline__ float row_sum(float v) {
+    return lane_group_sum<LR>(v);
+}
+template <int Ctrl>
+__device__ __forceinline__ double dpp64(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, Ctrl, 0xF, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), Ctrl, 0xF, 0xF, false);
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+template <int LR>
+__device__ __forceinline__ double row_sum(double v) {
+    v += dpp64<kDppXor1>(v);
+    v += dpp64<kDppXor2>(v);
+    v += dpp64<kDppHalfMirror>(v);
+    if constexpr (LR == 16) v += dpp64<kDppMirror>(v);
+    return v;
+}
+// The value LR / 2 lanes away in the row.
+template <int LR>
+__device__ __forceinline__ uint32_t partner(uint32_t v) {
+    if constexpr (LR == 16)
+        return __builtin_amdgcn_update_dpp(0, (int)v, DppRor<8>::value, 0xF, 0xF, false);
+    else
+        return __shfl_xor((int)v, LR / 2, kWave);
+}
+
+// x^-1/2 of a positive number: the hardware's estimate, in 64 bits one Newton
+// step further (its error, about 2^-29, squared).
+__device__ __forceinline__ float inv_root(float x) { return __builtin_amdgcn_rsqf(x); }
+__device__ __forceinline__ double inv_root(double x) {
+    const double r = __builtin_amdgcn_rsq(x);
+    return fma(0.5 * r, fma(-x * r, r, 1.0), r);
+}
+
+// The eight normed and rotated values of a lane, computed in T and rounded to
+// fp32.  Lane l of the LR that share a head row holds dims 8 l .. 8 l + 7; its
+// rotation partner, LR / 2 lanes away, holds the dims head_dim / 2 away.  wx,
+// wp: the norm's weights of both (ones without a norm); cs: cosines and sines
+// of the eight pairs.  Value times weight is exact in fp32 (two fp16 numbers),
+// and the norm's factor comes last: y = inv (x w_x cos -+ p w_p sin).
 template <typename T, int HD>
-__device__ __forceinline__ void norm_rotate(u32x4 raw, const uint16_t* w, float eps, const float* rope_row, int l,
-                                            T (&y)[8]) {
+__device__ __forceinline__ void norm_rotate(u32x4 raw, bool norm, u32x4 wx, u32x4 wp, float eps, const float2 (&cs)[8],
+                                            int l, float (&y)[8]) {
     constexpr int LR = HD / 8;
     u32x4 other;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) other[i] = __shfl_xor(raw[i], LR / 2, kWave);
-    T x[8], p[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        x[i] = (T)(float)half_at(raw, i);
-        p[i] = (T)(float)half_at(other, i);
-    }
-    if (w != nullptr) {
+    for (int i = 0; i < 4; ++i) other[i] = partner<LR>(raw[i]);
+    T inv = 1;
+    if (norm) {
         T s = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s += x[i] * x[i];
-        s = add_lanes(s, LR);
-        const T inv = (T)1 / sqrt(s / (T)HD + (T)eps);
-        const u32x4 wx = *reinterpret_cast<const u32x4*>(w + 8 * l);
-        const u32x4 wp = *reinterpret_cast<const u32x4*>(w + 8 * (l ^ (LR / 2)));
-#pragma unroll
         for (int i = 0; i < 8; ++i) {
-            x[i] = x[i] * inv * (T)(float)half_at(wx, i);
-            p[i] = p[i] * inv * (T)(float)half_at(wp, i);
+            const T x = (T)(float)half_at(raw, i);
+            s += x * x;
         }
+        inv = inv_root(row_sum<LR>(s) * (T)(1.0 / HD) + (T)eps);
     }
-    const float2* cs = reinterpret_cast<const float2*>(rope_row) + 8 * (l & (LR / 2 - 1));
-    const bool upper = l >= LR / 2;
+    // the lower half of the pairs takes - sin
+    const uint32_t flip = l < LR / 2 ? 0x80000000u : 0u;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float2 t = cs[i];
-        y[i] = upper ? p[i] * (T)t.y + x[i] * (T)t.x : x[i] * (T)t.x - p[i] * (T)t.y;
+        const float x = (float)half_at(raw, i) * (float)half_at(wx, i);
+        const float p = (float)half_at(other, i) * (float)half_at(wp, i);
+        const float sn = __uint_as_float(__float_as_uint(cs[i].y) ^ flip);
+        y[i] = (float)(inv * ((T)x * (T)cs[i].x + (T)p * (T)sn));
+        __builtin_amdgcn_sched_barrier(0);   // one at a time: few 64-bit numbers live
     }
 }
 
-// Codes of a lane's eight values; d and m (fp16 bits) are those of the four
-// lanes that share a group.
-__device__ __forceinline__ void quantise(const float (&in)[8], uint32_t (&code)[8], uint32_t& d16, uint32_t& m16) {
-#pragma clang fp contract(off)   // the codes are the formula's, with its division by d
-    float y[8], lo = INFINITY, hi = -INFINITY;
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        bad |= in[i] != in[i];
-        y[i] = fminf(fmaxf(in[i], -kKv4Limit), kKv4Limit);
-        lo = fminf(lo, y[i]);
-        hi = fmaxf(hi, y[i]);
-    }
-    if (bad) lo = -INFINITY;   // stays the least of the four lanes
-    lo = fminf(lo, dpp<kDppXor1>(lo));
-    lo = fminf(lo, dpp<kDppXor2>(lo));
-    hi = fmaxf(hi, dpp<kDppXor1>(hi));
-    hi = fmaxf(hi, dpp<kDppXor2>(hi));
-    bad = lo == -INFINITY;
-    m16 = bad ? 0x7e00u : f2h_rne(lo);
-    const float m = h2f((uint16_t)m16);
-    float step = (hi - m) * (1.f / 15.f);
+// Codes of a lane's eight values, four to a number: lo has those of values 0
+// .. 3 (or, kEven, of 0 2 4 6) from the low bits on, hi the others.  d and m
+// (fp16 bits) are those of the four lanes that share a group.
+// (y - m) / d rounded as fp32 division rounds it, from d's reciprocal: that is
+// correctly rounded after one Newton step for every fp16 d, and then one step
+// on the quotient is exact.
+template <bool kEven>
+__device__ __forceinline__ void quantise(const float (&y)[8], uint32_t& lo, uint32_t& hi, uint32_t& d16, uint32_t& m16) {
+    // a NaN stays through these two
+    auto min3 = [](float a, float b, float c) {
+        float r;
+        asm("v_minimum3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+        return r;
+    };
+    auto max3 = [](float a, float b, float c) {
+        float r;
+        asm("v_maximum3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+        return r;
+    };
+    float least = min3(min3(y[0], y[1], y[2]), min3(y[3], y[4], y[5]), min3(y[6], y[7], y[7]));
+    float most = max3(max3(y[0], y[1], y[2]), max3(y[3], y[4], y[5]), max3(y[6], y[7], y[7]));
+    const float l1 = dpp<kDppXor1>(least), m1 = dpp<kDppXor1>(most);
+    least = min3(least, l1, l1);
+    most = max3(most, m1, m1);
+    const float l2 = dpp<kDppXor2>(least), m2 = dpp<kDppXor2>(most);
+    least = min3(least, l2, l2);
+    most = max3(most, m2, m2);
+    const bool bad = least != least;
+    least = __builtin_amdgcn_fmed3f(least, -kKv4Limit, kKv4Limit);
+    most = __builtin_amdgcn_fmed3f(most, -kKv4Limit, kKv4Limit);
+    m16 = f2h_rne(least);
+    const float m = bad ? 0.f : h2f((uint16_t)m16);
+    float step = (most - m) * (1.f / 15.f);
     asm("" : "+v"(step));   // rounded to fp32 before fp16: no v_fma_mixlo_f16
     d16 = bad ? 0u : f2h_rne(step);
-    const float d = h2f((uint16_t)d16);
+    m16 = bad ? 0x7e00u : m16;
+    const float d = h2f((uint16_t)d16), top = 15.f * d;
+    float r = __builtin_amdgcn_rcpf(d);
+    r = d > 0.f ? fmaf(fmaf(-d, r, 1.f), r, r) : 0.f;
+    float c[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float c = d > 0.f ? rintf((y[i] - m) / d) : 0.f;
-        code[i] = bad ? 0u : (uint32_t)fminf(fmaxf(c, 0.f), 15.f);
+        const float x = __builtin_amdgcn_fmed3f(y[i] - m, 0.f, top);   // codes 0 .. 15; saturation as well
+        const float q = x * r;
+        c[i] = rintf(fmaf(fmaf(-q, d, x), r, q));
     }
+    auto four = [](float c0, float c1, float c2, float c3) {   // whole numbers below 2^16
+        return (uint32_t)fmaf(fmaf(fmaf(c3, 16.f, c2), 16.f, c1), 16.f, c0);
+    };
+    lo = kEven ? four(c[0], c[2], c[4], c[6]) : four(c[0], c[1], c[2], c[3]);
+    hi = kEven ? four(c[1], c[3], c[5], c[7]) : four(c[4], c[5], c[6], c[7]);
+    lo = bad ? 0u : lo;
+    hi = bad ? 0u : hi;
 }
 
-// One wave takes one head (query, key or value) of 512 / HD consecutive
-// tokens, 16 bytes a lane.
+// One wave takes `per` heads (all query, key or value heads) of 512 / HD
+// consecutive tokens, 16 bytes a lane and head, the next head's on their way:
+// the rotation's 64 bytes a lane, four times a head's, are read once for all.
+// 8192 tokens of 32/8 heads move 182 MB in 52.6 us (3.5 TB/s) against vector
+// work of about the same length; few tokens are bound by the chain position ->
+// table -> head.
 template <int HD>
-__global__ __launch_bounds__(kBlk) void kv4_append_kernel(Kv4View c, Kv4Append a) {
+__global__ __launch_bounds__(kBlk) void kv4_append_kernel(Kv4View c, Kv4Append a, int per) {
     constexpr int LR = HD / 8, kRows = kWave / LR;
     using L = Kv4Layout<HD>;
     const int lane = threadIdx.x & (kWave - 1), l = lane % LR;
-    const int slots_per_token = a.heads + 2 * c.kv_heads;
-    const long long unit = (long long)blockIdx.x * (kBlk / kWave) + threadIdx.x / kWave;
-    const int head = (int)(unit % slots_per_token);
-    const long long t = unit / slots_per_token * kRows + lane / LR;
+    const int q_units = (a.heads + per - 1) / per, kv_units = (c.kv_heads + per - 1) / per;
+    const int units = q_units + 2 * kv_units;
+    const long long at = (long long)blockIdx.x * (kBlk / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const long long group = at / units;
+    if (group * kRows >= a.tokens) return;   // uniform
+    int unit = (int)(at - group * units);
+    const bool is_q = unit < q_units, is_v = unit >= q_units + kv_units;
+    unit -= is_q ? 0 : is_v ? q_units + kv_units : q_units;
+    const int h0 = unit * per, h1 = min(is_q ? a.heads : c.kv_heads, h0 + per);
     // rows past the last token, and tokens without a position, take part in
     // the lane moves with row 0 and write nothing
+    const long long t = group * kRows + lane / LR;
     const bool real = t < a.tokens;
     const long long row = real ? t : 0;
-    const int pos = a.positions[row];
+    const uint16_t* src = (is_q ? a.q + row * a.q_stride : (is_v ? a.v : a.k) + row * a.kv_stride) + 8 * l;
+    const int pos = a.positions[row], slot = a.slots[row];
     const bool known = real && pos >= 0 && pos < a.rope_positions;
-    const float* rope_row = a.rope + (size_t)(known ? pos : 0) * HD;
-
-    if (head < a.heads) {
-        const u32x4 raw = *reinterpret_cast<const u32x4*>(a.q + row * a.q_stride + (size_t)head * HD + 8 * l);
-        float y[8];
-        norm_rotate<float, HD>(raw, a.q_norm, a.eps, rope_row, l, y);
-        if (known) {
-            u32x4 o;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = f2h_rne(y[2 * i]) | ((uint32_t)f2h_rne(y[2 * i + 1]) << 16);
-            *reinterpret_cast<u32x4*>(a.q_out + row * a.q_out_stride + (size_t)head * HD + 8 * l) = o;
-        }
-        return;
-    }
-    const bool is_k = head < a.heads + c.kv_heads;
-    const int kvh = head - a.heads - (is_k ? 0 : c.kv_heads);
-    const u32x4 raw =
-        *reinterpret_cast<const u32x4*>((is_k ? a.k : a.v) + row * a.kv_stride + (size_t)kvh * HD + 8 * l);
-    const int slot = a.slots[row];
-    const int P = 1 << c.page_shift;
+    const int P = 1 << c.page_shift, o = slot & (P - 1);
     const bool kept = known && slot >= 0 && (slot >> c.page_shift) < c.num_pages;
-    uint8_t* base = kv4_head<HD>(c, kept ? slot >> c.page_shift : 0, kvh);
-    const int o = slot & (P - 1);
-    float y[8];
-    uint32_t code[8], d16, m16;
-    if (is_k) {
-        double z[8];
-        norm_rotate<double, HD>(raw, a.k_norm, a.eps, rope_row, l, z);
+
+    float2 cs[8];
+    const uint32_t ones = 0x3c003c00u;
+    u32x4 wx{ones, ones, ones, ones}, wp = wx;
+    const uint16_t* w = is_q ? a.q_norm : a.k_norm;
+    if (!is_v) {
+        const float2* rope =
+            reinterpret_cast<const float2*>(a.rope + (size_t)(known ? pos : 0) * HD) + 8 * (l & (LR / 2 - 1));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = (float)z[i];
-        quantise(y, code, d16, m16);
-        if (!kept) return;
-        uint32_t w = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w |= (code[2 * i] | (code[2 * i + 1] << 16)) << (4 * i);
-        *reinterpret_cast<uint32_t*>(base + o * L::kCodes + 4 * l) = w;
-        if ((l & 3) == 0)
-            *reinterpret_cast<uint32_t*>(base + L::k_params(P) + o * L::kParams + l) = d16 | (m16 << 16);
-        return;
+        for (int i = 0; i < 8; ++i) cs[i] = rope[i];
+        if (w != nullptr) {
+            wx = *reinterpret_cast<const u32x4*>(w + 8 * l);
+            wp = *reinterpret_cast<const u32x4*>(w + 8 * (l ^ (LR / 2)));
+        }
     }
+    // values of neighbouring slots (an even one and the next) in neighbouring
+    // rows go out as words of two tokens
+    bool pairs = false;
+    if (is_v) {
+        const int next = __shfl_xor(slot, LR, kWave);
+        const bool even = ((lane / LR) & 1) == 0;
+        const bool good = kept && (even ? (slot & 1) == 0 && next == slot + 1 : (slot & 1) == 1 && next == slot - 1);
+        pairs = LR == 16 && __builtin_amdgcn_ballot_w64(!good) == 0;
+    }
+
+    u32x4 next = *reinterpret_cast<const u32x4*>(src + (size_t)h0 * HD);
+#pragma unroll 1
+    for (int h = h0; h < h1; ++h) {
+        const u32x4 raw = next;
+        next = *reinterpret_cast<const u32x4*>(src + (size_t)min(h + 1, h1 - 1) * HD);
+        if (is_q) {
+            float y[8];
+            norm_rotate<float, HD>(raw, w != nullptr, wx, wp, a.eps, cs, l, y);
+            if (known) {
+                u32x4 out;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = (float)half_at(raw, i);
-    quantise(y, code, d16, m16);
-    if (!kept) return;
-    uint16_t* vc = reinterpret_cast<uint16_t*>(base + L::v_codes(P)) + (o >> 2) * HD + (o & 3);
+                for (int i = 0; i < 4; ++i)
+                    out[i] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)y[2 * i], (_Float16)y[2 * i + 1]});
+                *reinterpret_cast<u32x4*>(a.q_out + row * a.q_out_stride + (size_t)h * HD + 8 * l) = out;
+            }
+            continue;
+        }
+        uint8_t* base = kv4_head<HD>(c, kept ? slot >> c.page_shift : 0, h);
+        float y[8];
+        uint32_t lo, hi, d16, m16;
+        if (!is_v) {
+            // widened here, for each head: 64 registers less to keep
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
-        vc[(2 * l + e) * 4] =
-            (uint16_t)(code[4 * e] | (code[4 * e + 1] << 4) | (code[4 * e + 2] << 8) | (code[4 * e + 3] << 12));
-    if ((l & 3) == 0) {
-        uint16_t* vp = reinterpret_cast<uint16_t*>(base + L::v_params(P)) +
-                       ((o >> 2) * (HD / kKv4Group) + (l >> 2)) * 8 + (o & 3);
-        vp[0] = (uint16_t)d16;
-        vp[4] = (uint16_t)m16;
+            for (int i = 0; i < 8; ++i) asm("" : "+v"(cs[i].x), "+v"(cs[i].y));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) asm("" : "+v"(wx[i]), "+v"(wp[i]));
+            norm_rotate<double, HD>(raw, w != nullptr, wx, wp, a.eps, cs, l, y);
+            quantise<true>(y, lo, hi, d16, m16);
+            if (!kept) continue;
+            *reinterpret_cast<uint32_t*>(base + o * L::kCodes + 4 * l) = lo | (hi << 16);
+            if ((l & 3) == 0)
+                *reinterpret_cast<uint32_t*>(base + L::k_params(P) + o * L::kParams + l) = d16 | (m16 << 16);
+            continue;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = (float)half_at(raw, i);
+        quantise<false>(y, lo, hi, d16, m16);   // dims 8 l .. and 8 l + 4 ..
+        uint16_t* vc = reinterpret_cast<uint16_t*>(base + L::v_codes(P)) + (o >> 2) * HD;
+        if (pairs) {
+            // row r gets both tokens' quad r & 1 (see swap16)
+            float q0 = __builtin_bit_cast(float, lo), q1 = __builtin_bit_cast(float, hi);
+            swap16(q0, q1);
+            *reinterpret_cast<uint32_t*>(vc + (2 * l + ((lane / LR) & 1)) * 4 + (o & 2)) =
+                __builtin_bit_cast(uint32_t, q0) | (__builtin_bit_cast(uint32_t, q1) << 16);
+        } else if (kept) {
+            vc[2 * l * 4 + (o & 3)] = (uint16_t)lo;
+            vc[(2 * l + 1) * 4 + (o & 3)] = (uint16_t)hi;
+        }
+        if (kept && (l & 3) == 0) {
+            uint16_t* vp = reinterpret_cast<uint16_t*>(base + L::v_params(P)) +
+                           ((o >> 2) * (HD / kKv4Group) + (l >> 2)) * 8 + (o & 3);
+            vp[0] = (uint16_t)d16;
+            vp[4] = (uint16_t)m16;
+        }
     }
 }
 
@@ -240,12 +330,18 @@ unsigned blocks_for(long long rows, int head_dim, long long heads) {
 }
 }  // namespace
 
+// Heads of a wave: as many of 16, 8, 4 or 2 as leave four waves per SIMD, else
+// one.  8192 tokens of 32/8 heads: 52.6 us with 16, 54.2 with 8, 57.7 with 4.
 hipError_t launch_kv4_append(const Kv4View& c, const Kv4Append& a, hipStream_t s) {
-    const dim3 grid(blocks_for(a.tokens, c.head_dim, a.heads + 2 * c.kv_heads));
+    const long long groups = (a.tokens + 512 / c.head_dim - 1) / (512 / c.head_dim);
+    auto waves = [&](int per) { return groups * ((a.heads + per - 1) / per + 2 * ((c.kv_heads + per - 1) / per)); };
+    int per = 16;
+    while (per > 1 && waves(per) < kEnoughWaves) per /= 2;
+    const dim3 grid((unsigned)((waves(per) + kBlk / kWave - 1) / (kBlk / kWave)));
     if (c.head_dim == 128)
-        launch_kernel(kv4_append_kernel<128>, grid, dim3(kBlk), 0, s, c, a);
+        launch_kernel(kv4_append_kernel<128>, grid, dim3(kBlk), 0, s, c, a, per);
     else
-        launch_kernel(kv4_append_kernel<64>, grid, dim3(kBlk), 0, s, c, a);
+        launch_kernel(kv4_append_kernel<64>, grid, dim3(kBlk), 0, s, c, a, per);
     return hipGetLastError();
 }
 
