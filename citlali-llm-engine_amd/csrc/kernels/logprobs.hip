@@ -1,12 +1,12 @@
 // logprobs.hip -- log probability and rank of a given token, entropy and the
 // most likely tokens of each row of logits, in one pass over them.
 //
-// With m a row's maximum, s = sum e^(x - m) and t = sum e^(x - m) (x - m):
-//   log p(x) = x - m - log s        H = log s - t / s
-// Every lane keeps (m, s, t) of its own logits, 16 at a time: the maximum
-// first, then one rescaling, then their exponentials, added in pairs.  A row is
-// cut into pieces of whole waves; lanes, waves and workgroups join by
-//   (m, s, t) + (m', s', t'):  s f + s' f',  f (t + s (m - M)) + ...,  f = e^(m - M).
+// With m a row's maximum, s = sum 2^y and t = sum 2^y y over y = (x - m) log2 e,
+//   log p(x) = x - m - log s        H = log s - ln 2 t / s.
+// Every lane keeps (m, s, t) of its own logits, 16 at a time: their maximum
+// first, then one rescaling, then their exponentials.  A row is cut into pieces
+// of whole waves; lanes, waves and workgroups join by
+//   (m, s, t) + (m', s', t'):  s f + s' f',  f (t + s d) + ...,  f = 2^d.
 //
 // The most likely tokens are kept as 64-bit keys (ordered bits of the logit,
 // then the complement of the id, so that equal logits go by the lower id):
@@ -15,15 +15,17 @@
 // sorted across the lanes and merged at a time.  The order is total, so the
 // result does not depend on the cut.
 //
-// Bound by reading the logits; beside them a wave issues about 11 instructions
-// per 64 logits, one of them the exponential.
+// Bound by reading the logits; beside them a wave issues about 8 vector
+// instructions per 64 logits, one of them the exponential.
 #include "device_common.hpp"
 #include "launch.hpp"
 
+#include <float.h>
 #include <limits.h>
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace citlali::hip {
 namespace {
@@ -46,26 +48,55 @@ __device__ __forceinline__ float key_logit(uint64_t k) {
 }
 
 // ---- a wave's largest keys --------------------------------------------------
+// Both of a lane's and its partner's (lane ^ kStride) values, in either order.
+template <int kStride>
+__device__ __forceinline__ void both(uint32_t v, uint32_t& a, uint32_t& b) {
+    a = b = v;
+    if constexpr (kStride >= 16) {
+        float x = __uint_as_float(v), y = x;
+        if constexpr (kStride == 16)
+            swap16(x, y);
+        else
+            swap32(x, y);
+        a = __float_as_uint(x);
+        b = __float_as_uint(y);
+    } else if constexpr (kStride == 4) {   // i ^ 7, then i ^ 3
+        const int t = __builtin_amdgcn_update_dpp(0, (int)v, kDppHalfMirror, 0xF, 0xF, false);
+        b = __builtin_amdgcn_update_dpp(0, t, 0x1B, 0xF, 0xF, false);
+    } else {
+        constexpr int kCtrl = kStride == 1 ? kDppXor1 : kStride == 2 ? kDppXor2 : DppRor<8>::value;
+        b = __builtin_amdgcn_update_dpp(0, (int)v, kCtrl, 0xF, 0xF, false);
+    }
+}
 // Larger of a lane's and its partner's key where `up`, else the smaller.
-__device__ __forceinline__ uint64_t exchange(uint64_t v, int stride, bool up) {
-    const uint64_t w = __shfl_xor((unsigned long long)v, stride, kWave);
-    return (v > w) == up ? v : w;
+template <int kStride>
+__device__ __forceinline__ uint64_t exchange(uint64_t v, bool up) {
+    uint32_t a0, a1, b0, b1;
+    both<kStride>((uint32_t)v, a0, b0);
+    both<kStride>((uint32_t)(v >> 32), a1, b1);
+    const uint64_t a = ((uint64_t)a1 << 32) | a0, b = ((uint64_t)b1 << 32) | b0;
+    return (a > b) == up ? a : b;
+}
+// The steps kStride, kStride / 2, .. 1 of a bitonic merge; each run of kSize
+// lanes descends where `down`.
+template <int kStride>
+__device__ __forceinline__ uint64_t merge_steps(uint64_t v, int lane, bool down) {
+    v = exchange<kStride>(v, ((lane & kStride) == 0) == down);
+    if constexpr (kStride > 1) v = merge_steps<kStride / 2>(v, lane, down);
+    return v;
 }
 __device__ __forceinline__ uint64_t sort_descending(uint64_t v, int lane) {
-#pragma unroll
-    for (int size = 2; size <= kWave; size <<= 1)
-#pragma unroll
-        for (int stride = size >> 1; stride > 0; stride >>= 1)
-            v = exchange(v, stride, ((lane & stride) == 0) == ((lane & size) == 0 || size == kWave));
-    return v;
+    v = merge_steps<1>(v, lane, (lane & 2) == 0);
+    v = merge_steps<2>(v, lane, (lane & 4) == 0);
+    v = merge_steps<4>(v, lane, (lane & 8) == 0);
+    v = merge_steps<8>(v, lane, (lane & 16) == 0);
+    v = merge_steps<16>(v, lane, (lane & 32) == 0);
+    return merge_steps<32>(v, lane, true);
 }
 // The 64 largest of two descending lists, descending.
 __device__ __forceinline__ uint64_t merge_descending(uint64_t a, uint64_t b, int lane) {
     const uint64_t w = __shfl((unsigned long long)b, kWave - 1 - lane, kWave);
-    uint64_t v = a > w ? a : w;
-#pragma unroll
-    for (int stride = kWave >> 1; stride > 0; stride >>= 1) v = exchange(v, stride, (lane & stride) == 0);
-    return v;
+    return merge_steps<32>(a > w ? a : w, lane, true);
 }
 __device__ __forceinline__ uint64_t lane_key(uint64_t v, int lane) {
     const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane);
@@ -73,9 +104,17 @@ __device__ __forceinline__ uint64_t lane_key(uint64_t v, int lane) {
     return ((uint64_t)hi << 32) | lo;
 }
 
+// `lane`, of which the compiler keeps no comparisons from one sort to the next
+// (they would fill the scalar registers of the whole kernel).
+__device__ __forceinline__ int hidden(int lane) {
+    asm("" : "+v"(lane));
+    return lane;
+}
+
 struct TopKeys {
     uint64_t mine = 0;    // lane i: the i-th largest
     uint64_t floor = 0;   // only keys above it can be among the k largest (uniform)
+    uint64_t theirs = 0;  // likewise, from the workgroup's other waves
     int waiting = 0;      // keys in `room` (uniform)
     uint64_t* room;       // 64 of LDS, the wave's own
     int lane, k;
@@ -84,19 +123,21 @@ struct TopKeys {
         wave_lds_sync();
         const uint64_t v = lane < waiting ? room[lane] : 0ull;
         wave_lds_sync();
-        mine = merge_descending(mine, sort_descending(v, lane), lane);
+        const int at = hidden(lane);
+        mine = merge_descending(mine, sort_descending(v, at), at);
         const uint64_t kth = lane_key(mine, k - 1);
         floor = kth > floor ? kth : floor;
         waiting = 0;
     }
     __device__ void add(uint64_t key) {
-        uint64_t who = __builtin_amdgcn_ballot_w64(key > floor);
+        const uint64_t least = floor > theirs ? floor : theirs;
+        uint64_t who = __builtin_amdgcn_ballot_w64(key > least);
         if (who == 0) return;
         if (waiting + __popcll(who) > kWave) {
             flush();
-            who = __builtin_amdgcn_ballot_w64(key > floor);
+            who = __builtin_amdgcn_ballot_w64(key > least);
         }
-        if (key > floor)
+        if (key > least)
             room[waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] =
                 key;
         waiting += __popcll(who);
@@ -104,23 +145,27 @@ struct TopKeys {
     // Before many keys at once, of which `best` are the lanes' largest: at
     // least k of them reach the k-th largest of those.
     __device__ void raise(uint64_t best) {
-        const uint64_t kth = lane_key(sort_descending(best, lane), k - 1);
+        const uint64_t kth = lane_key(sort_descending(best, hidden(lane)), k - 1);
         if (kth > floor) floor = kth - 1;
     }
 };
 
 // ---- sums --------------------------------------------------------------------
 struct Sums {
-    float m, s, t;   // t in base 2: sum e^(x - m) log2(e) (x - m)
+    float m, s, t;
 };
+// Sums rescaled to maximum m.
+__device__ __forceinline__ Sums rescaled(Sums a, float m) {
+    // without a logit above -inf s and t are 0 (or NaN, which stays)
+    const float d = a.m == -INFINITY ? 0.f : (a.m - m) * kLog2e, f = __builtin_amdgcn_exp2f(d);
+    // a factor of 0 takes t with it (d may be infinite), but for a NaN
+    return {m, a.s * f, f == 0.f ? 0.f * a.s : f * fmaf(a.s, d, a.t)};
+}
 __device__ __forceinline__ Sums join(Sums a, Sums b) {
-    const float M = fmaxf(a.m, b.m);
-    // a side without a logit above -inf has s and t 0 (or NaN, which stays)
-    const float da = a.m == -INFINITY ? 0.f : (a.m - M) * kLog2e, db = b.m == -INFINITY ? 0.f : (b.m - M) * kLog2e;
-    const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
-    // a factor of 0 takes its side's terms with it (its distance may be infinite)
-    const float ta = fa == 0.f ? 0.f * a.s : fa * fmaf(a.s, da, a.t), tb = fb == 0.f ? 0.f * b.s : fb * fmaf(b.s, db, b.t);
-    return {M, a.s * fa + b.s * fb, ta + tb};
+    const float m = fmaxf(a.m, b.m);
+    a = rescaled(a, m);
+    b = rescaled(b, m);
+    return {m, a.s + b.s, a.t + b.t};
 }
 __device__ __forceinline__ Sums wave_join(Sums v) {
     for (int o = 1; o < kWave; o <<= 1)
@@ -139,22 +184,56 @@ __device__ __forceinline__ float pair_sum(const float (&v)[kPer]) {
     return w[0];
 }
 
-__device__ __forceinline__ void add_logits(Sums& a, const float (&x)[kPer]) {
-    float mx = a.m;
+// 16 logits of a lane as they were loaded: fp32, or pairs of fp16.
+template <bool kHalf>
+struct Logits {
+    static constexpr int kVec = kHalf ? 8 : 4, kLoads = kPer / kVec;
+    u32x4 w[kLoads];
+    __device__ uint32_t word(int i) const { return w[i / kVec][kHalf ? i % kVec / 2 : i % kVec]; }
+    __device__ auto at(int i) const {
+        if constexpr (kHalf)
+            return __builtin_bit_cast(_Float16, (uint16_t)(i & 1 ? word(i) >> 16 : word(i)));
+        else
+            return __uint_as_float(word(i));
+    }
+    __device__ float largest() const {
+        if constexpr (kHalf) {
+            uint32_t m = word(0);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) mx = fmaxf(mx, x[i]);
-    const float M = mx == -INFINITY ? 0.f : mx;
-    const float d = a.m == -INFINITY ? 0.f : (a.m - M) * kLog2e, f = __builtin_amdgcn_exp2f(d);
-    float e[kPer], z[kPer];
+            for (int i = 2; i < kPer; i += 2) asm("v_pk_max_f16 %0, %1, %2" : "=v"(m) : "v"(m), "v"(word(i)));
+            return fmaxf((float)as_h2(m).x, (float)as_h2(m).y);
+        } else {
+            float m = at(0);
+#pragma unroll
+            for (int i = 1; i < kPer; ++i) m = fmaxf(m, at(i));
+            return m;
+        }
+    }
+    // y of logit i
+    __device__ float reach(int i, float m) const {
+        float d;
+        if constexpr (!kHalf)
+            d = at(i) - m;
+        else if (i & 1)
+            asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(word(i)), "v"(m));
+        else
+            asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(word(i)), "v"(m));
+        return d * kLog2e;
+    }
+};
+template <bool kHalf>
+__device__ __forceinline__ void add_logits(Sums& a, const Logits<kHalf>& x, float largest) {
+    const float m = fmaxf(a.m, largest), from = m == -INFINITY ? 0.f : m;
+    float e[kPer], z[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const float y = (x[i] - M) * kLog2e;
+        const float y = x.reach(i, from);
         e[i] = __builtin_amdgcn_exp2f(y);
-        z[i] = e[i] * fmaxf(y, -200.f);   // 0 for a logit of -inf
+        z[i % 4] = fmaf(e[i], fmaxf(y, -FLT_MAX), z[i % 4]);   // 0 for a logit of -inf
     }
-    a.t = (f == 0.f ? 0.f * a.s : f * fmaf(a.s, d, a.t)) + pair_sum(z);
-    a.s = a.s * f + pair_sum(e);
-    a.m = mx;
+    a = rescaled(a, m);
+    a.t += (z[0] + z[1]) + (z[2] + z[3]);
+    a.s += pair_sum(e);
 }
 
 template <bool kHalf>
@@ -167,15 +246,15 @@ __device__ __forceinline__ float logit_at(const void* row, int i) {
 
 // What one row comes to, from the joined sums.
 struct RowEnd {
-    float M, log_s;
-    __device__ RowEnd(Sums v) : M(v.m), log_s(v.s == 0.f ? NAN : logf(v.s)) {}
-    __device__ float logprob(float x) const { return x - M - log_s; }
+    float m, log_s;
+    __device__ RowEnd(Sums v) : m(v.m), log_s(v.s == 0.f ? NAN : logf(v.s)) {}
+    __device__ float logprob(float x) const { return x - m - log_s; }
 };
 __device__ __forceinline__ void write_row(const Logprobs& a, int r, Sums v, int rank, uint64_t top, int lane, float mine,
                                           bool given) {
     const RowEnd end(v);
     if (lane == 0) {
-        if (a.entropies) a.entropies[r] = end.log_s - v.t * kLn2 / v.s;
+        if (a.entropies) a.entropies[r] = end.log_s - kLn2 * (v.t / v.s);
         if (a.logprobs) a.logprobs[r] = given ? end.logprob(mine) : 0.f;
         if (a.ranks) a.ranks[r] = given ? rank : -1;
     }
@@ -193,135 +272,132 @@ struct alignas(16) Part {
 
 // Workgroup (row, piece); its four waves take `per_wave` steps of 1024 logits
 // each, 16-byte loads from the row's first aligned logit on, the next step's in
-// flight.  The logits before it go to the row's first wave, those behind the
-// last whole 16 bytes to its last.
+// flight.  What is left of the row, before that logit and behind the last whole
+// step, goes to the waves one logit a lane.
 template <bool kHalf>
 __global__ __launch_bounds__(kBlk) void logprobs_kernel(Logprobs a, int splits, int per_wave) {
-    constexpr int kVec = kHalf ? 8 : 4, kLoads = kPer / kVec;
+    using L = Logits<kHalf>;
+    using Logit = std::conditional_t<kHalf, _Float16, float>;
+    constexpr int kVecs = kWave * L::kLoads;   // vectors of a step
     __shared__ uint64_t room[kWaves][kWave];
     __shared__ Part parts[kWaves];
+    __shared__ uint64_t floors[kWaves];   // the waves' own, read without waiting for one another
     const int r = blockIdx.x / splits, split = blockIdx.x - r * splits;
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const char* row = static_cast<const char*>(a.logits) + (size_t)r * a.row_stride * (kHalf ? 2 : 4);
-    const int lead = (int)((16 - ((uintptr_t)row & 15)) & 15) / (kHalf ? 2 : 4);
-    const int head = min(lead, a.vocab);                   // logits before the aligned ones
-    const int vecs = (a.vocab - head) / kVec, behind = head + vecs * kVec;
-    const u32x4* body = reinterpret_cast<const u32x4*>(row + (size_t)head * (kHalf ? 2 : 4));
-    const int steps = (vecs + kWave * kLoads - 1) / (kWave * kLoads);
+    const int head = min(a.vocab, (int)((16 - ((uintptr_t)row & 15)) & 15) / (kHalf ? 2 : 4));
+    const int steps = (a.vocab - head) / kStep;
+    const u32x4* body = reinterpret_cast<const u32x4*>(row + (size_t)head * (kHalf ? 2 : 4)) + lane;
     const int piece = split * kWaves + wave;
-    const int first = min(steps, piece * per_wave), last = min(steps, first + per_wave);
+    // the workgroup's steps in turn over its waves: 8 or 16 KB of the row at a time
+    const int first = min(steps, split * kWaves * per_wave + wave), last = min(steps, (split + 1) * kWaves * per_wave);
 
     const int token = a.tokens ? a.tokens[r] : -1;
     const bool given = token >= 0 && token < a.vocab;
     const float mine = given ? logit_at<kHalf>(row, token) : NAN;
-    // before the token an equal logit counts too: x > the float below
-    const uint64_t my_key = logit_key(mine, 0);
-    const bool nan_token = given && mine != mine;          // every other logit is before a NaN
+    const Logit given_x = (Logit)mine;
+    const bool nan_token = given && mine != mine;   // every other logit is before a NaN
 
     Sums sums{-INFINITY, 0.f, 0.f};
-    int rank = 0;
+    int rank = 0;   // logits of the lane before the given one
     TopKeys top;
     top.room = room[wave];
     top.lane = lane;
     top.k = max(1, a.top_k);
 
-    // one logit a lane (id >= vocab: none)
-    auto add_one = [&](int id) {
-        const bool real = id < a.vocab;
-        const float x = real ? logit_at<kHalf>(row, id) : -INFINITY;
-        sums = join(sums, Sums{x, x == -INFINITY ? 0.f : x == INFINITY ? NAN : x - x + 1.f, x - x == 0.f || x == -INFINITY ? 0.f : NAN});
-        const uint64_t key = real ? logit_key(x, id) : 0ull;
-        if (given) rank += nan_token ? key != 0 : key > ((my_key & ~0xffffffffull) | (uint32_t)~(uint32_t)token);
-        if (a.top_k) top.add(key);
+    if (lane == 0) floors[wave] = 0;
+    __syncthreads();
+    L next;
+    auto load = [&](int step) {
+#pragma unroll
+        for (int i = 0; i < L::kLoads; ++i)
+            next.w[i] = __builtin_nontemporal_load(body + (size_t)step * kVecs + i * kWave);
     };
-
-    u32x4 raw[kLoads];
-    auto load = [&](int step) {   // steps past the last one read it again
-        const int at = min(step, steps - 1) * (kWave * kLoads) + lane;
+    if (first < last) load(first);
+    for (int step = first; step < last; step += kWaves) {
+        const L x = next;
+        load(min(step + kWaves, last - 1));
+        const int id0 = head + step * kStep;
+        auto id_of = [&](int i) { return id0 + (i / L::kVec * kWave + lane) * L::kVec + i % L::kVec; };
+        uint64_t others[kWaves];
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) raw[i] = __builtin_nontemporal_load(body + min(at + i * kWave, vecs - 1));
-    };
-    if (piece == 0 && head > 0) add_one(lane < head ? lane : INT_MAX);
-    if (first < last) {
-        load(first);
-        for (int step = first; step < last; ++step) {
-            float x[kPer];
+        for (int w = 0; w < kWaves; ++w)
+            others[w] = __hip_atomic_load(&floors[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        const float largest = x.largest();
+        add_logits(sums, x, largest);
+        if (given) {
+            if (nan_token) {
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i)
+                for (int i = 0; i < kPer; ++i) rank += x.at(i) == x.at(i);
+            } else if (token >= id0 + kStep) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if constexpr (kHalf) {
-                        const f16x2 h = as_h2(raw[i][j]);
-                        x[i * kVec + 2 * j] = (float)h.x;
-                        x[i * kVec + 2 * j + 1] = (float)h.y;
-                    } else {
-                        x[i * kVec + j] = __uint_as_float(raw[i][j]);
-                    }
-                }
-            load(step + 1);
-            const int vec0 = step * (kWave * kLoads) + lane;   // the lane's first; then every 64th
-            const bool whole = (step + 1) * (kWave * kLoads) <= vecs;
-            if (!whole) {
+                for (int i = 0; i < kPer; ++i) rank += x.at(i) >= given_x;
+            } else if (token < id0) {
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) rank += x.at(i) > given_x;
+            } else {
 #pragma unroll
                 for (int i = 0; i < kPer; ++i)
-                    if (vec0 + i / kVec * kWave >= vecs) x[i] = -INFINITY;
+                    rank += x.at(i) > given_x || (x.at(i) == given_x && id_of(i) < token);
             }
-            auto id_of = [&](int i) {
-                const int v = vec0 + i / kVec * kWave;
-                return whole || v < vecs ? head + v * kVec + i % kVec : INT_MAX;
-            };
-            add_logits(sums, x);
-            if (given) {
-                const int id0 = head + step * kStep;
-                if (nan_token) {
+        }
+        if (a.top_k) {
+            // ids only grow, so a later logit equal to the k-th is not above it
+            uint64_t theirs = 0;
 #pragma unroll
-                    for (int i = 0; i < kPer; ++i) rank += x[i] == x[i] && id_of(i) != INT_MAX;
-                } else if (whole && token >= id0 + kStep) {
+            for (int w = 0; w < kWaves; ++w) theirs = others[w] > theirs ? others[w] : theirs;
+            top.theirs = lane_key(theirs, 0);
+            // (one equal to another wave's may be, by its id)
+            const uint64_t over = __builtin_amdgcn_ballot_w64((top.floor == 0 || largest > key_logit(top.floor)) &&
+                                                              (top.theirs == 0 || largest >= key_logit(top.theirs)));
+            if (over != 0) {
+                const bool many = __popcll(over) > 16;
+                if (many) {
+                    uint64_t best = 0;
 #pragma unroll
-                    for (int i = 0; i < kPer; ++i) rank += x[i] >= mine;
-                } else if (token < id0) {
-#pragma unroll
-                    for (int i = 0; i < kPer; ++i) rank += x[i] > mine;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kPer; ++i) rank += x[i] > mine || (x[i] == mine && id_of(i) < token);
-                }
-            }
-            if (a.top_k) {
-                float mx = x[0];
-#pragma unroll
-                for (int i = 1; i < kPer; ++i) mx = fmaxf(mx, x[i]);
-                // ids only grow, so a later logit equal to the k-th is not above it
-                const uint64_t over = __builtin_amdgcn_ballot_w64(top.floor == 0 || mx > key_logit(top.floor));
-                if (over != 0) {
-                    if (__popcll(over) > 16) {
-                        uint64_t best = 0;
-#pragma unroll
-                        for (int i = 0; i < kPer; ++i) {
-                            const uint64_t key = id_of(i) == INT_MAX ? 0ull : logit_key(x[i], id_of(i));
-                            best = key > best ? key : best;
-                        }
-                        top.raise(best);
+                    for (int i = 0; i < kPer; ++i) {
+                        const uint64_t key = logit_key((float)x.at(i), id_of(i));
+                        best = key > best ? key : best;
                     }
-                    // registers i with a candidate, each added in turn
+                    top.raise(best);
+                }
+                // registers i with a candidate, each added in turn
+                uint32_t todo = 0;
+                if (many || top.floor == 0) {   // the k-th may be among them
                     const float least = top.floor == 0 ? -INFINITY : key_logit(top.floor);
-                    uint32_t todo = 0;
 #pragma unroll
                     for (int i = 0; i < kPer; ++i)
-                        todo |= (__builtin_amdgcn_ballot_w64(x[i] >= least) != 0 ? 1u : 0u) << i;
-                    while (todo != 0) {
-                        const int i = __builtin_ctz(todo);
-                        todo &= todo - 1;
-                        float xi = x[0];
+                        todo |= (__builtin_amdgcn_ballot_w64((float)x.at(i) >= least) != 0 ? 1u : 0u) << i;
+                } else {
+                    const float least = key_logit(top.floor);
 #pragma unroll
-                        for (int j = 1; j < kPer; ++j) xi = i == j ? x[j] : xi;
-                        top.add(id_of(i) == INT_MAX ? 0ull : logit_key(xi, id_of(i)));
-                    }
+                    for (int i = 0; i < kPer; ++i)
+                        todo |= (__builtin_amdgcn_ballot_w64((float)x.at(i) > least) != 0 ? 1u : 0u) << i;
                 }
+                while (todo != 0) {
+                    const int i = __builtin_ctz(todo);
+                    todo &= todo - 1;
+                    float xi = (float)x.at(0);
+#pragma unroll
+                    for (int j = 1; j < kPer; ++j) xi = i == j ? (float)x.at(j) : xi;
+                    top.add(logit_key(xi, id_of(i)));
+                }
+                if (lane == 0) __hip_atomic_store(&floors[wave], top.floor, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
             }
         }
     }
-    if (piece == splits * kWaves - 1 && behind < a.vocab) add_one(lane < a.vocab - behind ? behind + lane : INT_MAX);
+
+    const int rest = a.vocab - steps * kStep;   // the first `head` of them at the row's start
+    for (int j = piece * kWave; j < rest; j += splits * kWaves * kWave) {
+        const int n = j + lane, id = n < head ? n : n + steps * kStep;
+        const bool real = n < rest;
+        const float x = real ? logit_at<kHalf>(row, id) : -INFINITY;
+        const bool any = x > -INFINITY || x != x;
+        sums = join(sums, Sums{x, !any ? 0.f : x - x == 0.f ? 1.f : NAN, !any || x - x == 0.f ? 0.f : NAN});
+        const uint64_t key = real ? logit_key(x, id) : 0ull;
+        if (given) rank += key > logit_key(mine, token);
+        if (a.top_k) top.add(key);
+    }
 
     // the waves of the workgroup, then the piece or the row
     sums = wave_join(sums);
