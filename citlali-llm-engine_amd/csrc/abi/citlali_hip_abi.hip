@@ -606,6 +606,16 @@ CITLALI_EXPORT int citlali_hip_embed_at(const uint16_t* table, const int32_t* to
 
 // ---------------------------------------------------------------- paged 4-bit cache
 namespace {
+// heads per kv head the attention kernels have, and counts that a grid of fewer
+// than 2^32 threads (65535 workgroups in y) and 32-bit positions hold
+constexpr int kKv4MaxGroup = 16;
+constexpr int kKv4MaxHeads = 4096;
+constexpr int kKv4MaxContext = 65535 * 1024;           // the longest chunk, 65535 times
+constexpr long long kKv4MaxSeqHeads = 1ll << 23;       // a workgroup each
+constexpr long long kKv4MaxQueryHeads = 1ll << 25;     // a wave each in the merge
+constexpr long long kKv4MaxTokenHeads = 1ll << 31;     // of q: 256 GiB at head_dim 64
+constexpr long long kKv4MaxRows = 1ll << 27;           // head rows of one append or read, 8 or 16 lanes each
+
 int check_kv4(const char* who, const citlali_hip_kv4_cache* c, Kv4View* v) {
     REQUIRE(c && c->pages, "%s received a null cache", who);
     REQUIRE(c->num_pages > 0 && c->kv_heads > 0, "%s: num_pages (%d) and kv_heads (%d) must be positive", who,
@@ -615,18 +625,13 @@ int check_kv4(const char* who, const citlali_hip_kv4_cache* c, Kv4View* v) {
                     "%s: a cache of page_size %d and head_dim %d is not built (page_size 16, 32, 64, 128 or 256, "
                     "head_dim 64 or 128)",
                     who, c->page_size, c->head_dim);
+    REQUIRE(c->kv_heads <= kKv4MaxHeads, "%s: %d kv heads exceed %d", who, c->kv_heads, kKv4MaxHeads);
     REQUIRE((long long)c->num_pages * c->page_size <= INT_MAX, "%s: %d pages of %d tokens exceed the slot range", who,
             c->num_pages, c->page_size);
     REQUIRE(aligned(c->pages, 16), "%s: pages must be 16-byte aligned", who);
     *v = Kv4View{c->pages, c->num_pages, __builtin_ctz((unsigned)c->page_size), c->kv_heads, c->head_dim};
     return CITLALI_OK;
 }
-
-// heads per kv head the attention kernels have, and counts the grids hold
-constexpr int kKv4MaxGroup = 16;
-constexpr int kKv4MaxHeads = 4096;
-constexpr long long kKv4MaxQueryHeads = 1ll << 25;   // a wave each in the merge: 2^31 threads
-constexpr long long kKv4MaxRows = 1ll << 28;   // head rows of one append or read: 2^32 threads
 
 int check_kv4_attention(const char* who, int max_context, int max_query, int nseq, int tokens, int heads,
                         int kv_heads) {
@@ -636,6 +641,11 @@ int check_kv4_attention(const char* who, int max_context, int max_query, int nse
     REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "%s: heads (%d) must be a multiple of kv_heads (%d)",
             who, heads, kv_heads);
     REQUIRE(nseq <= 65535 && heads <= kKv4MaxHeads, "%s: at most 65535 sequences and %d heads", who, kKv4MaxHeads);
+    REQUIRE(max_context <= kKv4MaxContext, "%s: max_context (%d) exceeds %d", who, max_context, kKv4MaxContext);
+    REQUIRE((long long)nseq * kv_heads <= kKv4MaxSeqHeads, "%s: nseq (%d) times kv_heads (%d) exceeds %lld", who, nseq,
+            kv_heads, kKv4MaxSeqHeads);
+    REQUIRE((long long)tokens * heads <= kKv4MaxTokenHeads, "%s: tokens (%d) times heads (%d) exceeds %lld", who, tokens,
+            heads, kKv4MaxTokenHeads);
     REQUIRE((long long)max_query * heads <= kKv4MaxQueryHeads, "%s: max_query (%d) times heads (%d) exceeds %lld", who,
             max_query, heads, kKv4MaxQueryHeads);
     if (heads / kv_heads > kKv4MaxGroup)
@@ -646,7 +656,7 @@ int check_kv4_attention(const char* who, int max_context, int max_query, int nse
 }  // namespace
 
 CITLALI_EXPORT size_t citlali_hip_kv4_page_bytes(int page_size, int kv_heads, int head_dim) {
-    if (kv_heads <= 0 || !kv4_shape_ok(page_size, head_dim)) return 0;
+    if (kv_heads <= 0 || kv_heads > kKv4MaxHeads || !kv4_shape_ok(page_size, head_dim)) return 0;
     return (size_t)kv_heads * page_size * head_dim * 5 / 4;
 }
 
@@ -654,8 +664,8 @@ CITLALI_EXPORT int citlali_hip_rope_table(float* table, int positions, int head_
     REQUIRE(table, "rope_table received a null buffer");
     REQUIRE(positions > 0 && head_dim > 0 && head_dim % 2 == 0 && head_dim <= 2048,
             "rope_table: bad positions (%d) or head_dim (%d)", positions, head_dim);
-    REQUIRE((long long)positions * (head_dim / 2) < 1ll << 32, "rope_table: %d positions are too many", positions);
-    REQUIRE(theta > 0.f, "rope_table: theta must be positive");
+    REQUIRE((long long)positions * (head_dim / 2) <= 1ll << 31, "rope_table: %d positions are too many", positions);
+    REQUIRE(theta > 0.f && theta < INFINITY, "rope_table: theta must be positive and finite");
     REQUIRE(aligned(table, 8), "rope_table: table must be 8-byte aligned");
     HIP_TRY(launch_rope_table(table, positions, head_dim, theta, g_stream));
     return CITLALI_OK;
@@ -747,8 +757,13 @@ CITLALI_EXPORT int citlali_hip_kv4_attention(const citlali_hip_kv4_cache* cache,
 }
 
 // ---------------------------------------------------------------- log probabilities
+namespace {
+constexpr int kMaxLogitRows = 1 << 23;   // a workgroup each
+constexpr int kMaxVocab = 1 << 30;       // ids and what is rounded up from them stay in 32 bits
+}  // namespace
+
 CITLALI_EXPORT size_t citlali_hip_token_logprobs_workspace_bytes(int rows, int vocab, int top_k) {
-    if (rows <= 0 || vocab <= 0 || top_k < 0 || top_k > CITLALI_MAX_TOP_LOGPROBS) return 0;
+    if (rows <= 0 || rows > kMaxLogitRows || vocab <= 0 || vocab > kMaxVocab || top_k < 0 || top_k > CITLALI_MAX_TOP_LOGPROBS) return 0;
     return logprobs_workspace(rows, vocab, top_k);
 }
 
@@ -758,7 +773,8 @@ CITLALI_EXPORT int citlali_hip_token_logprobs(const void* logits, int gguf_type,
                                               void* workspace, size_t workspace_bytes) {
     REQUIRE(gguf_type == 0 || gguf_type == 1, "token_logprobs: GGUF type %d is not F32 or F16", gguf_type);
     REQUIRE(rows >= 0 && vocab > 0, "token_logprobs: bad rows (%d) or vocab (%d)", rows, vocab);
-    REQUIRE(rows <= 1 << 23, "token_logprobs: %d rows are too many", rows);
+    REQUIRE(rows <= kMaxLogitRows && vocab <= kMaxVocab, "token_logprobs: %d rows of %d exceed %d of %d", rows, vocab,
+            kMaxLogitRows, kMaxVocab);
     REQUIRE(logits, "token_logprobs received a null buffer");
     REQUIRE(row_stride >= vocab, "token_logprobs: row_stride (%lld) is shorter than vocab (%d)", row_stride, vocab);
     REQUIRE(aligned(logits, gguf_type == 0 ? 4 : 2), "token_logprobs: logits are not aligned to their type");

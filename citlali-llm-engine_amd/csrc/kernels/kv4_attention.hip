@@ -35,7 +35,7 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Attention& a, int seq) {
         end = seq + 1;
     }
     s.n = end - s.start;
-    s.context = a.context_lens[seq];
+    s.context = max(a.context_lens[seq], 0);
     s.cap = a.max_context;
     return s;
 }

@@ -343,8 +343,8 @@ int citlali_hip_matvec_norm(int gguf_type, const uint8_t* w, const uint16_t* x, 
  *   K params [page_size][head_dim / 32] fp16 pairs d, m
  *   V codes  [page_size / 4][head_dim / 4][4 tokens] 16-bit words of 4 dims
  *   V params [page_size / 4][head_dim / 32] fp16 d of 4 tokens, then m
- * page_size 16, 32, 64, 128 or 256; head_dim 64 or 128; pages 16-byte
- * aligned; num_pages * page_size at most INT_MAX. */
+ * page_size 16, 32, 64, 128 or 256; head_dim 64 or 128; kv_heads at most 4096;
+ * pages 16-byte aligned; num_pages * page_size at most INT_MAX. */
 typedef struct citlali_hip_kv4_cache {
     uint8_t* pages; /* [num_pages][kv_heads][page_bytes / kv_heads] */
     int num_pages;
@@ -357,7 +357,8 @@ size_t citlali_hip_kv4_page_bytes(int page_size, int kv_heads, int head_dim);
 
 /* cos and sin of position * theta^(-2i / head_dim), angles in 64 bits, for
  * citlali_hip_kv4_append: table [positions][head_dim / 2][cos, sin] floats.
- * Any other table of that shape (a scaled rotation, say) serves as well. */
+ * Any other table of that shape (a scaled rotation, say) serves as well.
+ * positions * head_dim / 2 at most 2^31. */
 int citlali_hip_rope_table(float* table, int positions, int head_dim, float theta);
 
 /* Appends `tokens` tokens of any sequences in one launch.  Token t's query
@@ -372,16 +373,16 @@ int citlali_hip_rope_table(float* table, int positions, int head_dim, float thet
  * Two tokens of one call must not name one slot: the slot then holds parts of
  * both.  q may be NULL with heads 0 (keys and values only); q_out may be q
  * when the strides agree.  q, k, v and q_out 16-byte aligned, strides multiples
- * of 8 (elements); q_norm, k_norm 16-byte, rope 8-byte aligned.
- * tokens 0 launches nothing. */
+ * of 8 (elements); q_norm, k_norm 16-byte, rope 8-byte aligned.  heads at most
+ * 4096, tokens * (heads + 2 kv_heads) 2^27.  tokens 0 launches nothing. */
 int citlali_hip_kv4_append(const citlali_hip_kv4_cache* cache, const uint16_t* q, const uint16_t* k,
                            const uint16_t* v, long long q_stride, long long kv_stride, const uint16_t* q_norm,
                            const uint16_t* k_norm, float eps, const float* rope, int rope_positions,
                            const int32_t* positions, const int32_t* slots, int tokens, int heads, uint16_t* q_out,
                            long long q_out_stride);
 /* The values that `count` slots hold, as fp16 rows [count][kv_heads][head_dim]
- * (16-byte aligned); a slot outside the cache reads as zeros.  count 0 launches
- * nothing. */
+ * (16-byte aligned); a slot outside the cache reads as zeros.  count * 2 *
+ * kv_heads at most 2^27; count 0 launches nothing. */
 int citlali_hip_kv4_read(const citlali_hip_kv4_cache* cache, const int32_t* slots, int count, uint16_t* k_out,
                          uint16_t* v_out);
 
@@ -393,20 +394,25 @@ int citlali_hip_kv4_read(const citlali_hip_kv4_cache* cache, const int32_t* slot
  *    (tokens == nseq).  Rows past the last sequence's are left as they were.
  *  - context_lens[s] positions are cached, the queries' own among them: with n
  *    queries, query i sees positions 0 .. context_lens[s] - n + i.  A query
- *    that sees none gives zeros.
+ *    that sees none, or only scores of -inf, gives zeros; a length below 0
+ *    counts as 0.
  *  - position p of sequence s is row p % page_size of page page_table[s *
  *    pages_per_seq + p / page_size]; a page outside the cache counts as not
  *    there (its positions take no part).
  *  - max_query and max_context bound the queries and the positions of a
  *    sequence: the launch is planned for them.  Queries past max_query are
  *    left as they were; positions past max_context are not read.
- *    max_context is at most pages_per_seq * page_size.
- * Slots past a sequence's positions may hold anything.  Weights are kept as
- * fp16 times 2^14 against the largest of their pass, sums in fp32.  heads /
- * kv_heads between 1 and 16.  Workspace:
+ *    max_context is at most pages_per_seq * page_size and 65535 * 1024.
+ * What a query does not see may hold anything: slots past a sequence's
+ * positions, and NaN in the keys or values of the queries behind it.  Scores
+ * and sums are fp32; weights go into the product with V as fp16, scaled so that
+ * the largest is between 2^10 and 2^14.  heads / kv_heads between 1 and 16,
+ * heads at most 4096, nseq at most 65535, nseq * kv_heads 2^23, max_query *
+ * heads 2^25, tokens * heads 2^31.  Workspace:
  * citlali_hip_kv4_attention_workspace_bytes() of the same bounds, 16-byte
- * aligned (may be NULL if that is 0); calls that overlap need one each.  q, out 16-byte aligned, strides
- * multiples of 8.  nseq 0 or tokens 0 launches nothing. */
+ * aligned (may be NULL if that is 0); calls that overlap need one each.  q and
+ * out 16-byte aligned, strides multiples of 8.  nseq 0 or tokens 0 launches
+ * nothing. */
 int citlali_hip_kv4_attention(const citlali_hip_kv4_cache* cache, const uint16_t* q, long long q_stride,
                               const int32_t* query_start, const int32_t* context_lens, const int32_t* page_table,
                               int pages_per_seq, int nseq, int tokens, int max_query, int max_context, int heads,
@@ -429,7 +435,7 @@ size_t citlali_hip_kv4_attention_workspace_bytes(int max_context, int max_query,
  * is never among them and before no token).  Fewer than top_k tokens to list:
  * id -1, log probability -inf.  Outputs may be NULL: logprobs and ranks (tokens
  * may then be NULL too), entropies, and top_ids with top_logprobs when top_k is
- * 0.  top_k at most CITLALI_MAX_TOP_LOGPROBS.  Workspace:
+ * 0.  top_k at most CITLALI_MAX_TOP_LOGPROBS, rows 2^23, vocab 2^30.  Workspace:
  * citlali_hip_token_logprobs_workspace_bytes(), 16-byte aligned (may be NULL if
  * that is 0); calls that overlap need one each.  rows 0 launches nothing. */
 #define CITLALI_MAX_TOP_LOGPROBS 64

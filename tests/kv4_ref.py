@@ -111,6 +111,7 @@ def attention(cache, q, query_start, lens, table, max_context=None, max_query=No
     for s, length in enumerate(lens):
         r0, r1 = int(query_start[s]), int(query_start[s + 1])
         n = r1 - r0
+        length = max(0, int(length))
         cap = length if max_context is None else min(length, max_context)
         p = np.arange(max(0, cap))
         pages = np.asarray(table[s])[p // page] if len(p) else np.zeros(0, int)

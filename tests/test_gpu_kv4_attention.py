@@ -117,6 +117,16 @@ def test_sequences_without_positions_or_queries(hip):
     Batch(hip, 4, 8, 2, 128, 16, [40, 40, 0, 40], asked=[0, 7, 0, 20]).upload().launch().check()
 
 
+def test_lengths_below_zero_count_as_zero(hip):
+    b = Batch(hip, 16, 8, 2, 128, 16, [0, 40, 0], asked=[2, 3, 40])
+    b.lens[[0, 2]] = -1, -2 ** 31
+    got = b.upload().launch().check()
+    assert not got[:2].any() and got[2:5].any() and not got[5:].any()
+    b = Batch(hip, 17, 8, 2, 64, 16, [0, 9000])
+    b.lens[0] = -2 ** 31
+    assert not b.upload().launch().check()[0].any()
+
+
 def test_queries_before_the_first_position(hip):
     """More queries than positions: the first ones see nothing."""
     got = Batch(hip, 5, 4, 2, 64, 16, [3, 30], asked=[9, 30]).upload().launch().check()
