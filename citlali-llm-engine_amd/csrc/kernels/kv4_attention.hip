@@ -2,6 +2,7 @@
 // values.
 #include "kv4.hpp"
 
+#include <limits.h>
 #include <math.h>
 
 #include <algorithm>
@@ -38,6 +39,22 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Attention& a, int seq) {
     s.context = max(a.context_lens[seq], 0);
     s.cap = a.max_context;
     return s;
+}
+
+// V of four positions that some rows do not see: a weight of 0 would not keep a
+// NaN from them.  Clears the scales (d of four positions, then m) of those whose
+// m is NaN -- their codes are 0 -- and returns them as bits.
+__device__ __forceinline__ uint32_t kv4_hide_nan(u32x4& dm) {
+    uint32_t nan = 0;
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+        const bool lo = (dm[2 + y] & 0x7fffu) > 0x7c00u, hi = (dm[2 + y] & 0x7fff0000u) > 0x7c000000u;
+        const uint32_t keep = (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+        dm[y] &= keep;
+        dm[2 + y] &= keep;
+        nan |= ((lo ? 1u : 0u) | (hi ? 2u : 0u)) << (2 * y);
+    }
+    return nan;
 }
 
 constexpr int kBlk = 256, kWaves = kBlk / kWave;
@@ -223,6 +240,24 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : 2) void kv4_decode_kernel(Kv
                 const uint32_t lo = left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
                 const uint32_t hi = left >= 4 ? 0xffffffffu : left == 3 ? 0xffffu : 0u;
                 xvp[u] &= u32x4{lo, hi, lo, hi};
+            }
+            // NaN in V: only for the rows that see it
+            const uint32_t nan = kv4_hide_nan(xvp[0]) | kv4_hide_nan(xvp[1]) << 4;
+            if (__builtin_amdgcn_ballot_w64(nan != 0) != 0) {
+                int first = INT_MAX;   // position of the first one in the lane's dims of O, a group
+#pragma unroll 1
+                for (int g = 0; g < HD / kKv4Group; ++g)
+#pragma unroll 1
+                    for (int b = 0; b < 8; ++b) {
+                        const uint64_t who = __builtin_amdgcn_ballot_w64(col / (512 / HD) == g && ((nan >> b) & 1) != 0);
+                        if (who == 0 || (HD == 128 ? grp : grp >> 1) != g) continue;
+                        first = min(first, t + 16 * (b / 4) + 4 * (__builtin_ctzll(who) / 16) + b % 4);
+                    }
+#pragma unroll
+                for (int n = 0; n < kCols; ++n)
+#pragma unroll
+                    for (int d = 0; d < kDims; ++d)
+                        if (see[n] > first) o[n][d] = f32x4{NAN, NAN, NAN, NAN};
             }
         }
 #pragma unroll
@@ -411,7 +446,9 @@ __global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Atten
     constexpr int kHalves = HD * kTile;                // of K (or V) in a buffer
     extern __shared__ __align__(16) float lds[];
     uint16_t* const buf = reinterpret_cast<uint16_t*>(lds);              // [2][K, V][kHalves]
-    int* const there_at = reinterpret_cast<int*>(buf + 4 * kHalves);     // [2][4 waves]: the 16 positions have a page
+    // [2][4 waves]: bit 0, the 16 positions have a page; bit 1, nan_at says where V is NaN
+    int* const there_at = reinterpret_cast<int*>(buf + 4 * kHalves);
+    int* const nan_at = there_at + 2 * kWaves;                           // [2][4 waves][4 groups of dims]
 
     // kv heads side by side, so that the workgroups of one meet in an XCD's L2
     // where there are eight of them; row tiles with the most positions first
@@ -448,6 +485,8 @@ __global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Atten
     const int wave_least = r_last < row0 + 32 * wave + 31 ? 0 : min(s.see((row0 + 32 * wave) / group), c1);
     const int wave_most = row0 + 32 * wave >= rows ? 0 : min(s.see(r_last / group), c1);
 
+    const int least = min(s.see(row0 / group), c1);   // positions that every row of the workgroup sees
+
     // ---- the wave's 16 positions of a tile: pages, loads, dequantisation ----
     const int P = 1 << c.page_shift;
     const int last_page = (max(c1, 1) - 1) >> c.page_shift;
@@ -462,7 +501,7 @@ __global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Atten
     u32x4 xvp;
     const uint32_t at_k = t16 * L::kCodes + g * (HD / 8), at_kp = t16 * L::kParams + (HD == 128 ? g : g >> 1) * 4;
     const uint32_t at_v = vb * (4 * L::kCodes) + t16 * (HD / 8), at_vp = vb * (4 * L::kParams) + t16 / (512 / HD) * 16;
-    int x_there = 0, x_pos = 0;
+    int x_there = 0, x_nan = 0, x_pos = 0;
     auto load = [&](int t) {
         const int p = t + 16 * wave, at = min(p >> c.page_shift, last_page);
         if (at >= window + kWave) {   // uniform
@@ -480,6 +519,25 @@ __global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Atten
         xv = *reinterpret_cast<const Vec*>(base + L::v_codes(P) + o * L::kCodes + at_v);
         xvp = *reinterpret_cast<const u32x4*>(base + L::v_params(P) + o * L::kParams + at_vp);
     };
+    // Before store(b): V of positions that no row, or not every row, sees.
+    auto hide = [&](int b) {
+        x_nan = 0;
+        if (x_there && x_pos + 16 <= least) return;   // uniform
+        // positions past the chunk or without a page: V counts as 0, whatever it holds
+        const int left = x_there ? c1 - (x_pos + 4 * vb) : 0;
+        const uint32_t lo = left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
+        const uint32_t hi = left >= 4 ? 0xffffffffu : left == 3 ? 0xffffu : 0u;
+        xvp &= u32x4{lo, hi, lo, hi};
+        const uint32_t nan = kv4_hide_nan(xvp);
+        if (__builtin_amdgcn_ballot_w64(nan != 0) == 0) return;
+        x_nan = 2;
+#pragma unroll 1
+        for (int dims = 0; dims < HD / kKv4Group; ++dims) {
+            int first = nan != 0 && t16 / (512 / HD) == dims ? x_pos + 4 * vb + __builtin_ctz(nan) : INT_MAX;
+            for (int d = 1; d < kWave; d <<= 1) first = min(first, __shfl_xor(first, d, kWave));
+            if (lane == 0) nan_at[(b * kWaves + wave) * 4 + dims] = first;
+        }
+    };
     auto store = [&](int b) {
         uint16_t* kb = buf + b * 2 * kHalves;
         uint16_t* vbuf = kb + kHalves;
@@ -492,11 +550,6 @@ __global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Atten
             *reinterpret_cast<half8*>(kb + ((g * kWords + w) * kTile + 16 * wave + t16) * 8) =
                 __builtin_bit_cast(half8, e);
         }
-        // positions past the chunk or without a page: V counts as 0, whatever it holds
-        const int left = x_there ? c1 - (x_pos + 4 * vb) : 0;
-        const uint32_t lo = left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
-        const uint32_t hi = left >= 4 ? 0xffffffffu : left == 3 ? 0xffffu : 0u;
-        xvp &= u32x4{lo, hi, lo, hi};
 #pragma unroll
         for (int h = 0; h < kWords / 2; ++h) {
             f16x2 e[2][4];
@@ -509,7 +562,7 @@ __global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Atten
                                           (vb >> 1) * 4) =
                     u32x2{__builtin_bit_cast(uint32_t, e[0][n]), __builtin_bit_cast(uint32_t, e[1][n])};
         }
-        if (lane == 0) there_at[b * 4 + wave] = x_there;
+        if (lane == 0) there_at[b * kWaves + wave] = x_there | x_nan;
     };
 
     f32x16 o[HD / 32];
@@ -520,17 +573,18 @@ __global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Atten
     float m_run = -INFINITY, l_run = 0.f;
 
     auto process = [&](int t, int b) {
+        hide(b ^ 1);
         if (t >= wave_most) {   // uniform: no row of the wave sees the tile
             store(b ^ 1);
             return;
         }
         const uint16_t* kb = buf + b * 2 * kHalves;
         const uint16_t* vbuf = kb + kHalves;
-        int there = 0;
+        int there = 0;   // two bits a wave
 #pragma unroll
-        for (int w = 0; w < 4; ++w) there |= (there_at[b * 4 + w] != 0) << w;
+        for (int w = 0; w < kWaves; ++w) there |= there_at[b * kWaves + w] << (2 * w);
         there = __builtin_amdgcn_readfirstlane(there);
-        const bool whole = there == 15 && t + kTile <= wave_least;
+        const bool whole = (there & 0x55) == 0x55 && t + kTile <= wave_least;
         __builtin_amdgcn_sched_barrier(0);
         f32x16 sc[2];
 #pragma unroll
@@ -558,9 +612,24 @@ __global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Atten
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int p = 32 * u + 8 * (e / 4) + 4 * half + e % 4;
-                    const bool seen = t + p < see && ((there >> (p >> 4)) & 1);
+                    const bool seen = t + p < see && ((there >> (p >> 4) * 2) & 1);
                     sc[u][e] = seen ? sc[u][e] : -INFINITY;
                 }
+        }
+        if ((there & 0xaa) != 0) {   // NaN in V: only for the rows that see it
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {   // elements e with e / 4 % 2 = y are of one group of dims
+                int first = INT_MAX;
+#pragma unroll 1
+                for (int w = 0; w < kWaves; ++w)
+                    if ((there >> (2 * w)) & 2)
+                        first = min(first, nan_at[(b * kWaves + w) * 4 + (HD == 128 ? 2 * y + half : y)]);
+#pragma unroll
+                for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (e / 4 % 2 == y) o[d][e] = see > first ? NAN : o[d][e];
+            }
         }
         float mt = -INFINITY;
 #pragma unroll
@@ -596,6 +665,7 @@ __global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Atten
     };
 
     load(c0);
+    hide(0);
     store(0);
     load(c0 + kTile);
     __syncthreads();
@@ -682,7 +752,7 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
     const int group = a.heads / c.kv_heads;
     const bool last = p.n_splits == 1;
     if (!p.few) {
-        const int lds = 4 * HD * kTile * (int)sizeof(uint16_t) + 8 * (int)sizeof(int);
+        const int lds = 4 * HD * kTile * (int)sizeof(uint16_t) + 2 * kWaves * 5 * (int)sizeof(int);
         const hipError_t e = allow_lds<kv4_prompt_kernel<HD>>(lds);
         if (e != hipSuccess) return e;
         launch_kernel_in_call(last, kv4_prompt_kernel<HD>, dim3(c.kv_heads * p.tiles * p.n_splits, a.nseq), dim3(kBlk), lds, s,

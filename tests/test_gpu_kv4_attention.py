@@ -61,10 +61,13 @@ class Batch:
         assert (out[:, row:] == 7).all()
         return out[:, :row].reshape(self.tokens, self.heads, self.hd)
 
+    def expected(self):
+        return kv4_ref.attention(self.cache, self.q, self.start, self.lens, self.table, self.max_context,
+                                 self.max_query)
+
     def check(self):
         got = self.result()
-        want, spread, reach = kv4_ref.attention(self.cache, self.q, self.start, self.lens, self.table,
-                                                self.max_context, self.max_query)
+        want, spread, reach = self.expected()
         asked = ~np.isnan(want[:, 0, 0])
         assert (got[~asked] == 7).all()                                   # rows nobody asks for
         got, want = got[asked].astype(np.float64), want[asked]
@@ -153,6 +156,62 @@ def test_slots_past_the_end_may_hold_anything(hip, asked):
             b.cache.raw[page, :, at:at + 2] = 0xFF
             b.cache.raw[page, :, at + 8:at + 10] = 0xFF
     assert np.array_equal(b.upload().launch().check(), clean)
+
+
+def _nan_tokens(b, where):
+    """Makes K and V NaN in one group of dims at (sequence, position, group)."""
+    _, kp, _, vp, _ = kv4_ref.head_layout(b.page, b.hd)
+    g, nan = b.hd // 32, np.frombuffer(np.float16(np.nan).tobytes(), np.uint8)
+    for s, p, j in where:
+        page, o = b.table[s, p // b.page], p % b.page
+        raw = b.cache.raw[page]
+        k, v = kp + (o * g + j) * 4, vp + (o // 4 * g + j) * 16 + o % 4 * 2
+        raw[:, k:k + 2], raw[:, k + 2:k + 4], raw[:, v:v + 2], raw[:, v + 8:v + 10] = 0, nan, 0, nan
+        raw[:, o * b.hd // 2 + j * 16:o * b.hd // 2 + j * 16 + 16] = 0
+        for w in range(8):
+            at = kp + g * 4 * b.page + (o // 4 * (b.hd // 4) + j * 8 + w) * 8 + o % 4 * 2
+            raw[:, at:at + 2] = 0
+    return b
+
+
+@pytest.mark.parametrize("hd,page", [(128, 16), (64, 64)])
+@pytest.mark.parametrize("heads,kv,asked", [(8, 2, [4, 2, 3]), (8, 2, [8, 1, 5]), (8, 2, [70, 9, 200])])
+def test_a_nan_is_kept_from_the_queries_before_it(hip, heads, kv, asked, hd, page):
+    """NaN keys and values at positions that the last queries see and the first
+    ones do not: the first ones' results are those of a cache without them."""
+    lens = [80, 33, 700]
+    b = Batch(hip, 18, heads, kv, hd, page, lens, asked)
+    want, spread, reach = b.expected()         # of the cache without them
+    near = kv4_ref.tolerance(want, spread, reach)
+    first = [lens[s] - max(1, n // 2) for s, n in enumerate(asked)]    # the first NaN position
+    _nan_tokens(b, [(s, p, (s + p) % (hd // 32)) for s in range(3) for p in range(first[s], lens[s], 3)])
+    got = b.upload().launch().result()[:b.start[-1]].astype(np.float64)
+    for s, n in enumerate(asked):
+        sees = lens[s] - n + np.arange(n) + 1 > first[s]
+        rows = slice(b.start[s], b.start[s + 1])
+        assert sees.any() and np.isnan(got[rows][sees]).all()
+        assert (np.abs(got[rows] - want[rows])[~sees] <= near[rows][~sees]).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("asked", [[4, 2], [70, 9]])
+def test_nan_values_reach_their_dims_alone(hip, hd, asked):
+    """Values (not keys) that are NaN in one group of dims."""
+    lens = [80, 33]
+    b = Batch(hip, 19, 8, 2, hd, 16, lens, asked)
+    want, spread, reach = b.expected()
+    near = kv4_ref.tolerance(want, spread, reach)
+    keys = b.cache.raw.copy()
+    where = [(0, 78, 1), (0, 79, 0), (1, 32, 1)]
+    _nan_tokens(b, where)
+    behind = kv4_ref.head_layout(16, hd)[2]
+    b.cache.raw[:, :, :behind] = keys[:, :, :behind]
+    got = b.upload().launch().result()[:b.start[-1]].astype(np.float64)
+    nan = np.zeros((len(got), hd // 32), bool)
+    for s, p, j in where:
+        nan[b.start[s]:b.start[s + 1], j] |= lens[s] - asked[s] + np.arange(asked[s]) + 1 > p
+    nan = np.repeat(nan, 32, axis=1)[:, None, :] & np.ones((1, 8, 1), bool)
+    assert np.isnan(got[nan]).all() and (np.abs(got - want)[~nan] <= near[~nan]).all()
 
 
 @pytest.mark.parametrize("asked", [None, [1, 6, 70]])
