@@ -157,6 +157,38 @@ def test_rows_that_are_no_distribution(hip):
     assert ids[1, 0] == 77 and ids[4, 0] == 2999 and (ids[2] == -1).all()
 
 
+@pytest.mark.parametrize("half", [False, True])
+def test_signalling_nans_hide_no_logit(hip, half):
+    """NaN logits of any kind beside the largest ones: the ids stay ordered."""
+    rng = np.random.default_rng(8)
+    x = _logits(rng, 6, 9001, half)
+    bits = x.view(np.uint16 if half else np.uint32)
+    for r, nan in enumerate((0x7c01, 0xfdff, 0x7e00) if half else (0x7f800001, 0xffbfffff, 0x7fc00000)):
+        bits[r, rng.random(9001) < 0.5] = nan
+        bits[r + 3, 1::2] = nan
+    _check(hip, x, [5, 6, 7, 8, 9, 10], 40)
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 151936), (9, 32000), (1100, 5000)])
+def test_equal_logits_over_a_row_in_pieces(hip, rows, vocab):
+    """A handful of values, so that waves and pieces end on equal logits; most
+    of the row at -inf or at the type's lowest value in others."""
+    rng = np.random.default_rng(vocab)
+    x = rng.integers(0, 3, (rows, vocab)).astype(np.float32)
+    x[0, rng.random(vocab) < 0.5] = 0
+    if rows > 1:
+        x[1] = np.finfo(np.float32).min
+        x[2] = -np.inf
+        x[2, rng.integers(0, vocab, 30)] = 1.5
+        x[3, :] = -np.inf
+        x[3, -70:] = 4
+        x[4, rng.random(vocab) < 0.999] = -np.inf
+        x[5, : vocab // 2] = 5
+        x[6, vocab // 2:] = 5
+    _check(hip, x, rng.integers(0, vocab, rows), 64)
+    _check(hip, x.astype(np.float16) if rows == 1 else x, rng.integers(0, vocab, rows), 3)
+
+
 def test_rows_without_a_token(hip):
     rng = np.random.default_rng(5)
     got, _, _ = _check(hip, _logits(rng, 4, 500), [-1, 499, 500, -2 ** 31], 2)
