@@ -57,43 +57,53 @@ __device__ __forceinline__ uint32_t kv4_hide_nan(u32x4& dm) {
     return nan;
 }
 
+// The sequence of workgroup x (of a layer of nseq sequences).  An XCD deals its
+// workgroups to its four shader engines in strict turn, those without work
+// too, so a sequence's place has to change from layer to layer: by nseq where
+// that is odd, else by one more.
+__device__ __forceinline__ int seq_of(int x, int layer, int nseq) {
+    return (x + (nseq & 1 ? 0 : layer)) % nseq;
+}
+
 constexpr int kBlk = 256, kWaves = kBlk / kWave;
-constexpr float kShift = 14.f;   // weights are kept times 2^14
+constexpr float kShift = 14.f;   // weights are kept times 2^14 (base 2)
 
 // ---------------------------------------------------------------------------
 // Few rows: one workgroup per (chunk of positions, kv head, sequence) serves
 // every query of the sequence for every head of the kv head's group, at most
 // 16 kCols rows (row r: query r / group, head r % group), so the cache is read
-// once.  The four waves take tiles of 32 positions in turn; no LDS until they
-// merge:
+// once.  The four waves take tiles of 32 positions in turn, without LDS until
+// they merge:
 //  * S^T[position][row] = K Q^T by v_mfma_f32_16x16x32_f16, 16 positions at a
 //    time: lane (col, grp) of the A operand holds position col's dims
 //    grp * HD/4 .. + HD/4 - 1, one 16-byte (head_dim 64: 8-byte) load of codes
-//    with one (d, m); Q, the B operand, is held in the same dim order.
+//    with one (d, m); Q, the B operand, is held in the same dim order (in LDS
+//    beyond 16 rows: that leaves registers for three waves per SIMD at 32).
 //  * online softmax down each column (row of Q): a lane has 8 of a tile's 32
 //    positions, the maximum takes two permlane swaps, the sum stays per lane
 //    until the end.
 //  * O^T[dim][row] += V^T P^T: the lanes' weights are the B operand as they
-//    stand (k index = grp 4 + i of the first 16 positions, then of the second);
-//    V lies in groups of four tokens, so lane (c, grp) loads the codes of its
-//    four positions and HD / 16 dims together, each word two positions' dims,
-//    and gets the A operand's pairs without a transposition.
+//    stand (k index = grp 4 + i of the first 16 positions, then of the second),
+//    rounded to fp16 -- times 2^14, so that weights down to 2^-28 of the largest
+//    keep all their bits; their sum takes them before.  V lies in groups of
+//    four tokens, so lane (c, grp) loads the codes of its four positions and
+//    HD / 16 dims together, each word two positions' dims, and gets the A
+//    operand's pairs without a transposition.
 // Bound by the cache's bytes: 5 KB a tile of head_dim 128 against about 300
 // vector instructions, a good half of what a CU issues meanwhile at 6 TB/s.
 // ---------------------------------------------------------------------------
 template <int HD, int kCols>
-__global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : 2) void kv4_decode_kernel(Kv4View c, Kv4Attention a, int chunk, int n_splits,
-                                                          float scale_log2) {
+__global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4_decode_kernel(
+    Kv4View c, Kv4Attention a, int chunk, int n_splits, float scale_log2) {
     using L = Kv4Layout<HD>;
     using Vec = std::conditional_t<HD == 128, u32x4, u32x2>;   // a lane's codes of 16 positions
     constexpr int kSteps = HD / 32, kDims = HD / 16;   // MFMA steps of a score; dims (and O tiles) of a V lane
-    // the waves' merge, rows_most of each: [wave][row][HD + 4], sums behind HD
+    // the waves' merge of 16 rows: [wave][row][HD + 4], sums behind HD
     extern __shared__ __align__(16) float lds[];
-    const int rows_most = a.max_query * (a.heads / c.kv_heads);
 
     // every sequence's first chunks before the second ones: the chunks that
     // short sequences lack then leave all XCDs alike
-    const int kvh = blockIdx.x % c.kv_heads, seq = blockIdx.x / c.kv_heads, split = blockIdx.y;
+    const int split = blockIdx.y, kvh = blockIdx.x % c.kv_heads, seq = seq_of(blockIdx.x / c.kv_heads, split, a.nseq);
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int col = lane & 15, grp = lane >> 4;
     // the chunk's pages, one a lane (a chunk has at most 64), with the lengths
@@ -108,8 +118,10 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : 2) void kv4_decode_kernel(Kv
     const int c1 = min(most, c0 + chunk);
     if (c0 >= most && split > 0) return;
     if (((first_page + lane) << c.page_shift) >= c1 || my_page >= c.num_pages) my_page = -1;
-    half8 q[kCols][kSteps];
+    constexpr bool kQInLds = kCols > 1;
+    half8 q[kQInLds ? 1 : kCols][kSteps];
     int see[kCols];
+    half8* const q_lds = reinterpret_cast<half8*>(lds);   // [column tile][step][lane]
 #pragma unroll
     for (int n = 0; n < kCols; ++n) {
         const int r = col + 16 * n, i = r / group;
@@ -121,7 +133,12 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : 2) void kv4_decode_kernel(Kv
         for (int t = 0; t < kSteps; ++t) {
             u32x4 v = *reinterpret_cast<const u32x4*>(qr + 8 * t);
             if (!real) v = u32x4{0u, 0u, 0u, 0u};
-            q[n][t] = __builtin_bit_cast(half8, v);
+            if constexpr (kQInLds) {
+                if ((n * kSteps + t) % kWaves == wave)
+                    q_lds[(n * kSteps + t) * kWave + lane] = __builtin_bit_cast(half8, v);
+            } else {
+                q[n][t] = __builtin_bit_cast(half8, v);
+            }
         }
     }
     const int least = s.see(0);   // positions every row sees
@@ -143,23 +160,27 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : 2) void kv4_decode_kernel(Kv
     u32x4 xvp[2];
     // uniform addresses plus a lane's own offsets
     const uint32_t at_k = col * L::kCodes + grp * (HD / 8), at_kp = col * L::kParams + (HD == 128 ? grp : grp >> 1) * 4;
-    const uint32_t at_v = grp * (4 * L::kCodes) + col * (HD / 8), at_vp = grp * (4 * L::kParams) + col / (512 / HD) * 16;
+    const uint32_t at_v = grp * (4 * L::kCodes) + col * (HD / 8);
+    const uint32_t at_vp = grp * (4 * L::kParams) + col / (512 / HD) * 16;
     const uint8_t* at_head[2];
+    auto read = [](auto* to, const uint8_t* from) {
+        *to = __builtin_nontemporal_load(reinterpret_cast<decltype(to)>(const_cast<uint8_t*>(from)));
+    };
     auto load_k = [&](int t) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int o = (t + 16 * u) & (P - 1) & ~15;
             at_head[u] = head_at(t + 16 * u);
-            xk[u] = __builtin_nontemporal_load(reinterpret_cast<const Vec*>(at_head[u] + o * L::kCodes + at_k));
-            xkp[u] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(at_head[u] + L::k_params(P) + o * L::kParams + at_kp));
+            read(&xk[u], at_head[u] + o * L::kCodes + at_k);
+            read(&xkp[u], at_head[u] + L::k_params(P) + o * L::kParams + at_kp);
         }
     };
     auto load_v = [&](int t) {   // of the positions that load_k took last
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int o = (t + 16 * u) & (P - 1) & ~15;
-            xv[u] = __builtin_nontemporal_load(reinterpret_cast<const Vec*>(at_head[u] + L::v_codes(P) + o * L::kCodes + at_v));
-            xvp[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at_head[u] + L::v_params(P) + o * L::kParams + at_vp));
+            read(&xv[u], at_head[u] + L::v_codes(P) + o * L::kCodes + at_v);
+            read(&xvp[u], at_head[u] + L::v_params(P) + o * L::kParams + at_vp);
         }
     };
 
@@ -175,11 +196,14 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : 2) void kv4_decode_kernel(Kv
 
     load_k(c0 + 32 * wave);
     load_v(c0 + 32 * wave);
+    if constexpr (kQInLds) lds_only_barrier();
     __builtin_amdgcn_sched_barrier(0);
     for (int t = c0 + 32 * wave; t < c1; t += 32 * kWaves) {
         const int there = (page_of(t) >= 0) | (page_of(t + 16) >= 0) << 1;
         const bool whole = there == 3 && t + 32 <= least;
         f32x4 sc[kCols][2];
+        int q_at = lane;
+        if constexpr (kQInLds) asm volatile("" : "+v"(q_at));   // read in every turn, not kept
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
@@ -192,8 +216,10 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : 2) void kv4_decode_kernel(Kv
                 kv4_pairs(xk[u][st], d, m, e);
                 const half8 k = __builtin_bit_cast(half8, e);
 #pragma unroll
-                for (int n = 0; n < kCols; ++n)
-                    sc[n][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[n][st], sc[n][u], 0, 0, 0);
+                for (int n = 0; n < kCols; ++n) {
+                    const half8 row = kQInLds ? q_lds[(n * kSteps + st) * kWave + q_at] : q[kQInLds ? 0 : n][st];
+                    sc[n][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, row, sc[n][u], 0, 0, 0);
+                }
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -249,7 +275,8 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : 2) void kv4_decode_kernel(Kv
                 for (int g = 0; g < HD / kKv4Group; ++g)
 #pragma unroll 1
                     for (int b = 0; b < 8; ++b) {
-                        const uint64_t who = __builtin_amdgcn_ballot_w64(col / (512 / HD) == g && ((nan >> b) & 1) != 0);
+                        const uint64_t who =
+                            __builtin_amdgcn_ballot_w64(col / (512 / HD) == g && ((nan >> b) & 1) != 0);
                         if (who == 0 || (HD == 128 ? grp : grp >> 1) != g) continue;
                         first = min(first, t + 16 * (b / 4) + 4 * (__builtin_ctzll(who) / 16) + b % 4);
                     }
@@ -282,16 +309,17 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : 2) void kv4_decode_kernel(Kv
         __builtin_amdgcn_sched_barrier(0);
     }
 
-    // merge the waves
+    // merge the waves, 16 rows at a time
+    const bool alone = most <= chunk;
 #pragma unroll
     for (int n = 0; n < kCols; ++n) {
-        l_run[n] = sum32(sum16(l_run[n]));
-        const int r = col + 16 * n;
-        if (r >= rows) continue;
-        float* to = lds + (wave * rows_most + r) * (HD + 4);
+        if (16 * n >= rows) break;   // uniform
+        if (kCols > 1) __syncthreads();   // Q, or the rows before, are read
+        const float l_sum = sum32(sum16(l_run[n]));
+        float* to = lds + (wave * 16 + col) * (HD + 4);
         if (grp == 0) {
             to[HD] = m_run[n];
-            to[HD + 1] = l_run[n];
+            to[HD + 1] = l_sum;
         }
         // lane (col, grp) has dims kDims (4 grp + i) + d of its column
 #pragma unroll
@@ -300,39 +328,38 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : 2) void kv4_decode_kernel(Kv
             for (int d = 0; d < kDims; d += 4)
                 *reinterpret_cast<f32x4*>(to + kDims * (4 * grp + i) + d) =
                     f32x4{o[n][d][i], o[n][d + 1][i], o[n][d + 2][i], o[n][d + 3][i]};
-    }
-    __syncthreads();
-    const bool alone = most <= chunk;
-    for (int idx = threadIdx.x; idx < rows * (HD / 4); idx += kBlk) {
-        const int r = idx / (HD / 4), d = idx % (HD / 4) * 4, i = r / group;
-        const float* from = lds + r * (HD + 4);
-        const int step = rows_most * (HD + 4);
-        float M = -INFINITY;
+        __syncthreads();
+        for (int idx = threadIdx.x; idx < min(rows - 16 * n, 16) * (HD / 4); idx += kBlk) {
+            const int r = 16 * n + idx / (HD / 4), d = idx % (HD / 4) * 4, i = r / group;
+            const float* from = lds + idx / (HD / 4) * (HD + 4);
+            const int step = 16 * (HD + 4);
+            float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) M = fmaxf(M, from[w * step + HD]);
-        float l = 0.f;
-        f32x4 acc{0.f, 0.f, 0.f, 0.f};
+            for (int w = 0; w < kWaves; ++w) M = fmaxf(M, from[w * step + HD]);
+            float l = 0.f;
+            f32x4 acc{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const float m = from[w * step + HD];
-            const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
-            l += from[w * step + HD + 1] * f;
-            acc += *reinterpret_cast<const f32x4*>(from + w * step + d) * f;
-        }
-        const size_t head = (size_t)kvh * group + (r - i * group);
-        if (alone) {
-            const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-            u32x2 w;
-            w.x = f2h_rne(acc.x * inv) | ((uint32_t)f2h_rne(acc.y * inv) << 16);
-            w.y = f2h_rne(acc.z * inv) | ((uint32_t)f2h_rne(acc.w * inv) << 16);
-            *reinterpret_cast<u32x2*>(a.out + (size_t)(s.start + i) * a.out_stride + head * HD + d) = w;
-        } else {
-            const size_t at = ((size_t)(s.start + i) * a.heads + head) * n_splits + split;
-            *reinterpret_cast<f32x4*>(a.workspace + at * HD + d) = acc;
-            if (d == 0) {
-                float* ml = a.workspace + (size_t)a.tokens * a.heads * n_splits * HD + 2 * at;
-                ml[0] = M;
-                ml[1] = l;
+            for (int w = 0; w < kWaves; ++w) {
+                const float m = from[w * step + HD];
+                const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+                l += from[w * step + HD + 1] * f;
+                acc += *reinterpret_cast<const f32x4*>(from + w * step + d) * f;
+            }
+            const size_t head = (size_t)kvh * group + (r - i * group);
+            if (alone) {
+                const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+                u32x2 w;
+                w.x = f2h_rne(acc.x * inv) | ((uint32_t)f2h_rne(acc.y * inv) << 16);
+                w.y = f2h_rne(acc.z * inv) | ((uint32_t)f2h_rne(acc.w * inv) << 16);
+                *reinterpret_cast<u32x2*>(a.out + (size_t)(s.start + i) * a.out_stride + head * HD + d) = w;
+            } else {
+                const size_t at = ((size_t)(s.start + i) * a.heads + head) * n_splits + split;
+                *reinterpret_cast<f32x4*>(a.workspace + at * HD + d) = acc;
+                if (d == 0) {
+                    float* ml = a.workspace + (size_t)a.tokens * a.heads * n_splits * HD + 2 * at;
+                    ml[0] = M;
+                    ml[1] = l;
+                }
             }
         }
     }
@@ -451,13 +478,17 @@ __global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Atten
     int* const nan_at = there_at + 2 * kWaves;                           // [2][4 waves][4 groups of dims]
 
     // kv heads side by side, so that the workgroups of one meet in an XCD's L2
-    // where there are eight of them; row tiles with the most positions first
-    const int kvh = blockIdx.x % c.kv_heads, seq = blockIdx.y, rest = blockIdx.x / c.kv_heads;
-    const int split = rest % n_splits, tile = gridDim.x / (c.kv_heads * n_splits) - 1 - rest / n_splits;
+    // where there are eight of them; row tiles with the most positions first,
+    // every sequence's before the next tile (6 prompts of 100 .. 2500 tokens:
+    // 88 us against 85 with one sequence's tiles after another's, but 29.5 against
+    // 35.1 for two of 761, 43 against 50 for three pieces of 636 behind a prefix)
+    const int kvh = blockIdx.x % c.kv_heads;
+    const int group = a.heads / c.kv_heads, tiles = (a.max_query * group + kRowTile - 1) / kRowTile;
+    const int rest = blockIdx.z * gridDim.y + blockIdx.y, split = rest % n_splits, tile = tiles - 1 - rest / n_splits;
+    const int seq = seq_of(blockIdx.x / c.kv_heads, rest, a.nseq);
     const Kv4Seq s = kv4_seq(a, seq);
-    const int group = a.heads / c.kv_heads, rows = min(s.n, a.max_query) * group;
-    const int row0 = tile * kRowTile;
-    if (row0 >= rows) return;
+    const int rows = min(s.n, a.max_query) * group, row0 = tile * kRowTile;
+    if (tile < 0 || row0 >= rows) return;
     const int most = max(0, s.see((min(rows, row0 + kRowTile) - 1) / group));
     const int c0 = split * chunk, c1 = min(most, c0 + chunk);
     if (c0 >= most && split > 0) return;
@@ -716,12 +747,28 @@ __global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Atten
     }
 }
 
-// The few-row kernel takes up to 32 rows.  Its workgroups take whole turns of
-// their four waves, at most 1024 positions (a lane per page), about eight
-// workgroups per CU where the bound allows.  The prompt kernel splits the
-// positions only where its row tiles leave CUs without work.
-constexpr int kFewRows = 32, kChunkStep = 32 * kWaves, kChunkMost = 1024, kFewBlocks = 1024;
-constexpr int kPromptBlocks = 512, kPromptChunk = 512;
+// us below: 8 kv heads, head_dim 128, wall clock per call.
+// Which kernel: the few-row kernel up to 48 rows, where it beats the prompt
+// kernel from about 300 positions on and does not lose before (16 sequences of
+// 2000 / 6000 positions, few-row against prompt kernel: 32 rows 24 / 39 against
+// 30 / 59, 40 rows 26 / 54 against 32 / 67; built for 64 rows 37 / 82 against
+// 33 / 68).
+constexpr int kFewRows = 48;
+// Its chunks: whole turns of the four waves, as long as leaves one round of
+// resident workgroups (four, three or two per CU for 16, 32 or 48 rows), at
+// most 1024 positions (a lane per page) and at least 256 (16 sequences of 2000
+// positions, 15 rows: chunks of 128 16.3, 256 13.6, 512 13.3).  Short contexts
+// stay in one chunk, without a merge (64 sequences of 4 rows: 512 positions
+// 12.1 against 20.9 in chunks, 768 15.3 against 23.7; one sequence of 42 rows and
+// 512 positions 14.1 against 13.0, 768 17.4 against 13.5).
+constexpr int kChunkStep = 32 * kWaves, kChunkLeast = 256, kChunkMost = 1024, kFewBlocks = 1024;
+constexpr int kAlone = 768, kAloneWide = 512;   // positions of one chunk, up to 16 rows and above
+// The prompt kernel splits the positions only where its row tiles leave CUs
+// without work: chunks of 192 on up to one workgroup per CU, of 512 up to two
+// (64 rows of 600 positions 15.2, 21.2 with 512 alone; 4 sequences of 64 rows and
+// 1000 positions 16.3, 33.0; 2 prompts of 500 x 4 rows behind 500 positions, which
+// fill the CUs, 34.9, and 46.3 with 192 up to two).
+constexpr int kPromptBlocks = 256, kPromptChunk = 192, kPromptChunkFull = 512;
 struct Kv4Plan {
     bool few;
     int cols, tiles, chunk, n_splits;
@@ -730,16 +777,21 @@ Kv4Plan kv4_plan(int max_context, int max_query, int nseq, int heads, int kv_hea
     Kv4Plan p{};
     const long long rows = (long long)max_query * (heads / kv_heads);
     p.few = rows <= kFewRows;
-    p.cols = rows <= 16 ? 1 : 2;
+    p.cols = p.few ? (int)(rows + 15) / 16 : 0;
     p.tiles = (int)((rows + kRowTile - 1) / kRowTile);
+    auto whole = [](long long positions, int step) { return (int)((positions + step - 1) / step * step); };
     if (p.few) {
-        const long long want = ((long long)max_context * nseq * kv_heads + kFewBlocks - 1) / kFewBlocks;
-        p.chunk = (int)std::min<long long>(kChunkMost, std::max<long long>(1, (want + kChunkStep - 1) / kChunkStep) * kChunkStep);
+        const int blocks = p.cols == 1 ? kFewBlocks : p.cols == 2 ? kFewBlocks * 3 / 4 : kFewBlocks / 2;
+        const long long share = ((long long)max_context * nseq * kv_heads + blocks - 1) / blocks;
+        p.chunk = max_context <= (p.cols == 1 ? kAlone : kAloneWide)
+                      ? whole(max_context, kChunkStep)
+                      : whole(std::max<long long>(kChunkLeast, std::min<long long>(kChunkMost, share)), kChunkStep);
     } else {
         const long long blocks = (long long)p.tiles * kv_heads * nseq;
-        const long long splits = std::max<long long>(1, std::min<long long>(kPromptBlocks / blocks, max_context / kPromptChunk));
-        p.chunk = (int)((max_context + splits - 1) / splits);
-        p.chunk = (p.chunk + kTile - 1) / kTile * kTile;
+        auto least = [&](long long most, int chunk) { return std::min<long long>(most / blocks, max_context / chunk); };
+        const long long splits =
+            std::max({1ll, least(kPromptBlocks, kPromptChunk), least(2 * kPromptBlocks, kPromptChunkFull)});
+        p.chunk = whole((max_context + splits - 1) / splits, kTile);
     }
     p.n_splits = (max_context + p.chunk - 1) / p.chunk;
     return p;
@@ -753,22 +805,25 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
     const bool last = p.n_splits == 1;
     if (!p.few) {
         const int lds = 4 * HD * kTile * (int)sizeof(uint16_t) + 2 * kWaves * 5 * (int)sizeof(int);
+        const int units = p.tiles * p.n_splits, y = std::min(units, 32768);   // at most 65535 in y
         const hipError_t e = allow_lds<kv4_prompt_kernel<HD>>(lds);
         if (e != hipSuccess) return e;
-        launch_kernel_in_call(last, kv4_prompt_kernel<HD>, dim3(c.kv_heads * p.tiles * p.n_splits, a.nseq), dim3(kBlk), lds, s,
-                              c, a, p.chunk, p.n_splits, scale_log2);
+        const dim3 grid(c.kv_heads * a.nseq, y, (units + y - 1) / y);
+        launch_kernel_in_call(last, kv4_prompt_kernel<HD>, grid, dim3(kBlk), lds, s, c, a, p.chunk, p.n_splits,
+                              scale_log2);
     } else {
         const dim3 grid(c.kv_heads * a.nseq, p.n_splits);
-        const int lds = kWaves * a.max_query * group * (HD + 4) * (int)sizeof(float);
-        if (p.cols == 1) {
-            launch_kernel_in_call(last, kv4_decode_kernel<HD, 1>, grid, dim3(kBlk), lds, s, c, a, p.chunk, p.n_splits,
-                                  scale_log2);
-        } else {
-            const hipError_t e = allow_lds<kv4_decode_kernel<HD, 2>>(lds);
-            if (e != hipSuccess) return e;
-            launch_kernel_in_call(last, kv4_decode_kernel<HD, 2>, grid, dim3(kBlk), lds, s, c, a, p.chunk, p.n_splits,
-                                  scale_log2);
-        }
+        const int lds = std::max(kWaves * 16 * (HD + 4) * (int)sizeof(float),
+                                 p.cols > 1 ? p.cols * (HD / 32) * kWave * 16 : 0);
+        auto go = [&](auto kernel) {
+            launch_kernel_in_call(last, kernel, grid, dim3(kBlk), lds, s, c, a, p.chunk, p.n_splits, scale_log2);
+        };
+        if (p.cols == 1)
+            go(kv4_decode_kernel<HD, 1>);
+        else if (p.cols == 2)
+            go(kv4_decode_kernel<HD, 2>);
+        else
+            go(kv4_decode_kernel<HD, 3>);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || last) return e;
@@ -776,11 +831,11 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
     const long long units = (long long)a.max_query * a.heads;
     const int tile_rows = p.few ? kFewRows : kRowTile;
     if (p.n_splits <= 4 * kWave / (HD / 4))
-        launch_kernel(kv4_merge_kernel<HD, 1>, dim3((unsigned)((units + kWaves - 1) / kWaves), a.nseq), dim3(kBlk), 0, s, a,
-                      group, tile_rows, p.chunk, p.n_splits);
+        launch_kernel(kv4_merge_kernel<HD, 1>, dim3((unsigned)((units + kWaves - 1) / kWaves), a.nseq), dim3(kBlk), 0, s,
+                      a, group, tile_rows, p.chunk, p.n_splits);
     else
-        launch_kernel(kv4_merge_kernel<HD, kWaves>, dim3((unsigned)units, a.nseq), dim3(kBlk), 0, s, a, group, tile_rows,
-                      p.chunk, p.n_splits);
+        launch_kernel(kv4_merge_kernel<HD, kWaves>, dim3((unsigned)units, a.nseq), dim3(kBlk), 0, s, a, group,
+                      tile_rows, p.chunk, p.n_splits);
     return hipGetLastError();
 }
 

@@ -108,7 +108,11 @@ def test_a_large_weight_beside_small_ones(hip):
     (16, 2, 128, 64, [300, 129], [129, 65]),                  # chunks behind a prefix
     (6, 2, 128, 128, [513], [200]),
     (32, 2, 64, 16, [90, 20], [31, 20]),
-    (5, 5, 128, 16, [70, 300], [70, 40])])
+    (5, 5, 128, 16, [70, 300], [70, 40]),
+    (14, 2, 128, 16, [40, 7, 1300], [6, 7, 5]),               # 33 to 64 rows of a kv head
+    (16, 2, 64, 32, [100, 2100, 5], [5, 4, 5]),
+    (8, 2, 128, 128, [640, 64, 15], [16, 12, 15]),
+    (3, 3, 64, 16, [900, 61], [64, 61])])
 def test_several_queries(hip, heads, kv, hd, page, lens, asked):
     Batch(hip, sum(lens), heads, kv, hd, page, lens, asked, behind=3).upload().launch().check()
 
@@ -175,7 +179,8 @@ def _nan_tokens(b, where):
 
 
 @pytest.mark.parametrize("hd,page", [(128, 16), (64, 64)])
-@pytest.mark.parametrize("heads,kv,asked", [(8, 2, [4, 2, 3]), (8, 2, [8, 1, 5]), (8, 2, [70, 9, 200])])
+@pytest.mark.parametrize("heads,kv,asked", [(8, 2, [4, 2, 3]), (8, 2, [8, 1, 5]), (8, 2, [12, 9, 16]),
+                                            (8, 2, [70, 9, 200])])
 def test_a_nan_is_kept_from_the_queries_before_it(hip, heads, kv, asked, hd, page):
     """NaN keys and values at positions that the last queries see and the first
     ones do not: the first ones' results are those of a cache without them."""
