@@ -70,6 +70,12 @@ __device__ __forceinline__ void both(uint32_t v, uint32_t& a, uint32_t& b) {
 }
 // Larger of a lane's and its partner's key where `up`, else the smaller.
 template <int kStride>
+__device__ __forceinline__ uint32_t exchange(uint32_t v, bool up) {
+    uint32_t a, b;
+    both<kStride>(v, a, b);
+    return (a > b) == up ? a : b;
+}
+template <int kStride>
 __device__ __forceinline__ uint64_t exchange(uint64_t v, bool up) {
     uint32_t a0, a1, b0, b1;
     both<kStride>((uint32_t)v, a0, b0);
@@ -79,13 +85,14 @@ __device__ __forceinline__ uint64_t exchange(uint64_t v, bool up) {
 }
 // The steps kStride, kStride / 2, .. 1 of a bitonic merge; each run of kSize
 // lanes descends where `down`.
-template <int kStride>
-__device__ __forceinline__ uint64_t merge_steps(uint64_t v, int lane, bool down) {
+template <int kStride, typename T>
+__device__ __forceinline__ T merge_steps(T v, int lane, bool down) {
     v = exchange<kStride>(v, ((lane & kStride) == 0) == down);
     if constexpr (kStride > 1) v = merge_steps<kStride / 2>(v, lane, down);
     return v;
 }
-__device__ __forceinline__ uint64_t sort_descending(uint64_t v, int lane) {
+template <typename T>
+__device__ __forceinline__ T sort_descending(T v, int lane) {
     v = merge_steps<1>(v, lane, (lane & 2) == 0);
     v = merge_steps<2>(v, lane, (lane & 4) == 0);
     v = merge_steps<4>(v, lane, (lane & 8) == 0);
@@ -111,6 +118,20 @@ __device__ __forceinline__ int hidden(int lane) {
     return lane;
 }
 
+// v[i] for an i of the lane's own.
+template <typename T>
+__device__ __forceinline__ T pick(const T (&v)[kPer], int i) {
+    T a[kPer / 2];
+    auto half = [](bool second, T x, T y) { return second ? y : x; };   // of values: the array stays in registers
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] = half(i & 1, v[2 * j], v[2 * j + 1]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a[j] = half(i & 2, a[2 * j], a[2 * j + 1]);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) a[j] = half(i & 4, a[2 * j], a[2 * j + 1]);
+    return half(i & 8, a[0], a[1]);
+}
+
 struct TopKeys {
     uint64_t mine = 0;    // lane i: the i-th largest
     uint64_t floor = 0;   // only keys above it can be among the k largest (uniform)
@@ -119,34 +140,64 @@ struct TopKeys {
     uint64_t* room;       // 64 of LDS, the wave's own
     int lane, k;
 
+    __device__ uint64_t least() const { return floor > theirs ? floor : theirs; }
     __device__ void flush() {
         wave_lds_sync();
         const uint64_t v = lane < waiting ? room[lane] : 0ull;
         wave_lds_sync();
         const int at = hidden(lane);
-        mine = merge_descending(mine, sort_descending(v, at), at);
+        const uint64_t sorted = sort_descending(v, at);
+        mine = lane_key(mine, 0) == 0 ? sorted : merge_descending(mine, sorted, at);
         const uint64_t kth = lane_key(mine, k - 1);
         floor = kth > floor ? kth : floor;
         waiting = 0;
     }
     __device__ void add(uint64_t key) {
-        const uint64_t least = floor > theirs ? floor : theirs;
-        uint64_t who = __builtin_amdgcn_ballot_w64(key > least);
+        const uint64_t low = least();
+        uint64_t who = __builtin_amdgcn_ballot_w64(key > low);
         if (who == 0) return;
         if (waiting + __popcll(who) > kWave) {
             flush();
-            who = __builtin_amdgcn_ballot_w64(key > least);
+            who = __builtin_amdgcn_ballot_w64(key > least());
         }
-        if (key > least)
-            room[waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] =
-                key;
+        if (key > least()) room[waiting + below(who)] = key;
         waiting += __popcll(who);
     }
-    // Before many keys at once, of which `best` are the lanes' largest: at
-    // least k of them reach the k-th largest of those.
-    __device__ void raise(uint64_t best) {
-        const uint64_t kth = lane_key(sort_descending(best, hidden(lane)), k - 1);
-        if (kth > floor) floor = kth - 1;
+    // The keys key_of(i) of the lane's marks (one not above least() does no harm).
+    template <typename F>
+    __device__ void add_marked(uint32_t marks, F key_of) {
+        const int count = __builtin_popcount(marks);
+        int before = 0, total = 0;   // over the lanes, the counts' bits in turn
+#pragma unroll
+        for (int b = 0; 1 << b <= kPer; ++b) {
+            const uint64_t who = __builtin_amdgcn_ballot_w64((count >> b & 1) != 0);
+            before += below(who) << b;
+            total += __popcll(who) << b;
+        }
+        const bool fits = waiting + total <= kWave;
+        int at = waiting + before;
+        waiting += fits ? total : 0;
+        while (__builtin_amdgcn_ballot_w64(marks != 0) != 0) {   // a key of each lane
+            const uint64_t key = marks != 0 ? key_of(__builtin_ctz(marks)) : 0ull;
+            if (!fits)
+                add(key);
+            else if (marks != 0)
+                room[at++] = key;
+            marks &= marks - 1;
+        }
+    }
+    // Before many keys at once, of which `best` are the lanes' largest (their
+    // upper halves): at least k of them reach the k-th largest of those.
+    __device__ void raise(uint32_t best) {
+        const uint64_t kth = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)sort_descending(best, hidden(lane)), k - 1)
+                             << 32;
+        floor = kth > floor ? kth : floor;
+    }
+
+private:
+    // lanes of `who` below this one
+    __device__ static int below(uint64_t who) {
+        return __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
     }
 };
 
@@ -342,46 +393,33 @@ __global__ __launch_bounds__(kBlk) void logprobs_kernel(Logprobs a, int splits, 
             }
         }
         if (a.top_k) {
-            // ids only grow, so a later logit equal to the k-th is not above it
             uint64_t theirs = 0;
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) theirs = others[w] > theirs ? others[w] : theirs;
             top.theirs = lane_key(theirs, 0);
-            // (one equal to another wave's may be, by its id)
-            const uint64_t over = __builtin_amdgcn_ballot_w64((top.floor == 0 || largest > key_logit(top.floor)) &&
-                                                              (top.theirs == 0 || largest >= key_logit(top.theirs)));
+            // the least logit of a key above least(); an equal one only where its id may be lower
+            auto limit = [&] {
+                const uint64_t least = top.least();
+                const uint64_t next = (uint64_t)((uint32_t)id0 >= ~(uint32_t)least) << 32;
+                return least == 0 ? -INFINITY : key_logit(least + next);
+            };
+            float low = limit();
+            // (beside a NaN `largest` may miss a logit: a signalling one makes the
+            // maximum a NaN, whatever came before)
+            const uint64_t over = __builtin_amdgcn_ballot_w64(largest >= low || sums.s != sums.s);
             if (over != 0) {
-                const bool many = __popcll(over) > 16;
-                if (many) {
-                    uint64_t best = 0;
-#pragma unroll
-                    for (int i = 0; i < kPer; ++i) {
-                        const uint64_t key = logit_key((float)x.at(i), id_of(i));
-                        best = key > best ? key : best;
-                    }
-                    top.raise(best);
+                if (__popcll(over) > 16) {
+                    top.raise((uint32_t)(logit_key(largest, 0) >> 32));
+                    low = limit();
                 }
-                // registers i with a candidate, each added in turn
-                uint32_t todo = 0;
-                if (many || top.floor == 0) {   // the k-th may be among them
-                    const float least = top.floor == 0 ? -INFINITY : key_logit(top.floor);
+                float v[kPer];
+                uint32_t marks = 0;
 #pragma unroll
-                    for (int i = 0; i < kPer; ++i)
-                        todo |= (__builtin_amdgcn_ballot_w64((float)x.at(i) >= least) != 0 ? 1u : 0u) << i;
-                } else {
-                    const float least = key_logit(top.floor);
-#pragma unroll
-                    for (int i = 0; i < kPer; ++i)
-                        todo |= (__builtin_amdgcn_ballot_w64((float)x.at(i) > least) != 0 ? 1u : 0u) << i;
+                for (int i = 0; i < kPer; ++i) {
+                    v[i] = (float)x.at(i);
+                    marks |= (v[i] >= low ? 1u : 0u) << i;
                 }
-                while (todo != 0) {
-                    const int i = __builtin_ctz(todo);
-                    todo &= todo - 1;
-                    float xi = (float)x.at(0);
-#pragma unroll
-                    for (int j = 1; j < kPer; ++j) xi = i == j ? (float)x.at(j) : xi;
-                    top.add(logit_key(xi, id_of(i)));
-                }
+                top.add_marked(marks, [&](int i) { return logit_key(pick(v, i), id_of(i)); });
                 if (lane == 0) __hip_atomic_store(&floors[wave], top.floor, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
             }
         }
@@ -459,9 +497,11 @@ __global__ __launch_bounds__(kWave) void logprobs_join_kernel(Logprobs a, int sp
             }
 #pragma unroll
             for (int i = 0; i < kPer; ++i) best = key[i] > best ? key[i] : best;
-            top.raise(best);
+            top.raise((uint32_t)(best >> 32));
+            uint32_t marks = 0;
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) top.add(key[i]);
+            for (int i = 0; i < kPer; ++i) marks |= (key[i] > top.least() ? 1u : 0u) << i;
+            top.add_marked(marks, [&](int i) { return pick(key, i); });
         }
         top.flush();
     }

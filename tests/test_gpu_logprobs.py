@@ -167,6 +167,8 @@ def test_signalling_nans_hide_no_logit(hip, half):
         bits[r, rng.random(9001) < 0.5] = nan
         bits[r + 3, 1::2] = nan
     _check(hip, x, [5, 6, 7, 8, 9, 10], 40)
+    many = np.tile(x.view(bits.dtype), (171, 1)).view(x.dtype)        # a wave has several steps of a row
+    _check(hip, many, rng.integers(0, 9001, len(many)), 40)
 
 
 @pytest.mark.parametrize("rows,vocab", [(1, 151936), (9, 32000), (1100, 5000)])
