@@ -763,7 +763,8 @@ constexpr int kMaxVocab = 1 << 30;       // ids and what is rounded up from them
 }  // namespace
 
 CITLALI_EXPORT size_t citlali_hip_token_logprobs_workspace_bytes(int rows, int vocab, int top_k) {
-    if (rows <= 0 || rows > kMaxLogitRows || vocab <= 0 || vocab > kMaxVocab || top_k < 0 || top_k > CITLALI_MAX_TOP_LOGPROBS) return 0;
+    if (rows <= 0 || rows > kMaxLogitRows || vocab <= 0 || vocab > kMaxVocab) return 0;
+    if (top_k < 0 || top_k > CITLALI_MAX_TOP_LOGPROBS) return 0;
     return logprobs_workspace(rows, vocab, top_k);
 }
 

@@ -61,40 +61,43 @@ __device__ __forceinline__ double inv_root(double x) {
     return fma(0.5 * r, fma(-x * r, r, 1.0), r);
 }
 
-// The eight normed and rotated values of a lane, computed in T and rounded to
-// fp32.  Lane l of the LR that share a head row holds dims 8 l .. 8 l + 7; its
-// rotation partner, LR / 2 lanes away, holds the dims head_dim / 2 away.  wx,
-// wp: the norm's weights of both (ones without a norm); cs: cosines and sines
-// of the eight pairs.  Value times weight is exact in fp32 (two fp16 numbers),
-// and the norm's factor comes last: y = inv (x w_x cos -+ p w_p sin).
+// Norm and rotation of a lane's eight values, in T.  Lane l of the LR that share
+// a head row holds dims 8 l .. 8 l + 7; its rotation partner, LR / 2 lanes away,
+// holds the dims head_dim / 2 away.  y = inv (x a + p b), inv the norm's factor,
+// a = w_x cos and b = -+ w_p sin once for all heads (wx, wp: the norm's weights of
+// both lanes, ones without a norm; cs: cosines and sines of the eight pairs).
+// In 64 bits a, b and x a are exact.
 template <typename T, int HD>
-__device__ __forceinline__ void norm_rotate(u32x4 raw, bool norm, u32x4 wx, u32x4 wp, float eps, const float2 (&cs)[8],
-                                            int l, float (&y)[8]) {
-    constexpr int LR = HD / 8;
-    u32x4 other;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) other[i] = partner<LR>(raw[i]);
-    T inv = 1;
-    if (norm) {
-        T s = 0;
+struct Rotation {
+    static constexpr int LR = HD / 8;
+    T a[8], b[8];
+    __device__ Rotation(const float2 (&cs)[8], u32x4 wx, u32x4 wp, int l) {
+        const uint32_t flip = l < LR / 2 ? 0x80000000u : 0u;   // the lower half of the pairs takes - sin
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const T x = (T)(float)half_at(raw, i);
-            s += x * x;
+            a[i] = (T)(float)half_at(wx, i) * (T)cs[i].x;
+            b[i] = (T)(float)half_at(wp, i) * (T)__uint_as_float(__float_as_uint(cs[i].y) ^ flip);
         }
-        inv = inv_root(row_sum<LR>(s) * (T)(1.0 / HD) + (T)eps);
     }
-    // the lower half of the pairs takes - sin
-    const uint32_t flip = l < LR / 2 ? 0x80000000u : 0u;
+    __device__ void operator()(u32x4 raw, bool norm, float eps, float (&y)[8]) const {
+        u32x4 other;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float x = (float)half_at(raw, i) * (float)half_at(wx, i);
-        const float p = (float)half_at(other, i) * (float)half_at(wp, i);
-        const float sn = __uint_as_float(__float_as_uint(cs[i].y) ^ flip);
-        y[i] = (float)(inv * ((T)x * (T)cs[i].x + (T)p * (T)sn));
-        __builtin_amdgcn_sched_barrier(0);   // one at a time: few 64-bit numbers live
+        for (int i = 0; i < 4; ++i) other[i] = partner<LR>(raw[i]);
+        T inv = 1;
+        if (norm) {
+            T s = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const T x = (T)(float)half_at(raw, i);
+                s += x * x;
+            }
+            inv = inv_root(row_sum<LR>(s) * (T)(1.0 / HD) + (T)eps);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            y[i] = (float)(inv * ((T)(float)half_at(raw, i) * a[i] + (T)(float)half_at(other, i) * b[i]));
     }
-}
+};
 
 // Codes of a lane's eight values, four to a number: lo has those of values 0
 // .. 3 (or, kEven, of 0 2 4 6) from the low bits on, hi the others.  d and m
@@ -154,9 +157,10 @@ __device__ __forceinline__ void quantise(const float (&y)[8], uint32_t& lo, uint
 // One wave takes `per` heads (all query, key or value heads) of 512 / HD
 // consecutive tokens, 16 bytes a lane and head, the next head's on their way:
 // the rotation's 64 bytes a lane, four times a head's, are read once for all.
-// 8192 tokens of 32/8 heads move 182 MB in 52.6 us (3.5 TB/s) against vector
-// work of about the same length; few tokens are bound by the chain position ->
-// table -> head.
+// Bound by HBM: 8192 tokens of 32/8 heads move 182 MB in 43.7 us (4.2 TB/s; a
+// copy of as many bytes takes 36), with the streams read and written
+// nontemporal (4 us more without); few tokens (250: 4.8 us, one: 3.6) by the
+// chain position -> table -> head.
 template <int HD>
 __global__ __launch_bounds__(kBlk) void kv4_append_kernel(Kv4View c, Kv4Append a, int per) {
     constexpr int LR = HD / 8, kRows = kWave / LR;
@@ -207,42 +211,52 @@ __global__ __launch_bounds__(kBlk) void kv4_append_kernel(Kv4View c, Kv4Append a
     }
 
     u32x4 next = *reinterpret_cast<const u32x4*>(src + (size_t)h0 * HD);
-#pragma unroll 1
-    for (int h = h0; h < h1; ++h) {
+    auto head = [&](int h) {   // head h; the next one's are on their way
         const u32x4 raw = next;
-        next = *reinterpret_cast<const u32x4*>(src + (size_t)min(h + 1, h1 - 1) * HD);
-        if (is_q) {
-            float y[8];
-            norm_rotate<float, HD>(raw, w != nullptr, wx, wp, a.eps, cs, l, y);
-            if (known) {
-                u32x4 out;
+        const uint16_t* ahead = src + (size_t)min(h + 1, h1 - 1) * HD;
+        next = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(ahead));
+        return raw;
+    };
+    float y[8];
+    if (is_q) {
+        const Rotation<float, HD> rotate(cs, wx, wp, l);
+#pragma unroll 1
+        for (int h = h0; h < h1; ++h) {
+            rotate(head(h), w != nullptr, a.eps, y);
+            if (!known) continue;
+            u32x4 out;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    out[i] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)y[2 * i], (_Float16)y[2 * i + 1]});
-                *reinterpret_cast<u32x4*>(a.q_out + row * a.q_out_stride + (size_t)h * HD + 8 * l) = out;
-            }
-            continue;
+            for (int i = 0; i < 4; ++i)
+                out[i] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)y[2 * i], (_Float16)y[2 * i + 1]});
+            uint16_t* to = a.q_out + row * a.q_out_stride + (size_t)h * HD + 8 * l;
+            __builtin_nontemporal_store(out, reinterpret_cast<u32x4*>(to));
         }
-        uint8_t* base = kv4_head<HD>(c, kept ? slot >> c.page_shift : 0, h);
-        float y[8];
-        uint32_t lo, hi, d16, m16;
-        if (!is_v) {
-            // widened here, for each head: 64 registers less to keep
-#pragma unroll
-            for (int i = 0; i < 8; ++i) asm("" : "+v"(cs[i].x), "+v"(cs[i].y));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) asm("" : "+v"(wx[i]), "+v"(wp[i]));
-            norm_rotate<double, HD>(raw, w != nullptr, wx, wp, a.eps, cs, l, y);
+        return;
+    }
+    uint32_t lo, hi, d16, m16;
+    uint8_t* const page = kv4_head<HD>(c, kept ? slot >> c.page_shift : 0, 0);
+    const size_t head_bytes = (size_t)L::kToken << c.page_shift;
+    if (!is_v) {
+        const Rotation<double, HD> rotate(cs, wx, wp, l);
+#pragma unroll 1
+        for (int h = h0; h < h1; ++h) {
+            rotate(head(h), w != nullptr, a.eps, y);
             quantise<true>(y, lo, hi, d16, m16);
             if (!kept) continue;
+            uint8_t* base = page + h * head_bytes;
             *reinterpret_cast<uint32_t*>(base + o * L::kCodes + 4 * l) = lo | (hi << 16);
             if ((l & 3) == 0)
                 *reinterpret_cast<uint32_t*>(base + L::k_params(P) + o * L::kParams + l) = d16 | (m16 << 16);
-            continue;
         }
+        return;
+    }
+#pragma unroll 1
+    for (int h = h0; h < h1; ++h) {
+        const u32x4 raw = head(h);
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = (float)half_at(raw, i);
         quantise<false>(y, lo, hi, d16, m16);   // dims 8 l .. and 8 l + 4 ..
+        uint8_t* base = page + h * head_bytes;
         uint16_t* vc = reinterpret_cast<uint16_t*>(base + L::v_codes(P)) + (o >> 2) * HD;
         if (pairs) {
             // row r gets both tokens' quad r & 1 (see swap16)
@@ -330,12 +344,12 @@ unsigned blocks_for(long long rows, int head_dim, long long heads) {
 }
 }  // namespace
 
-// Heads of a wave: as many of 16, 8, 4 or 2 as leave four waves per SIMD, else
-// one.  8192 tokens of 32/8 heads: 52.6 us with 16, 54.2 with 8, 57.7 with 4.
+// Heads of a wave: as many of 8, 4 or 2 as leave four waves per SIMD, else one.
+// 8192 tokens of 32/8 heads: 45.2 us with 16, 43.7 with 8, 48.4 with 4.
 hipError_t launch_kv4_append(const Kv4View& c, const Kv4Append& a, hipStream_t s) {
     const long long groups = (a.tokens + 512 / c.head_dim - 1) / (512 / c.head_dim);
     auto waves = [&](int per) { return groups * ((a.heads + per - 1) / per + 2 * ((c.kv_heads + per - 1) / per)); };
-    int per = 16;
+    int per = 8;
     while (per > 1 && waves(per) < kEnoughWaves) per /= 2;
     const dim3 grid((unsigned)((waves(per) + kBlk / kWave - 1) / (kBlk / kWave)));
     if (c.head_dim == 128)
