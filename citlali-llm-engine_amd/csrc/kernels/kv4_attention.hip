@@ -60,7 +60,8 @@ __device__ __forceinline__ uint32_t kv4_hide_nan(u32x4& dm) {
 // The sequence of workgroup x (of a layer of nseq sequences).  An XCD deals its
 // workgroups to its four shader engines in strict turn, those without work
 // too, so a sequence's place has to change from layer to layer: by nseq where
-// that is odd, else by one more.
+// that is odd, else by one more (16 long contexts 87.7 -> 82.0 us, 24 sequences
+// of 20 rows 40.3 -> 36.8).
 __device__ __forceinline__ int seq_of(int x, int layer, int nseq) {
     return (x + (nseq & 1 ? 0 : layer)) % nseq;
 }
@@ -89,8 +90,12 @@ constexpr float kShift = 14.f;   // weights are kept times 2^14 (base 2)
 //    four tokens, so lane (c, grp) loads the codes of its four positions and
 //    HD / 16 dims together, each word two positions' dims, and gets the A
 //    operand's pairs without a transposition.
-// Bound by the cache's bytes: 5 KB a tile of head_dim 128 against about 300
-// vector instructions, a good half of what a CU issues meanwhile at 6 TB/s.
+// Bound by the cache's bytes, next by the vector unit (about 300 instructions a
+// tile of 5 KB at head_dim 128, 215 a tile of 2.5 KB at 64) and the round trips
+// of a workgroup's start.  32/8 heads of 128: 16 sequences of 4096 .. 32768
+// positions, 403 MB, in 78 us (5.1 TB/s), 64 of 200 .. 4000, 174 MB, in 38.7 (4.5);
+// 20 rows, 24 sequences of 500 .. 6000, 101 MB, in 31.0; 16/8 heads of 64, 100
+// sequences of 150 .. 1500, 52.6 MB, in 18.6.
 // ---------------------------------------------------------------------------
 template <int HD, int kCols>
 __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4_decode_kernel(
@@ -369,7 +374,9 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4
 // lanes read a chunk's sums 16 bytes each, the teams of a wave (and the waves)
 // take different chunks, kBatch at once.  The first batch is read before the
 // number of chunks is known (all lie in the workspace), so that the kernel is
-// one round trip behind the lengths.
+// one round trip behind the lengths.  Up to 8 chunks (head_dim 64: 16) it takes 3.2
+// to 4.7 us by one wave, by four 3.6 to 7.3; 32 chunks of 16 x 32 heads 4.7 by four,
+// 6.4 by one.
 template <int HD, int kTeam>
 __global__ __launch_bounds__(kBlk) void kv4_merge_kernel(Kv4Attention a, int group, int tile_rows, int chunk,
                                                          int n_splits) {
@@ -458,7 +465,11 @@ __global__ __launch_bounds__(kBlk) void kv4_merge_kernel(Kv4Attention a, int gro
 //  * V's dim HD/16 c + n lies at 16 n + c, so that the 16 lanes that write one n
 //    use different banks.
 //  * the maximum a row's weights refer to moves only when it is exceeded by
-//    kSlack (base 2), which spares O its rescaling in most tiles.
+//    kSlack (base 2), which spares O its rescaling in most tiles (583 us below,
+//    599 without).
+// 2048 queries behind 14336 positions, 32/8 heads of 128 (515 GFLOP): 583 us, 883
+// TFLOP/s (a large fp16 product: 1162); of 631 us of an early form the products
+// alone took 330, and 256 rows by eight waves as long as 128 by four.
 // ---------------------------------------------------------------------------
 constexpr int kRowTile = 128, kTile = 64;   // rows of a workgroup; positions of a step
 constexpr float kSlack = 4.f;
@@ -831,8 +842,8 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
     const long long units = (long long)a.max_query * a.heads;
     const int tile_rows = p.few ? kFewRows : kRowTile;
     if (p.n_splits <= 4 * kWave / (HD / 4))
-        launch_kernel(kv4_merge_kernel<HD, 1>, dim3((unsigned)((units + kWaves - 1) / kWaves), a.nseq), dim3(kBlk), 0, s,
-                      a, group, tile_rows, p.chunk, p.n_splits);
+        launch_kernel(kv4_merge_kernel<HD, 1>, dim3((unsigned)((units + kWaves - 1) / kWaves), a.nseq), dim3(kBlk), 0,
+                      s, a, group, tile_rows, p.chunk, p.n_splits);
     else
         launch_kernel(kv4_merge_kernel<HD, kWaves>, dim3((unsigned)units, a.nseq), dim3(kBlk), 0, s, a, group,
                       tile_rows, p.chunk, p.n_splits);

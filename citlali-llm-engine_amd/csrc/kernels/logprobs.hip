@@ -10,13 +10,18 @@
 //
 // The most likely tokens are kept as 64-bit keys (ordered bits of the logit,
 // then the complement of the id, so that equal logits go by the lower id):
-// lane i of a wave has the wave's i-th largest.  Logits below the k-th cost one
-// comparison per 16; those above it are gathered in LDS, and 64 of them are
-// sorted across the lanes and merged at a time.  The order is total, so the
+// lane i of a wave has the wave's i-th largest.  Logits below the k-th, the
+// wave's own or another's of the workgroup, cost one comparison per 16; those
+// above it are gathered in LDS, and 64 of them are sorted across the lanes and
+// merged at a time.  Where many lanes have one (a row's first steps), a sort of
+// the lanes' largest raises the threshold first.  The order is total, so the
 // result does not depend on the cut.
 //
-// Bound by reading the logits; beside them a wave issues about 8 vector
-// instructions per 64 logits, one of them the exponential.
+// Bound by reading the logits where there are many rows: 2048 rows of 151936
+// fp16 logits, 622 MB, in 122 us (5.1 TB/s); beside them a wave issues about 8
+// vector instructions per 64 logits, one of them the exponential.  A few rows
+// are a chain of latencies, the sorts its longest part: 8 rows 7.8 us and the
+// join of their pieces 4.6.
 #include "device_common.hpp"
 #include "launch.hpp"
 
@@ -189,8 +194,8 @@ struct TopKeys {
     // Before many keys at once, of which `best` are the lanes' largest (their
     // upper halves): at least k of them reach the k-th largest of those.
     __device__ void raise(uint32_t best) {
-        const uint64_t kth = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)sort_descending(best, hidden(lane)), k - 1)
-                             << 32;
+        const uint32_t reach = __builtin_amdgcn_readlane((int)sort_descending(best, hidden(lane)), k - 1);
+        const uint64_t kth = (uint64_t)reach << 32;
         floor = kth > floor ? kth : floor;
     }
 
@@ -301,8 +306,8 @@ struct RowEnd {
     __device__ RowEnd(Sums v) : m(v.m), log_s(v.s == 0.f ? NAN : logf(v.s)) {}
     __device__ float logprob(float x) const { return x - m - log_s; }
 };
-__device__ __forceinline__ void write_row(const Logprobs& a, int r, Sums v, int rank, uint64_t top, int lane, float mine,
-                                          bool given) {
+__device__ __forceinline__ void write_row(const Logprobs& a, int r, Sums v, int rank, uint64_t top, int lane,
+                                          float mine, bool given) {
     const RowEnd end(v);
     if (lane == 0) {
         if (a.entropies) a.entropies[r] = end.log_s - kLn2 * (v.t / v.s);
@@ -420,7 +425,8 @@ __global__ __launch_bounds__(kBlk) void logprobs_kernel(Logprobs a, int splits, 
                     marks |= (v[i] >= low ? 1u : 0u) << i;
                 }
                 top.add_marked(marks, [&](int i) { return logit_key(pick(v, i), id_of(i)); });
-                if (lane == 0) __hip_atomic_store(&floors[wave], top.floor, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                if (lane == 0)
+                    __hip_atomic_store(&floors[wave], top.floor, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
             }
         }
     }
@@ -509,14 +515,17 @@ __global__ __launch_bounds__(kWave) void logprobs_join_kernel(Logprobs a, int sp
 }
 
 // Pieces of a row: about four workgroups per CU over all rows, each wave with a
-// whole step at least.
-constexpr int kTargetBlocks = 1024;
+// whole step at least; rows as many as CUs stay whole.  us for 151936 fp32 logits,
+// 20 listed: 8 rows 12.9 with one step a wave, 14.3 with two, 18.5 with four; 100
+// rows 27.4 (half or twice as many workgroups 27.6, 28.9), 200 rows of fp16 34.1
+// (40.9); 300 rows whole 45.8, in three pieces 48.6, 500 rows 52.2, in two 64.6.
+constexpr int kTargetBlocks = 1024, kWholeRows = 256;
 struct Cut {
     int splits, per_wave;
 };
 Cut cut_row(int rows, int vocab) {
     const int steps = std::max(1, (vocab + kStep - 1) / kStep);
-    const int want = std::max(1, std::min((steps + kWaves - 1) / kWaves, kTargetBlocks / std::min(rows, kTargetBlocks)));
+    const int want = rows > kWholeRows ? 1 : std::min((steps + kWaves - 1) / kWaves, kTargetBlocks / rows);
     Cut c;
     c.per_wave = (steps + want * kWaves - 1) / (want * kWaves);
     c.splits = (steps + c.per_wave * kWaves - 1) / (c.per_wave * kWaves);
