@@ -824,8 +824,8 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
                               scale_log2);
     } else {
         const dim3 grid(c.kv_heads * a.nseq, p.n_splits);
-        const int lds = std::max(kWaves * 16 * (HD + 4) * (int)sizeof(float),
-                                 p.cols > 1 ? p.cols * (HD / 32) * kWave * 16 : 0);
+        const int lds = kWaves * 16 * (HD + 4) * (int)sizeof(float);   // the merge; Q takes less
+        static_assert(kFewRows * HD * 2 <= kWaves * 16 * (HD + 4) * 4);
         auto go = [&](auto kernel) {
             launch_kernel_in_call(last, kernel, grid, dim3(kBlk), lds, s, c, a, p.chunk, p.n_splits, scale_log2);
         };

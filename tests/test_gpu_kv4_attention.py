@@ -89,7 +89,7 @@ def test_every_group(hip, group):
     Batch(hip, group, group * 2, 2, 128 if group % 2 else 64, 16, [77, 5]).upload().launch().check()
 
 
-@pytest.mark.parametrize("lens", [[5000], [9000, 40, 1], [2049] * 3])
+@pytest.mark.parametrize("lens", [[5000], [9000, 40, 1], [2049] * 3, [768, 513], [769, 256, 512], [20000]])
 def test_long_contexts(hip, lens):
     Batch(hip, len(lens), 8, 2, 128, 64, lens).upload().launch().check()
 
@@ -109,6 +109,7 @@ def test_a_large_weight_beside_small_ones(hip):
     (6, 2, 128, 128, [513], [200]),
     (32, 2, 64, 16, [90, 20], [31, 20]),
     (5, 5, 128, 16, [70, 300], [70, 40]),
+    (16, 2, 64, 32, [900, 500], [20, 9]),                     # chunks of a prompt's positions
     (14, 2, 128, 16, [40, 7, 1300], [6, 7, 5]),               # 33 to 64 rows of a kv head
     (16, 2, 64, 32, [100, 2100, 5], [5, 4, 5]),
     (8, 2, 128, 128, [640, 64, 15], [16, 12, 15]),
