@@ -467,25 +467,31 @@ __global__ __launch_bounds__(kBlk) void kv4_merge_kernel(Kv4Attention a, int gro
 //  * the maximum a row's weights refer to moves only when it is exceeded by
 //    kSlack (base 2), which spares O its rescaling in most tiles (583 us below,
 //    599 without).
+//  * kParts = 2: eight waves, four for every other tile, each with buffers of
+//    their own; the second four's sums join the first's at the end.  For grids
+//    that leave a CU one workgroup, whose waves would wait for their own reads.
 // 2048 queries behind 14336 positions, 32/8 heads of 128 (515 GFLOP): 583 us, 883
 // TFLOP/s (a large fp16 product: 1162); of 631 us of an early form the products
 // alone took 330, and 256 rows by eight waves as long as 128 by four.
 // ---------------------------------------------------------------------------
 constexpr int kRowTile = 128, kTile = 64;   // rows of a workgroup; positions of a step
+constexpr int kPromptNotes = 10 * kWaves;   // words that a part's waves leave one another
 constexpr float kSlack = 4.f;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-template <int HD>
-__global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Attention a, int chunk, int n_splits,
-                                                             float scale_log2) {
+template <int HD, int kParts>
+__global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Attention a, int chunk,
+                                                                      int n_splits, float scale_log2) {
     using L = Kv4Layout<HD>;
     using Vec = std::conditional_t<HD == 128, u32x4, u32x2>;
     constexpr int kWords = HD / 32;                    // words of codes a thread has of a position (K) or of 4 (V)
     constexpr int kHalves = HD * kTile;                // of K (or V) in a buffer
     extern __shared__ __align__(16) float lds[];
-    uint16_t* const buf = reinterpret_cast<uint16_t*>(lds);              // [2][K, V][kHalves]
+    const int part = kParts == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kBlk);
+    uint16_t* const buf = reinterpret_cast<uint16_t*>(lds) + part * 4 * kHalves;   // [2][K, V][kHalves]
     // [2][4 waves]: bit 0, the 16 positions have a page; bit 1, nan_at says where V is NaN
-    int* const there_at = reinterpret_cast<int*>(buf + 4 * kHalves);
+    int* const notes = reinterpret_cast<int*>(reinterpret_cast<uint16_t*>(lds) + kParts * 4 * kHalves);
+    int* const there_at = notes + part * kPromptNotes;
     int* const nan_at = there_at + 2 * kWaves;                           // [2][4 waves][4 groups of dims]
 
     // kv heads side by side, so that the workgroups of one meet in an XCD's L2
@@ -503,7 +509,8 @@ __global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Atten
     const int most = max(0, s.see((min(rows, row0 + kRowTile) - 1) / group));
     const int c0 = split * chunk, c1 = min(most, c0 + chunk);
     if (c0 >= most && split > 0) return;
-    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) % kWaves;   // of the part
     const int col = lane & 31, half = lane >> 5;
 
     // this lane's row of Q
@@ -706,19 +713,44 @@ __global__ __launch_bounds__(kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Atten
             }
     };
 
-    load(c0);
+    constexpr int kTurn = kParts * kTile;
+    const int mine = part * kTile;
+    load(c0 + mine);
     hide(0);
     store(0);
-    load(c0 + kTile);
+    load(c0 + mine + kTurn);
     __syncthreads();
-    for (int t = c0, b = 0; t < c1; t += kTile, b ^= 1) {
-        process(t, b);
-        load(t + 2 * kTile);
+    for (int t = c0, b = 0; t < c1; t += kTurn, b ^= 1) {
+        process(t + mine, b);
+        load(t + mine + 2 * kTurn);
         __syncthreads();
     }
 
     // ---- out: O^T's rows back in dim order through LDS, a wave's rows at a time ----
-    const float l = sum32(l_run);
+    float l = sum32(l_run);
+    if constexpr (kParts == 2) {   // the second part's sums, lane by lane, through its own buffers
+        float* const sums = lds + 2 * kHalves + wave * (HD / 2) * kWave + lane;
+        float* const ml = reinterpret_cast<float*>(notes + 2 * kPromptNotes) + 2 * (wave * kWave + lane);
+        if (part == 1) {
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sums[(16 * d + e) * kWave] = o[d][e];
+            ml[0] = m_run;
+            ml[1] = l;
+        }
+        __syncthreads();
+        if (part == 1) return;
+        const float m = fmaxf(m_run, ml[0]);
+        const float f0 = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m);
+        const float f1 = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m);
+        m_run = m;
+        l = l * f0 + ml[1] * f1;
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] = o[d][e] * f0 + sums[(16 * d + e) * kWave] * f1;
+    }
     const bool alone = most <= chunk;
     if (alone) {
         constexpr int kPitch = HD + 8;
@@ -780,6 +812,13 @@ constexpr int kAlone = 768, kAloneWide = 512;   // positions of one chunk, up to
 // 1000 positions 16.3, 33.0; 2 prompts of 500 x 4 rows behind 500 positions, which
 // fill the CUs, 34.9, and 46.3 with 192 up to two).
 constexpr int kPromptBlocks = 256, kPromptChunk = 192, kPromptChunkFull = 512;
+// Two parts up to 384 workgroups, one and a half per CU, that take all of more than
+// 256 positions (one prompt of 32/8 heads: 1100 tokens, 280 workgroups, 33.8
+// against 40.8 with one part, 1500, 376, 44.0 against 53.4, 2048, 512, 59.6
+// against 62.7; but two of 1024, 512, 40.7 against 39.1, four of 700, 704, 43.5
+// against 36.3, 288 workgroups of half of 1390 positions 54.6 against 48.5, 312 of
+// 44 positions 11.7 against 9.4).
+constexpr int kTwoPartBlocks = 384, kTwoPartContext = 256;
 struct Kv4Plan {
     bool few;
     int cols, tiles, chunk, n_splits;
@@ -815,13 +854,22 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
     const int group = a.heads / c.kv_heads;
     const bool last = p.n_splits == 1;
     if (!p.few) {
-        const int lds = 4 * HD * kTile * (int)sizeof(uint16_t) + 2 * kWaves * 5 * (int)sizeof(int);
         const int units = p.tiles * p.n_splits, y = std::min(units, 32768);   // at most 65535 in y
-        const hipError_t e = allow_lds<kv4_prompt_kernel<HD>>(lds);
-        if (e != hipSuccess) return e;
         const dim3 grid(c.kv_heads * a.nseq, y, (units + y - 1) / y);
-        launch_kernel_in_call(last, kv4_prompt_kernel<HD>, grid, dim3(kBlk), lds, s, c, a, p.chunk, p.n_splits,
-                              scale_log2);
+        const int part = 4 * HD * kTile * (int)sizeof(uint16_t) + kPromptNotes * (int)sizeof(int);
+        hipError_t e;
+        if (last && a.max_context > kTwoPartContext && (long long)units * c.kv_heads * a.nseq <= kTwoPartBlocks) {
+            const int lds = 2 * part + 2 * kBlk * (int)sizeof(float);
+            e = allow_lds<kv4_prompt_kernel<HD, 2>>(lds);
+            if (e != hipSuccess) return e;
+            launch_kernel_in_call(last, kv4_prompt_kernel<HD, 2>, grid, dim3(2 * kBlk), lds, s, c, a, p.chunk,
+                                  p.n_splits, scale_log2);
+        } else {
+            e = allow_lds<kv4_prompt_kernel<HD, 1>>(part);
+            if (e != hipSuccess) return e;
+            launch_kernel_in_call(last, kv4_prompt_kernel<HD, 1>, grid, dim3(kBlk), part, s, c, a, p.chunk, p.n_splits,
+                                  scale_log2);
+        }
     } else {
         const dim3 grid(c.kv_heads * a.nseq, p.n_splits);
         const int lds = kWaves * 16 * (HD + 4) * (int)sizeof(float);   // the merge; Q takes less

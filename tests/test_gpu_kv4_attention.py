@@ -109,6 +109,8 @@ def test_a_large_weight_beside_small_ones(hip):
     (6, 2, 128, 128, [513], [200]),
     (32, 2, 64, 16, [90, 20], [31, 20]),
     (5, 5, 128, 16, [70, 300], [70, 40]),
+    (64, 32, 128, 16, [131, 66, 5, 90, 300], [130, 66, 5, 65, 33]),   # more workgroups than fit the CUs at once
+    (64, 32, 64, 32, [131, 66, 5, 90, 300], [130, 66, 5, 65, 33]),
     (16, 2, 64, 32, [900, 500], [20, 9]),                     # chunks of a prompt's positions
     (14, 2, 128, 16, [40, 7, 1300], [6, 7, 5]),               # 33 to 64 rows of a kv head
     (16, 2, 64, 32, [100, 2100, 5], [5, 4, 5]),
