@@ -112,7 +112,9 @@ def test_a_large_weight_beside_small_ones(hip):
     (64, 32, 128, 16, [131, 66, 5, 90, 300], [130, 66, 5, 65, 33]),   # more workgroups than fit the CUs at once
     (64, 32, 64, 32, [131, 66, 5, 90, 300], [130, 66, 5, 65, 33]),
     (16, 2, 64, 32, [900, 500], [20, 9]),                     # chunks of a prompt's positions
-    (14, 2, 128, 16, [40, 7, 1300], [6, 7, 5]),               # 33 to 64 rows of a kv head
+    (32, 2, 128, 16, [900, 33, 5], [3, 3, 1]),                # 33 to 48 rows of a kv head
+    (10, 2, 128, 64, [1300, 40], [8, 3]),
+    (14, 2, 128, 16, [40, 7, 1300], [6, 7, 5]),               # 49 to 64
     (16, 2, 64, 32, [100, 2100, 5], [5, 4, 5]),
     (8, 2, 128, 128, [640, 64, 15], [16, 12, 15]),
     (3, 3, 64, 16, [900, 61], [64, 61])])
@@ -182,7 +184,8 @@ def _nan_tokens(b, where):
 
 
 @pytest.mark.parametrize("hd,page", [(128, 16), (64, 64)])
-@pytest.mark.parametrize("heads,kv,asked", [(8, 2, [4, 2, 3]), (8, 2, [8, 1, 5]), (8, 2, [12, 9, 16]),
+@pytest.mark.parametrize("heads,kv,asked", [(8, 2, [4, 2, 3]), (8, 2, [8, 1, 5]), (8, 2, [10, 9, 12]),
+                                            (8, 2, [12, 9, 16]),
                                             (8, 2, [70, 9, 200])])
 def test_a_nan_is_kept_from_the_queries_before_it(hip, heads, kv, asked, hd, page):
     """NaN keys and values at positions that the last queries see and the first

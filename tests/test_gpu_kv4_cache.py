@@ -189,3 +189,27 @@ def test_rope_table(hip, positions, hd, theta):
     want = np.stack((np.cos(angle), np.sin(angle)), -1)
     # the angle itself, at most 40000 and some roundings of 2^-53 off
     assert np.abs(got - want).max() <= 2.0 ** -25 + 40000 * 2.0 ** -50
+
+
+@pytest.mark.parametrize("tokens,heads,kv,hd", [(2500, 32, 8, 128), (5003, 7, 3, 64), (9001, 4, 2, 128), (4099, 0, 5, 64)])
+def test_many_tokens_equal_few_at_a_time(hip, tokens, heads, kv, hd):
+    """Queries and every byte of the cache do not depend on the call's size."""
+    rng = np.random.default_rng(tokens)
+    s = Step(hip, rng, tokens, heads, kv, hd, 16)
+    s.at[rng.integers(0, tokens, 30)] = -1
+    row = heads * hd
+    up = hip.DeviceArray.from_numpy
+    d_qkv, d_qn, d_kn, d_t, d_at, d_s = (up(x) for x in (s.qkv, s.q_norm, s.k_norm, s.table, s.at, s.slots))
+    got = []
+    for step in (tokens, 97):
+        d_pages, d_out = up(s.cache.raw), up(np.full((tokens, row + 8), 7, np.float16))
+        view = hip.device.kv4_cache(d_pages, s.cache.num_pages, 16, kv, hd)
+        for t in range(0, tokens, step):
+            base = d_qkv.ptr + t * s.width * 2
+            hip.device.kv4_append(view, base if heads else None, base + 2 * row, base + 2 * (row + kv * hd), s.width,
+                                  s.width, d_qn, d_kn, EPS, d_t, len(s.table), d_at.ptr + 4 * t, d_s.ptr + 4 * t,
+                                  min(step, tokens - t), heads, d_out.ptr + t * (row + 8) * 2 if heads else None,
+                                  row + 8)
+        got.append((d_pages.download(np.uint8), d_out.download(np.uint16)))
+    assert np.array_equal(got[0][0], got[1][0]) and np.array_equal(got[0][1], got[1][1])
+    assert (got[0][0] != 0x5A).mean() > 0.5
