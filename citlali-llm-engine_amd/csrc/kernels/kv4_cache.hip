@@ -169,10 +169,10 @@ __global__ __launch_bounds__(kBlk) void kv4_append_kernel(Kv4View c, Kv4Append a
     const int lane = threadIdx.x & (kWave - 1), l = lane % LR;
     const int q_units = (a.heads + per - 1) / per, kv_units = (c.kv_heads + per - 1) / per;
     const int units = q_units + 2 * kv_units;
-    const long long at = (long long)blockIdx.x * (kBlk / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const long long group = at / units;
+    const uint32_t at = blockIdx.x * (kBlk / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const long long group = at / (uint32_t)units;
     if (group * kRows >= a.tokens) return;   // uniform
-    int unit = (int)(at - group * units);
+    int unit = (int)(at % (uint32_t)units);
     const bool is_q = unit < q_units, is_v = unit >= q_units + kv_units;
     unit -= is_q ? 0 : is_v ? q_units + kv_units : q_units;
     const int h0 = unit * per, h1 = min(is_q ? a.heads : c.kv_heads, h0 + per);
@@ -278,48 +278,44 @@ __global__ __launch_bounds__(kBlk) void kv4_append_kernel(Kv4View c, Kv4Append a
     }
 }
 
-// Lanes as in the append: one wave reads the K or V values of one head in
-// 512 / HD slots.  8192 slots of 8 heads of 128, 44 MB, in 11.7 us (3.7 TB/s).
+// Lanes as in the append: one wave reads the K and V values of one head in
+// 512 / HD slots.  8192 slots of 8 heads of 128, 44 MB, in 10.4 us
+// (4.2 TB/s; K and V in a wave each 11.8).
 template <int HD>
 __global__ __launch_bounds__(kBlk) void kv4_read_kernel(Kv4View c, const int32_t* __restrict__ slots, int count,
                                                         uint16_t* __restrict__ k_out, uint16_t* __restrict__ v_out) {
     constexpr int LR = HD / 8, kRows = kWave / LR;
     using L = Kv4Layout<HD>;
     const int lane = threadIdx.x & (kWave - 1), l = lane % LR;
-    const long long unit = (long long)blockIdx.x * (kBlk / kWave) + threadIdx.x / kWave;
-    const int head = (int)(unit % (2 * c.kv_heads));
-    const long long t = unit / (2 * c.kv_heads) * kRows + lane / LR;
+    const uint32_t unit = blockIdx.x * (kBlk / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t group = unit / (uint32_t)c.kv_heads;
+    const int kvh = (int)(unit - group * c.kv_heads);
+    const long long t = (long long)group * kRows + lane / LR;
     if (t >= count) return;
-    const bool is_k = head < c.kv_heads;
-    const int kvh = is_k ? head : head - c.kv_heads;
     const int slot = slots[t];
     const int P = 1 << c.page_shift, o = slot & (P - 1);
-    u32x4 out{0u, 0u, 0u, 0u};
+    u32x4 k{0u, 0u, 0u, 0u}, v = k;
     if (slot >= 0 && (slot >> c.page_shift) < c.num_pages) {
         const uint8_t* base = kv4_head<HD>(c, slot >> c.page_shift, kvh);
-        f16x2 v[4];
-        if (is_k) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(base + o * L::kCodes + 4 * l);
-            const f16x2 dm = as_h2(
-                *reinterpret_cast<const uint32_t*>(base + L::k_params(P) + o * L::kParams + (l & ~3)));
-            kv4_pairs(w, f16x2{dm.x, dm.x}, f16x2{dm.y, dm.y}, v);
-        } else {
-            const uint16_t* vc = reinterpret_cast<const uint16_t*>(base + L::v_codes(P)) + (o >> 2) * HD + (o & 3);
-            const _Float16* vp = reinterpret_cast<const _Float16*>(base + L::v_params(P)) +
-                                 ((o >> 2) * (HD / kKv4Group) + (l >> 2)) * 8 + (o & 3);
-            const _Float16 d = vp[0], m = vp[4];
-            const uint32_t lo = vc[8 * l], hi = vc[8 * l + 4];
-            f16x2 s[4];   // pair i: dims i and i + 4 of the lane
-            kv4_pairs(lo | (hi << 16), f16x2{d, d}, f16x2{m, m}, s);
-            v[0] = f16x2{s[0].x, s[1].x};
-            v[1] = f16x2{s[2].x, s[3].x};
-            v[2] = f16x2{s[0].y, s[1].y};
-            v[3] = f16x2{s[2].y, s[3].y};
-        }
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(base + o * L::kCodes + 4 * l);
+        const f16x2 dm =
+            as_h2(*reinterpret_cast<const uint32_t*>(base + L::k_params(P) + o * L::kParams + (l & ~3)));
+        const uint16_t* vc = reinterpret_cast<const uint16_t*>(base + L::v_codes(P)) + (o >> 2) * HD + (o & 3);
+        const _Float16* vp = reinterpret_cast<const _Float16*>(base + L::v_params(P)) +
+                             ((o >> 2) * (HD / kKv4Group) + (l >> 2)) * 8 + (o & 3);
+        const _Float16 d = vp[0], m = vp[4];
+        const uint32_t lo = vc[8 * l], hi = vc[8 * l + 4];
+        f16x2 e[4];
+        kv4_pairs(w, f16x2{dm.x, dm.x}, f16x2{dm.y, dm.y}, e);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) out[i] = __builtin_bit_cast(uint32_t, v[i]);
+        for (int i = 0; i < 4; ++i) k[i] = __builtin_bit_cast(uint32_t, e[i]);
+        kv4_pairs(lo | (hi << 16), f16x2{d, d}, f16x2{m, m}, e);   // pair i: dims i and i + 4 of the lane
+        const f16x2 in_order[4] = {{e[0].x, e[1].x}, {e[2].x, e[3].x}, {e[0].y, e[1].y}, {e[2].y, e[3].y}};
+        v = __builtin_bit_cast(u32x4, in_order);
     }
-    *reinterpret_cast<u32x4*>((is_k ? k_out : v_out) + ((size_t)t * c.kv_heads + kvh) * HD + 8 * l) = out;
+    const size_t at = ((size_t)t * c.kv_heads + kvh) * HD + 8 * l;
+    __builtin_nontemporal_store(k, reinterpret_cast<u32x4*>(k_out + at));
+    __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(v_out + at));
 }
 
 }  // namespace
@@ -362,7 +358,7 @@ hipError_t launch_kv4_append(const Kv4View& c, const Kv4Append& a, hipStream_t s
 
 hipError_t launch_kv4_read(const Kv4View& c, const int32_t* slots, int count, uint16_t* k_out, uint16_t* v_out,
                            hipStream_t s) {
-    const dim3 grid(blocks_for(count, c.head_dim, 2 * c.kv_heads));
+    const dim3 grid(blocks_for(count, c.head_dim, c.kv_heads));
     if (c.head_dim == 128)
         launch_kernel(kv4_read_kernel<128>, grid, dim3(kBlk), 0, s, c, slots, count, k_out, v_out);
     else
