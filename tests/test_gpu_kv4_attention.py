@@ -295,3 +295,37 @@ def test_pages_past_four_gigabytes(hip):
     b.view = hip.device.kv4_cache(pages, num, page, kv, hd)
     b.d_table = hip.DeviceArray.from_numpy(np.where(b.table >= 0, num - 1 - b.table, -1).astype(np.int32))
     assert np.array_equal(b.launch().check(), want)
+
+
+@pytest.mark.parametrize("hd,asked", [(64, None), (128, None), (128, [40, 30]), (64, [40, 33])])
+def test_infinite_queries(hip, hd, asked):
+    """Scores that are all -inf give zeros, +inf among them NaN; other rows keep theirs."""
+    b = Batch(hip, 20, 4, 2, hd, 16, [40, 33], asked)
+    want, spread, reach = b.expected()
+    sign = np.sign(b.cache.k[..., 5].astype(np.float64))
+    b.q[0, 1] = 0
+    b.q[0, 1, 5] = -np.inf
+    b.q[-1, 2] = 0
+    pages = b.table[0, :3]
+    raw = kv4_ref.Cache(b.cache.num_pages, 16, 2, hd)
+    raw.raw, raw.k, raw.v = b.cache.raw, b.cache.k, b.cache.v
+    for p in range(40):                                        # sequence 0, kv head 0: dim 5 of every key above 0
+        k, v = raw.read(pages[p // 16] * 16 + p % 16)
+        k = np.abs(k.astype(np.float32)) + np.float32(0.5) if p or asked is None else k.astype(np.float32)
+        raw.write(pages[p // 16] * 16 + p % 16, k, v.astype(np.float32))
+    got = b.upload().launch().result()[:b.start[-1]].astype(np.float64)
+    if asked is None:
+        assert not got[0, 1].any()                             # every score -inf
+    else:
+        first = sign[pages[0], 0, 0]                           # the first row sees position 0 alone
+        assert not got[0, 1].any() if first > 0 else np.isnan(got[0, 1]).all()
+    seen = b.cache.v[b.table[1, np.arange(33) // 16], 1, np.arange(33) % 16].astype(np.float64)
+    near = np.abs(seen).mean(0) * 2.0 ** -9 + 2.0 ** -20
+    assert (np.abs(got[-1, 2] - seen.mean(0)) <= near).all()   # equal scores
+    off = np.abs(got - want) - kv4_ref.tolerance(want, spread, reach)
+    other = np.ones(got.shape[:2], bool)
+    other[0], other[-1, 2] = False, False
+    if asked is None:
+        assert (off[other] <= 0).all()
+    else:                                                      # sequence 1, whose keys are as they were
+        assert (off[40:][other[40:]] <= 0).all()
