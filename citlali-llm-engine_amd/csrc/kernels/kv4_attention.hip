@@ -465,13 +465,13 @@ __global__ __launch_bounds__(kBlk) void kv4_merge_kernel(Kv4Attention a, int gro
 //  * V's dim HD/16 c + n lies at 16 n + c, so that the 16 lanes that write one n
 //    use different banks.
 //  * the maximum a row's weights refer to moves only when it is exceeded by
-//    kSlack (base 2), which spares O its rescaling in most tiles (583 us below,
-//    599 without).
+//    kSlack (base 2), which spares O its rescaling in most tiles (593 us for the
+//    case below against 599 without, six fresh prompts 88 against 91).
 //  * kParts = 2: eight waves, four for every other tile, each with buffers of
 //    their own; the second four's sums join the first's at the end.  For grids
 //    that leave a CU one workgroup, whose waves would wait for their own reads.
-// 2048 queries behind 14336 positions, 32/8 heads of 128 (515 GFLOP): 583 us, 883
-// TFLOP/s (a large fp16 product: 1162); of 631 us of an early form the products
+// 2048 queries behind 14336 positions, 32/8 heads of 128 (515 GFLOP): 583 to
+// 593 us, 870 to 884 TFLOP/s (a large fp16 product: 1162); of 631 us of an early form the products
 // alone took 330, and 256 rows by eight waves as long as 128 by four.
 // ---------------------------------------------------------------------------
 constexpr int kRowTile = 128, kTile = 64;   // rows of a workgroup; positions of a step
