@@ -53,12 +53,13 @@ __device__ __forceinline__ uint32_t partner(uint32_t v) {
         return __shfl_xor((int)v, LR / 2, kWave);
 }
 
-// x^-1/2 of a positive number: the hardware's estimate, in 64 bits one Newton
-// step further (its error, about 2^-29, squared).
+// x^-1/2 of a positive number, 0 of infinity: the hardware's estimate, in 64 bits
+// one Newton step further (its error, about 2^-29, squared), which a 0 does without
+// (its x r would be a NaN).
 __device__ __forceinline__ float inv_root(float x) { return __builtin_amdgcn_rsqf(x); }
 __device__ __forceinline__ double inv_root(double x) {
     const double r = __builtin_amdgcn_rsq(x);
-    return fma(0.5 * r, fma(-x * r, r, 1.0), r);
+    return r == 0.0 ? 0.0 : fma(0.5 * r, fma(-x * r, r, 1.0), r);
 }
 
 // Norm and rotation of a lane's eight values, in T.  Lane l of the LR that share

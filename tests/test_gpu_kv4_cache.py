@@ -213,3 +213,27 @@ def test_many_tokens_equal_few_at_a_time(hip, tokens, heads, kv, hd):
         got.append((d_pages.download(np.uint8), d_out.download(np.uint16)))
     assert np.array_equal(got[0][0], got[1][0]) and np.array_equal(got[0][1], got[1][1])
     assert (got[0][0] != 0x5A).mean() > 0.5
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_infinities_under_a_norm(hip, hd):
+    """A head with an infinity has an infinite root mean square: its finite dims
+    become 0, the infinite one and its rotation partner NaN, in queries and (a
+    group of 32 at a time) in keys."""
+    step = Step(hip, np.random.default_rng(7), 9, 2, 2, hd, 16)
+    x = step.qkv.reshape(9, 6, hd)
+    x[2, :4, 3] = np.inf
+    x[5, :4, hd // 2 + 1] = -np.inf
+    x[7, :4, 0], x[7, :4, hd - 1] = np.inf, np.inf
+    step.run()
+    rows = [2, 5, 7]
+    with np.errstate(invalid="ignore"):
+        q, k = (_rotated(x[rows, lo:lo + 2], w, step.table, step.at[rows])[0]
+                for lo, w in ((0, step.q_norm), (2, step.k_norm)))
+    got = step.q_out[rows, :2 * hd].reshape(3, 2, hd)
+    assert np.array_equal(np.isnan(got), np.isnan(q)) and np.isnan(q).sum() == 2 * (2 + 2 + 4)
+    assert not got[~np.isnan(q)].any()
+    want = kv4_ref.values(*kv4_ref.quantise(k.astype(np.float32)))
+    assert np.array_equal(step.k[rows], want, equal_nan=True)
+    finite = ~np.isnan(want)
+    assert finite.any() == (hd == 128) and not step.k[rows][finite].any()
