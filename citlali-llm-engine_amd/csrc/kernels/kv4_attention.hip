@@ -69,6 +69,14 @@ __device__ __forceinline__ int seq_of(int x, int layer, int nseq) {
 constexpr int kBlk = 256, kWaves = kBlk / kWave;
 constexpr float kShift = 14.f;   // weights are kept times 2^14 (base 2)
 
+// 2^((a - b) scale) of scores a <= b, of which -inf is none at all.  The maxima
+// that weights and sums refer to are kept as scores: a difference of scores is as
+// exact as they are, one of their multiples of scale_log2 need not be, and from
+// 2^25 on (queries and keys of some thousands) is off by any factor.
+__device__ __forceinline__ float score_factor(float a, float b, float scale_log2) {
+    return a == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((a - b) * scale_log2);
+}
+
 // ---------------------------------------------------------------------------
 // Few rows: one workgroup per (chunk of positions, kv head, sequence) serves
 // every query of the sequence for every head of the kv head's group, at most
@@ -245,21 +253,21 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4
             }
             float mt = max3(max3(sc[n][0][0], sc[n][0][1], sc[n][0][2]), sc[n][0][3], sc[n][1][0]);
             mt = max3(mt, sc[n][1][1], max3(sc[n][1][2], sc[n][1][3], sc[n][1][3]));
-            mt = max32(max16(mt)) * scale_log2;
+            mt = max32(max16(mt));
             if (__builtin_amdgcn_ballot_w64(mt > m_run[n]) != 0) {
                 const float m_new = fmaxf(m_run[n], mt);
-                const float f = m_run[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[n] - m_new);
+                const float f = score_factor(m_run[n], m_new, scale_log2);
                 m_run[n] = m_new;
                 l_run[n] *= f;
 #pragma unroll
                 for (int d = 0; d < kDims; ++d) o[n][d] *= f;
             }
-            const float off = kShift - (m_run[n] == -INFINITY ? 0.f : m_run[n]);
+            const float ref = m_run[n] == -INFINITY ? 0.f : m_run[n];
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float w = __builtin_amdgcn_exp2f(fmaf(sc[n][u][i], scale_log2, off));
+                    const float w = __builtin_amdgcn_exp2f(fmaf(sc[n][u][i] - ref, scale_log2, kShift));
                     l_run[n] += w;
                     pw[n][4 * u + i] = (_Float16)w;
                 }
@@ -346,7 +354,7 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) {
                 const float m = from[w * step + HD];
-                const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+                const float f = score_factor(m, M, scale_log2);
                 l += from[w * step + HD + 1] * f;
                 acc += *reinterpret_cast<const f32x4*>(from + w * step + d) * f;
             }
@@ -379,7 +387,7 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4
 // 6.4 by one.
 template <int HD, int kTeam>
 __global__ __launch_bounds__(kBlk) void kv4_merge_kernel(Kv4Attention a, int group, int tile_rows, int chunk,
-                                                         int n_splits) {
+                                                         int n_splits, float scale_log2) {
     constexpr int kLanes = HD / 4, kTeams = kTeam * kWave / kLanes, kBatch = 4;
     __shared__ __align__(16) float lds[kTeam > 1 ? kTeam : 1][HD];
     const int seq = blockIdx.y, lane = threadIdx.x & (kWave - 1);
@@ -415,7 +423,7 @@ __global__ __launch_bounds__(kBlk) void kv4_merge_kernel(Kv4Attention a, int gro
     float M = lane < n ? mine.x : -INFINITY;
     for (int j = lane + kWave; j < n; j += kWave) M = fmaxf(M, ml[j].x);
     M = wave_max(M);
-    auto factor = [&](float m) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M); };
+    auto factor = [&](float m) { return score_factor(m, M, scale_log2); };
     float l = lane < n ? mine.y * factor(mine.x) : 0.f;
     for (int j = lane + kWave; j < n; j += kWave) l += ml[j].y * factor(ml[j].x);
     l = wave_sum(l);
@@ -476,7 +484,7 @@ __global__ __launch_bounds__(kBlk) void kv4_merge_kernel(Kv4Attention a, int gro
 // ---------------------------------------------------------------------------
 constexpr int kRowTile = 128, kTile = 64;   // rows of a workgroup; positions of a step
 constexpr int kPromptNotes = 10 * kWaves;   // words that a part's waves leave one another
-constexpr float kSlack = 4.f;
+constexpr float kSlack = 4.f, kFar = 1024.f;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 template <int HD, int kParts>
@@ -486,6 +494,7 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
     using Vec = std::conditional_t<HD == 128, u32x4, u32x2>;
     constexpr int kWords = HD / 32;                    // words of codes a thread has of a position (K) or of 4 (V)
     constexpr int kHalves = HD * kTile;                // of K (or V) in a buffer
+    constexpr float kSlackScore = kSlack * 0.693147181f * (HD == 128 ? 11.3137085f : 8.f);   // kSlack / scale_log2
     extern __shared__ __align__(16) float lds[];
     const int part = kParts == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kBlk);
     uint16_t* const buf = reinterpret_cast<uint16_t*>(lds) + part * 4 * kHalves;   // [2][K, V][kHalves]
@@ -685,16 +694,27 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int e = 0; e < 16; e += 2) mt = max3(mt, sc[u][e], sc[u][e + 1]);
-        mt = max32(mt) * scale_log2;
-        if (__builtin_amdgcn_ballot_w64(mt > m_run + kSlack || (m_run == -INFINITY && mt > m_run)) != 0) {
+        mt = max32(mt);
+        if (__builtin_amdgcn_ballot_w64(mt - m_run > kSlackScore) != 0) {
             const float m_new = fmaxf(m_run, mt);
-            const float f = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
+            const float f = score_factor(m_run, m_new, scale_log2);
             m_run = m_new;
             l_run *= f;
 #pragma unroll
             for (int d = 0; d < HD / 32; ++d) o[d] *= f;
         }
-        const float off = kShift - kSlack - (m_run == -INFINITY ? 0.f : m_run);
+        // A weight is 2^((score - ref) scale + shift), here as one fma with off =
+        // shift - ref scale (with the difference first, as few rows take it: 603 us
+        // for 584).  Beyond kFar the rounding of off would count, 2^-15 of a weight
+        // there; those tiles take the difference first.
+        const float ref = m_run == -INFINITY ? 0.f : m_run;
+        float off = fmaf(-ref, scale_log2, kShift - kSlack);
+        if (__builtin_amdgcn_ballot_w64(fabsf(off) > kFar) != 0) {
+            asm volatile("");   // a branch: most tiles skip it
+            sc[0] -= ref;
+            sc[1] -= ref;
+            off = kShift - kSlack;
+        }
         half8 pw[4];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -742,8 +762,7 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
         __syncthreads();
         if (part == 1) return;
         const float m = fmaxf(m_run, ml[0]);
-        const float f0 = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m);
-        const float f1 = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m);
+        const float f0 = score_factor(m_run, m, scale_log2), f1 = score_factor(ml[0], m, scale_log2);
         m_run = m;
         l = l * f0 + ml[1] * f1;
 #pragma unroll
@@ -891,10 +910,10 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
     const int tile_rows = p.few ? kFewRows : kRowTile;
     if (p.n_splits <= 4 * kWave / (HD / 4))
         launch_kernel(kv4_merge_kernel<HD, 1>, dim3((unsigned)((units + kWaves - 1) / kWaves), a.nseq), dim3(kBlk), 0,
-                      s, a, group, tile_rows, p.chunk, p.n_splits);
+                      s, a, group, tile_rows, p.chunk, p.n_splits, scale_log2);
     else
         launch_kernel(kv4_merge_kernel<HD, kWaves>, dim3((unsigned)units, a.nseq), dim3(kBlk), 0, s, a, group,
-                      tile_rows, p.chunk, p.n_splits);
+                      tile_rows, p.chunk, p.n_splits, scale_log2);
     return hipGetLastError();
 }
 

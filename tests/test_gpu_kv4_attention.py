@@ -329,3 +329,39 @@ def test_infinite_queries(hip, hd, asked):
         assert (off[other] <= 0).all()
     else:                                                      # sequence 1, whose keys are as they were
         assert (off[40:][other[40:]] <= 0).all()
+
+
+@pytest.mark.parametrize("hd,big", [(64, 3000.0), (128, 3000.0), (128, 40000.0)])
+@pytest.mark.parametrize("heads,kv,lens,asked", [
+    (8, 2, [300, 37], None), (8, 2, [5000], None),           # one query: in one chunk, in several
+    (8, 2, [700, 60], [8, 3]), (32, 2, [900, 33], [3, 2]),   # 17 to 48 rows
+    (16, 2, [900, 500], [20, 9]),                            # a prompt's positions in chunks
+    (8, 8, [300], [200])])                                   # and in two parts
+def test_scores_of_large_queries_and_keys(hip, heads, kv, lens, asked, hd, big):
+    """Finite queries and keys whose scores lie far beyond 2^20: a row whose
+    largest score leads the next by more than the scores' own rounding (2^-16
+    of their terms, both ways, and 30 for the exponential) is the value of that
+    position: half a step for the weight, half for the output."""
+    with np.errstate(over="ignore"):                         # infinities saturate
+        b = Batch(hip, 21, heads, kv, hd, 16, lens, asked, big=big)
+        b.q = np.clip(b.q.astype(np.float32) * big, -65504, 65504).astype(np.float16)
+    got = b.upload().launch().result().astype(np.float64)
+    assert np.isfinite(got).all()
+    tested = 0
+    for s, length in enumerate(lens):
+        n = b.start[s + 1] - b.start[s]
+        p = np.arange(length)
+        k, v = (x[b.table[s, p // 16], :, p % 16].astype(np.float64) for x in (b.cache.k, b.cache.v))
+        for i in range(n):
+            seen = length - n + i + 1
+            for h in range(heads):
+                q = b.q[b.start[s] + i, h].astype(np.float64)
+                x = k[:seen, h // (heads // kv)] @ q / np.sqrt(hd)
+                reach = (np.abs(k[:seen, h // (heads // kv)]) @ np.abs(q)).max() / np.sqrt(hd)
+                best = x.argmax()
+                if seen > 1 and np.delete(x, best).max() > x[best] - 2 * reach * 2.0 ** -16 - 30:
+                    continue
+                tested += 1
+                want = v[best, h // (heads // kv)]
+                assert (np.abs(got[b.start[s] + i, h] - want) <= np.abs(want) * 2.0 ** -10 + 2.0 ** -24).all()
+    assert tested >= 0.9 * heads * b.start[-1]
