@@ -11,12 +11,12 @@
 namespace citlali::hip {
 namespace {
 
-// The largest of three, as one instruction (fmaxf first makes a quiet NaN of
-// each operand that a matrix instruction wrote).
+// The largest of three (a NaN stays): one v_maximum3_f32.  Not asm: its operands
+// come from matrix instructions, and only for an instruction of its own does the
+// compiler keep the wait states between the two.  Not fmaxf: that first makes a
+// quiet NaN of each operand.
 __device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 
 // The queries of sequence `seq`: rows start .. start + n - 1 of q, the cached
