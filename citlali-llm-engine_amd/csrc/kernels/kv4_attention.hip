@@ -19,6 +19,15 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 
+// l + the sum of eight weights as the product with V takes them: what their
+// rounding to fp16 does is then in numerator and denominator alike.
+__device__ __forceinline__ float add_weights(half8 w, float l) {
+    const u32x4 pairs = __builtin_bit_cast(u32x4, w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) l = dot2(pairs[i], 0x3c003c00u, l);   // times 1, 1
+    return l;
+}
+
 // The queries of sequence `seq`: rows start .. start + n - 1 of q, the cached
 // positions that exist, and how many of them query i sees (see()).
 struct Kv4Seq {
@@ -94,7 +103,7 @@ __device__ __forceinline__ float score_factor(float a, float b, float scale_log2
 //  * O^T[dim][row] += V^T P^T: the lanes' weights are the B operand as they
 //    stand (k index = grp 4 + i of the first 16 positions, then of the second),
 //    rounded to fp16 -- times 2^14, so that weights down to 2^-28 of the largest
-//    keep all their bits; their sum takes them before.  V lies in groups of
+//    keep all their bits; their sum takes them so too.  V lies in groups of
 //    four tokens, so lane (c, grp) loads the codes of its four positions and
 //    HD / 16 dims together, each word two positions' dims, and gets the A
 //    operand's pairs without a transposition.
@@ -266,11 +275,10 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float w = __builtin_amdgcn_exp2f(fmaf(sc[n][u][i] - ref, scale_log2, kShift));
-                    l_run[n] += w;
-                    pw[n][4 * u + i] = (_Float16)w;
-                }
+                for (int i = 0; i < 4; ++i)
+                    pw[n][4 * u + i] =
+                        (_Float16)__builtin_amdgcn_exp2f(fmaf(sc[n][u][i] - ref, scale_log2, kShift));
+            l_run[n] = add_weights(pw[n], l_run[n]);
         }
         if (!whole) {   // positions no row may use: their V counts as 0, whatever it holds
 #pragma unroll
@@ -719,11 +727,10 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float w = __builtin_amdgcn_exp2f(fmaf(sc[u][e], scale_log2, off));
-                l_run += w;
-                pw[2 * u + e / 8][e % 8] = (_Float16)w;
-            }
+            for (int e = 0; e < 16; ++e)
+                pw[2 * u + e / 8][e % 8] = (_Float16)__builtin_amdgcn_exp2f(fmaf(sc[u][e], scale_log2, off));
+#pragma unroll
+        for (int st = 0; st < 4; ++st) l_run = add_weights(pw[st], l_run);
 #pragma unroll
         for (int st = 0; st < 4; ++st)
 #pragma unroll

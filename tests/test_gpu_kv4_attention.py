@@ -365,3 +365,29 @@ def test_scores_of_large_queries_and_keys(hip, heads, kv, lens, asked, hd, big):
                 want = v[best, h // (heads // kv)]
                 assert (np.abs(got[b.start[s] + i, h] - want) <= np.abs(want) * 2.0 ** -10 + 2.0 ** -24).all()
     assert tested >= 0.9 * heads * b.start[-1]
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("heads,kv,lens,asked", [
+    (16, 2, [200, 40], None), (16, 2, [1500], None),         # one query: in one chunk, in several
+    (16, 2, [200], [4]), (16, 1, [200, 90], [3, 3]),         # 17 to 48 rows
+    (16, 2, [200], [20]), (8, 8, [300], [200])])             # prompts: in chunks, in two parts
+def test_equal_values_come_out_as_they_are(hip, heads, kv, lens, asked, hd):
+    """Every position has the same value and the weights are of two kinds: what
+    rounding does to them is in the numerator and in their sum alike, so the
+    value comes out to the bit (fp32 sums of at most 1500 terms are off by less
+    than 2^-13, half a step is at least 2^-12 of the value)."""
+    b = Batch(hip, 22, heads, kv, hd, 16, lens, asked)
+    rng = np.random.default_rng(22)
+    b.cache.raw[:] = 0
+    value = np.repeat(1.999 - np.arange(kv * hd // 32) / (kv * hd // 32), 32).reshape(kv, hd).astype(np.float16)
+    key = np.zeros((kv, hd), np.float32)
+    for s, length in enumerate(lens):
+        for p in range(length):
+            key[:, :32] = 0 if p % 97 else 1                 # a group of one value is kept as it is
+            b.cache.write(b.table[s, p // 16] * 16 + p % 16, key, value)
+    b.q[:] = 0
+    b.q[..., 0] = rng.uniform(2, 40, b.q.shape[:2])          # weights 1 and e^(-q / sqrt(hd)), e^-0.2 to e^-5
+    got = b.upload().launch().result()
+    want = np.repeat(value, heads // kv, axis=0)
+    assert np.array_equal(got, np.broadcast_to(want, got.shape))
