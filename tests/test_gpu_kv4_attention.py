@@ -391,3 +391,48 @@ def test_equal_values_come_out_as_they_are(hip, heads, kv, lens, asked, hd):
     got = b.upload().launch().result()
     want = np.repeat(value, heads // kv, axis=0)
     assert np.array_equal(got, np.broadcast_to(want, got.shape))
+
+
+@pytest.mark.parametrize("nseq", [33, 49])                   # two parts of the positions, one
+@pytest.mark.parametrize("hd,page,lens", [(64, 16, [3300, 1030, 2049]), (128, 16, [2500, 1100]),
+                                          (64, 32, [2300, 4200]), (128, 64, [4500])])
+def test_long_prompts_in_one_chunk(hip, nseq, hd, page, lens):
+    """A prompt kernel's chunk of more pages than the lanes hold at once (64), of
+    shuffled pages, more than twice as many too; sequences enough for no split."""
+    asked = [60, 49, 60][:len(lens)]
+    short = nseq - len(lens)
+    b = Batch(hip, 23, 8, 8, hd, page, lens + [40] * short, asked + [2] * short).upload()
+    assert b.bytes == 0 and max(lens) > 64 * page
+    b.launch().check()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("keys", [False, True])
+def test_nan_in_two_parts_of_the_positions(hip, hd, keys):
+    """As the two tests above, where two groups of waves share the positions."""
+    lens, asked = [300, 290], [200, 65]
+    b = Batch(hip, 24, 8, 8, hd, 16, lens, asked)
+    want, spread, reach = b.expected()
+    near = kv4_ref.tolerance(want, spread, reach)
+    clean = b.cache.raw.copy()
+    where = [(0, 150, 0), (0, 200, 1), (0, 259, 0), (0, 299, 1), (1, 255, 1), (1, 288, 0)]
+    _nan_tokens(b, where)
+    if not keys:
+        behind = kv4_ref.head_layout(16, hd)[2]
+        b.cache.raw[:, :, :behind] = clean[:, :, :behind]
+    got = b.upload().launch().result().astype(np.float64)
+    assert b.bytes == 0
+    nan = np.zeros((len(got), hd // 32), bool)
+    for s, p, j in where:
+        nan[b.start[s]:b.start[s + 1], slice(None) if keys else j] |= (
+            lens[s] - asked[s] + np.arange(asked[s]) + 1 > p)[(slice(None),) + (None,) * keys]
+    nan = np.repeat(nan, 32, axis=1)[:, None, :] & np.ones((1, 8, 1), bool)
+    assert nan.any() and not nan.all()
+    assert np.isnan(got[nan]).all() and (np.abs(got - want)[~nan] <= near[~nan]).all()
+
+
+def test_a_bound_of_very_many_queries(hip):
+    """A plan whose row tiles pass one dimension of a grid."""
+    b = Batch(hip, 25, 16, 1, 64, 16, [130, 9], asked=[120, 2])
+    b.max_query = 270000
+    b.upload().launch().check()
