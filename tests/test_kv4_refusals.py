@@ -142,3 +142,19 @@ def test_page_bytes():
                                   (A, 2 ** 31 - 1, 64, 1e4)])
 def test_rope_table(args):
     _refused(device.rope_table, INVALID, *args)
+
+
+def test_short_workspaces_are_refused():
+    """The sizes that the queries give are what the calls insist on."""
+    need = device.kv4_attention_workspace_bytes(100000, 1, 1, 1, 8, 2, 128)
+    call = {**ATTENTION, "nseq": 1, "tokens": 1, "max_context": 100000, "pages_per_seq": 100000 // 16}
+    assert need > 0 and need % (8 * (128 + 2) * 4) == 0        # parts of 8 heads
+    for change in (dict(workspace=A, workspace_bytes=need - 1), dict(workspace=A, workspace_bytes=0),
+                   dict(workspace=None, workspace_bytes=need), dict(workspace=A + 4, workspace_bytes=need)):
+        _refused(device.kv4_attention, INVALID, _cache(), **{**call, **change})
+    need = device.token_logprobs_workspace_bytes(1, 151936, 20)
+    call = {**LOGPROBS, "rows": 1, "vocab": 151936, "row_stride": 151936, "top_k": 20}
+    assert need > 0 and need % (16 + 8 * 20) == 0              # sums and 20 listed of each piece
+    for change in (dict(workspace=A, workspace_bytes=need - 1), dict(workspace=A, workspace_bytes=0),
+                   dict(workspace=None, workspace_bytes=need), dict(workspace=A + 8, workspace_bytes=need)):
+        _refused(device.token_logprobs, INVALID, **{**call, **change})
