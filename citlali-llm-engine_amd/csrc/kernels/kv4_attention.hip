@@ -107,9 +107,11 @@ __device__ __forceinline__ float score_factor(float a, float b, float scale_log2
 //    four tokens, so lane (c, grp) loads the codes of its four positions and
 //    HD / 16 dims together, each word two positions' dims, and gets the A
 //    operand's pairs without a transposition.
-// Bound by the cache's bytes, next by the vector unit (about 300 instructions a
-// tile of 5 KB at head_dim 128, 215 a tile of 2.5 KB at 64) and the round trips
-// of a workgroup's start.  32/8 heads of 128: 16 sequences of 4096 .. 32768
+// Bound by the cache's bytes where contexts are long; else by the round trips of a
+// workgroup's start and by the unequal lengths of the one round of workgroups: the
+// vector unit (about 300 instructions a tile of 5 KB at head_dim 128, 215 a tile of
+// 2.5 KB at 64) is busy for half of the time in each case below but the first.
+// 32/8 heads of 128: 16 sequences of 4096 .. 32768
 // positions, 403 MB, in 78 us (5.1 TB/s), 64 of 200 .. 4000, 174 MB, in 38.7 (4.5);
 // 20 rows, 24 sequences of 500 .. 6000, 101 MB, in 31.0; 16/8 heads of 64, 100
 // sequences of 150 .. 1500, 52.6 MB, in 18.6.
@@ -486,8 +488,9 @@ __global__ __launch_bounds__(kBlk) void kv4_merge_kernel(Kv4Attention a, int gro
 //  * kParts = 2: eight waves, four for every other tile, each with buffers of
 //    their own; the second four's sums join the first's at the end.  For grids
 //    that leave a CU one workgroup, whose waves would wait for their own reads.
-// 2048 queries behind 14336 positions, 32/8 heads of 128 (515 GFLOP): 583 to
-// 593 us, 870 to 884 TFLOP/s (a large fp16 product: 1162); of 631 us of an early form the products
+// 2048 queries behind 14336 positions, 32/8 heads of 128 (515 GFLOP): 573 to
+// 578 us, 893 TFLOP/s (a large fp16 product: 1162), the matrix units busy for 36%
+// of it and the vector units for 46%; of 631 us of an early form the products
 // alone took 330, and 256 rows by eight waves as long as 128 by four.
 // ---------------------------------------------------------------------------
 constexpr int kRowTile = 128, kTile = 64;   // rows of a workgroup; positions of a step
