@@ -114,7 +114,7 @@ __device__ __forceinline__ float score_factor(float a, float b, float scale_log2
 // 32/8 heads of 128: 16 sequences of 4096 .. 32768
 // positions, 403 MB, in 78 us (5.1 TB/s), 64 of 200 .. 4000, 174 MB, in 38.7 (4.5);
 // 20 rows, 24 sequences of 500 .. 6000, 101 MB, in 31.0; 16/8 heads of 64, 100
-// sequences of 150 .. 1500, 52.6 MB, in 18.6.
+// sequences of 150 .. 1500, 52.6 MB, in 17.6.
 // ---------------------------------------------------------------------------
 template <int HD, int kCols>
 __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4_decode_kernel(

@@ -334,8 +334,8 @@ int citlali_hip_matvec_norm(int gguf_type, const uint8_t* w, const uint16_t* x, 
  * 32 dims of one token share two fp16 numbers, m = fp16(min) and
  * d = fp16((max - m) * fp32(1 / 15)); a dim's code is clamp(round((y - m) / d), 0, 15)
  * (ties to even; 0 where d is not above 0: values closer together than m's
- * rounding) and stands for fp16(d * code + m).  Values
- * saturate at +-61440 first; a NaN makes its 32 dims NaN.
+ * rounding) and stands for fp16(d * code + m).  Values saturate at +-61440
+ * first; a NaN makes its 32 dims NaN.
  *
  * A slot is page * page_size + row.  One kv head's part of a page
  * (page_bytes / kv_heads, heads in order):
@@ -409,11 +409,11 @@ int citlali_hip_kv4_read(const citlali_hip_kv4_cache* cache, const int32_t* slot
  * and sums are fp32; weights go into the product with V and into their sum as
  * fp16, scaled so that the largest is between 2^10 and 2^14.  A call is planned
  * for max_query queries of every sequence: where pieces of prompts stand beside
- * sequences with a few queries each, one call for either kind is faster (512
+ * sequences with a few queries each, a call for each kind is faster (512
  * queries of one sequence and one each of 32, 32/8 heads of 128: 84 us against
- * 232).  heads / kv_heads between 1 and 16,
- * heads at most 4096, nseq at most 65535, nseq * kv_heads 2^23, max_query *
- * heads 2^25, tokens * heads 2^31.  Workspace:
+ * 232 in one call).  heads / kv_heads between 1 and 16, heads at most 4096,
+ * nseq at most 65535, nseq * kv_heads 2^23, max_query * heads 2^25, tokens *
+ * heads 2^31.  Workspace:
  * citlali_hip_kv4_attention_workspace_bytes() of the same bounds, 16-byte
  * aligned (may be NULL if that is 0); calls that overlap need one each.  q and
  * out 16-byte aligned, strides multiples of 8.  nseq 0 or tokens 0 launches
