@@ -726,33 +726,170 @@ CITLALI_EXPORT size_t citlali_hip_kv4_attention_workspace_bytes(int max_context,
     return kv4_attention_workspace(max_context, max_query, nseq, tokens, heads, kv_heads, head_dim);
 }
 
+namespace {
+// citlali_hip_kv4_attention, and with masks citlali_hip_kv4_tree_attention
+int kv4_attend(const char* who, const citlali_hip_kv4_cache* cache, const uint16_t* q, long long q_stride,
+               const int32_t* query_start, const int32_t* context_lens, const uint64_t* masks,
+               const int32_t* page_table, int pages_per_seq, int nseq, int tokens, int max_query, int max_context,
+               int heads, void* workspace, size_t workspace_bytes, uint16_t* out, long long out_stride) {
+    Kv4View c{};
+    int st = check_kv4(who, cache, &c);
+    if (st) return st;
+    st = check_kv4_attention(who, max_context, max_query, nseq, tokens, heads, c.kv_heads);
+    if (st) return st;
+    REQUIRE(q && context_lens && page_table && out, "%s received a null buffer", who);
+    REQUIRE(query_start || tokens == nseq, "%s: without query_start tokens (%d) must be nseq (%d)", who, tokens, nseq);
+    REQUIRE(pages_per_seq > 0 && max_context <= (long long)pages_per_seq << c.page_shift,
+            "%s: max_context (%d) exceeds %d pages of %d", who, max_context, pages_per_seq, 1 << c.page_shift);
+    const long long row = (long long)heads * c.head_dim;
+    REQUIRE(q_stride >= row && out_stride >= row, "%s: a stride is shorter than its row", who);
+    REQUIRE(q_stride % 8 == 0 && out_stride % 8 == 0, "%s: strides must be multiples of 8", who);
+    REQUIRE(aligned(q, 16) && aligned(out, 16), "%s: q and out must be 16-byte aligned", who);
+    if (nseq == 0 || tokens == 0) return CITLALI_OK;
+    const size_t need = kv4_attention_workspace(max_context, max_query, nseq, tokens, heads, c.kv_heads, c.head_dim);
+    REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned(workspace, 16))),
+            "%s: workspace of %zu bytes needed, %zu given", who, need, workspace_bytes);
+    const Kv4Attention a{q,      q_stride,  query_start, context_lens, page_table, pages_per_seq, nseq,
+                         tokens, max_query, max_context, heads,        static_cast<float*>(workspace), out, out_stride,
+                         reinterpret_cast<const uint32_t*>(masks), 2 * ((max_query + 63) / 64)};
+    HIP_TRY(launch_kv4_attention(c, a, g_stream));
+    return CITLALI_OK;
+}
+}  // namespace
+
 CITLALI_EXPORT int citlali_hip_kv4_attention(const citlali_hip_kv4_cache* cache, const uint16_t* q,
                                              long long q_stride, const int32_t* query_start,
                                              const int32_t* context_lens, const int32_t* page_table,
                                              int pages_per_seq, int nseq, int tokens, int max_query, int max_context,
                                              int heads, void* workspace, size_t workspace_bytes, uint16_t* out,
                                              long long out_stride) {
-    Kv4View c{};
-    int st = check_kv4("kv4_attention", cache, &c);
-    if (st) return st;
-    st = check_kv4_attention("kv4_attention", max_context, max_query, nseq, tokens, heads, c.kv_heads);
-    if (st) return st;
-    REQUIRE(q && context_lens && page_table && out, "kv4_attention received a null buffer");
-    REQUIRE(query_start || tokens == nseq, "kv4_attention: without query_start tokens (%d) must be nseq (%d)", tokens,
+    return kv4_attend("kv4_attention", cache, q, q_stride, query_start, context_lens, nullptr, page_table,
+                      pages_per_seq, nseq, tokens, max_query, max_context, heads, workspace, workspace_bytes, out,
+                      out_stride);
+}
+
+// ---------------------------------------------------------------- trees of drafted tokens
+static_assert(kMaxTree == CITLALI_MAX_TREE && kKeepLayers == CITLALI_MAX_KEEP_CACHES);
+
+CITLALI_EXPORT int citlali_hip_draft_tree(const int32_t* parents, const int32_t* query_start,
+                                          const int32_t* context_lens, int nseq, int tokens, int max_query,
+                                          uint64_t* masks, int32_t* positions) {
+    REQUIRE(nseq >= 0 && tokens >= 0, "draft_tree: nseq (%d) and tokens (%d) must not be negative", nseq, tokens);
+    REQUIRE(max_query > 0 && max_query <= CITLALI_MAX_TREE, "draft_tree: max_query (%d) is not in 1..%d", max_query,
+            CITLALI_MAX_TREE);
+    REQUIRE(nseq <= 65535, "draft_tree: at most 65535 sequences");
+    REQUIRE(parents && context_lens && masks, "draft_tree received a null buffer");
+    REQUIRE(query_start || tokens == nseq, "draft_tree: without query_start tokens (%d) must be nseq (%d)", tokens,
             nseq);
-    REQUIRE(pages_per_seq > 0 && max_context <= (long long)pages_per_seq << c.page_shift,
-            "kv4_attention: max_context (%d) exceeds %d pages of %d", max_context, pages_per_seq, 1 << c.page_shift);
-    const long long row = (long long)heads * c.head_dim;
-    REQUIRE(q_stride >= row && out_stride >= row, "kv4_attention: a stride is shorter than its row");
-    REQUIRE(q_stride % 8 == 0 && out_stride % 8 == 0, "kv4_attention: strides must be multiples of 8");
-    REQUIRE(aligned(q, 16) && aligned(out, 16), "kv4_attention: q and out must be 16-byte aligned");
+    REQUIRE(aligned(masks, 8), "draft_tree: masks must be 8-byte aligned");
     if (nseq == 0 || tokens == 0) return CITLALI_OK;
-    const size_t need = kv4_attention_workspace(max_context, max_query, nseq, tokens, heads, c.kv_heads, c.head_dim);
+    HIP_TRY(launch_draft_tree(
+        DraftTree{parents, query_start, context_lens, nseq, tokens, max_query, masks, positions}, g_stream));
+    return CITLALI_OK;
+}
+
+CITLALI_EXPORT int citlali_hip_kv4_tree_attention(const citlali_hip_kv4_cache* cache, const uint16_t* q,
+                                                  long long q_stride, const int32_t* query_start,
+                                                  const int32_t* context_lens, const uint64_t* masks,
+                                                  const int32_t* page_table, int pages_per_seq, int nseq, int tokens,
+                                                  int max_query, int max_context, int heads, void* workspace,
+                                                  size_t workspace_bytes, uint16_t* out, long long out_stride) {
+    REQUIRE(masks && aligned(masks, 8), "kv4_tree_attention: masks must be given, 8-byte aligned");
+    REQUIRE(max_query <= CITLALI_MAX_TREE, "kv4_tree_attention: max_query (%d) exceeds %d", max_query,
+            CITLALI_MAX_TREE);
+    return kv4_attend("kv4_tree_attention", cache, q, q_stride, query_start, context_lens, masks, page_table,
+                      pages_per_seq, nseq, tokens, max_query, max_context, heads, workspace, workspace_bytes, out,
+                      out_stride);
+}
+
+CITLALI_EXPORT int citlali_hip_kv4_keep(const citlali_hip_kv4_cache* caches, int n_caches, const int32_t* page_table,
+                                        int pages_per_seq, int nseq, const int32_t* first, const int32_t* kept,
+                                        long long kept_stride, const int32_t* counts, int max_count) {
+    REQUIRE(n_caches > 0 && n_caches <= CITLALI_MAX_KEEP_CACHES, "kv4_keep: %d caches are not in 1..%d", n_caches,
+            CITLALI_MAX_KEEP_CACHES);
+    REQUIRE(caches, "kv4_keep received a null cache");
+    Kv4View c{};
+    Kv4Keep a{};
+    for (int i = 0; i < n_caches; ++i) {
+        const int st = check_kv4("kv4_keep", caches + i, &c);
+        if (st) return st;
+        REQUIRE(caches[i].num_pages == caches[0].num_pages && caches[i].page_size == caches[0].page_size &&
+                    caches[i].kv_heads == caches[0].kv_heads && caches[i].head_dim == caches[0].head_dim,
+                "kv4_keep: cache %d has another shape than the first", i);
+        for (int j = 0; j < i; ++j) REQUIRE(caches[j].pages != caches[i].pages, "kv4_keep: caches %d and %d are one", j, i);
+        a.pages[i] = c.pages;
+    }
+    REQUIRE(nseq >= 0 && nseq <= 65535, "kv4_keep: nseq (%d) is not in 0..65535", nseq);
+    REQUIRE(pages_per_seq > 0 && max_count >= 0, "kv4_keep: bad pages_per_seq (%d) or max_count (%d)", pages_per_seq,
+            max_count);
+    REQUIRE((long long)nseq * c.kv_heads <= kKv4MaxSeqHeads, "kv4_keep: nseq (%d) times kv_heads (%d) exceeds %lld",
+            nseq, c.kv_heads, kKv4MaxSeqHeads);
+    REQUIRE(page_table && first && kept && counts, "kv4_keep received a null buffer");
+    REQUIRE(kept_stride >= max_count, "kv4_keep: kept_stride (%lld) is shorter than max_count (%d)", kept_stride,
+            max_count);
+    if (nseq == 0 || max_count == 0) return CITLALI_OK;
+    a.page_table = page_table;
+    a.first = first;
+    a.kept = kept;
+    a.counts = counts;
+    a.kept_stride = kept_stride;
+    a.pages_per_seq = pages_per_seq;
+    a.nseq = nseq;
+    a.max_count = max_count;
+    a.layers = n_caches;
+    HIP_TRY(launch_kv4_keep(c, a, g_stream));
+    return CITLALI_OK;
+}
+
+namespace {
+constexpr int kMaxVerifyVocab = 1 << 30;              // ids and what is rounded up from them stay in 32 bits
+constexpr long long kMaxVerifyLogits = 1ll << 40;     // nseq * max_query * vocab: a wave per 2048 of them
+int check_verify(int nseq, int rows, int max_query, int vocab) {
+    REQUIRE(nseq >= 0 && rows >= 0 && vocab > 0, "verify_drafts: bad nseq (%d), rows (%d) or vocab (%d)", nseq, rows,
+            vocab);
+    REQUIRE(max_query > 0 && max_query <= CITLALI_MAX_TREE, "verify_drafts: max_query (%d) is not in 1..%d", max_query,
+            CITLALI_MAX_TREE);
+    REQUIRE(nseq <= 65535 && rows <= 65535 * CITLALI_MAX_TREE && vocab <= kMaxVerifyVocab,
+            "verify_drafts: at most 65535 sequences of %d rows and %d tokens", CITLALI_MAX_TREE, kMaxVerifyVocab);
+    REQUIRE((long long)nseq * max_query * vocab <= kMaxVerifyLogits,
+            "verify_drafts: %d sequences of %d rows of %d logits are too many", nseq, max_query, vocab);
+    return CITLALI_OK;
+}
+}  // namespace
+
+CITLALI_EXPORT size_t citlali_hip_verify_drafts_workspace_bytes(int nseq, int rows, int max_query, int vocab,
+                                                                int drafts) {
+    if (check_verify(nseq, rows, max_query, vocab) || nseq == 0) return 0;
+    return verify_drafts_workspace(nseq, rows, vocab, drafts != 0);
+}
+
+CITLALI_EXPORT int citlali_hip_verify_drafts(const void* logits, int gguf_type, long long row_stride, int vocab,
+                                             const void* draft_logits, long long draft_row_stride,
+                                             const int32_t* tokens, const int32_t* parents,
+                                             const int32_t* query_start, int nseq, int rows, int max_query,
+                                             const float* temperatures, const float* uniforms, int32_t* paths,
+                                             int32_t* counts, int32_t* next_tokens, float* token_probs,
+                                             void* workspace, size_t workspace_bytes) {
+    REQUIRE(gguf_type == 0 || gguf_type == 1, "verify_drafts: GGUF type %d is not F32 or F16", gguf_type);
+    const int st = check_verify(nseq, rows, max_query, vocab);
+    if (st) return st;
+    const int size = gguf_type == 0 ? 4 : 2;
+    REQUIRE(logits && uniforms && next_tokens, "verify_drafts received a null buffer");
+    REQUIRE(tokens || max_query == 1, "verify_drafts: drafts need tokens");
+    REQUIRE(query_start || rows == nseq, "verify_drafts: without query_start rows (%d) must be nseq (%d)", rows, nseq);
+    REQUIRE(!draft_logits || !parents, "verify_drafts: drafts of a tree are taken as given, without draft logits");
+    REQUIRE(row_stride >= vocab && (!draft_logits || draft_row_stride >= vocab),
+            "verify_drafts: a row stride is shorter than vocab (%d)", vocab);
+    REQUIRE(aligned(logits, size) && aligned(draft_logits, size), "verify_drafts: logits are not aligned to their type");
+    if (nseq == 0) return CITLALI_OK;
+    const size_t need = verify_drafts_workspace(nseq, rows, vocab, draft_logits != nullptr);
     REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned(workspace, 16))),
-            "kv4_attention: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
-    const Kv4Attention a{q,      q_stride,  query_start, context_lens, page_table, pages_per_seq, nseq,
-                         tokens, max_query, max_context, heads,        static_cast<float*>(workspace), out, out_stride};
-    HIP_TRY(launch_kv4_attention(c, a, g_stream));
+            "verify_drafts: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    HIP_TRY(launch_verify_drafts(
+        VerifyDrafts{logits, gguf_type == 1, row_stride, vocab, draft_logits, draft_row_stride, tokens, parents,
+                     query_start, nseq, rows, max_query, temperatures, uniforms, paths, counts, next_tokens,
+                     token_probs, workspace},
+        g_stream));
     return CITLALI_OK;
 }
 

@@ -1,5 +1,5 @@
-// kv4_attention.hip -- causal attention over the paged cache of 4-bit keys and
-// values.
+// kv4_attention.hip -- attention over the paged cache of 4-bit keys and values:
+// causal, or of a tree of drafted tokens.
 #include "kv4.hpp"
 
 #include <limits.h>
@@ -29,13 +29,24 @@ __device__ __forceinline__ float add_weights(half8 w, float l) {
 }
 
 // The queries of sequence `seq`: rows start .. start + n - 1 of q, the cached
-// positions that exist, and how many of them query i sees (see()).
+// positions that exist, how many of them query i sees some of (see()), and how
+// many every query from i on sees all of (all()).  In a tree the n last positions
+// are the rows' own; which of them a row sees its mask says.
+template <bool kTree>
 struct Kv4Seq {
     int start, n, context, cap;
-    __device__ int see(int i) const { return min(context - n + i + 1, cap); }
+    __device__ int see(int i) const { return min(kTree ? context : context - n + i + 1, cap); }
+    __device__ int all(int i) const { return kTree ? min(before(), cap) : see(i); }
+    __device__ int before() const { return context - n; }
 };
-__device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Attention& a, int seq) {
-    Kv4Seq s;
+// Bits p .. p + 31 of a row's mask: set before it (p < 0), clear behind it.
+__device__ __forceinline__ uint32_t tree_bits(const uint32_t* row, int words, int p) {
+    auto word = [&](int k) { return k < 0 ? 0xffffffffu : k < words ? row[k] : 0u; };
+    return __builtin_amdgcn_alignbit(word((p >> 5) + 1), word(p >> 5), p & 31);
+}
+template <bool kTree>
+__device__ __forceinline__ Kv4Seq<kTree> kv4_seq(const Kv4Attention& a, int seq) {
+    Kv4Seq<kTree> s;
     int end;
     if (a.query_start != nullptr) {
         s.start = min(max(a.query_start[seq], 0), a.tokens);
@@ -116,7 +127,7 @@ __device__ __forceinline__ float score_factor(float a, float b, float scale_log2
 // 20 rows, 24 sequences of 500 .. 6000, 101 MB, in 31.0; 16/8 heads of 64, 100
 // sequences of 150 .. 1500, 52.6 MB, in 17.6.
 // ---------------------------------------------------------------------------
-template <int HD, int kCols>
+template <int HD, int kCols, bool kTree>
 __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4_decode_kernel(
     Kv4View c, Kv4Attention a, int chunk, int n_splits, float scale_log2) {
     using L = Kv4Layout<HD>;
@@ -134,7 +145,7 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4
     // still on their way
     const int c0 = split * chunk, first_page = c0 >> c.page_shift;
     int my_page = a.page_table[(size_t)seq * a.pages_per_seq + min(first_page + lane, a.pages_per_seq - 1)];
-    const Kv4Seq s = kv4_seq(a, seq);
+    const Kv4Seq<kTree> s = kv4_seq<kTree>(a, seq);
     const int asked = min(s.n, a.max_query);
     if (asked <= 0) return;
     const int group = a.heads / c.kv_heads, rows = asked * group;
@@ -144,13 +155,13 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4
     if (((first_page + lane) << c.page_shift) >= c1 || my_page >= c.num_pages) my_page = -1;
     constexpr bool kQInLds = kCols > 1;
     half8 q[kQInLds ? 1 : kCols][kSteps];
-    int see[kCols];
+    int see[kCols];   // positions a row sees; in a tree the row (-1: none)
     half8* const q_lds = reinterpret_cast<half8*>(lds);   // [column tile][step][lane]
 #pragma unroll
     for (int n = 0; n < kCols; ++n) {
         const int r = col + 16 * n, i = r / group;
         const bool real = r < rows;
-        see[n] = real ? s.see(i) : 0;
+        see[n] = kTree ? (real ? s.start + i : -1) : real ? s.see(i) : 0;
         const uint16_t* qr = a.q + (size_t)(s.start + (real ? i : 0)) * a.q_stride +
                              (size_t)(kvh * group + (real ? r - i * group : 0)) * HD + grp * (HD / 4);
 #pragma unroll
@@ -165,7 +176,7 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4
             }
         }
     }
-    const int least = s.see(0);   // positions every row sees
+    const int least = s.all(0);   // positions every row sees
 
     const int P = 1 << c.page_shift;
     // The page of the 16 positions at p (-1: none).  Past the chunk it is the
@@ -250,15 +261,22 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4
         load_k(t + 32 * kWaves);   // in flight through the softmax and V
         __builtin_amdgcn_sched_barrier(0);
         half8 pw[kCols];
+        uint32_t sees[kTree ? kCols : 1];   // of a tree's row, the tile's positions
 #pragma unroll
         for (int n = 0; n < kCols; ++n) {
             if (!whole) {
                 asm volatile("");   // a branch: most tiles skip it
+                if constexpr (kTree)
+                    sees[n] = see[n] < 0 ? 0u
+                                         : tree_bits(a.masks + (size_t)see[n] * a.mask_words, a.mask_words,
+                                                     t - s.before());
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const bool seen = ((there >> u) & 1) && t + 16 * u + 4 * grp + i < min(see[n], c1);
+                        const int p = 16 * u + 4 * grp + i;
+                        const bool seen = ((there >> u) & 1) && (kTree ? t + p < c1 && (sees[kTree ? n : 0] >> p & 1)
+                                                                       : t + p < min(see[n], c1));
                         sc[n][u][i] = seen ? sc[n][u][i] : -INFINITY;
                     }
             }
@@ -294,6 +312,7 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4
             const uint32_t nan = kv4_hide_nan(xvp[0]) | kv4_hide_nan(xvp[1]) << 4;
             if (__builtin_amdgcn_ballot_w64(nan != 0) != 0) {
                 int first = INT_MAX;   // position of the first one in the lane's dims of O, a group
+                uint32_t where = 0;    // in a tree, of all of them in the tile
 #pragma unroll 1
                 for (int g = 0; g < HD / kKv4Group; ++g)
 #pragma unroll 1
@@ -302,12 +321,16 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4
                             __builtin_amdgcn_ballot_w64(col / (512 / HD) == g && ((nan >> b) & 1) != 0);
                         if (who == 0 || (HD == 128 ? grp : grp >> 1) != g) continue;
                         first = min(first, t + 16 * (b / 4) + 4 * (__builtin_ctzll(who) / 16) + b % 4);
+                        if constexpr (kTree)
+                            for (int y = 0; y < 4; ++y)
+                                where |= (who >> (16 * y) & 0xffff) != 0 ? 1u << (16 * (b / 4) + 4 * y + b % 4) : 0u;
                     }
 #pragma unroll
                 for (int n = 0; n < kCols; ++n)
 #pragma unroll
                     for (int d = 0; d < kDims; ++d)
-                        if (see[n] > first) o[n][d] = f32x4{NAN, NAN, NAN, NAN};
+                        if (kTree ? (sees[kTree ? n : 0] & where) != 0 : see[n] > first)
+                            o[n][d] = f32x4{NAN, NAN, NAN, NAN};
             }
         }
 #pragma unroll
@@ -395,7 +418,7 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4
 // one round trip behind the lengths.  Up to 8 chunks (head_dim 64: 16) it takes 3.2
 // to 4.7 us by one wave, by four 3.6 to 7.3; 32 chunks of 16 x 32 heads 4.7 by four,
 // 6.4 by one.
-template <int HD, int kTeam>
+template <int HD, int kTeam, bool kTree>
 __global__ __launch_bounds__(kBlk) void kv4_merge_kernel(Kv4Attention a, int group, int tile_rows, int chunk,
                                                          int n_splits, float scale_log2) {
     constexpr int kLanes = HD / 4, kTeams = kTeam * kWave / kLanes, kBatch = 4;
@@ -405,7 +428,7 @@ __global__ __launch_bounds__(kBlk) void kv4_merge_kernel(Kv4Attention a, int gro
     const int unit = kTeam > 1 ? blockIdx.x : blockIdx.x * kWaves + wave;
     const int i = unit / a.heads, head = unit - i * a.heads;
     if (i >= a.max_query) return;
-    const Kv4Seq s = kv4_seq(a, seq);
+    const Kv4Seq<kTree> s = kv4_seq<kTree>(a, seq);
     const size_t token = min(s.start + i, a.tokens - 1);   // i may be past the sequence's queries
     const size_t at = (token * a.heads + head) * n_splits;
     const int team = (kTeam > 1 ? wave * (kWave / kLanes) : 0) + lane / kLanes, d = lane % kLanes * 4;
@@ -498,7 +521,7 @@ constexpr int kPromptNotes = 10 * kWaves;   // words that a part's waves leave o
 constexpr float kSlack = 4.f, kFar = 1024.f;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-template <int HD, int kParts>
+template <int HD, int kParts, bool kTree>
 __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Attention a, int chunk,
                                                                       int n_splits, float scale_log2) {
     using L = Kv4Layout<HD>;
@@ -509,7 +532,8 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
     extern __shared__ __align__(16) float lds[];
     const int part = kParts == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kBlk);
     uint16_t* const buf = reinterpret_cast<uint16_t*>(lds) + part * 4 * kHalves;   // [2][K, V][kHalves]
-    // [2][4 waves]: bit 0, the 16 positions have a page; bit 1, nan_at says where V is NaN
+    // [2][4 waves]: bit 0, the 16 positions have a page; bit 1, nan_at says where V is
+    // NaN first (in a tree: at which of the 16)
     int* const notes = reinterpret_cast<int*>(reinterpret_cast<uint16_t*>(lds) + kParts * 4 * kHalves);
     int* const there_at = notes + part * kPromptNotes;
     int* const nan_at = there_at + 2 * kWaves;                           // [2][4 waves][4 groups of dims]
@@ -523,7 +547,7 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
     const int group = a.heads / c.kv_heads, tiles = (a.max_query * group + kRowTile - 1) / kRowTile;
     const int rest = blockIdx.z * gridDim.y + blockIdx.y, split = rest % n_splits, tile = tiles - 1 - rest / n_splits;
     const int seq = seq_of(blockIdx.x / c.kv_heads, rest, a.nseq);
-    const Kv4Seq s = kv4_seq(a, seq);
+    const Kv4Seq<kTree> s = kv4_seq<kTree>(a, seq);
     const int rows = min(s.n, a.max_query) * group, row0 = tile * kRowTile;
     if (tile < 0 || row0 >= rows) return;
     const int most = max(0, s.see((min(rows, row0 + kRowTile) - 1) / group));
@@ -551,10 +575,10 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
     }
     // positions that every / any row of the wave sees
     const int r_last = min(rows - 1, row0 + 32 * wave + 31);
-    const int wave_least = r_last < row0 + 32 * wave + 31 ? 0 : min(s.see((row0 + 32 * wave) / group), c1);
+    const int wave_least = r_last < row0 + 32 * wave + 31 ? 0 : min(s.all((row0 + 32 * wave) / group), c1);
     const int wave_most = row0 + 32 * wave >= rows ? 0 : min(s.see(r_last / group), c1);
 
-    const int least = min(s.see(row0 / group), c1);   // positions that every row of the workgroup sees
+    const int least = min(s.all(row0 / group), c1);   // positions that every row of the workgroup sees
 
     // ---- the wave's 16 positions of a tile: pages, loads, dequantisation ----
     const int P = 1 << c.page_shift;
@@ -603,7 +627,11 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
 #pragma unroll 1
         for (int dims = 0; dims < HD / kKv4Group; ++dims) {
             int first = nan != 0 && t16 / (512 / HD) == dims ? x_pos + 4 * vb + __builtin_ctz(nan) : INT_MAX;
-            for (int d = 1; d < kWave; d <<= 1) first = min(first, __shfl_xor(first, d, kWave));
+            if constexpr (kTree) first = t16 / (512 / HD) == dims ? (int)(nan << 4 * vb) : 0;
+            for (int d = 1; d < kWave; d <<= 1) {
+                const int other = __shfl_xor(first, d, kWave);
+                first = kTree ? first | other : min(first, other);
+            }
             if (lane == 0) nan_at[(b * kWaves + wave) * 4 + dims] = first;
         }
     };
@@ -675,13 +703,21 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
             __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
+        uint32_t sees[kTree ? 2 : 1];   // of a tree's row, the tile's positions
         if (!whole) {
+            if constexpr (kTree) {
+                const uint32_t* row = a.masks + (size_t)(s.start + i) * a.mask_words;
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    sees[u] = real ? tree_bits(row, a.mask_words, t + 32 * u - s.before()) : 0u;
+            }
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int p = 32 * u + 8 * (e / 4) + 4 * half + e % 4;
-                    const bool seen = t + p < see && ((there >> (p >> 4) * 2) & 1);
+                    const bool seen = t + p < see && ((there >> (p >> 4) * 2) & 1) &&
+                                      (!kTree || (sees[kTree ? u : 0] >> (p & 31) & 1));
                     sc[u][e] = seen ? sc[u][e] : -INFINITY;
                 }
         }
@@ -689,15 +725,21 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
 #pragma unroll
             for (int y = 0; y < 2; ++y) {   // elements e with e / 4 % 2 = y are of one group of dims
                 int first = INT_MAX;
+                bool meets = false;   // in a tree: the row sees one of them
 #pragma unroll 1
                 for (int w = 0; w < kWaves; ++w)
-                    if ((there >> (2 * w)) & 2)
-                        first = min(first, nan_at[(b * kWaves + w) * 4 + (HD == 128 ? 2 * y + half : y)]);
+                    if ((there >> (2 * w)) & 2) {
+                        const int at = nan_at[(b * kWaves + w) * 4 + (HD == 128 ? 2 * y + half : y)];
+                        if constexpr (kTree)
+                            meets |= ((w < 2 ? sees[0] : sees[1]) >> (16 * (w & 1)) & (uint32_t)at) != 0;
+                        else
+                            first = min(first, at);
+                    }
 #pragma unroll
                 for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        if (e / 4 % 2 == y) o[d][e] = see > first ? NAN : o[d][e];
+                        if (e / 4 % 2 == y) o[d][e] = (kTree ? meets : see > first) ? NAN : o[d][e];
             }
         }
         float mt = -INFINITY;
@@ -876,7 +918,7 @@ Kv4Plan kv4_plan(int max_context, int max_query, int nseq, int heads, int kv_hea
     return p;
 }
 
-template <int HD>
+template <int HD, bool kTree>
 hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
     const Kv4Plan p = kv4_plan(a.max_context, a.max_query, a.nseq, a.heads, c.kv_heads);
     const float scale_log2 = 1.44269504088896340736f / sqrtf((float)HD);
@@ -889,14 +931,14 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
         hipError_t e;
         if (last && a.max_context > kTwoPartContext && (long long)units * c.kv_heads * a.nseq <= kTwoPartBlocks) {
             const int lds = 2 * part + 2 * kBlk * (int)sizeof(float);
-            e = allow_lds<kv4_prompt_kernel<HD, 2>>(lds);
+            e = allow_lds<kv4_prompt_kernel<HD, 2, kTree>>(lds);
             if (e != hipSuccess) return e;
-            launch_kernel_in_call(last, kv4_prompt_kernel<HD, 2>, grid, dim3(2 * kBlk), lds, s, c, a, p.chunk,
+            launch_kernel_in_call(last, kv4_prompt_kernel<HD, 2, kTree>, grid, dim3(2 * kBlk), lds, s, c, a, p.chunk,
                                   p.n_splits, scale_log2);
         } else {
-            e = allow_lds<kv4_prompt_kernel<HD, 1>>(part);
+            e = allow_lds<kv4_prompt_kernel<HD, 1, kTree>>(part);
             if (e != hipSuccess) return e;
-            launch_kernel_in_call(last, kv4_prompt_kernel<HD, 1>, grid, dim3(kBlk), part, s, c, a, p.chunk, p.n_splits,
+            launch_kernel_in_call(last, kv4_prompt_kernel<HD, 1, kTree>, grid, dim3(kBlk), part, s, c, a, p.chunk, p.n_splits,
                                   scale_log2);
         }
     } else {
@@ -907,11 +949,11 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
             launch_kernel_in_call(last, kernel, grid, dim3(kBlk), lds, s, c, a, p.chunk, p.n_splits, scale_log2);
         };
         if (p.cols == 1)
-            go(kv4_decode_kernel<HD, 1>);
+            go(kv4_decode_kernel<HD, 1, kTree>);
         else if (p.cols == 2)
-            go(kv4_decode_kernel<HD, 2>);
+            go(kv4_decode_kernel<HD, 2, kTree>);
         else
-            go(kv4_decode_kernel<HD, 3>);
+            go(kv4_decode_kernel<HD, 3, kTree>);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || last) return e;
@@ -919,10 +961,10 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
     const long long units = (long long)a.max_query * a.heads;
     const int tile_rows = p.few ? kFewRows : kRowTile;
     if (p.n_splits <= 4 * kWave / (HD / 4))
-        launch_kernel(kv4_merge_kernel<HD, 1>, dim3((unsigned)((units + kWaves - 1) / kWaves), a.nseq), dim3(kBlk), 0,
+        launch_kernel(kv4_merge_kernel<HD, 1, kTree>, dim3((unsigned)((units + kWaves - 1) / kWaves), a.nseq), dim3(kBlk), 0,
                       s, a, group, tile_rows, p.chunk, p.n_splits, scale_log2);
     else
-        launch_kernel(kv4_merge_kernel<HD, kWaves>, dim3((unsigned)units, a.nseq), dim3(kBlk), 0, s, a, group,
+        launch_kernel(kv4_merge_kernel<HD, kWaves, kTree>, dim3((unsigned)units, a.nseq), dim3(kBlk), 0, s, a, group,
                       tile_rows, p.chunk, p.n_splits, scale_log2);
     return hipGetLastError();
 }
@@ -937,7 +979,8 @@ size_t kv4_attention_workspace(int max_context, int max_query, int nseq, int tok
 }
 
 hipError_t launch_kv4_attention(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
-    return c.head_dim == 128 ? launch_for<128>(c, a, s) : launch_for<64>(c, a, s);
+    if (a.masks) return c.head_dim == 128 ? launch_for<128, true>(c, a, s) : launch_for<64, true>(c, a, s);
+    return c.head_dim == 128 ? launch_for<128, false>(c, a, s) : launch_for<64, false>(c, a, s);
 }
 
 }  // namespace citlali::hip

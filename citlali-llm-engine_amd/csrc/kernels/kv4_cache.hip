@@ -319,6 +319,79 @@ __global__ __launch_bounds__(kBlk) void kv4_read_kernel(Kv4View c, const int32_t
     __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(v_out + at));
 }
 
+// ---------------------------------------------------------------------------
+// Position first[s] + kept[s][j] of sequence s moves to first[s] + j.  One
+// workgroup per (kv head, sequence, cache) takes its moves in order, 4 kTokens at a
+// time: all are read before any is written, so that a position which one of them
+// takes may be where another comes from.  Later moves come from behind (kept
+// ascends), so the next ones are read before these are written.
+// A token's part of a head is HD / 2 lanes' work: HD / 8 words of K codes, HD / 32
+// of K params, then HD / 4 pairs of bytes of V codes and HD / 16 of V params.
+// ---------------------------------------------------------------------------
+template <int HD>
+__global__ __launch_bounds__(kBlk) void kv4_keep_kernel(Kv4View c, Kv4Keep a) {
+    using L = Kv4Layout<HD>;
+    constexpr int kLanes = HD / 2, kRows = kBlk / kLanes, kTokens = 4;
+    constexpr int kWords = HD / 8 + HD / 32;   // lanes that have a word of K
+    const int kvh = blockIdx.x, seq = blockIdx.y;
+    c.pages = a.pages[blockIdx.z];
+    const int n = min(a.counts[seq], a.max_count), first = a.first[seq];
+    if (n <= 0 || first < 0) return;
+    const int l = threadIdx.x % kLanes, mine = threadIdx.x / kLanes;
+    const int32_t* kept = a.kept + (size_t)seq * a.kept_stride;
+    const int32_t* table = a.page_table + (size_t)seq * a.pages_per_seq;
+    const int P = 1 << c.page_shift;
+    // the lane's bytes of the token at a position; null: a position without a page
+    auto place = [&](long long position) -> uint8_t* {
+        const long long at = position >> c.page_shift;
+        if (at >= a.pages_per_seq) return nullptr;
+        const int page = table[at];
+        if (page < 0 || page >= c.num_pages) return nullptr;
+        uint8_t* base = kv4_head<HD>(c, page, kvh);
+        const int o = (int)position & (P - 1);
+        if (l < HD / 8) return base + o * L::kCodes + 4 * l;
+        if (l < kWords) return base + L::k_params(P) + o * L::kParams + 4 * (l - HD / 8);
+        const int h = l - kWords;
+        if (h < HD / 4) return base + L::v_codes(P) + (((o >> 2) * (HD / 4) + h) * 4 + (o & 3)) * 2;
+        if (h < HD / 4 + HD / 16) return base + L::v_params(P) + (((o >> 2) * (HD / 16) + h - HD / 4) * 4 + (o & 3)) * 2;
+        return nullptr;
+    };
+    auto load = [&](int j0, uint32_t (&v)[kTokens], uint8_t* (&to)[kTokens]) {
+#pragma unroll
+        for (int k = 0; k < kTokens; ++k) {
+            const int j = j0 + k * kRows + mine, from = j < n ? kept[j] : -1;
+            to[k] = nullptr;
+            if (from <= j) continue;   // already there, or behind: nothing moves
+            const uint8_t* src = place((long long)first + from);
+            if (src == nullptr) continue;
+            to[k] = place((long long)first + j);
+            if (l < kWords)
+                v[k] = *reinterpret_cast<const uint32_t*>(src);
+            else
+                v[k] = *reinterpret_cast<const uint16_t*>(src);
+        }
+    };
+    uint32_t v[kTokens], w[kTokens];
+    uint8_t *to[kTokens], *to_next[kTokens];
+    load(0, v, to);
+    for (int j0 = 0; j0 < n; j0 += kTokens * kRows) {
+        wait_vm<0>();   // in registers, not on the way, before another wave may write there
+        __syncthreads();
+        load(j0 + kTokens * kRows, w, to_next);
+#pragma unroll
+        for (int k = 0; k < kTokens; ++k) {
+            if (to[k] != nullptr) {
+                if (l < kWords)
+                    *reinterpret_cast<uint32_t*>(to[k]) = v[k];
+                else
+                    *reinterpret_cast<uint16_t*>(to[k]) = (uint16_t)v[k];
+            }
+            v[k] = w[k];
+            to[k] = to_next[k];
+        }
+    }
+}
+
 }  // namespace
 
 bool kv4_shape_ok(int page_size, int head_dim) {
@@ -364,6 +437,15 @@ hipError_t launch_kv4_read(const Kv4View& c, const int32_t* slots, int count, ui
         launch_kernel(kv4_read_kernel<128>, grid, dim3(kBlk), 0, s, c, slots, count, k_out, v_out);
     else
         launch_kernel(kv4_read_kernel<64>, grid, dim3(kBlk), 0, s, c, slots, count, k_out, v_out);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv4_keep(const Kv4View& c, const Kv4Keep& a, hipStream_t s) {
+    const dim3 grid(c.kv_heads, a.nseq, a.layers);
+    if (c.head_dim == 128)
+        launch_kernel(kv4_keep_kernel<128>, grid, dim3(kBlk), 0, s, c, a);
+    else
+        launch_kernel(kv4_keep_kernel<64>, grid, dim3(kBlk), 0, s, c, a);
     return hipGetLastError();
 }
 

@@ -233,10 +233,63 @@ struct Kv4Attention {
     float* workspace;
     uint16_t* out;
     long long out_stride;
+    // a tree of drafts: bit j of row r's mask_words words says whether it sees the
+    // row j of its sequence; null: causal
+    const uint32_t* masks;
+    int mask_words;
 };
 size_t kv4_attention_workspace(int max_context, int max_query, int nseq, int tokens, int heads, int kv_heads,
                                int head_dim);
 hipError_t launch_kv4_attention(const Kv4View& c, const Kv4Attention& a, hipStream_t s);
+
+// Positions first[s] + kept[s][j] move to first[s] + j, in `layers` caches.
+constexpr int kKeepLayers = 128;   // pages of one launch's layers: 1 KB of arguments
+struct Kv4Keep {
+    uint8_t* pages[kKeepLayers];
+    const int32_t *page_table, *first, *kept, *counts;
+    long long kept_stride;
+    int pages_per_seq, nseq, max_count, layers;
+};
+hipError_t launch_kv4_keep(const Kv4View& c, const Kv4Keep& a, hipStream_t s);
+
+// ---- trees of drafted tokens (drafts.hip) ----
+constexpr int kMaxTree = 256;   // rows of a sequence
+// Sequence seq's rows start .. start + n - 1, of `total` that it has.
+struct DraftRows {
+    int start, n, total;
+};
+__device__ __forceinline__ DraftRows draft_rows(const int32_t* query_start, int seq, int rows, int max_query) {
+    DraftRows d{seq, 1, 1};
+    if (query_start != nullptr) {
+        d.start = min(max(query_start[seq], 0), rows);
+        d.total = min(max(query_start[seq + 1], d.start), rows) - d.start;
+    }
+    d.n = min(d.total, max_query);
+    return d;
+}
+struct DraftTree {
+    const int32_t *parents, *query_start, *context_lens;
+    int nseq, tokens, max_query;
+    uint64_t* masks;
+    int32_t* positions;
+};
+hipError_t launch_draft_tree(const DraftTree& a, hipStream_t s);
+struct VerifyDrafts {
+    const void* logits;
+    bool half;
+    long long stride;
+    int vocab;
+    const void* draft;   // logits, or null: the drafts are taken as given
+    long long draft_stride;
+    const int32_t *tokens, *parents, *query_start;
+    int nseq, rows, max_query;
+    const float *temperatures, *uniforms;
+    int32_t *paths, *counts, *next_tokens;
+    float* token_probs;
+    void* workspace;
+};
+size_t verify_drafts_workspace(int nseq, int rows, int vocab, bool drafts);
+hipError_t launch_verify_drafts(const VerifyDrafts& a, hipStream_t s);
 
 // ---- log probabilities (logprobs.hip) ----
 struct Logprobs {

@@ -465,6 +465,53 @@ def kv4_attention(cache, q, q_stride: int, query_start, context_lens, page_table
               workspace_bytes, _at(out), out_stride)
 
 
+# ---- trees of drafted tokens --------------------------------------------------
+def draft_tree(parents, query_start, context_lens, nseq: int, tokens: int, max_query: int, masks, positions) -> None:
+    """Which rows of its tree each row sees, uint64 [tokens][(max_query + 63) // 64],
+    and its position (None: not wanted).  See citlali_hip_draft_tree."""
+    _lib.call("citlali_hip_draft_tree", _at(parents), _at(query_start), _at(context_lens), nseq, tokens, max_query,
+              _at(masks), _at(positions))
+
+
+def kv4_tree_attention(cache, q, q_stride: int, query_start, context_lens, masks, page_table, pages_per_seq: int,
+                       nseq: int, tokens: int, max_query: int, max_context: int, heads: int, workspace,
+                       workspace_bytes: int, out, out_stride: int) -> None:
+    """kv4_attention where a query sees the positions before its tree and those
+    that its mask names; the same workspace.  See citlali_hip_kv4_tree_attention."""
+    _lib.call("citlali_hip_kv4_tree_attention", cache, _at(q), q_stride, _at(query_start), _at(context_lens),
+              _at(masks), _at(page_table), pages_per_seq, nseq, tokens, max_query, max_context, heads, _at(workspace),
+              workspace_bytes, _at(out), out_stride)
+
+
+def verify_drafts_workspace_bytes(nseq: int, rows: int, max_query: int, vocab: int, drafts: bool) -> int:
+    return int(_lib.load().citlali_hip_verify_drafts_workspace_bytes(nseq, rows, max_query, vocab, int(drafts)))
+
+
+def verify_drafts(logits, kind: str, row_stride: int, vocab: int, draft_logits, draft_row_stride: int, tokens, parents,
+                  query_start, nseq: int, rows: int, max_query: int, temperatures, uniforms, paths, counts,
+                  next_tokens, token_probs, workspace, workspace_bytes: int) -> None:
+    """The path of drafted tokens that stays and the token after it; kind in
+    {"fp32", "fp16"}; draft_logits None: the drafts are taken as given; parents
+    None: chains.  See citlali_hip_verify_drafts."""
+    _lib.call("citlali_hip_verify_drafts", _at(logits), _LOGIT_TYPE[kind], row_stride, vocab, _at(draft_logits),
+              draft_row_stride, _at(tokens), _at(parents), _at(query_start), nseq, rows, max_query, _at(temperatures),
+              _at(uniforms), _at(paths), _at(counts), _at(next_tokens), _at(token_probs), _at(workspace),
+              workspace_bytes)
+
+
+def kv4_caches(caches):
+    """The caches of a model's layers, for kv4_keep."""
+    return (_lib.Kv4Cache * len(caches))(*caches)
+
+
+def kv4_keep(caches, page_table, pages_per_seq: int, nseq: int, first, kept, kept_stride: int, counts,
+             max_count: int) -> None:
+    """Moves positions first + kept[j] of each sequence to first + j, in every
+    cache of `caches` (kv4_caches).  See citlali_hip_kv4_keep."""
+    _lib.call("citlali_hip_kv4_keep", caches, len(caches), _at(page_table), pages_per_seq, nseq, _at(first), _at(kept),
+              kept_stride, _at(counts), max_count)
+
+
 # ---- log probabilities --------------------------------------------------------
 _LOGIT_TYPE = {"fp32": 0, "fp16": 1}
 

@@ -425,6 +425,102 @@ int citlali_hip_kv4_attention(const citlali_hip_kv4_cache* cache, const uint16_t
 size_t citlali_hip_kv4_attention_workspace_bytes(int max_context, int max_query, int nseq, int tokens, int heads,
                                                  int kv_heads, int head_dim);
 
+/* ---- trees of drafted tokens (no reference counterpart) -------------------- *
+ * Speculative decoding: a step drafts several tokens of each sequence, the model
+ * runs over all of them at once, and some of them stay.  A sequence's rows are
+ * query_start[s] .. query_start[s + 1] - 1 as in citlali_hip_kv4_attention, at
+ * most CITLALI_MAX_TREE.  Row 0 is the token the step before ended with; a row's
+ * parent is an earlier row of the sequence, by its index there, or -1 (only the
+ * positions before the tree are above it).  A chain of drafts has parents -1, 0,
+ * 1, ...  One step, per layer the third and fourth call:
+ *   citlali_hip_draft_tree         masks and positions of the rows
+ *   (embedding, projections)
+ *   citlali_hip_kv4_append         the rows' K and V, in order, as the sequence's
+ *                                  last slots, rotated by those positions
+ *   citlali_hip_kv4_tree_attention
+ *   (output projection)
+ *   citlali_hip_verify_drafts      the path that stays, and the token after it
+ *   citlali_hip_kv4_keep           the path's K and V moved up, in all layers   */
+#define CITLALI_MAX_TREE 256
+
+/* masks [tokens][(max_query + 63) / 64]: bit j of a row's mask (bit j % 64 of word
+ * j / 64) says whether the row sees row j of its sequence, that is itself and the
+ * rows above it.  positions (may be NULL) [tokens]: the row's place in the text,
+ * context_lens[s] - rows + rows above it, with the sequence's rows among the
+ * context_lens[s] cached positions.  A row whose parent is neither -1 nor an
+ * earlier row, and every row below it, sees nothing and has position -1.  Rows
+ * past max_query, and past the last sequence's, are left as they were.  masks
+ * 8-byte aligned; nseq at most 65535.  nseq 0 or tokens 0 launches nothing. */
+int citlali_hip_draft_tree(const int32_t* parents, const int32_t* query_start, const int32_t* context_lens, int nseq,
+                           int tokens, int max_query, uint64_t* masks, int32_t* positions);
+
+/* citlali_hip_kv4_attention, with its arguments and limits, but for what a query
+ * sees: the positions before the tree, 0 .. context_lens[s] - n - 1 of a sequence
+ * with n rows, and position context_lens[s] - n + j where bit j of its mask is set
+ * (any masks of that layout, not only a tree's; bits past the row count are
+ * ignored).  max_query is at most CITLALI_MAX_TREE.  Workspace:
+ * citlali_hip_kv4_attention_workspace_bytes() of the same bounds. */
+int citlali_hip_kv4_tree_attention(const citlali_hip_kv4_cache* cache, const uint16_t* q, long long q_stride,
+                                   const int32_t* query_start, const int32_t* context_lens, const uint64_t* masks,
+                                   const int32_t* page_table, int pages_per_seq, int nseq, int tokens, int max_query,
+                                   int max_context, int heads, void* workspace, size_t workspace_bytes, uint16_t* out,
+                                   long long out_stride);
+
+/* Which drafted tokens stay, so that the tokens that come out are distributed as
+ * if the model had drawn them one by one.  Row r's logits (element r * row_stride
+ * on; gguf_type 0 = F32 or 1 = F16) are the model's after row r's token; p is
+ * softmax(logits / temperatures[s]) (NULL: 1), or, where the temperature is not
+ * above 0, 1 for the largest logit (the lowest id of equal ones).  uniforms has a
+ * random number of [0, 1) for each row.
+ *  - From row 0 on, the children of the current row are tried in order.  Child c,
+ *    whose token is x, becomes the current row if u_c R < p(x), where R is 1 for a
+ *    row's first child; else R loses p(x), and p(x) becomes 0.
+ *  - The next token is drawn from what is left of p at the row where the path
+ *    ends: the first id whose running sum exceeds u_0 times the total.
+ *  - With draft_logits (chains only: parents NULL), row r's are those that row
+ *    r + 1's token was drawn from, at the same temperature, q their distribution.
+ *    The token becomes the current row if u q(x) < p(x); else what is left is
+ *    max(p - q, 0).
+ *  - Where nothing is left (numbers outside [0, 1), which count as the nearest in
+ *    it, NaN as 0), the next token is drawn from p as it was.
+ * parents NULL: chains.  query_start NULL: one row each, whose next token is drawn
+ * (then tokens may be NULL).  A token outside [0, vocab) and one whose parent is
+ * not an earlier row are never accepted; a logit of -inf is a token that cannot
+ * come.  A row with a NaN, +inf or nothing above -inf has no distribution: no
+ * child of it is accepted, and if the path ends there the next token is -1; with
+ * such draft logits a row's child is rejected and the token drawn from p.
+ * Outputs: paths [nseq][max_query], the path's rows by their index in the
+ * sequence, row 0 first, then -1; counts [nseq], their number (0 for a sequence
+ * without rows); next_tokens [nseq] (-1 likewise); token_probs [rows], each
+ * token's p under its parent row, 0 for row 0.  paths, counts and token_probs may
+ * be NULL.  Probabilities and their sums are 64-bit floats.  Rows past max_query
+ * take no part.  nseq at most 65535, vocab 2^30, nseq * max_query * vocab 2^40.
+ * Workspace: citlali_hip_verify_drafts_workspace_bytes() (drafts: with draft
+ * logits or not), 16-byte aligned; calls that overlap need one each.  nseq 0
+ * launches nothing. */
+int citlali_hip_verify_drafts(const void* logits, int gguf_type, long long row_stride, int vocab,
+                              const void* draft_logits, long long draft_row_stride, const int32_t* tokens,
+                              const int32_t* parents, const int32_t* query_start, int nseq, int rows, int max_query,
+                              const float* temperatures, const float* uniforms, int32_t* paths, int32_t* counts,
+                              int32_t* next_tokens, float* token_probs, void* workspace, size_t workspace_bytes);
+size_t citlali_hip_verify_drafts_workspace_bytes(int nseq, int rows, int max_query, int vocab, int drafts);
+
+/* Moves cached tokens up within their sequences, in the caches of many layers at
+ * once (same shape and page tables; n_caches at most CITLALI_MAX_KEEP_CACHES):
+ * position first[s] + kept[s * kept_stride + j] of sequence s goes to position
+ * first[s] + j, for j below counts[s] and max_count.  kept ascends.  After
+ * citlali_hip_verify_drafts, first is the length before the tree, kept and counts
+ * are its paths and counts, and the sequence's new length first[s] + counts[s];
+ * any other positions of a sequence may be dropped the same way.  An entry not
+ * above its j, and one whose position (or the one it goes to) has no page, moves
+ * nothing; a negative first moves nothing of the sequence.  Sequences that share a
+ * page must not move anything to it.  nseq * kv_heads at most 2^23.  nseq or
+ * max_count 0 launches nothing. */
+#define CITLALI_MAX_KEEP_CACHES 128
+int citlali_hip_kv4_keep(const citlali_hip_kv4_cache* caches, int n_caches, const int32_t* page_table,
+                         int pages_per_seq, int nseq, const int32_t* first, const int32_t* kept,
+                         long long kept_stride, const int32_t* counts, int max_count);
+
 /* ---- log probabilities (no reference counterpart) -------------------------- *
  * For each of `rows` rows of logits (row r at element r * row_stride; gguf_type
  * 0 = F32 or 1 = F16), with natural logarithms and fp32 sums:
