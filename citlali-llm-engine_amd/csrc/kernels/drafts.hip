@@ -87,13 +87,47 @@ __device__ __forceinline__ double weight(float x, float m, double c) {
     return x == -INFINITY ? 0. : exp2_64(((double)x - (double)m) * c);
 }
 
-template <typename T, typename F>
-__device__ __forceinline__ T wave_fold(T v, F f) {
-    for (int o = 1; o < kWave; o <<= 1) v = f(v, __shfl_xor(v, o, kWave));
-    return v;
+// ---- 64-bit moves between lanes --------------------------------------------------
+template <int Ctrl, int kRows = 0xF>
+__device__ __forceinline__ double dpp64(double v) {   // 0 where no lane is meant
+    const u32x2 w = __builtin_bit_cast(u32x2, v);
+    return __builtin_bit_cast(double, u32x2{(uint32_t)__builtin_amdgcn_update_dpp(0, (int)w.x, Ctrl, kRows, 0xF, false),
+                                            (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w.y, Ctrl, kRows, 0xF, false)});
+}
+__device__ __forceinline__ double lane64(double v, int lane) {
+    const u32x2 w = __builtin_bit_cast(u32x2, v);
+    return __builtin_bit_cast(double, u32x2{(uint32_t)__builtin_amdgcn_readlane((int)w.x, lane),
+                                            (uint32_t)__builtin_amdgcn_readlane((int)w.y, lane)});
+}
+// Sum over each row of 16 lanes, in all of them.
+__device__ __forceinline__ double row_sum64(double v) {
+    v += dpp64<kDppXor1>(v);
+    v += dpp64<kDppXor2>(v);
+    v += dpp64<DppRor<4>::value>(v);
+    return v + dpp64<DppRor<8>::value>(v);
 }
 __device__ __forceinline__ double wave_sum64(double v) {
-    return wave_fold(v, [](double a, double b) { return a + b; });
+    v = row_sum64(v);
+    return (lane64(v, 0) + lane64(v, 16)) + (lane64(v, 32) + lane64(v, 48));
+}
+// Sum over the lanes up to this one.
+__device__ __forceinline__ double wave_scan64(double v) {
+    v += dpp64<0x111>(v);   // row_shr 1, 2, 4, 8
+    v += dpp64<0x112>(v);
+    v += dpp64<0x114>(v);
+    v += dpp64<0x118>(v);
+    v += dpp64<0x142, 0xA>(v);   // lane 15 of a row to the next row, then lane 31 to the upper half
+    return v + dpp64<0x143, 0xC>(v);
+}
+__device__ __forceinline__ float row_max(float v) {
+    v = fmaxf(v, dpp<kDppXor1>(v));
+    v = fmaxf(v, dpp<kDppXor2>(v));
+    v = fmaxf(v, dpp<DppRor<4>::value>(v));
+    return fmaxf(v, dpp<DppRor<8>::value>(v));
+}
+__device__ __forceinline__ int row_min(int v) {
+    for (int o = 1; o < 16; o <<= 1) v = min(v, __shfl_xor(v, o, kWave));
+    return v;
 }
 
 template <bool kHalf>
@@ -142,10 +176,46 @@ __device__ __forceinline__ float temperature(const VerifyDrafts& a, int seq) {
 }
 constexpr double kLog2e = 1.4426950408889634074;
 
+// A segment's logits as one wave has them: element e of a lane is id
+// seg * kSeg + (e / kVec * 64 + lane) * kVec + e % kVec; -inf behind the last id.
+template <bool kHalf>
+struct Logits {
+    static constexpr int kVec = kHalf ? 8 : 4;
+    float x[kPer];
+    __device__ Logits(const void* row, int vocab, int seg, int lane) {
+        const int id0 = seg * kSeg;
+        if (id0 + kSeg <= vocab) {
+            const char* at = static_cast<const char*>(row) + (size_t)id0 * (kHalf ? 2 : 4) + lane * 16;
+#pragma unroll
+            for (int l = 0; l < kPer / kVec; ++l) {
+                const u32x4 v = *reinterpret_cast<const u32x4_a2*>(at + l * kWave * 16);
+#pragma unroll
+                for (int e = 0; e < kVec; ++e)
+                    x[l * kVec + e] = kHalf ? h2f((uint16_t)(v[e / 2] >> (e % 2 * 16))) : __uint_as_float(v[e]);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+                const int id = id_of(seg, e, lane);
+                x[e] = id < vocab ? logit<kHalf>(row, id) : -INFINITY;
+            }
+        }
+    }
+    __device__ static int id_of(int seg, int e, int lane) {
+        return seg * kSeg + (e / kVec * kWave + lane) * kVec + e % kVec;
+    }
+    // of the lane's weights against m > -inf
+    __device__ double sum(double m, double c) const {
+        double s[2] = {0., 0.};
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) s[e % 2] += exp2_64(((double)x[e] - m) * c);
+        return s[0] + s[1];
+    }
+};
+
 // Workgroup (4 segments, row, sequence), a segment a wave.
 template <bool kHalf>
 __global__ __launch_bounds__(kBlk) void verify_sums_kernel(VerifyDrafts a, int segs) {
-    constexpr int kVec = kHalf ? 8 : 4, kLoads = kPer / kVec;
     const int seq = blockIdx.z;
     const bool draft = (int)blockIdx.y >= a.max_query;
     const int i = blockIdx.y - (draft ? a.max_query : 0);
@@ -156,351 +226,385 @@ __global__ __launch_bounds__(kBlk) void verify_sums_kernel(VerifyDrafts a, int s
     if (seg >= segs) return;
     const float t = temperature(a, seq);
     const int r = rows.start + i;
-    const void* row = draft ? logit_row<kHalf>(a.draft, a.draft_stride, r) : logit_row<kHalf>(a.logits, a.stride, r);
-    const int id0 = seg * kSeg;
-    float x[kPer];
-    if (id0 + kSeg <= a.vocab) {
-        const char* at = static_cast<const char*>(row) + (size_t)id0 * (kHalf ? 2 : 4) + lane * 16;
+    const Logits<kHalf> x(draft ? logit_row<kHalf>(a.draft, a.draft_stride, r) : logit_row<kHalf>(a.logits, a.stride, r),
+                          a.vocab, seg, lane);
+    float top = x.x[0];
 #pragma unroll
-        for (int l = 0; l < kLoads; ++l) {
-            u32x4 v = *reinterpret_cast<const u32x4_a2*>(at + l * kWave * 16);
-#pragma unroll
-            for (int e = 0; e < kVec; ++e)
-                x[l * kVec + e] = kHalf ? h2f((uint16_t)(v[e / 2] >> (e % 2 * 16))) : __uint_as_float(v[e]);
-        }
-    } else {
-#pragma unroll
-        for (int l = 0; l < kPer; ++l) {
-            const int id = id0 + (l / kVec * kWave + lane) * kVec + l % kVec;
-            x[l] = id < a.vocab ? logit<kHalf>(row, id) : -INFINITY;
-        }
-    }
-    float top = x[0];
-#pragma unroll
-    for (int l = 1; l < kPer; ++l) top = __builtin_elementwise_maximum(top, x[l]);   // a NaN stays
+    for (int e = 1; e < kPer; ++e) top = __builtin_elementwise_maximum(top, x.x[e]);   // a NaN stays
     const bool bad = __builtin_amdgcn_ballot_w64(!(top < INFINITY)) != 0;
     top = wave_max(top);
     Segment out{0., bad ? NAN : top, 0};
     if (!bad && top > -INFINITY) {
         if (t > 0.f) {
-            const double c = kLog2e / (double)t, m = top;
-            double s[2] = {0., 0.};
-#pragma unroll
-            for (int l = 0; l < kPer; ++l) s[l % 2] += exp2_64(((double)x[l] - m) * c);
-            out.sum = wave_sum64(s[0] + s[1]);
+            out.sum = wave_sum64(x.sum(top, kLog2e / (double)t));
         } else {
             int first = INT_MAX;
 #pragma unroll
-            for (int l = kPer - 1; l >= 0; --l)
-                if (x[l] == top) first = id0 + (l / kVec * kWave + lane) * kVec + l % kVec;
-            out.first = wave_fold(first, [](int p, int q) { return min(p, q); });
-            out.sum = 1.;
+            for (int e = kPer - 1; e >= 0; --e)
+                if (x.x[e] == top) first = x.id_of(seg, e, lane);
+            first = row_min(first);
+            out.first = min(min(__builtin_amdgcn_readlane(first, 0), __builtin_amdgcn_readlane(first, 16)),
+                            min(__builtin_amdgcn_readlane(first, 32), __builtin_amdgcn_readlane(first, 48)));
         }
     }
     if (lane == 0) work_of(a, segs).segments[((size_t)(draft ? a.rows : 0) + r) * segs + seg] = out;
 }
 
-// Largest logit, sum and first id of a row from its segments, by one wave.
+// ---- a draw by a workgroup of kWalk threads ---------------------------------------
+constexpr int kWalk = 512, kWalkWaves = kWalk / kWave;
+constexpr int kRun = kSeg / kWalk;   // ids of a thread
+
+// Sums over the threads before this one, and over all.
+struct Scan {
+    double before, total;
+};
+__device__ Scan block_scan(double v, double* room) {
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const double run = wave_scan64(v);
+    if (lane == kWave - 1) room[wave] = run;
+    __syncthreads();
+    double base = 0., total = 0.;
+#pragma unroll
+    for (int w = 0; w < kWalkWaves; ++w) {
+        base = w == wave ? total : base;
+        total += room[w];
+    }
+    return Scan{base + (run - v), total};
+}
+
+// The `at` and `before` of the first thread that is `here`, and the `at` of the last
+// that has `any` (INT_MAX and -1 without one).
+struct Found {
+    int at, last;
+    double before;
+};
+__device__ Found block_find(bool here, bool any, int at, double before, Found* room) {
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint64_t who = __builtin_amdgcn_ballot_w64(here), have = __builtin_amdgcn_ballot_w64(any);
+    if (lane == (who != 0 ? __builtin_ctzll(who) : 0)) {
+        room[wave].at = who != 0 ? at : INT_MAX;
+        room[wave].before = before;
+    }
+    if (lane == (have != 0 ? 63 - __builtin_clzll(have) : 0)) room[wave].last = have != 0 ? at : -1;
+    __syncthreads();
+    Found f{INT_MAX, -1, 0.};
+#pragma unroll
+    for (int w = kWalkWaves - 1; w >= 0; --w) {
+        const Found g = room[w];
+        if (g.at < INT_MAX) {
+            f.at = g.at;
+            f.before = g.before;
+        }
+        f.last = max(f.last, g.last);
+    }
+    return f;
+}
+__device__ __forceinline__ float unit(float u) { return u >= 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f; }
+
+// The first id whose running sum of weights exceeds u times their total; -1 where
+// the total is 0.  value(j): the sum of segment j's weights; weights(id, w): those of
+// the kRun ids from `id` on.
+template <typename V, typename W>
+__device__ int pick(int segs, float u, V value, W weights) {
+    __shared__ double sums[3][kWalkWaves];
+    __shared__ Found finds[2][kWalkWaves];
+    const int tid = threadIdx.x;
+    double v = tid < segs ? value(tid) : 0.;
+    Scan s = block_scan(v, sums[0]);
+    double total = s.total, base = 0.;
+    for (int j0 = kWalk; j0 < segs; j0 += kWalk) {
+        __syncthreads();
+        total += block_scan(j0 + tid < segs ? value(j0 + tid) : 0., sums[1]).total;
+    }
+    if (!(total > 0.)) return -1;
+    const double t = (double)unit(u) * total;
+    Found f = block_find(s.before + v > t, v > 0., tid, s.before, finds[0]);
+    for (int j0 = kWalk; j0 < segs && f.at == INT_MAX; j0 += kWalk) {
+        base += s.total;
+        __syncthreads();
+        v = j0 + tid < segs ? value(j0 + tid) : 0.;
+        s = block_scan(v, sums[1]);
+        const Found g = block_find(base + s.before + v > t, v > 0., j0 + tid, base + s.before, finds[0]);
+        f = Found{g.at, max(f.last, g.last), g.before};
+    }
+    // where rounding leaves no segment, or none of its ids, the last that has a weight
+    const bool none = f.at == INT_MAX;
+    const int id0 = (none ? f.last : f.at) * kSeg + tid * kRun;
+    double w[kRun], sum = 0.;
+    weights(id0, w);
+#pragma unroll
+    for (int e = 0; e < kRun; ++e) sum += w[e];
+    s = block_scan(sum, sums[2]);
+    double run = f.before + s.before;
+    int at = INT_MAX, last = -1;
+#pragma unroll
+    for (int e = 0; e < kRun; ++e) {
+        run += w[e];
+        if (w[e] > 0.) {
+            last = id0 + e;
+            if (at == INT_MAX && !none && run > t) at = last;
+        }
+    }
+    const Found hit = block_find(at < INT_MAX, false, at, 0., finds[1]);
+    if (hit.at < INT_MAX) return hit.at;
+    __syncthreads();
+    return block_find(false, last >= 0, last, 0., finds[1]).last;
+}
+// kRun logits of a row from id on, -inf behind the last.
+template <bool kHalf>
+__device__ __forceinline__ void load_run(const void* row, int id, int vocab, float (&x)[kRun]) {
+    static_assert(kRun == 4);
+    if (id + kRun <= vocab) {
+        if constexpr (kHalf) {
+            const u32x2 v = *reinterpret_cast<const u32x2_a2*>(static_cast<const uint16_t*>(row) + id);
+#pragma unroll
+            for (int e = 0; e < kRun; ++e) x[e] = h2f((uint16_t)(v[e / 2] >> (e % 2 * 16)));
+        } else {
+            const u32x4 v = *reinterpret_cast<const u32x4_a2*>(static_cast<const float*>(row) + id);
+#pragma unroll
+            for (int e = 0; e < kRun; ++e) x[e] = __uint_as_float(v[e]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < kRun; ++e) x[e] = id + e < vocab ? logit<kHalf>(row, id + e) : -INFINITY;
+    }
+}
+
+// Largest logit, sum and first id of a row.
 struct RowSum {
     double s;
     float m;   // NaN: no distribution
     int first;
 };
-__device__ RowSum join_segments(const Segment* at, int segs, bool greedy, double c, int lane) {
+// A row's segments joined by 16 lanes.
+constexpr int kRowLanes = 16;
+__device__ RowSum join_segments(const Segment* at, int segs, bool greedy, double c) {
+    constexpr int kBatch = 5;
+    const int lane = threadIdx.x & (kWave - 1);
     float m = -INFINITY;
     double s = 0.;
     int first = INT_MAX;
     bool bad = false;
-    for (int j = lane; j < segs; j += kWave) {
-        const Segment g = at[j];
-        bad |= g.top != g.top;
-        if (!(g.top > -INFINITY)) continue;
-        if (greedy) {
-            if (g.top > m) {
-                m = g.top;
-                first = g.first;
-            }
-        } else if (g.top > m) {
-            s = fma(s, m == -INFINITY ? 0. : weight(m, g.top, c), g.sum);
-            m = g.top;
-        } else {
-            s = fma(g.sum, weight(g.top, m, c), s);
+    for (int j0 = lane % kRowLanes; j0 < segs; j0 += kBatch * kRowLanes) {
+        Segment g[kBatch];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const int j = j0 + b * kRowLanes;
+            g[b] = at[min(j, segs - 1)];
+            if (j >= segs) g[b].top = -INFINITY;
         }
+        float most = m;
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            bad |= g[b].top != g[b].top;
+            most = fmaxf(most, g[b].top);
+        }
+        if (greedy) {
+            int here = INT_MAX;   // (the lowest ids come first)
+#pragma unroll
+            for (int b = kBatch - 1; b >= 0; --b)
+                if (g[b].top == most) here = g[b].first;
+            first = most > m ? here : first;
+        } else if (most > -INFINITY) {
+            s *= weight(m, most, c);
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) s = fma(g[b].sum, weight(g[b].top, most, c), s);
+        }
+        m = most;
     }
-    RowSum r;
-    r.m = wave_max(m);
-    bad = __builtin_amdgcn_ballot_w64(bad) != 0 || r.m == -INFINITY;
-    if (greedy) {
-        r.first = wave_fold(m == r.m ? first : INT_MAX, [](int p, int q) { return min(p, q); });
-        r.s = 1.;
-    } else {
-        r.first = 0;
-        r.s = wave_sum64(m == -INFINITY ? 0. : s * weight(m, r.m, c));
-    }
-    if (bad) r.m = NAN;
+    RowSum r{0., row_max(m), 0};
+    if (greedy)
+        r.first = row_min(m == r.m ? first : INT_MAX);
+    else if (r.m > -INFINITY)
+        r.s = row_sum64(s * weight(m, r.m, c));
+    const uint64_t any = __builtin_amdgcn_ballot_w64(bad);
+    if ((any >> (lane & 48) & 0xffff) != 0 || r.m == -INFINITY) r.m = NAN;
     return r;
 }
 
-// Running sum over the threads, and the workgroup's total.
-struct Scan {
-    double before, total;
-};
-__device__ Scan block_scan(double v, double* room) {
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    double run = v;
-    for (int o = 1; o < kWave; o <<= 1) {
-        const double w = __shfl_up(run, o, kWave);
-        if (lane >= o) run += w;
-    }
-    __syncthreads();
-    if (lane == kWave - 1) room[wave] = run;
-    __syncthreads();
-    Scan s{run - v, 0.};
-    for (int w = 0; w < kWaves; ++w) {
-        if (w < wave) s.before += room[w];
-        s.total += room[w];
-    }
-    return s;
-}
-
-// The first id whose running sum of weights exceeds u times their total; -1 where
-// the total is 0.  value(j): sum of segment j's weights; weight_of(id).
-template <typename V, typename W>
-__device__ int pick(int vocab, int segs, float u, V value, W weight_of) {
-    __shared__ double room[kWaves];
-    __shared__ int found, last;
-    __shared__ double found_before;
-    u = u >= 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
-    double total = 0.;
-    for (int j0 = 0; j0 < segs; j0 += kBlk) {
-        const int j = j0 + threadIdx.x;
-        total += block_scan(j < segs ? value(j) : 0., room).total;
-    }
-    if (!(total > 0.)) return -1;
-    const double t = (double)u * total;
-    if (threadIdx.x == 0) {
-        found = INT_MAX;
-        last = -1;
-    }
-    double base = 0.;
-    for (int j0 = 0; j0 < segs; j0 += kBlk) {
-        const int j = j0 + threadIdx.x;
-        const double v = j < segs ? value(j) : 0.;
-        const Scan s = block_scan(v, room);
-        if (v > 0.) {
-            if (base + s.before + v > t) atomicMin(&found, j);
-            atomicMax(&last, j);
-        }
-        __syncthreads();
-        const bool here = found == j;
-        if (here) found_before = base + s.before;
-        base += s.total;
-        if (found < INT_MAX) break;   // uniform
-    }
-    __syncthreads();
-    // (where rounding leaves no segment, the last one that has any)
-    const int seg = found < INT_MAX ? found : last;
-    const double before = found < INT_MAX ? found_before : 0., bar = found < INT_MAX ? t : INFINITY;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        found = INT_MAX;
-        last = -1;
-    }
-    constexpr int kRun = kSeg / kBlk;
-    const int id0 = seg * kSeg + (int)threadIdx.x * kRun;
-    double w[kRun], sum = 0.;
-#pragma unroll
-    for (int e = 0; e < kRun; ++e) {
-        w[e] = id0 + e < vocab ? weight_of(id0 + e) : 0.;
-        sum += w[e];
-    }
-    double run = before + block_scan(sum, room).before;
-    int mine = INT_MAX;
-#pragma unroll
-    for (int e = 0; e < kRun; ++e) {
-        run += w[e];
-        if (w[e] > 0.) {
-            if (run > bar && mine == INT_MAX) mine = id0 + e;
-            atomicMax(&last, id0 + e);
-        }
-    }
-    if (mine < INT_MAX) atomicMin(&found, mine);
-    __syncthreads();
-    return found < INT_MAX ? found : last;
-}
-
-// One workgroup per sequence: the rows' sums, the drafted tokens' probabilities,
-// the path, and the next token but where it comes from what q leaves of p.
+// ---------------------------------------------------------------------------
+// One workgroup per sequence: the rows' sums, the drafted tokens' probabilities, the
+// path, and the next token but where it comes from what q leaves of p.
+// ---------------------------------------------------------------------------
 template <bool kHalf>
-__global__ __launch_bounds__(kBlk) void verify_walk_kernel(VerifyDrafts a, int segs) {
-    __shared__ RowSum target[kMaxTree], drafted[kMaxTree];
-    __shared__ int parent[kMaxTree], token[kMaxTree], gone[kMaxTree];
-    __shared__ double p[kMaxTree], bar[kMaxTree];
-    __shared__ int end_row, end_gone;
-    const int seq = blockIdx.x, lane = threadIdx.x & (kWave - 1);
+__global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerifyDrafts a, int segs) {
+    __shared__ RowSum sums[2 * kMaxTree];   // the rows', then their drafts'
+    __shared__ int parent[kMaxTree], token[kMaxTree], gone[kMaxTree], path[kMaxTree];
+    __shared__ double p[kMaxTree], bar[kMaxTree], gone_sum[kMaxTree];
+    __shared__ int end_row, end_lost, end_count;
+    const int seq = blockIdx.x, lane = threadIdx.x & (kWave - 1), tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const DraftRows rows = draft_rows(a.query_start, seq, a.rows, a.max_query);
     const Work work = work_of(a, segs);
     if (rows.n <= 0) {
         if (a.paths)
-            for (int i = threadIdx.x; i < a.max_query; i += kBlk) a.paths[(size_t)seq * a.max_query + i] = -1;
-        if (threadIdx.x == 0) {
+            for (int i = tid; i < a.max_query; i += kWalk) a.paths[(size_t)seq * a.max_query + i] = -1;
+        if (tid == 0) {
             if (a.counts) a.counts[seq] = 0;
             a.next_tokens[seq] = -1;
             if (a.draft) work.ends[seq].rest = 0;
         }
         return;
     }
-    const float t = temperature(a, seq);
-    const bool greedy = !(t > 0.f);
-    const double c = greedy ? 0. : kLog2e / (double)t;
-    const Segment* segments = work.segments + (size_t)rows.start * segs;
-    const Segment* draft_segments = segments + (size_t)a.rows * segs;
-    for (int i = wave; i < rows.n; i += kWaves) {
-        const RowSum r = join_segments(segments + (size_t)i * segs, segs, greedy, c, lane);
-        if (lane == 0) target[i] = r;
-        if (a.draft && i + 1 < rows.n) {
-            const RowSum d = join_segments(draft_segments + (size_t)i * segs, segs, greedy, c, lane);
-            if (lane == 0) drafted[i] = d;
+    const float heat = temperature(a, seq);
+    const bool greedy = !(heat > 0.f);
+    const double c = greedy ? 0. : kLog2e / (double)heat;
+    const float u0 = a.uniforms[rows.start];
+    // a row's draft and its logits, on their way beside the rows' sums
+    int up = -1, x = -1;
+    float u = 0.f, x_logit = -INFINITY, x_draft = -INFINITY;
+    if (tid < rows.n) {
+        const int r = rows.start + tid;
+        up = a.parents ? a.parents[r] : tid - 1;
+        if (up < 0 || up >= tid) up = -1;
+        x = up >= 0 ? a.tokens[r] : -1;
+        u = unit(a.uniforms[r]);
+        if (x < 0 || x >= a.vocab) x = -1;
+        if (x >= 0) {
+            x_logit = logit<kHalf>(logit_row<kHalf>(a.logits, a.stride, rows.start + up), x);
+            if (a.draft) x_draft = logit<kHalf>(logit_row<kHalf>(a.draft, a.draft_stride, rows.start + up), x);
         }
     }
+    const int joined = rows.n + (a.draft ? rows.n - 1 : 0);
+    for (int v = tid / kRowLanes; v < joined; v += kWalk / kRowLanes) {
+        const bool of_draft = v >= rows.n;
+        const int i = of_draft ? v - rows.n : v;
+        const RowSum r = join_segments(
+            work.segments + ((size_t)(of_draft ? a.rows : 0) + rows.start + i) * segs, segs, greedy, c);
+        if (tid % kRowLanes == 0) sums[(of_draft ? kMaxTree : 0) + i] = r;
+    }
     __syncthreads();
-    const int i = threadIdx.x;
-    float u = 0.f;
-    if (i < rows.n) {
-        const int r = rows.start + i;
-        int up = a.parents ? a.parents[r] : i - 1;
-        if (up < 0 || up >= i) up = -1;
-        const int x = up >= 0 ? a.tokens[r] : -1;
-        u = a.uniforms[r];
-        u = u >= 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
+    if (tid < rows.n) {
         double mine = 0., against = 1.;
-        if (up >= 0 && x >= 0 && x < a.vocab) {
-            const RowSum s = target[up];
-            if (s.m == s.m) {
-                if (greedy)
-                    mine = x == s.first;
-                else
-                    mine = weight(logit<kHalf>(logit_row<kHalf>(a.logits, a.stride, rows.start + up), x), s.m, c) / s.s;
-            }
-            if (a.draft) {
-                const RowSum d = drafted[up];
-                if (d.m != d.m)
-                    against = INFINITY;   // no distribution: rejected
-                else if (greedy)
-                    against = x == d.first;
-                else
-                    against =
-                        weight(logit<kHalf>(logit_row<kHalf>(a.draft, a.draft_stride, rows.start + up), x), d.m, c) / d.s;
-            }
+        if (x >= 0) {
+            const RowSum s = sums[up];
+            if (s.m == s.m) mine = greedy ? x == s.first : weight(x_logit, s.m, c) / s.s;
         }
-        parent[i] = up;
-        token[i] = x;
-        p[i] = mine;
-        bar[i] = a.draft ? (u == 0.f && against == INFINITY ? INFINITY : (double)u * against) : (double)u;
-        if (a.token_probs) a.token_probs[r] = (float)mine;
+        if (a.draft && up >= 0) {
+            const RowSum d = sums[kMaxTree + up];
+            against = d.m != d.m ? INFINITY   // no distribution: rejected
+                      : x < 0    ? 0.
+                      : greedy   ? x == d.first
+                                 : weight(x_draft, d.m, c) / d.s;
+        }
+        parent[tid] = up;
+        token[tid] = x;
+        p[tid] = mine;
+        bar[tid] = against == INFINITY ? INFINITY : (double)u * against;
+        if (a.token_probs) a.token_probs[rows.start + tid] = (float)mine;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        int current = 0, count = 1, lost = 0;
+    if (wave == 0) {   // the path; lanes look for the current row's children
+        int above[kMaxTree / kWave];
+#pragma unroll
+        for (int k = 0; k < kMaxTree / kWave; ++k) above[k] = k * kWave + lane < rows.n ? parent[k * kWave + lane] : -1;
+        int current = 0, at = 0, count = 1, lost = 0;
         double left = 1.;
-        if (a.paths) a.paths[(size_t)seq * a.max_query] = 0;
-        for (int k = 1; k < rows.n; ++k) {
-            if (parent[k] != current) continue;
-            double mine = p[k];
-            for (int g = 0; g < lost; ++g)
-                if (gone[g] == token[k]) mine = 0.;
-            if (bar[k] * (a.draft ? 1. : left) < mine) {
-                current = k;
-                if (a.paths) a.paths[(size_t)seq * a.max_query + count] = k;
+        for (;;) {
+            int next = INT_MAX;
+#pragma unroll
+            for (int k = kMaxTree / kWave - 1; k >= 0; --k) {
+                const uint64_t who = __builtin_amdgcn_ballot_w64(above[k] == current && k * kWave + lane > at);
+                if (who != 0) next = k * kWave + __builtin_ctzll(who);
+            }
+            if (next == INT_MAX) break;
+            at = next;
+            const int mark = token[at];
+            double mine = p[at];
+            for (int g = 0; g < lost; ++g) mine = gone[g] == mark ? 0. : mine;
+            if (bar[at] * (a.draft ? 1. : left) < mine) {
+                current = at;
+                if (lane == 0) path[count] = at;
                 ++count;
                 lost = 0;
                 left = 1.;
             } else {
                 left -= mine;
-                gone[lost++] = token[k];
+                if (lane == 0) gone[lost] = mark;
+                ++lost;
+                wave_lds_sync();
             }
         }
-        if (a.counts) a.counts[seq] = count;
-        if (a.paths)
-            for (int k = count; k < a.max_query; ++k) a.paths[(size_t)seq * a.max_query + k] = -1;
-        end_row = current;
-        end_gone = lost;
+        if (lane == 0) {
+            path[0] = 0;
+            end_row = current;
+            end_lost = lost;
+            end_count = count;
+        }
     }
     __syncthreads();
-    const int f = end_row, lost = end_gone;
-    const RowSum s = target[f];
-    const bool rest = a.draft && lost > 0 && s.m == s.m && !greedy && drafted[f].m == drafted[f].m;
-    if (a.draft && threadIdx.x == 0) {
-        PathEnd e{};
-        e.rest = rest;
-        if (rest) {
-            e.s = s.s;
-            e.m = s.m;
-            e.s_draft = drafted[f].s;
-            e.m_draft = drafted[f].m;
-            e.row = rows.start + f;
-            e.c = c;
-        }
-        work.ends[seq] = e;
+    const int f = end_row, lost = end_lost;
+    if (a.paths)
+        for (int i = tid; i < a.max_query; i += kWalk)
+            a.paths[(size_t)seq * a.max_query + i] = i < end_count ? path[i] : -1;
+    if (a.counts && tid == 0) a.counts[seq] = end_count;
+    const RowSum s = sums[f];
+    bool rest = false;
+    if (a.draft) {
+        const RowSum d = sums[kMaxTree + f];
+        rest = lost > 0 && s.m == s.m && !greedy && d.m == d.m;
+        if (tid == 0)
+            work.ends[seq] = rest ? PathEnd{s.s, d.s, s.m, d.m, rows.start + f, 1, c} : PathEnd{};
     }
     if (rest) return;
     int next = -1;
-    if (s.m != s.m) {
-        // no distribution
-    } else if (greedy) {
-        next = s.first;
-    } else {
-        const void* row = logit_row<kHalf>(a.logits, a.stride, rows.start + f);
-        Segment* mine = work.segments + ((size_t)rows.start + f) * segs;
-        auto of = [&](int id) { return weight(logit<kHalf>(row, id), s.m, c); };
-        auto value = [&](int j) {
-            const Segment g = mine[j];
-            return g.top > -INFINITY ? g.sum * weight(g.top, s.m, c) : 0.;
-        };
-        const int out = a.draft ? 0 : lost;   // rejected tokens to leave out
-        auto left_of = [&](int id) {
-            for (int g = 0; g < out; ++g)
-                if (gone[g] == id) return 0.;
-            return of(id);
-        };
-        // their segments anew, without them, by a wave each
-        auto resum = [&](bool all) {
-            for (int g = wave; g < out; g += kWaves) {
-                if (gone[g] < 0 || gone[g] >= a.vocab) continue;
-                const int seg = gone[g] / kSeg, id1 = min(a.vocab, (seg + 1) * kSeg);
-                double sum = 0.;
-                for (int id = seg * kSeg + lane; id < id1; id += kWave) sum += all ? of(id) : left_of(id);
-                sum = wave_sum64(sum);
-                if (lane == 0) mine[seg] = Segment{sum, s.m, 0};
+    if (s.m == s.m) {
+        if (greedy) {
+            next = s.first;
+        } else {
+            const void* row = logit_row<kHalf>(a.logits, a.stride, rows.start + f);
+            const Segment* mine = work.segments + ((size_t)rows.start + f) * segs;
+            const int out = a.draft ? 0 : lost;   // rejected tokens, left out
+            // their segments anew, a wave each
+            for (int g = wave; g < out; g += kWalkWaves) {
+                const int mark = __builtin_amdgcn_readfirstlane(gone[g]), seg = mark / kSeg;
+                if (mark < 0) continue;
+                Logits<kHalf> l(row, a.vocab, seg, lane);
+                for (int k = 0; k < out; ++k) {
+                    const int other = __builtin_amdgcn_readfirstlane(gone[k]);
+                    if (other < 0 || other / kSeg != seg) continue;
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) l.x[e] = l.id_of(seg, e, lane) == other ? -INFINITY : l.x[e];
+                }
+                const double sum = wave_sum64(l.sum(s.m, c));
+                if (lane == 0) gone_sum[g] = sum;
             }
-            __syncthreads();
-        };
-        if (out > 0) resum(false);
-        next = pick(a.vocab, segs, a.uniforms[rows.start], value, left_of);
-        if (next < 0) {   // nothing is left
-            __syncthreads();
-            resum(true);
-            next = pick(a.vocab, segs, a.uniforms[rows.start], value, of);
+            if (out > 0) __syncthreads();
+            auto draw = [&](int left_out) {
+                auto value = [&](int j) {
+                    const Segment g = mine[j];
+                    double v = g.top > -INFINITY ? g.sum * weight(g.top, s.m, c) : 0.;
+                    for (int k = 0; k < left_out; ++k) v = gone[k] >= 0 && gone[k] / kSeg == j ? gone_sum[k] : v;
+                    return v;
+                };
+                return pick(segs, u0, value, [&](int id, double (&w)[kRun]) {
+                    float l[kRun];
+                    load_run<kHalf>(row, id, a.vocab, l);
+                    for (int k = 0; k < left_out; ++k)
+#pragma unroll
+                        for (int e = 0; e < kRun; ++e) l[e] = gone[k] == id + e ? -INFINITY : l[e];
+#pragma unroll
+                    for (int e = 0; e < kRun; ++e) w[e] = weight(l[e], s.m, c);
+                });
+            };
+            next = draw(out);
+            if (next < 0) {   // nothing is left
+                __syncthreads();
+                next = draw(0);
+            }
         }
     }
-    if (threadIdx.x == 0) a.next_tokens[seq] = next;
+    if (tid == 0) a.next_tokens[seq] = next;
 }
 
-template <bool kHalf>
-struct Rest {   // max(p - q, 0)
-    const void *row, *draft_row;
+// max(p - q, 0) of logits of the two rows
+struct Rest {
     PathEnd e;
     double inv, inv_draft;
-    __device__ Rest(const VerifyDrafts& a, const PathEnd& end)
-        : row(logit_row<kHalf>(a.logits, a.stride, end.row)),
-          draft_row(logit_row<kHalf>(a.draft, a.draft_stride, end.row)), e(end), inv(1. / end.s),
-          inv_draft(1. / end.s_draft) {}
-    __device__ double operator()(int id) const {
+    __device__ Rest(const PathEnd& end) : e(end), inv(1. / end.s), inv_draft(1. / end.s_draft) {}
+    __device__ double operator()(float x, float x_draft) const {
 #pragma clang fp contract(off)   // equal p and q leave nothing
-        return fmax(weight(logit<kHalf>(row, id), e.m, e.c) * inv -
-                        weight(logit<kHalf>(draft_row, id), e.m_draft, e.c) * inv_draft,
-                    0.);
+        return fmax(weight(x, e.m, e.c) * inv - weight(x_draft, e.m_draft, e.c) * inv_draft, 0.);
     }
 };
 
@@ -512,33 +616,49 @@ __global__ __launch_bounds__(kBlk) void verify_rest_kernel(VerifyDrafts a, int s
     const Work work = work_of(a, segs);
     const PathEnd e = work.ends[seq];
     if (!e.rest || seg >= segs) return;
-    const Rest<kHalf> rest(a, e);
-    const int id1 = min(a.vocab, (seg + 1) * kSeg);
+    const Logits<kHalf> x(logit_row<kHalf>(a.logits, a.stride, e.row), a.vocab, seg, lane);
+    const Logits<kHalf> d(logit_row<kHalf>(a.draft, a.draft_stride, e.row), a.vocab, seg, lane);
+    const Rest rest(e);
     double sum = 0.;
-#pragma unroll 4
-    for (int id = seg * kSeg + lane; id < id1; id += kWave) sum += rest(id);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) sum += rest(x.x[k], d.x[k]);
     sum = wave_sum64(sum);
     if (lane == 0) work.rest[(size_t)seq * segs + seg] = sum;
 }
 
 template <bool kHalf>
-__global__ __launch_bounds__(kBlk) void verify_pick_kernel(VerifyDrafts a, int segs) {
+__global__ __launch_bounds__(kWalk) void verify_pick_kernel(VerifyDrafts a, int segs) {
     const int seq = blockIdx.x;
     const Work work = work_of(a, segs);
     const PathEnd e = work.ends[seq];
     if (!e.rest) return;
     const DraftRows rows = draft_rows(a.query_start, seq, a.rows, a.max_query);
-    const Rest<kHalf> rest(a, e);
+    const void* row = logit_row<kHalf>(a.logits, a.stride, e.row);
+    const void* draft_row = logit_row<kHalf>(a.draft, a.draft_stride, e.row);
     const float u = a.uniforms[rows.start];
-    int next = pick(a.vocab, segs, u, [&](int j) { return work.rest[(size_t)seq * segs + j]; }, rest);
+    const Rest rest(e);
+    int next = pick(
+        segs, u, [&](int j) { return work.rest[(size_t)seq * segs + j]; },
+        [&](int id, double (&w)[kRun]) {
+            float x[kRun], d[kRun];
+            load_run<kHalf>(row, id, a.vocab, x);
+            load_run<kHalf>(draft_row, id, a.vocab, d);
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) w[k] = rest(x[k], d[k]);
+        });
     if (next < 0) {   // nothing is left
+        __syncthreads();
         const Segment* mine = work.segments + (size_t)e.row * segs;
         auto value = [&](int j) {
             const Segment g = mine[j];
             return g.top > -INFINITY ? g.sum * weight(g.top, e.m, e.c) : 0.;
         };
-        __syncthreads();
-        next = pick(a.vocab, segs, u, value, [&](int id) { return weight(logit<kHalf>(rest.row, id), e.m, e.c); });
+        next = pick(segs, u, value, [&](int id, double (&w)[kRun]) {
+            float x[kRun];
+            load_run<kHalf>(row, id, a.vocab, x);
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) w[k] = weight(x[k], e.m, e.c);
+        });
     }
     if (threadIdx.x == 0) a.next_tokens[seq] = next;
 }
@@ -550,10 +670,10 @@ void launch_for(const VerifyDrafts& a, hipStream_t s) {
     const int segs = segments_of(a.vocab), blocks = (segs + kWaves - 1) / kWaves;
     launch_kernel_in_call(false, verify_sums_kernel<kHalf>, dim3(blocks, a.max_query * (a.draft ? 2 : 1), a.nseq),
                           dim3(kBlk), 0, s, a, segs);
-    launch_kernel_in_call(!a.draft, verify_walk_kernel<kHalf>, dim3(a.nseq), dim3(kBlk), 0, s, a, segs);
+    launch_kernel_in_call(!a.draft, verify_walk_kernel<kHalf>, dim3(a.nseq), dim3(kWalk), 0, s, a, segs);
     if (!a.draft) return;
     launch_kernel_in_call(false, verify_rest_kernel<kHalf>, dim3(blocks, a.nseq), dim3(kBlk), 0, s, a, segs);
-    launch_kernel(verify_pick_kernel<kHalf>, dim3(a.nseq), dim3(kBlk), 0, s, a, segs);
+    launch_kernel(verify_pick_kernel<kHalf>, dim3(a.nseq), dim3(kWalk), 0, s, a, segs);
 }
 
 }  // namespace
