@@ -82,6 +82,50 @@ __device__ __forceinline__ double exp2_64(double z) {
     r = fma(r, f, 1.);
     return ldexp(r, (int)k);
 }
+// The same for many z = d c: z is n / 256 + r with a whole n, 2^(n / 256) comes from a
+// table of 256 and 2^r, |r| <= 1/512, by a polynomial of degree 3; off by 1e-13 at
+// most, 2^0 is 1.  Adding 1.5 * 2^44 rounds z to 256ths and leaves n in the low bits;
+// entry j's upper half is less by j << 12, so that n << 12 added to it is the
+// exponent.  d is kept from -1000 / c on: 2^-1000 for all below.
+struct Exp2Table {
+    static constexpr int kEntries = 256;
+    const double* table;   // of LDS
+    double c, least;
+    // by kThreads threads; they meet without waiting for their loads
+    template <int kThreads>
+    __device__ void make(double* room, double c_) {
+        table = room;
+        c = c_;
+        least = -1000. / c_;
+        for (int j = threadIdx.x; j < kEntries; j += kThreads) {
+            u32x2 w = __builtin_bit_cast(u32x2, exp2_64(j * (1. / kEntries) - 1.));
+            w.y += (1u << 20) - ((uint32_t)j << 12);   // (times 2)
+            room[j] = __builtin_bit_cast(double, w);
+        }
+        lds_only_barrier();
+    }
+    struct Parts {
+        double e, p;   // whose product it is
+    };
+    __device__ Parts parts(double d) const {
+        d = fmax(d, least);
+        constexpr double kRound = 0x1.8p44;
+        const double t = fma(d, c, kRound), r = fma(d, c, kRound - t);
+        const uint32_t n = __builtin_bit_cast(u32x2, t).x;
+        u32x2 w = __builtin_bit_cast(u32x2, table[n & (kEntries - 1)]);
+        w.y += n << 12;
+        return {__builtin_bit_cast(double, w),
+                fma(fma(fma(0.05550411247958329, r, 0.24022653447679007), r, 0.6931471805599453), r, 1.)};
+    }
+    __device__ double operator()(double d) const {
+        const Parts v = parts(d);
+        return v.e * v.p;
+    }
+    __device__ double add(double sum, double d) const {
+        const Parts v = parts(d);
+        return fma(v.e, v.p, sum);
+    }
+};
 // Weight of a logit x against one of m >= x; c = log2(e) / T.
 __device__ __forceinline__ double weight(float x, float m, double c) {
     return x == -INFINITY ? 0. : exp2_64(((double)x - (double)m) * c);
@@ -180,42 +224,44 @@ constexpr double kLog2e = 1.4426950408889634074;
 // seg * kSeg + (e / kVec * 64 + lane) * kVec + e % kVec; -inf behind the last id.
 template <bool kHalf>
 struct Logits {
-    static constexpr int kVec = kHalf ? 8 : 4;
-    float x[kPer];
-    __device__ Logits(const void* row, int vocab, int seg, int lane) {
+    static constexpr int kVec = kHalf ? 8 : 4, kLoads = kPer / kVec;
+    u32x4 w[kLoads];   // fp32, or pairs of fp16
+    __device__ void load(const void* row, int vocab, int seg, int lane) {
         const int id0 = seg * kSeg;
         if (id0 + kSeg <= vocab) {
             const char* at = static_cast<const char*>(row) + (size_t)id0 * (kHalf ? 2 : 4) + lane * 16;
 #pragma unroll
-            for (int l = 0; l < kPer / kVec; ++l) {
-                const u32x4 v = *reinterpret_cast<const u32x4_a2*>(at + l * kWave * 16);
-#pragma unroll
-                for (int e = 0; e < kVec; ++e)
-                    x[l * kVec + e] = kHalf ? h2f((uint16_t)(v[e / 2] >> (e % 2 * 16))) : __uint_as_float(v[e]);
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) {
-                const int id = id_of(seg, e, lane);
-                x[e] = id < vocab ? logit<kHalf>(row, id) : -INFINITY;
-            }
+            for (int l = 0; l < kLoads; ++l) w[l] = *reinterpret_cast<const u32x4_a2*>(at + l * kWave * 16);
+            return;
         }
+#pragma unroll
+        for (int l = 0; l < kLoads; ++l)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int id = id_of(seg, l * kVec + i * (kVec / 4), lane);
+                if constexpr (kHalf) {
+                    const uint16_t* x = static_cast<const uint16_t*>(row);   // all of them on their way at once
+                    const uint32_t lo = x[min(id, vocab - 1)], hi = x[min(id + 1, vocab - 1)];
+                    w[l][i] = (id < vocab ? lo : 0xfc00u) | (id + 1 < vocab ? hi : 0xfc00u) << 16;
+                } else {
+                    const uint32_t x = static_cast<const uint32_t*>(row)[min(id, vocab - 1)];
+                    w[l][i] = id < vocab ? x : 0xff800000u;
+                }
+            }
+    }
+    __device__ float at(int e) const {
+        const uint32_t v = w[e / kVec][kHalf ? e % kVec / 2 : e % kVec];
+        return kHalf ? h2f((uint16_t)(e & 1 ? v >> 16 : v)) : __uint_as_float(v);
     }
     __device__ static int id_of(int seg, int e, int lane) {
         return seg * kSeg + (e / kVec * kWave + lane) * kVec + e % kVec;
-    }
-    // of the lane's weights against m > -inf
-    __device__ double sum(double m, double c) const {
-        double s[2] = {0., 0.};
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) s[e % 2] += exp2_64(((double)x[e] - m) * c);
-        return s[0] + s[1];
     }
 };
 
 // Workgroup (4 segments, row, sequence), a segment a wave.
 template <bool kHalf>
 __global__ __launch_bounds__(kBlk) void verify_sums_kernel(VerifyDrafts a, int segs) {
+    __shared__ double table[Exp2Table::kEntries];
     const int seq = blockIdx.z;
     const bool draft = (int)blockIdx.y >= a.max_query;
     const int i = blockIdx.y - (draft ? a.max_query : 0);
@@ -223,25 +269,31 @@ __global__ __launch_bounds__(kBlk) void verify_sums_kernel(VerifyDrafts a, int s
     if (i >= rows.n || (draft && i + 1 >= rows.n)) return;   // the last row's draft has no child
     const int lane = threadIdx.x & (kWave - 1);
     const int seg = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    if (seg >= segs) return;
     const float t = temperature(a, seq);
     const int r = rows.start + i;
-    const Logits<kHalf> x(draft ? logit_row<kHalf>(a.draft, a.draft_stride, r) : logit_row<kHalf>(a.logits, a.stride, r),
-                          a.vocab, seg, lane);
-    float top = x.x[0];
+    Logits<kHalf> x;
+    x.load(draft ? logit_row<kHalf>(a.draft, a.draft_stride, r) : logit_row<kHalf>(a.logits, a.stride, r), a.vocab,
+           min(seg, segs - 1), lane);
+    Exp2Table exp2;
+    exp2.make<kBlk>(table, kLog2e / (double)t);
+    if (seg >= segs) return;
+    float top = x.at(0);
 #pragma unroll
-    for (int e = 1; e < kPer; ++e) top = __builtin_elementwise_maximum(top, x.x[e]);   // a NaN stays
+    for (int e = 1; e < kPer; ++e) top = __builtin_elementwise_maximum(top, x.at(e));   // a NaN stays
     const bool bad = __builtin_amdgcn_ballot_w64(!(top < INFINITY)) != 0;
     top = wave_max(top);
     Segment out{0., bad ? NAN : top, 0};
     if (!bad && top > -INFINITY) {
         if (t > 0.f) {
-            out.sum = wave_sum64(x.sum(top, kLog2e / (double)t));
+            double s[2] = {0., 0.};
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) s[e % 2] = exp2.add(s[e % 2], (double)x.at(e) - (double)top);
+            out.sum = wave_sum64(s[0] + s[1]);
         } else {
             int first = INT_MAX;
 #pragma unroll
             for (int e = kPer - 1; e >= 0; --e)
-                if (x.x[e] == top) first = x.id_of(seg, e, lane);
+                if (x.at(e) == top) first = x.id_of(seg, e, lane);
             first = row_min(first);
             out.first = min(min(__builtin_amdgcn_readlane(first, 0), __builtin_amdgcn_readlane(first, 16)),
                             min(__builtin_amdgcn_readlane(first, 32), __builtin_amdgcn_readlane(first, 48)));
@@ -366,7 +418,10 @@ __device__ __forceinline__ void load_run(const void* row, int id, int vocab, flo
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < kRun; ++e) x[e] = id + e < vocab ? logit<kHalf>(row, id + e) : -INFINITY;
+        for (int e = 0; e < kRun; ++e) {
+            const float v = logit<kHalf>(row, min(id + e, vocab - 1));
+            x[e] = id + e < vocab ? v : -INFINITY;
+        }
     }
 }
 
@@ -431,6 +486,7 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerifyDrafts a, int 
     __shared__ RowSum sums[2 * kMaxTree];   // the rows', then their drafts'
     __shared__ int parent[kMaxTree], token[kMaxTree], gone[kMaxTree], path[kMaxTree];
     __shared__ double p[kMaxTree], bar[kMaxTree], gone_sum[kMaxTree];
+    __shared__ double table[Exp2Table::kEntries];
     __shared__ int end_row, end_lost, end_count;
     const int seq = blockIdx.x, lane = threadIdx.x & (kWave - 1), tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -556,17 +612,28 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerifyDrafts a, int 
             const Segment* mine = work.segments + ((size_t)rows.start + f) * segs;
             const int out = a.draft ? 0 : lost;   // rejected tokens, left out
             // their segments anew, a wave each
+            Exp2Table exp2;
+            if (out > 0) exp2.make<kWalk>(table, c);
             for (int g = wave; g < out; g += kWalkWaves) {
                 const int mark = __builtin_amdgcn_readfirstlane(gone[g]), seg = mark / kSeg;
                 if (mark < 0) continue;
-                Logits<kHalf> l(row, a.vocab, seg, lane);
+                Logits<kHalf> l;
+                l.load(row, a.vocab, seg, lane);
+                uint32_t here = 0;   // of the lane's elements
                 for (int k = 0; k < out; ++k) {
                     const int other = __builtin_amdgcn_readfirstlane(gone[k]);
                     if (other < 0 || other / kSeg != seg) continue;
 #pragma unroll
-                    for (int e = 0; e < kPer; ++e) l.x[e] = l.id_of(seg, e, lane) == other ? -INFINITY : l.x[e];
+                    for (int e = 0; e < kPer; ++e) here |= (l.id_of(seg, e, lane) == other ? 1u : 0u) << e;
                 }
-                const double sum = wave_sum64(l.sum(s.m, c));
+                // (what is left may be nothing, or far below the largest)
+                double sum = 0.;
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) {
+                    const double v = exp2((double)l.at(e) - (double)s.m);
+                    sum += (here >> e & 1) != 0 || l.at(e) == -INFINITY ? 0. : v;
+                }
+                sum = wave_sum64(sum);
                 if (lane == 0) gone_sum[g] = sum;
             }
             if (out > 0) __syncthreads();
@@ -602,28 +669,40 @@ struct Rest {
     PathEnd e;
     double inv, inv_draft;
     __device__ Rest(const PathEnd& end) : e(end), inv(1. / end.s), inv_draft(1. / end.s_draft) {}
-    __device__ double operator()(float x, float x_draft) const {
+    __device__ double of(double w, double w_draft) const {
 #pragma clang fp contract(off)   // equal p and q leave nothing
-        return fmax(weight(x, e.m, e.c) * inv - weight(x_draft, e.m_draft, e.c) * inv_draft, 0.);
+        return fmax(w * inv - w_draft * inv_draft, 0.);
+    }
+    __device__ double operator()(float x, float x_draft) const {
+        return of(weight(x, e.m, e.c), weight(x_draft, e.m_draft, e.c));
     }
 };
 
 // Workgroup (4 segments, sequence): what q leaves of p where a draft was rejected.
 template <bool kHalf>
 __global__ __launch_bounds__(kBlk) void verify_rest_kernel(VerifyDrafts a, int segs) {
+    __shared__ double table[Exp2Table::kEntries];
     const int seq = blockIdx.y, lane = threadIdx.x & (kWave - 1);
-    const int seg = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), seg = blockIdx.x * kWaves + wave;
     const Work work = work_of(a, segs);
     const PathEnd e = work.ends[seq];
-    if (!e.rest || seg >= segs) return;
-    const Logits<kHalf> x(logit_row<kHalf>(a.logits, a.stride, e.row), a.vocab, seg, lane);
-    const Logits<kHalf> d(logit_row<kHalf>(a.draft, a.draft_stride, e.row), a.vocab, seg, lane);
+    if (!e.rest) return;
+    Logits<kHalf> x, d;
+    x.load(logit_row<kHalf>(a.logits, a.stride, e.row), a.vocab, min(seg, segs - 1), lane);
+    d.load(logit_row<kHalf>(a.draft, a.draft_stride, e.row), a.vocab, min(seg, segs - 1), lane);
     const Rest rest(e);
-    double sum = 0.;
+    Exp2Table exp2;
+    exp2.make<kBlk>(table, e.c);
+    if (seg >= segs) return;
+    double sum[2] = {0., 0.};
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) sum += rest(x.x[k], d.x[k]);
-    sum = wave_sum64(sum);
-    if (lane == 0) work.rest[(size_t)seq * segs + seg] = sum;
+    for (int k = 0; k < kPer; ++k) {
+        const double dx = (double)x.at(k) - (double)e.m, dd = (double)d.at(k) - (double)e.m_draft;
+        const double w = exp2(dx), w_draft = exp2(dd);
+        sum[k % 2] += rest.of(dx > exp2.least ? w : 0., dd > exp2.least ? w_draft : 0.);
+    }
+    const double all = wave_sum64(sum[0] + sum[1]);
+    if (lane == 0) work.rest[(size_t)seq * segs + seg] = all;
 }
 
 template <bool kHalf>

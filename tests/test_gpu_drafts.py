@@ -1,7 +1,9 @@
 """Masks and positions of trees of drafted tokens, and which drafts stay, against
 numpy in 64 bits.  Bars: masks, positions, paths, counts and tokens are equal;
 probabilities are one fp32 rounding (2^-24) of 64-bit values that are off by
-less than 1e-12 (an exponential by 4e-14, the sums of up to 2^18 terms by less)."""
+less than 1e-12 (an exponential by 1e-13, as are then their sums; 2^18 additions by
+2^-53 each of what they have reached add less than 3e-11 in the worst case, and the
+sums run over 32, 64 and 149 terms: 3e-14)."""
 from __future__ import annotations
 
 import numpy as np
