@@ -820,8 +820,8 @@ CITLALI_EXPORT int citlali_hip_kv4_keep(const citlali_hip_kv4_cache* caches, int
         a.pages[i] = c.pages;
     }
     REQUIRE(nseq >= 0 && nseq <= 65535, "kv4_keep: nseq (%d) is not in 0..65535", nseq);
-    REQUIRE(pages_per_seq > 0 && max_count >= 0, "kv4_keep: bad pages_per_seq (%d) or max_count (%d)", pages_per_seq,
-            max_count);
+    REQUIRE(pages_per_seq > 0 && max_count >= 0 && max_count <= 1 << 30,
+            "kv4_keep: bad pages_per_seq (%d) or max_count (%d)", pages_per_seq, max_count);
     REQUIRE((long long)nseq * c.kv_heads <= kKv4MaxSeqHeads, "kv4_keep: nseq (%d) times kv_heads (%d) exceeds %lld",
             nseq, c.kv_heads, kKv4MaxSeqHeads);
     REQUIRE(page_table && first && kept && counts, "kv4_keep received a null buffer");

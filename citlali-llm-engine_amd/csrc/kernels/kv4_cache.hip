@@ -5,6 +5,8 @@
 
 #include <math.h>
 
+#include <algorithm>
+
 namespace citlali::hip {
 namespace {
 
@@ -320,74 +322,148 @@ __global__ __launch_bounds__(kBlk) void kv4_read_kernel(Kv4View c, const int32_t
 }
 
 // ---------------------------------------------------------------------------
-// Position first[s] + kept[s][j] of sequence s moves to first[s] + j.  One
-// workgroup per (kv head, sequence, cache) takes its moves in order, 4 kTokens at a
-// time: all are read before any is written, so that a position which one of them
-// takes may be where another comes from.  Later moves come from behind (kept
-// ascends), so the next ones are read before these are written.
-// A token's part of a head is HD / 2 lanes' work: HD / 8 words of K codes, HD / 32
-// of K params, then HD / 4 pairs of bytes of V codes and HD / 16 of V params.
+// Position first[s] + kept[s][j] of sequence s moves to first[s] + j.  One workgroup
+// per (kv head, sequence, cache), and one more for the V codes, which are as many
+// bytes as the rest, takes its moves in order, some hundred at a time:
+// all are read before any is written, so that a position which one of them takes
+// may be where another comes from.  Later moves come from behind (kept ascends), so
+// the next ones are read before these are written.
+// kQuad lanes take four positions of the target in a row: for K 16 bytes of a token's
+// codes or its params, for V a word of the four tokens' codes or params, gathered
+// from four places and stored at once.  Where the tokens come from and go to is looked up for kAhead of them at a
+// time, a thread a token.
 // ---------------------------------------------------------------------------
+constexpr int kKeepWaves = 8, kAhead = 2048;
 template <int HD>
-__global__ __launch_bounds__(kBlk) void kv4_keep_kernel(Kv4View c, Kv4Keep a) {
+struct KeepTurn {
+    static constexpr int kQuad = HD / 4;   // lanes of four tokens
+    static constexpr int kSteps = 4;
+    static constexpr int kTokens = kSteps * 4 * (kWave / kQuad);   // of a wave
+    static_assert(kAhead % (kKeepWaves * kTokens) == 0);
+};
+template <int HD>
+__global__ __launch_bounds__(kKeepWaves * kWave) void kv4_keep_kernel(Kv4View c, Kv4Keep a) {
     using L = Kv4Layout<HD>;
-    constexpr int kLanes = HD / 2, kRows = kBlk / kLanes, kTokens = 4;
-    constexpr int kWords = HD / 8 + HD / 32;   // lanes that have a word of K
-    const int kvh = blockIdx.x, seq = blockIdx.y;
+    using T = KeepTurn<HD>;
+    constexpr int kSteps = T::kSteps, kTokens = T::kTokens;
+    constexpr int kCodeLanes = HD / 8, kKLanes = kCodeLanes + 4;   // of K: 16-byte pieces, then params
+    constexpr int kVCodes = HD / 4, kVParams = HD / 16;            // words of V a quad of tokens
+    static_assert(kKLanes + kVParams <= T::kQuad && kVCodes <= T::kQuad);
+    // the parts of pages (their first byte << 8 | row) that tokens come from and go to;
+    // -1 for none
+    __shared__ __align__(16) long long from_at[kAhead], to_at[kAhead];
+    const bool codes = blockIdx.x & 1;   // of V
+    const int kvh = blockIdx.x / 2, seq = blockIdx.y;
     c.pages = a.pages[blockIdx.z];
     const int n = min(a.counts[seq], a.max_count), first = a.first[seq];
     if (n <= 0 || first < 0) return;
-    const int l = threadIdx.x % kLanes, mine = threadIdx.x / kLanes;
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int l = lane % T::kQuad, quad = lane / T::kQuad;
     const int32_t* kept = a.kept + (size_t)seq * a.kept_stride;
     const int32_t* table = a.page_table + (size_t)seq * a.pages_per_seq;
-    const int P = 1 << c.page_shift;
-    // the lane's bytes of the token at a position; null: a position without a page
-    auto place = [&](long long position) -> uint8_t* {
+    const int P = 1 << c.page_shift, lead = first & 3;   // target positions of the first quad that stay
+    const int turn = blockDim.x / kWave * kTokens;
+    const int end = lead + n;
+
+    auto part_of = [&](long long position) {
         const long long at = position >> c.page_shift;
-        if (at >= a.pages_per_seq) return nullptr;
-        const int page = table[at];
-        if (page < 0 || page >= c.num_pages) return nullptr;
-        uint8_t* base = kv4_head<HD>(c, page, kvh);
-        const int o = (int)position & (P - 1);
-        if (l < HD / 8) return base + o * L::kCodes + 4 * l;
-        if (l < kWords) return base + L::k_params(P) + o * L::kParams + 4 * (l - HD / 8);
-        const int h = l - kWords;
-        if (h < HD / 4) return base + L::v_codes(P) + (((o >> 2) * (HD / 4) + h) * 4 + (o & 3)) * 2;
-        if (h < HD / 4 + HD / 16) return base + L::v_params(P) + (((o >> 2) * (HD / 16) + h - HD / 4) * 4 + (o & 3)) * 2;
-        return nullptr;
+        const int page = at < a.pages_per_seq ? table[at] : -1;
+        if (page < 0 || page >= c.num_pages) return -1ll;
+        return (long long)(kv4_head<HD>(c, page, kvh) - c.pages) << 8 | (position & (P - 1));
     };
-    auto load = [&](int j0, uint32_t (&v)[kTokens], uint8_t* (&to)[kTokens]) {
+    // a lane's bytes of a token in row o of its part: lane_at + (o >> lane_shift) *
+    // lane_row, and for V 2 (o & 3) more
+    const bool is_k = !codes && l < kKLanes, is_v = codes || (!is_k && l < kKLanes + kVParams);
+    const bool k_codes = is_k && l < kCodeLanes;
+    const int lane_shift = is_k ? 0 : 2, lane_and = is_k ? 0 : 3;
+    const int lane_row = k_codes ? L::kCodes : is_k ? L::kParams : 8 * (codes ? kVCodes : kVParams);
+    const int lane_at = k_codes  ? l % (HD / 32) * 16
+                        : is_k   ? L::k_params(P)
+                        : codes  ? L::v_codes(P) + 8 * l
+                                 : L::v_params(P) + 8 * (l - kKLanes);
+    auto place = [&](long long part) {
+        const int o = (int)part & 255;
+        return c.pages + (part >> 8) + (lane_at + (o >> lane_shift) * lane_row + 2 * (o & lane_and));
+    };
+    const int k_token = k_codes ? l / (HD / 32) : l - kCodeLanes;   // of the quad
+    const bool wide = HD == 128 || k_codes;                          // 16 bytes of K, else 8
+    const int my_quad = wave * kTokens + quad * 4;
+    constexpr int kStride = 4 * (kWave / T::kQuad);   // of a step's tokens
+    // without branches on what moves: the cache's first bytes are read in the place of none
+    auto load = [&](int t, u32x4 (&v)[kSteps]) {
+        const long long* at = from_at + t + my_quad;
+        if (is_k) {
 #pragma unroll
-        for (int k = 0; k < kTokens; ++k) {
-            const int j = j0 + k * kRows + mine, from = j < n ? kept[j] : -1;
-            to[k] = nullptr;
-            if (from <= j) continue;   // already there, or behind: nothing moves
-            const uint8_t* src = place((long long)first + from);
-            if (src == nullptr) continue;
-            to[k] = place((long long)first + j);
-            if (l < kWords)
-                v[k] = *reinterpret_cast<const uint32_t*>(src);
-            else
-                v[k] = *reinterpret_cast<const uint16_t*>(src);
+            for (int s = 0; s < kSteps; ++s) {
+                const uint8_t* src = place(max(at[s * kStride + k_token], 0ll));
+                if (wide) {
+                    v[s] = *reinterpret_cast<const u32x4*>(src);
+                } else {
+                    const u32x2 w = *reinterpret_cast<const u32x2*>(src);
+                    v[s].x = w.x;
+                    v[s].y = w.y;
+                }
+            }
+        } else if (is_v) {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    v[s][k] = *reinterpret_cast<const uint16_t*>(place(max(at[s * kStride + k], 0ll)));
         }
     };
-    uint32_t v[kTokens], w[kTokens];
-    uint8_t *to[kTokens], *to_next[kTokens];
-    load(0, v, to);
-    for (int j0 = 0; j0 < n; j0 += kTokens * kRows) {
-        wait_vm<0>();   // in registers, not on the way, before another wave may write there
-        __syncthreads();
-        load(j0 + kTokens * kRows, w, to_next);
+    auto store = [&](int t, const u32x4 (&v)[kSteps]) {
+        const long long* at = to_at + t + my_quad;
+        if (is_k) {
 #pragma unroll
-        for (int k = 0; k < kTokens; ++k) {
-            if (to[k] != nullptr) {
-                if (l < kWords)
-                    *reinterpret_cast<uint32_t*>(to[k]) = v[k];
+            for (int s = 0; s < kSteps; ++s) {
+                const long long to = at[s * kStride + k_token];
+                if (to < 0) continue;
+                if (wide)
+                    *reinterpret_cast<u32x4*>(place(to)) = v[s];
                 else
-                    *reinterpret_cast<uint16_t*>(to[k]) = (uint16_t)v[k];
+                    *reinterpret_cast<u32x2*>(place(to)) = u32x2{v[s].x, v[s].y};
             }
-            v[k] = w[k];
-            to[k] = to_next[k];
+        } else if (is_v) {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                long long to[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) to[k] = at[s * kStride + k];
+                if ((to[0] | to[1] | to[2] | to[3]) >= 0) {
+                    *reinterpret_cast<u32x2*>(place(to[0])) = u32x2{v[s].x | v[s].y << 16, v[s].z | v[s].w << 16};
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (to[k] >= 0) *reinterpret_cast<uint16_t*>(place(to[k])) = (uint16_t)v[s][k];
+                }
+            }
+        }
+    };
+
+    u32x4 v[kSteps], w[kSteps];
+    for (int t0 = 0; t0 < end; t0 += kAhead) {   // (all bounds are the same for the workgroup's waves)
+        const int some = min(kAhead, (end - t0 + turn - 1) / turn * turn);
+        __syncthreads();
+        for (int i = threadIdx.x; i < some; i += blockDim.x) {
+            const int j = t0 + i - lead, source = j >= 0 && j < n ? kept[j] : -1;
+            long long from = -1, to = -1;
+            if (j >= 0 && source > j) {
+                from = part_of((long long)first + source);
+                to = part_of((long long)first + j);
+            }
+            from_at[i] = from;
+            to_at[i] = from < 0 ? -1 : to;
+        }
+        __syncthreads();
+        load(0, v);
+        for (int t = 0; t < some; t += turn) {
+            wait_vm<0>();   // in registers, not on the way, before another wave may write there
+            __syncthreads();
+            if (t + turn < some) load(t + turn, w);
+            store(t, v);
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) v[s] = w[s];
         }
     }
 }
@@ -441,11 +517,13 @@ hipError_t launch_kv4_read(const Kv4View& c, const int32_t* slots, int count, ui
 }
 
 hipError_t launch_kv4_keep(const Kv4View& c, const Kv4Keep& a, hipStream_t s) {
-    const dim3 grid(c.kv_heads, a.nseq, a.layers);
+    const dim3 grid(2 * c.kv_heads, a.nseq, a.layers);
+    const int tokens = c.head_dim == 128 ? KeepTurn<128>::kTokens : KeepTurn<64>::kTokens;
+    const int waves = std::min<long long>(kKeepWaves, ((long long)a.max_count + 3 + tokens - 1) / tokens);
     if (c.head_dim == 128)
-        launch_kernel(kv4_keep_kernel<128>, grid, dim3(kBlk), 0, s, c, a);
+        launch_kernel(kv4_keep_kernel<128>, grid, dim3(waves * kWave), 0, s, c, a);
     else
-        launch_kernel(kv4_keep_kernel<64>, grid, dim3(kBlk), 0, s, c, a);
+        launch_kernel(kv4_keep_kernel<64>, grid, dim3(waves * kWave), 0, s, c, a);
     return hipGetLastError();
 }
 

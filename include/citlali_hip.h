@@ -514,8 +514,8 @@ size_t citlali_hip_verify_drafts_workspace_bytes(int nseq, int rows, int max_que
  * any other positions of a sequence may be dropped the same way.  An entry not
  * above its j, and one whose position (or the one it goes to) has no page, moves
  * nothing; a negative first moves nothing of the sequence.  Sequences that share a
- * page must not move anything to it.  nseq * kv_heads at most 2^23.  nseq or
- * max_count 0 launches nothing. */
+ * page must not move anything to it.  nseq * kv_heads at most 2^23, max_count 2^30.
+ * nseq or max_count 0 launches nothing. */
 #define CITLALI_MAX_KEEP_CACHES 128
 int citlali_hip_kv4_keep(const citlali_hip_kv4_cache* caches, int n_caches, const int32_t* page_table,
                          int pages_per_seq, int nseq, const int32_t* first, const int32_t* kept,

@@ -104,7 +104,8 @@ def test_verify_type_and_workspace():
 
 @pytest.mark.parametrize("change", [
     dict(page_table=None), dict(first=None), dict(kept=None), dict(counts=None), dict(pages_per_seq=0),
-    dict(nseq=-1), dict(nseq=1 << 16), dict(max_count=-1), dict(max_count=9)])
+    dict(nseq=-1), dict(nseq=1 << 16), dict(max_count=-1), dict(max_count=9),
+    dict(max_count=(1 << 30) + 1, kept_stride=1 << 31)])
 def test_keep(change):
     _refused(device.kv4_keep, INVALID, device.kv4_caches([_cache()]), **{**KEEP, **change})
 
