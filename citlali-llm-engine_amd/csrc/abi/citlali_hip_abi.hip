@@ -723,7 +723,7 @@ CITLALI_EXPORT size_t citlali_hip_kv4_attention_workspace_bytes(int max_context,
     if (check_kv4_attention("kv4_attention", max_context, max_query, nseq, tokens, heads, kv_heads) ||
         !kv4_shape_ok(16, head_dim) || nseq == 0 || tokens == 0)
         return 0;
-    return kv4_attention_workspace(max_context, max_query, nseq, tokens, heads, kv_heads, head_dim);
+    return kv4_attention_workspace(false, max_context, max_query, nseq, tokens, heads, kv_heads, head_dim);
 }
 
 namespace {
@@ -746,7 +746,8 @@ int kv4_attend(const char* who, const citlali_hip_kv4_cache* cache, const uint16
     REQUIRE(q_stride % 8 == 0 && out_stride % 8 == 0, "%s: strides must be multiples of 8", who);
     REQUIRE(aligned(q, 16) && aligned(out, 16), "%s: q and out must be 16-byte aligned", who);
     if (nseq == 0 || tokens == 0) return CITLALI_OK;
-    const size_t need = kv4_attention_workspace(max_context, max_query, nseq, tokens, heads, c.kv_heads, c.head_dim);
+    const size_t need =
+        kv4_attention_workspace(masks != nullptr, max_context, max_query, nseq, tokens, heads, c.kv_heads, c.head_dim);
     REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned(workspace, 16))),
             "%s: workspace of %zu bytes needed, %zu given", who, need, workspace_bytes);
     const Kv4Attention a{q,      q_stride,  query_start, context_lens, page_table, pages_per_seq, nseq,
@@ -786,6 +787,15 @@ CITLALI_EXPORT int citlali_hip_draft_tree(const int32_t* parents, const int32_t*
     HIP_TRY(launch_draft_tree(
         DraftTree{parents, query_start, context_lens, nseq, tokens, max_query, masks, positions}, g_stream));
     return CITLALI_OK;
+}
+
+CITLALI_EXPORT size_t citlali_hip_kv4_tree_attention_workspace_bytes(int max_context, int max_query, int nseq,
+                                                                     int tokens, int heads, int kv_heads,
+                                                                     int head_dim) {
+    if (check_kv4_attention("kv4_tree_attention", max_context, max_query, nseq, tokens, heads, kv_heads) ||
+        max_query > CITLALI_MAX_TREE || !kv4_shape_ok(16, head_dim) || nseq == 0 || tokens == 0)
+        return 0;
+    return kv4_attention_workspace(true, max_context, max_query, nseq, tokens, heads, kv_heads, head_dim);
 }
 
 CITLALI_EXPORT int citlali_hip_kv4_tree_attention(const citlali_hip_kv4_cache* cache, const uint16_t* q,

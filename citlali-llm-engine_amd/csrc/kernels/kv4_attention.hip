@@ -61,6 +61,12 @@ __device__ __forceinline__ Kv4Seq<kTree> kv4_seq(const Kv4Attention& a, int seq)
     return s;
 }
 
+// Chunks of a sequence whose rows all see some of its last positions; one where there
+// are no positions.
+__device__ __forceinline__ int kv4_chunks(const Kv4Seq<true>& s, int chunk) {
+    return max(1, (min(s.context, s.cap) + chunk - 1) / chunk);
+}
+
 // V of four positions that some rows do not see: a weight of 0 would not keep a
 // NaN from them.  Clears the scales (d of four positions, then m) of those whose
 // m is NaN -- their codes are 0 -- and returns them as bits.
@@ -88,6 +94,11 @@ __device__ __forceinline__ int seq_of(int x, int layer, int nseq) {
 
 constexpr int kBlk = 256, kWaves = kBlk / kWave;
 constexpr float kShift = 14.f;   // weights are kept times 2^14 (base 2)
+// The maximum that weights refer to moves only when it is exceeded by kSlack (base
+// 2; kSlackScore of a score); beyond kFar a reference is taken off the scores first.
+constexpr float kSlack = 4.f, kFar = 1024.f;
+template <int HD>
+constexpr float kSlackScore = kSlack * 0.693147181f * (HD == 128 ? 11.3137085f : 8.f);   // kSlack / scale_log2
 
 // 2^((a - b) scale) of scores a <= b, of which -inf is none at all.  The maxima
 // that weights and sums refer to are kept as scores: a difference of scores is as
@@ -128,7 +139,7 @@ __device__ __forceinline__ float score_factor(float a, float b, float scale_log2
 // sequences of 150 .. 1500, 52.6 MB, in 17.6.
 // ---------------------------------------------------------------------------
 template <int HD, int kCols, bool kTree>
-__global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4_decode_kernel(
+__global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 || (kTree && HD == 64) ? 3 : 2) void kv4_decode_kernel(
     Kv4View c, Kv4Attention a, int chunk, int n_splits, float scale_log2) {
     using L = Kv4Layout<HD>;
     using Vec = std::conditional_t<HD == 128, u32x4, u32x2>;   // a lane's codes of 16 positions
@@ -233,7 +244,13 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4
     load_v(c0 + 32 * wave);
     if constexpr (kQInLds) lds_only_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    for (int t = c0 + 32 * wave; t < c1; t += 32 * kWaves) {
+    // A tree's tiles with positions of its rows have a loop of their own: with the masks
+    // in one the compiler keeps less in registers (64 rows of 16384 positions on the
+    // prompt kernel, below: 121 us for 95).
+    int t = c0 + 32 * wave;
+#pragma unroll
+    for (int phase = kTree ? 0 : 1; phase < 2; ++phase)
+    for (const bool tail = kTree && phase == 1; t < (kTree && !tail ? min(c1, s.before() - 31) : c1); t += 32 * kWaves) {
         const int there = (page_of(t) >= 0) | (page_of(t + 16) >= 0) << 1;
         const bool whole = there == 3 && t + 32 <= least;
         f32x4 sc[kCols][2];
@@ -266,7 +283,7 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4
         for (int n = 0; n < kCols; ++n) {
             if (!whole) {
                 asm volatile("");   // a branch: most tiles skip it
-                if constexpr (kTree)
+                if (kTree && tail)
                     sees[n] = see[n] < 0 ? 0u
                                          : tree_bits(a.masks + (size_t)see[n] * a.mask_words, a.mask_words,
                                                      t - s.before());
@@ -275,15 +292,16 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int p = 16 * u + 4 * grp + i;
-                        const bool seen = ((there >> u) & 1) && (kTree ? t + p < c1 && (sees[kTree ? n : 0] >> p & 1)
-                                                                       : t + p < min(see[n], c1));
+                        const bool seen = ((there >> u) & 1) && t + p < (kTree ? c1 : min(see[n], c1)) &&
+                                          (!kTree || !tail || (sees[kTree ? n : 0] >> p & 1));
                         sc[n][u][i] = seen ? sc[n][u][i] : -INFINITY;
                     }
             }
             float mt = max3(max3(sc[n][0][0], sc[n][0][1], sc[n][0][2]), sc[n][0][3], sc[n][1][0]);
             mt = max3(mt, sc[n][1][1], max3(sc[n][1][2], sc[n][1][3], sc[n][1][3]));
             mt = max32(max16(mt));
-            if (__builtin_amdgcn_ballot_w64(mt > m_run[n]) != 0) {
+            // (rows of a tree in the prompt kernel's way, see there)
+            if (__builtin_amdgcn_ballot_w64(kTree ? mt - m_run[n] > kSlackScore<HD> : mt > m_run[n]) != 0) {
                 const float m_new = fmaxf(m_run[n], mt);
                 const float f = score_factor(m_run[n], m_new, scale_log2);
                 m_run[n] = m_new;
@@ -292,12 +310,22 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4
                 for (int d = 0; d < kDims; ++d) o[n][d] *= f;
             }
             const float ref = m_run[n] == -INFINITY ? 0.f : m_run[n];
+            float off = 0.f;
+            if constexpr (kTree) {
+                off = fmaf(-ref, scale_log2, kShift - kSlack);
+                if (__builtin_amdgcn_ballot_w64(fabsf(off) > kFar) != 0) {
+                    asm volatile("");
+                    sc[n][0] -= ref;
+                    sc[n][1] -= ref;
+                    off = kShift - kSlack;
+                }
+            }
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    pw[n][4 * u + i] =
-                        (_Float16)__builtin_amdgcn_exp2f(fmaf(sc[n][u][i] - ref, scale_log2, kShift));
+                    pw[n][4 * u + i] = (_Float16)__builtin_amdgcn_exp2f(
+                        kTree ? fmaf(sc[n][u][i], scale_log2, off) : fmaf(sc[n][u][i] - ref, scale_log2, kShift));
             l_run[n] = add_weights(pw[n], l_run[n]);
         }
         if (!whole) {   // positions no row may use: their V counts as 0, whatever it holds
@@ -321,7 +349,7 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4
                             __builtin_amdgcn_ballot_w64(col / (512 / HD) == g && ((nan >> b) & 1) != 0);
                         if (who == 0 || (HD == 128 ? grp : grp >> 1) != g) continue;
                         first = min(first, t + 16 * (b / 4) + 4 * (__builtin_ctzll(who) / 16) + b % 4);
-                        if constexpr (kTree)
+                        if (kTree && tail)
                             for (int y = 0; y < 4; ++y)
                                 where |= (who >> (16 * y) & 0xffff) != 0 ? 1u << (16 * (b / 4) + 4 * y + b % 4) : 0u;
                     }
@@ -329,7 +357,7 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 ? 3 : 2) void kv4
                 for (int n = 0; n < kCols; ++n)
 #pragma unroll
                     for (int d = 0; d < kDims; ++d)
-                        if (kTree ? (sees[kTree ? n : 0] & where) != 0 : see[n] > first)
+                        if (!kTree ? see[n] > first : tail ? (sees[kTree ? n : 0] & where) != 0 : first < INT_MAX)
                             o[n][d] = f32x4{NAN, NAN, NAN, NAN};
             }
         }
@@ -518,7 +546,6 @@ __global__ __launch_bounds__(kBlk) void kv4_merge_kernel(Kv4Attention a, int gro
 // ---------------------------------------------------------------------------
 constexpr int kRowTile = 128, kTile = 64;   // rows of a workgroup; positions of a step
 constexpr int kPromptNotes = 10 * kWaves;   // words that a part's waves leave one another
-constexpr float kSlack = 4.f, kFar = 1024.f;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 template <int HD, int kParts, bool kTree>
@@ -528,7 +555,6 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
     using Vec = std::conditional_t<HD == 128, u32x4, u32x2>;
     constexpr int kWords = HD / 32;                    // words of codes a thread has of a position (K) or of 4 (V)
     constexpr int kHalves = HD * kTile;                // of K (or V) in a buffer
-    constexpr float kSlackScore = kSlack * 0.693147181f * (HD == 128 ? 11.3137085f : 8.f);   // kSlack / scale_log2
     extern __shared__ __align__(16) float lds[];
     const int part = kParts == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kBlk);
     uint16_t* const buf = reinterpret_cast<uint16_t*>(lds) + part * 4 * kHalves;   // [2][K, V][kHalves]
@@ -545,9 +571,18 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
     // 35.1 for two of 761, 43 against 50 for three pieces of 636 behind a prefix)
     const int kvh = blockIdx.x % c.kv_heads;
     const int group = a.heads / c.kv_heads, tiles = (a.max_query * group + kRowTile - 1) / kRowTile;
-    const int rest = blockIdx.z * gridDim.y + blockIdx.y, split = rest % n_splits, tile = tiles - 1 - rest / n_splits;
+    const int rest = blockIdx.z * gridDim.y + blockIdx.y;
     const int seq = seq_of(blockIdx.x / c.kv_heads, rest, a.nseq);
     const Kv4Seq<kTree> s = kv4_seq<kTree>(a, seq);
+    int split, tile;
+    if constexpr (kTree) {   // every sequence's last chunk, the short one, last (304 -> 207 us, see below)
+        tile = rest % tiles;
+        split = rest / tiles - (n_splits - kv4_chunks(s, chunk));
+        if (split < 0) return;
+    } else {
+        split = rest % n_splits;
+        tile = tiles - 1 - rest / n_splits;
+    }
     const int rows = min(s.n, a.max_query) * group, row0 = tile * kRowTile;
     if (tile < 0 || row0 >= rows) return;
     const int most = max(0, s.see((min(rows, row0 + kRowTile) - 1) / group));
@@ -669,7 +704,8 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
         for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
     float m_run = -INFINITY, l_run = 0.f;
 
-    auto process = [&](int t, int b) {
+    // kTail: of a tree, positions of its rows among the tile's
+    auto process = [&](int t, int b, auto kTail) __attribute__((always_inline)) {
         hide(b ^ 1);
         if (t >= wave_most) {   // uniform: no row of the wave sees the tile
             store(b ^ 1);
@@ -703,9 +739,9 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
             __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
-        uint32_t sees[kTree ? 2 : 1];   // of a tree's row, the tile's positions
+        uint32_t sees[kTail ? 2 : 1];   // of a tree's row, the tile's positions
         if (!whole) {
-            if constexpr (kTree) {
+            if constexpr (kTail) {
                 const uint32_t* row = a.masks + (size_t)(s.start + i) * a.mask_words;
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
@@ -717,7 +753,7 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
                 for (int e = 0; e < 16; ++e) {
                     const int p = 32 * u + 8 * (e / 4) + 4 * half + e % 4;
                     const bool seen = t + p < see && ((there >> (p >> 4) * 2) & 1) &&
-                                      (!kTree || (sees[kTree ? u : 0] >> (p & 31) & 1));
+                                      (!kTail || (sees[kTail ? u : 0] >> (p & 31) & 1));
                     sc[u][e] = seen ? sc[u][e] : -INFINITY;
                 }
         }
@@ -730,8 +766,10 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
                 for (int w = 0; w < kWaves; ++w)
                     if ((there >> (2 * w)) & 2) {
                         const int at = nan_at[(b * kWaves + w) * 4 + (HD == 128 ? 2 * y + half : y)];
-                        if constexpr (kTree)
+                        if constexpr (kTail)
                             meets |= ((w < 2 ? sees[0] : sees[1]) >> (16 * (w & 1)) & (uint32_t)at) != 0;
+                        else if constexpr (kTree)
+                            meets |= at != 0;
                         else
                             first = min(first, at);
                     }
@@ -748,7 +786,7 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
 #pragma unroll
             for (int e = 0; e < 16; e += 2) mt = max3(mt, sc[u][e], sc[u][e + 1]);
         mt = max32(mt);
-        if (__builtin_amdgcn_ballot_w64(mt - m_run > kSlackScore) != 0) {
+        if (__builtin_amdgcn_ballot_w64(mt - m_run > kSlackScore<HD>) != 0) {
             const float m_new = fmaxf(m_run, mt);
             const float f = score_factor(m_run, m_new, scale_log2);
             m_run = m_new;
@@ -792,11 +830,17 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
     store(0);
     load(c0 + mine + kTurn);
     __syncthreads();
-    for (int t = c0, b = 0; t < c1; t += kTurn, b ^= 1) {
-        process(t + mine, b);
+    int t = c0, b = 0;
+    auto turn = [&](auto kTail) __attribute__((always_inline)) {
+        process(t + mine, b, kTail);
         load(t + mine + 2 * kTurn);
         __syncthreads();
-    }
+        t += kTurn;
+        b ^= 1;
+    };
+    if constexpr (kTree)
+        while (t < c1 && t + kTurn <= s.before()) turn(std::false_type{});
+    while (t < c1) turn(std::bool_constant<kTree>{});
 
     // ---- out: O^T's rows back in dim order through LDS, a wave's rows at a time ----
     float l = sum32(l_run);
@@ -890,11 +934,19 @@ constexpr int kPromptBlocks = 256, kPromptChunk = 192, kPromptChunkFull = 512;
 // against 36.3, 288 workgroups of half of 1390 positions 54.6 against 48.5, 312 of
 // 44 positions 11.7 against 9.4).
 constexpr int kTwoPartBlocks = 384, kTwoPartContext = 256;
+// Trees have few rows behind contexts of any length: the prompt kernel's grid is cut
+// finer than a prompt's, into about kTreeBlocks workgroups were all contexts the
+// longest (four sequences of 38 to 60 rows of 5 heads behind 22452 to 32000 positions:
+// kernel and merge 215 us, cut for one round of workgroups 263, into 1280 232; 25 of 17
+// to 33 rows of 2 heads of 64 behind 176 to 2500 37, 45 and 40).  The merge takes one
+// wave a head from kMergeUnits heads on (180 rows of 40 heads in 15 parts: 12.1 us, by
+// four waves 18.5).
+constexpr int kTreeBlocks = 700, kMergeUnits = 2048;
 struct Kv4Plan {
     bool few;
     int cols, tiles, chunk, n_splits;
 };
-Kv4Plan kv4_plan(int max_context, int max_query, int nseq, int heads, int kv_heads) {
+Kv4Plan kv4_plan(bool tree, int max_context, int max_query, int nseq, int heads, int kv_heads) {
     Kv4Plan p{};
     const long long rows = (long long)max_query * (heads / kv_heads);
     p.few = rows <= kFewRows;
@@ -911,7 +963,8 @@ Kv4Plan kv4_plan(int max_context, int max_query, int nseq, int heads, int kv_hea
         const long long blocks = (long long)p.tiles * kv_heads * nseq;
         auto least = [&](long long most, int chunk) { return std::min<long long>(most / blocks, max_context / chunk); };
         const long long splits =
-            std::max({1ll, least(kPromptBlocks, kPromptChunk), least(2 * kPromptBlocks, kPromptChunkFull)});
+            tree ? std::max(1ll, least(kTreeBlocks, kPromptChunk))
+                 : std::max({1ll, least(kPromptBlocks, kPromptChunk), least(2 * kPromptBlocks, kPromptChunkFull)});
         p.chunk = whole((max_context + splits - 1) / splits, kTile);
     }
     p.n_splits = (max_context + p.chunk - 1) / p.chunk;
@@ -920,7 +973,7 @@ Kv4Plan kv4_plan(int max_context, int max_query, int nseq, int heads, int kv_hea
 
 template <int HD, bool kTree>
 hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
-    const Kv4Plan p = kv4_plan(a.max_context, a.max_query, a.nseq, a.heads, c.kv_heads);
+    const Kv4Plan p = kv4_plan(kTree, a.max_context, a.max_query, a.nseq, a.heads, c.kv_heads);
     const float scale_log2 = 1.44269504088896340736f / sqrtf((float)HD);
     const int group = a.heads / c.kv_heads;
     const bool last = p.n_splits == 1;
@@ -960,7 +1013,7 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
     // one wave covers 4 chunks a lane group at once; with more of them four waves share a head
     const long long units = (long long)a.max_query * a.heads;
     const int tile_rows = p.few ? kFewRows : kRowTile;
-    if (p.n_splits <= 4 * kWave / (HD / 4))
+    if (p.n_splits <= 4 * kWave / (HD / 4) || (kTree && units * a.nseq > kMergeUnits))
         launch_kernel(kv4_merge_kernel<HD, 1, kTree>, dim3((unsigned)((units + kWaves - 1) / kWaves), a.nseq), dim3(kBlk), 0,
                       s, a, group, tile_rows, p.chunk, p.n_splits, scale_log2);
     else
@@ -971,9 +1024,9 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
 
 }  // namespace
 
-size_t kv4_attention_workspace(int max_context, int max_query, int nseq, int tokens, int heads, int kv_heads,
-                               int head_dim) {
-    const Kv4Plan p = kv4_plan(max_context, max_query, nseq, heads, kv_heads);
+size_t kv4_attention_workspace(bool tree, int max_context, int max_query, int nseq, int tokens, int heads,
+                               int kv_heads, int head_dim) {
+    const Kv4Plan p = kv4_plan(tree, max_context, max_query, nseq, heads, kv_heads);
     if (p.n_splits == 1) return 0;
     return (size_t)tokens * heads * p.n_splits * (head_dim + 2) * sizeof(float);
 }

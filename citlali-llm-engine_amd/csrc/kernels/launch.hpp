@@ -238,8 +238,8 @@ struct Kv4Attention {
     const uint32_t* masks;
     int mask_words;
 };
-size_t kv4_attention_workspace(int max_context, int max_query, int nseq, int tokens, int heads, int kv_heads,
-                               int head_dim);
+size_t kv4_attention_workspace(bool tree, int max_context, int max_query, int nseq, int tokens, int heads,
+                               int kv_heads, int head_dim);
 hipError_t launch_kv4_attention(const Kv4View& c, const Kv4Attention& a, hipStream_t s);
 
 // Positions first[s] + kept[s][j] move to first[s] + j, in `layers` caches.

@@ -115,6 +115,7 @@ SIGNATURES = [
     ("citlali_hip_draft_tree", c_int, [_P, _P, _P, c_int, c_int, c_int, _P, _P]),
     ("citlali_hip_kv4_tree_attention", c_int, [POINTER(Kv4Cache), _P, c_longlong, _P, _P, _P, _P, c_int, c_int, c_int,
                                                c_int, c_int, c_int, _P, c_size_t, _P, c_longlong]),
+    ("citlali_hip_kv4_tree_attention_workspace_bytes", c_size_t, [c_int] * 7),
     ("citlali_hip_verify_drafts", c_int, [_P, c_int, c_longlong, c_int, _P, c_longlong, _P, _P, _P, c_int, c_int,
                                           c_int, _P, _P, _P, _P, _P, _P, _P, c_size_t]),
     ("citlali_hip_verify_drafts_workspace_bytes", c_size_t, [c_int] * 5),

@@ -473,11 +473,17 @@ def draft_tree(parents, query_start, context_lens, nseq: int, tokens: int, max_q
               _at(masks), _at(positions))
 
 
+def kv4_tree_attention_workspace_bytes(max_context: int, max_query: int, nseq: int, tokens: int, heads: int,
+                                       kv_heads: int, head_dim: int) -> int:
+    return int(_lib.load().citlali_hip_kv4_tree_attention_workspace_bytes(max_context, max_query, nseq, tokens, heads,
+                                                                          kv_heads, head_dim))
+
+
 def kv4_tree_attention(cache, q, q_stride: int, query_start, context_lens, masks, page_table, pages_per_seq: int,
                        nseq: int, tokens: int, max_query: int, max_context: int, heads: int, workspace,
                        workspace_bytes: int, out, out_stride: int) -> None:
     """kv4_attention where a query sees the positions before its tree and those
-    that its mask names; the same workspace.  See citlali_hip_kv4_tree_attention."""
+    that its mask names.  See citlali_hip_kv4_tree_attention."""
     _lib.call("citlali_hip_kv4_tree_attention", cache, _at(q), q_stride, _at(query_start), _at(context_lens),
               _at(masks), _at(page_table), pages_per_seq, nseq, tokens, max_query, max_context, heads, _at(workspace),
               workspace_bytes, _at(out), out_stride)

@@ -459,12 +459,14 @@ int citlali_hip_draft_tree(const int32_t* parents, const int32_t* query_start, c
  * with n rows, and position context_lens[s] - n + j where bit j of its mask is set
  * (any masks of that layout, not only a tree's; bits past the row count are
  * ignored).  max_query is at most CITLALI_MAX_TREE.  Workspace:
- * citlali_hip_kv4_attention_workspace_bytes() of the same bounds. */
+ * citlali_hip_kv4_tree_attention_workspace_bytes() of the same bounds. */
 int citlali_hip_kv4_tree_attention(const citlali_hip_kv4_cache* cache, const uint16_t* q, long long q_stride,
                                    const int32_t* query_start, const int32_t* context_lens, const uint64_t* masks,
                                    const int32_t* page_table, int pages_per_seq, int nseq, int tokens, int max_query,
                                    int max_context, int heads, void* workspace, size_t workspace_bytes, uint16_t* out,
                                    long long out_stride);
+size_t citlali_hip_kv4_tree_attention_workspace_bytes(int max_context, int max_query, int nseq, int tokens, int heads,
+                                                      int kv_heads, int head_dim);
 
 /* Which drafted tokens stay, so that the tokens that come out are distributed as
  * if the model had drawn them one by one.  Row r's logits (element r * row_stride

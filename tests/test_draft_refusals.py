@@ -63,12 +63,16 @@ def test_attention(change, status):
 
 def test_attention_names_itself_and_its_workspace():
     call = {**ATTENTION, "nseq": 1, "tokens": 8, "max_context": 100000, "pages_per_seq": 100000 // 16}
-    need = device.kv4_attention_workspace_bytes(100000, 8, 1, 8, 8, 2, 128)
+    need = device.kv4_tree_attention_workspace_bytes(100000, 8, 1, 8, 8, 2, 128)
     assert need > 0
     for change in (dict(workspace=A, workspace_bytes=need - 1), dict(workspace=None, workspace_bytes=need),
                    dict(workspace=A + 4, workspace_bytes=need)):
         _refused(device.kv4_tree_attention, INVALID, _cache(), **{**call, **change})
         assert "kv4_tree_attention" in pycitlali.last_error()
+    lib = pycitlali.load()
+    for bad in ((0, 8, 1, 8, 8, 2, 128), (9, 0, 1, 8, 8, 2, 128), (9, 257, 1, 8, 8, 2, 128), (9, 8, -1, 8, 8, 2, 128),
+                (9, 8, 1, 8, 9, 2, 128), (9, 8, 1, 8, 8, 2, 100), (9, 8, 1, 8, 34, 2, 128), (9, 8, 0, 0, 8, 2, 128)):
+        assert lib.citlali_hip_kv4_tree_attention_workspace_bytes(*bad) == 0
     for cache in (_cache(page_size=24), _cache(head_dim=96)):
         _refused(device.kv4_tree_attention, UNSUPPORTED, cache, **ATTENTION)
 

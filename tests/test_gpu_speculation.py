@@ -28,7 +28,7 @@ class Speculator(Server):
         heads, kv, hd = self.dims
         d = self.hip.device
         self.spaces = [(self.hip.DeviceArray(max(16, b)), b) for b in (
-            d.kv4_attention_workspace_bytes(self.most, ROWS, self.nseq, n, heads, kv, hd),
+            d.kv4_tree_attention_workspace_bytes(self.most, ROWS, self.nseq, n, heads, kv, hd),
             d.verify_drafts_workspace_bytes(self.nseq, n, ROWS, VOCAB, False))]
 
     def speculate(self):
