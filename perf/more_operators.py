@@ -344,7 +344,8 @@ def prepare(case, seed):
     if own:
         dev = _hip()
         s["cache"] = dev.kv4_cache(s["pages"].data_ptr(), pages, page, kv, hd)
-        s["bytes"] = dev.kv4_attention_workspace_bytes(s["max_context"], c["nodes"], c["seqs"], start[-1], h, kv, hd)
+        s["bytes"] = dev.kv4_tree_attention_workspace_bytes(s["max_context"], c["nodes"], c["seqs"], start[-1], h, kv,
+                                                            hd)
         s["space"] = torch.empty(max(16, s["bytes"]), dtype=torch.uint8, device="cuda")
     return s
 
