@@ -456,14 +456,19 @@ __global__ __launch_bounds__(kKeepWaves * kWave) void kv4_keep_kernel(Kv4View c,
             to_at[i] = from < 0 ? -1 : to;
         }
         __syncthreads();
-        load(0, v);
-        for (int t = 0; t < some; t += turn) {
-            wait_vm<0>();   // in registers, not on the way, before another wave may write there
-            __syncthreads();
-            if (t + turn < some) load(t + turn, w);
-            store(t, v);
+        // two turns' tokens on their way while a third's are stored
+        auto go = [&](int t, u32x4 (&x)[kSteps]) {
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) v[s] = w[s];
+            for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(x[s]));   // in registers, not on the way,
+            lds_only_barrier();                                              // before another wave may write there
+            store(t, x);
+            if (t + 2 * turn < some) load(t + 2 * turn, x);
+        };
+        load(0, v);
+        if (turn < some) load(turn, w);
+        for (int t = 0; t < some; t += 2 * turn) {
+            go(t, v);
+            if (t + turn < some) go(t + turn, w);
         }
     }
 }
