@@ -306,101 +306,96 @@ __global__ __launch_bounds__(kBlk) void verify_sums_kernel(VerifyDrafts a, int s
 constexpr int kWalk = 512, kWalkWaves = kWalk / kWave;
 constexpr int kRun = kSeg / kWalk;   // ids of a thread
 
-// Sums over the threads before this one, and over all.
-struct Scan {
-    double before, total;
-};
-__device__ Scan block_scan(double v, double* room) {
-    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const double run = wave_scan64(v);
-    if (lane == kWave - 1) room[wave] = run;
-    __syncthreads();
-    double base = 0., total = 0.;
-#pragma unroll
-    for (int w = 0; w < kWalkWaves; ++w) {
-        base = w == wave ? total : base;
-        total += room[w];
-    }
-    return Scan{base + (run - v), total};
-}
-
-// The `at` and `before` of the first thread that is `here`, and the `at` of the last
-// that has `any` (INT_MAX and -1 without one).
-struct Found {
-    int at, last;
-    double before;
-};
-__device__ Found block_find(bool here, bool any, int at, double before, Found* room) {
-    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const uint64_t who = __builtin_amdgcn_ballot_w64(here), have = __builtin_amdgcn_ballot_w64(any);
-    if (lane == (who != 0 ? __builtin_ctzll(who) : 0)) {
-        room[wave].at = who != 0 ? at : INT_MAX;
-        room[wave].before = before;
-    }
-    if (lane == (have != 0 ? 63 - __builtin_clzll(have) : 0)) room[wave].last = have != 0 ? at : -1;
-    __syncthreads();
-    Found f{INT_MAX, -1, 0.};
-#pragma unroll
-    for (int w = kWalkWaves - 1; w >= 0; --w) {
-        const Found g = room[w];
-        if (g.at < INT_MAX) {
-            f.at = g.at;
-            f.before = g.before;
-        }
-        f.last = max(f.last, g.last);
-    }
-    return f;
-}
 __device__ __forceinline__ float unit(float u) { return u >= 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f; }
+
+// The first of `count` values whose running sum exceeds t(total), and the sum before
+// it; where rounding leaves none, the last that is above 0, with t infinite; -1 where
+// the total is 0.  By every wave for itself: 64 blocks of them at a time, then the
+// block that has it.
+struct Place {
+    int at;
+    double before, t;
+};
+template <typename V>
+__device__ __forceinline__ Place find_place(int count, float u, V value) {
+    const int lane = threadIdx.x & (kWave - 1);
+    Place f{0, 0., -1.};
+    for (int n = count;;) {   // n values from f.at on
+        const int each = (n + kWave - 1) / kWave;
+        double v = 0.;
+        for (int k = 0; k < each; ++k) {
+            const int j = lane * each + k;
+            v += j < n ? value(f.at + j) : 0.;
+        }
+        const double upto = wave_scan64(v);
+        if (f.t < 0.) {
+            const double total = lane64(upto, kWave - 1);
+            if (!(total > 0.)) return {-1, 0., 0.};
+            f.t = (double)unit(u) * total;
+        }
+        uint64_t who = __builtin_amdgcn_ballot_w64(f.before + upto > f.t);
+        if (who == 0) {
+            who = __builtin_amdgcn_ballot_w64(v > 0.);
+            if (who == 0) return {-1, 0., 0.};
+            who = 1ull << (63 - __builtin_clzll(who));
+            f.t = INFINITY;
+        }
+        const int l = __builtin_ctzll(who);
+        f.before += lane64(upto - v, l);
+        f.at += l * each;
+        if (each == 1) return f;
+        n = min(each, n - l * each);
+    }
+}
 
 // The first id whose running sum of weights exceeds u times their total; -1 where
 // the total is 0.  value(j): the sum of segment j's weights; weights(id, w): those of
 // the kRun ids from `id` on.
 template <typename V, typename W>
 __device__ int pick(int segs, float u, V value, W weights) {
-    __shared__ double sums[3][kWalkWaves];
-    __shared__ Found finds[2][kWalkWaves];
-    const int tid = threadIdx.x;
-    double v = tid < segs ? value(tid) : 0.;
-    Scan s = block_scan(v, sums[0]);
-    double total = s.total, base = 0.;
-    for (int j0 = kWalk; j0 < segs; j0 += kWalk) {
-        __syncthreads();
-        total += block_scan(j0 + tid < segs ? value(j0 + tid) : 0., sums[1]).total;
-    }
-    if (!(total > 0.)) return -1;
-    const double t = (double)unit(u) * total;
-    Found f = block_find(s.before + v > t, v > 0., tid, s.before, finds[0]);
-    for (int j0 = kWalk; j0 < segs && f.at == INT_MAX; j0 += kWalk) {
-        base += s.total;
-        __syncthreads();
-        v = j0 + tid < segs ? value(j0 + tid) : 0.;
-        s = block_scan(v, sums[1]);
-        const Found g = block_find(base + s.before + v > t, v > 0., j0 + tid, base + s.before, finds[0]);
-        f = Found{g.at, max(f.last, g.last), g.before};
-    }
-    // where rounding leaves no segment, or none of its ids, the last that has a weight
-    const bool none = f.at == INT_MAX;
-    const int id0 = (none ? f.last : f.at) * kSeg + tid * kRun;
+    __shared__ double sums[kWalkWaves];
+    __shared__ int hits[kWalkWaves], lasts[kWalkWaves];
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const Place f = find_place(segs, u, value);
+    if (f.at < 0) return -1;
+    const int id0 = f.at * kSeg + (int)threadIdx.x * kRun;
     double w[kRun], sum = 0.;
     weights(id0, w);
 #pragma unroll
     for (int e = 0; e < kRun; ++e) sum += w[e];
-    s = block_scan(sum, sums[2]);
-    double run = f.before + s.before;
-    int at = INT_MAX, last = -1;
+    const double upto = wave_scan64(sum);
+    if (lane == kWave - 1) sums[wave] = upto;
+    __syncthreads();
+    double run = f.before;
+#pragma unroll
+    for (int k = 0; k < kWalkWaves - 1; ++k) run += k < wave ? sums[k] : 0.;
+    run += upto - sum;
+    int hit = INT_MAX, last = -1;
 #pragma unroll
     for (int e = 0; e < kRun; ++e) {
         run += w[e];
         if (w[e] > 0.) {
             last = id0 + e;
-            if (at == INT_MAX && !none && run > t) at = last;
+            hit = hit == INT_MAX && run > f.t ? last : hit;
         }
     }
-    const Found hit = block_find(at < INT_MAX, false, at, 0., finds[1]);
-    if (hit.at < INT_MAX) return hit.at;
+    // the wave's first hit, and its last id with a weight: for where rounding leaves no hit
+    const uint64_t who = __builtin_amdgcn_ballot_w64(hit < INT_MAX), have = __builtin_amdgcn_ballot_w64(last >= 0);
+    if (lane == 0) {
+        hits[wave] = INT_MAX;
+        lasts[wave] = -1;
+    }
+    wave_lds_sync();
+    if (who != 0 && lane == __builtin_ctzll(who)) hits[wave] = hit;
+    if (have != 0 && lane == 63 - __builtin_clzll(have)) lasts[wave] = last;
     __syncthreads();
-    return block_find(false, last >= 0, last, 0., finds[1]).last;
+    int first = INT_MAX, end = -1;
+#pragma unroll
+    for (int k = 0; k < kWalkWaves; ++k) {
+        first = min(first, hits[k]);
+        end = max(end, lasts[k]);
+    }
+    return first < INT_MAX ? first : end;
 }
 // kRun logits of a row from id on, -inf behind the last.
 template <bool kHalf>
@@ -485,8 +480,8 @@ template <bool kHalf>
 __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerifyDrafts a, int segs) {
     __shared__ RowSum sums[2 * kMaxTree];   // the rows', then their drafts'
     __shared__ int parent[kMaxTree], token[kMaxTree], gone[kMaxTree], path[kMaxTree];
-    __shared__ double p[kMaxTree], bar[kMaxTree], gone_sum[kMaxTree];
-    __shared__ double table[Exp2Table::kEntries];
+    __shared__ double p[kMaxTree], bar[kMaxTree], gone_p[kMaxTree], gone_sum[kMaxTree];
+    __shared__ double end_left;
     __shared__ int end_row, end_lost, end_count;
     const int seq = blockIdx.x, lane = threadIdx.x & (kWave - 1), tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -550,25 +545,33 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerifyDrafts a, int 
         if (a.token_probs) a.token_probs[rows.start + tid] = (float)mine;
     }
     __syncthreads();
-    if (wave == 0) {   // the path; lanes look for the current row's children
-        int above[kMaxTree / kWave];
-#pragma unroll
-        for (int k = 0; k < kMaxTree / kWave; ++k) above[k] = k * kWave + lane < rows.n ? parent[k * kWave + lane] : -1;
-        int current = 0, at = 0, count = 1, lost = 0;
+    if (wave == 0) {   // the path; the lanes have 64 rows at a time
+        int above = -1, mark = -1;
+        double chance = 0., limit = 0.;
+        auto look_at = [&](int from) {
+            const int i = min(from + lane, rows.n - 1);
+            above = from + lane < rows.n ? parent[i] : -1;
+            mark = token[i];
+            chance = p[i];
+            limit = bar[i];
+        };
+        int current = 0, at = 0, from = 0, count = 1, lost = 0;
         double left = 1.;
+        look_at(0);
         for (;;) {
-            int next = INT_MAX;
-#pragma unroll
-            for (int k = kMaxTree / kWave - 1; k >= 0; --k) {
-                const uint64_t who = __builtin_amdgcn_ballot_w64(above[k] == current && k * kWave + lane > at);
-                if (who != 0) next = k * kWave + __builtin_ctzll(who);
+            const uint64_t who = __builtin_amdgcn_ballot_w64(above == current && from + lane > at);
+            if (who == 0) {
+                from += kWave;
+                if (from >= rows.n) break;
+                look_at(from);
+                continue;
             }
-            if (next == INT_MAX) break;
-            at = next;
-            const int mark = token[at];
-            double mine = p[at];
-            for (int g = 0; g < lost; ++g) mine = gone[g] == mark ? 0. : mine;
-            if (bar[at] * (a.draft ? 1. : left) < mine) {
+            const int l = __builtin_ctzll(who), its_mark = __builtin_amdgcn_readlane(mark, l);
+            at = from + l;
+            bool again = false;   // rejected before
+            for (int g = lane; g < lost; g += kWave) again |= gone[g] == its_mark;
+            const double mine = __builtin_amdgcn_ballot_w64(again) != 0 ? 0. : lane64(chance, l);
+            if (lane64(limit, l) * (a.draft ? 1. : left) < mine) {
                 current = at;
                 if (lane == 0) path[count] = at;
                 ++count;
@@ -576,7 +579,10 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerifyDrafts a, int 
                 left = 1.;
             } else {
                 left -= mine;
-                if (lane == 0) gone[lost] = mark;
+                if (lane == 0) {
+                    gone[lost] = its_mark;
+                    gone_p[lost] = mine;
+                }
                 ++lost;
                 wave_lds_sync();
             }
@@ -586,6 +592,7 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerifyDrafts a, int 
             end_row = current;
             end_lost = lost;
             end_count = count;
+            end_left = left;
         }
     }
     __syncthreads();
@@ -611,29 +618,28 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerifyDrafts a, int 
             const void* row = logit_row<kHalf>(a.logits, a.stride, rows.start + f);
             const Segment* mine = work.segments + ((size_t)rows.start + f) * segs;
             const int out = a.draft ? 0 : lost;   // rejected tokens, left out
-            // their segments anew, a wave each
-            Exp2Table exp2;
-            if (out > 0) exp2.make<kWalk>(table, c);
+            // What is left of their segments, a wave each: the sum less their weights, an
+            // error of 2^-43 of p in all; summed anew without them (some 10 us) where that
+            // counts, with less than a sixteenth of p left, or leaves hardly more than it.
             for (int g = wave; g < out; g += kWalkWaves) {
                 const int mark = __builtin_amdgcn_readfirstlane(gone[g]), seg = mark / kSeg;
                 if (mark < 0) continue;
-                Logits<kHalf> l;
-                l.load(row, a.vocab, seg, lane);
-                uint32_t here = 0;   // of the lane's elements
-                for (int k = 0; k < out; ++k) {
-                    const int other = __builtin_amdgcn_readfirstlane(gone[k]);
-                    if (other < 0 || other / kSeg != seg) continue;
-#pragma unroll
-                    for (int e = 0; e < kPer; ++e) here |= (l.id_of(seg, e, lane) == other ? 1u : 0u) << e;
+                const Segment whole = mine[seg];
+                const double all = whole.sum * weight(whole.top, s.m, c);
+                double sum = all;
+                for (int k = 0; k < out; ++k) sum -= gone[k] >= 0 && gone[k] / kSeg == seg ? gone_p[k] * s.s : 0.;
+                if (end_left < 0.0625 || !(sum >= all * 0x1p-40)) {
+                    const int id1 = min(a.vocab, (seg + 1) * kSeg);
+                    sum = 0.;
+#pragma unroll 4
+                    for (int id = seg * kSeg + lane; id < id1; id += kWave) {
+                        bool is_out = false;
+                        for (int k = 0; k < out; ++k) is_out |= gone[k] == id;
+                        const double v = weight(logit<kHalf>(row, id), s.m, c);
+                        sum += is_out ? 0. : v;
+                    }
+                    sum = wave_sum64(sum);
                 }
-                // (what is left may be nothing, or far below the largest)
-                double sum = 0.;
-#pragma unroll
-                for (int e = 0; e < kPer; ++e) {
-                    const double v = exp2((double)l.at(e) - (double)s.m);
-                    sum += (here >> e & 1) != 0 || l.at(e) == -INFINITY ? 0. : v;
-                }
-                sum = wave_sum64(sum);
                 if (lane == 0) gone_sum[g] = sum;
             }
             if (out > 0) __syncthreads();
