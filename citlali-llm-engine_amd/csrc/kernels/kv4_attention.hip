@@ -168,6 +168,7 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 || (kTree && HD =
     half8 q[kQInLds ? 1 : kCols][kSteps];
     int see[kCols];   // positions a row sees; in a tree the row (-1: none)
     half8* const q_lds = reinterpret_cast<half8*>(lds);   // [column tile][step][lane]
+    u32x4 mine[kTree && kQInLds ? kCols : 1];             // (a row that is none has another's)
 #pragma unroll
     for (int n = 0; n < kCols; ++n) {
         const int r = col + 16 * n, i = r / group;
@@ -175,6 +176,10 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 || (kTree && HD =
         see[n] = kTree ? (real ? s.start + i : -1) : real ? s.see(i) : 0;
         const uint16_t* qr = a.q + (size_t)(s.start + (real ? i : 0)) * a.q_stride +
                              (size_t)(kvh * group + (real ? r - i * group : 0)) * HD + grp * (HD / 4);
+        if constexpr (kTree && kQInLds) {   // a piece a wave, written once all are on their way
+            mine[n] = *reinterpret_cast<const u32x4*>(qr + 8 * (wave % kSteps));
+            continue;
+        }
 #pragma unroll
         for (int t = 0; t < kSteps; ++t) {
             u32x4 v = *reinterpret_cast<const u32x4*>(qr + 8 * t);
@@ -242,6 +247,12 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 || (kTree && HD =
 
     load_k(c0 + 32 * wave);
     load_v(c0 + 32 * wave);
+    if constexpr (kTree && kQInLds) {
+#pragma unroll
+        for (int n = 0; n < kCols; ++n)
+            if (kSteps == kWaves || wave / kSteps == (n & 1))
+                q_lds[(n * kSteps + wave % kSteps) * kWave + lane] = __builtin_bit_cast(half8, mine[n]);
+    }
     if constexpr (kQInLds) lds_only_barrier();
     __builtin_amdgcn_sched_barrier(0);
     // A tree's tiles with positions of its rows have a loop of their own: with the masks
