@@ -335,12 +335,5 @@ __device__ __forceinline__ void copy16_to_lds(const uint8_t* src, uint8_t* dst_w
                                      (__attribute__((address_space(3))) void*)dst_wave_base, 16, 0,
                                      kNontemporal ? 2 : 0);
 }
-// 4 bytes per lane, likewise at dst_wave_base + 4 lane
-template <bool kNontemporal = false>
-__device__ __forceinline__ void copy4_to_lds(const uint8_t* src, uint8_t* dst_wave_base) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                     (__attribute__((address_space(3))) void*)dst_wave_base, 4, 0,
-                                     kNontemporal ? 2 : 0);
-}
 
 }  // namespace citlali::hip

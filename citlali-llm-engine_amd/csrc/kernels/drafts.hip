@@ -228,10 +228,25 @@ struct Logits {
     u32x4 w[kLoads];   // fp32, or pairs of fp16
     __device__ void load(const void* row, int vocab, int seg, int lane) {
         const int id0 = seg * kSeg;
+        constexpr int kSize = kHalf ? 2 : 4;
         if (id0 + kSeg <= vocab) {
-            const char* at = static_cast<const char*>(row) + (size_t)id0 * (kHalf ? 2 : 4) + lane * 16;
+            const char* at = static_cast<const char*>(row) + (size_t)id0 * kSize + lane * 16;
 #pragma unroll
             for (int l = 0; l < kLoads; ++l) w[l] = *reinterpret_cast<const u32x4_a2*>(at + l * kWave * 16);
+            return;
+        }
+        if (vocab >= kVec) {   // the row's last: what would reach behind it is read from before and moved down
+#pragma unroll
+            for (int l = 0; l < kLoads; ++l) {
+                const int id = id_of(seg, l * kVec, lane);
+                w[l] = *reinterpret_cast<const u32x4_a2*>(static_cast<const char*>(row) +
+                                                          (size_t)min(id, vocab - kVec) * kSize);
+            }
+#pragma unroll
+            for (int l = 0; l < kLoads; ++l) {
+                const int by = id_of(seg, l * kVec, lane) - (vocab - kVec);
+                w[l] = by <= 0 ? w[l] : by >= kVec ? u32x4{kNone, kNone, kNone, kNone} : moved(w[l], by);
+            }
             return;
         }
 #pragma unroll
@@ -240,14 +255,22 @@ struct Logits {
             for (int i = 0; i < 4; ++i) {
                 const int id = id_of(seg, l * kVec + i * (kVec / 4), lane);
                 if constexpr (kHalf) {
-                    const uint16_t* x = static_cast<const uint16_t*>(row);   // all of them on their way at once
-                    const uint32_t lo = x[min(id, vocab - 1)], hi = x[min(id + 1, vocab - 1)];
-                    w[l][i] = (id < vocab ? lo : 0xfc00u) | (id + 1 < vocab ? hi : 0xfc00u) << 16;
+                    const uint16_t* x = static_cast<const uint16_t*>(row);
+                    w[l][i] = (id < vocab ? x[id] : kNone & 0xffffu) | (id + 1 < vocab ? x[id + 1] : kNone >> 16) << 16;
                 } else {
-                    const uint32_t x = static_cast<const uint32_t*>(row)[min(id, vocab - 1)];
-                    w[l][i] = id < vocab ? x : 0xff800000u;
+                    w[l][i] = id < vocab ? static_cast<const uint32_t*>(row)[id] : kNone;
                 }
             }
+    }
+    static constexpr uint32_t kNone = kHalf ? 0xfc00fc00u : 0xff800000u;   // -inf
+    // elements `by` .. of v, -inf behind them
+    __device__ static u32x4 moved(u32x4 v, int by) {
+        const int words = kHalf ? by >> 1 : by;
+        if (words & 2) v = u32x4{v.z, v.w, kNone, kNone};
+        if (words & 1) v = u32x4{v.y, v.z, v.w, kNone};
+        if (kHalf && (by & 1))
+            v = u32x4{v.x >> 16 | v.y << 16, v.y >> 16 | v.z << 16, v.z >> 16 | v.w << 16, v.w >> 16 | kNone << 16};
+        return v;
     }
     __device__ float at(int e) const {
         const uint32_t v = w[e / kVec][kHalf ? e % kVec / 2 : e % kVec];
@@ -472,6 +495,53 @@ __device__ RowSum join_segments(const Segment* at, int segs, bool greedy, double
     return r;
 }
 
+// max(p - q, 0) of the row where a path ended.
+template <bool kHalf>
+struct Rest {
+    const void *row, *draft_row;
+    PathEnd e;
+    double inv, inv_draft;
+    __device__ Rest(const VerifyDrafts& a, const PathEnd& end)
+        : row(logit_row<kHalf>(a.logits, a.stride, end.row)),
+          draft_row(logit_row<kHalf>(a.draft, a.draft_stride, end.row)), e(end), inv(1. / end.s),
+          inv_draft(1. / end.s_draft) {}
+    __device__ double of(double w, double w_draft) const {
+#pragma clang fp contract(off)   // equal p and q leave nothing
+        return fmax(w * inv - w_draft * inv_draft, 0.);
+    }
+    // of kRun ids from id on
+    __device__ void run(int id, int vocab, double (&w)[kRun]) const {
+        float x[kRun], d[kRun];
+        load_run<kHalf>(row, id, vocab, x);
+        load_run<kHalf>(draft_row, id, vocab, d);
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) w[k] = of(weight(x[k], e.m, e.c), weight(d[k], e.m_draft, e.c));
+    }
+};
+// A segment of it, by one wave.
+template <bool kHalf>
+struct RestLogits {
+    Logits<kHalf> x, d;
+    __device__ void load(const Rest<kHalf>& r, int vocab, int seg, int lane) {
+        x.load(r.row, vocab, seg, lane);
+        d.load(r.draft_row, vocab, seg, lane);
+    }
+    __device__ double sum(const Rest<kHalf>& r, const Exp2Table& exp2) const {
+        double sum[2] = {0., 0.};
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const double dx = (double)x.at(k) - (double)r.e.m, dd = (double)d.at(k) - (double)r.e.m_draft;
+            const double w = exp2(dx), w_draft = exp2(dd);
+            sum[k % 2] += r.of(dx > exp2.least ? w : 0., dd > exp2.least ? w_draft : 0.);
+        }
+        return wave_sum64(sum[0] + sum[1]);
+    }
+};
+// Rows of up to kAloneSegs segments, two a wave: the workgroup that finds the path sums
+// what q leaves of them too (150 sequences of 32003 tokens: 12.3 us), without the two
+// launches that take longer rows' (14.7).
+constexpr int kAloneSegs = 2 * kWalkWaves;
+
 // ---------------------------------------------------------------------------
 // One workgroup per sequence: the rows' sums, the drafted tokens' probabilities, the
 // path, and the next token but where it comes from what q leaves of p.
@@ -482,6 +552,7 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerifyDrafts a, int 
     __shared__ int parent[kMaxTree], token[kMaxTree], gone[kMaxTree], path[kMaxTree];
     __shared__ double p[kMaxTree], bar[kMaxTree], gone_p[kMaxTree], gone_sum[kMaxTree];
     __shared__ double end_left;
+    __shared__ double table[Exp2Table::kEntries], rest_sum[kAloneSegs];
     __shared__ int end_row, end_lost, end_count;
     const int seq = blockIdx.x, lane = threadIdx.x & (kWave - 1), tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -606,10 +677,30 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerifyDrafts a, int 
     if (a.draft) {
         const RowSum d = sums[kMaxTree + f];
         rest = lost > 0 && s.m == s.m && !greedy && d.m == d.m;
-        if (tid == 0)
-            work.ends[seq] = rest ? PathEnd{s.s, d.s, s.m, d.m, rows.start + f, 1, c} : PathEnd{};
+        const PathEnd end = rest ? PathEnd{s.s, d.s, s.m, d.m, rows.start + f, 1, c} : PathEnd{};
+        if (tid == 0) work.ends[seq] = end;
+        if (rest && segs > kAloneSegs) return;
+        if (rest) {
+            const Rest<kHalf> left(a, end);
+            Exp2Table exp2;
+            exp2.make<kWalk>(table, c);
+            for (int seg = wave; seg < segs; seg += kWalkWaves) {
+                RestLogits<kHalf> l;
+                l.load(left, a.vocab, seg, lane);
+                const double sum = l.sum(left, exp2);
+                if (lane == 0) rest_sum[seg] = sum;
+            }
+            __syncthreads();
+            const int next = pick(
+                segs, u0, [&](int j) { return rest_sum[j]; },
+                [&](int id, double (&w)[kRun]) { left.run(id, a.vocab, w); });
+            if (next >= 0) {
+                if (tid == 0) a.next_tokens[seq] = next;
+                return;
+            }
+            __syncthreads();   // nothing is left: the token comes from p
+        }
     }
-    if (rest) return;
     int next = -1;
     if (s.m == s.m) {
         if (greedy) {
@@ -670,45 +761,23 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerifyDrafts a, int 
     if (tid == 0) a.next_tokens[seq] = next;
 }
 
-// max(p - q, 0) of logits of the two rows
-struct Rest {
-    PathEnd e;
-    double inv, inv_draft;
-    __device__ Rest(const PathEnd& end) : e(end), inv(1. / end.s), inv_draft(1. / end.s_draft) {}
-    __device__ double of(double w, double w_draft) const {
-#pragma clang fp contract(off)   // equal p and q leave nothing
-        return fmax(w * inv - w_draft * inv_draft, 0.);
-    }
-    __device__ double operator()(float x, float x_draft) const {
-        return of(weight(x, e.m, e.c), weight(x_draft, e.m_draft, e.c));
-    }
-};
-
 // Workgroup (4 segments, sequence): what q leaves of p where a draft was rejected.
 template <bool kHalf>
 __global__ __launch_bounds__(kBlk) void verify_rest_kernel(VerifyDrafts a, int segs) {
     __shared__ double table[Exp2Table::kEntries];
     const int seq = blockIdx.y, lane = threadIdx.x & (kWave - 1);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), seg = blockIdx.x * kWaves + wave;
+    const int seg = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const Work work = work_of(a, segs);
     const PathEnd e = work.ends[seq];
     if (!e.rest) return;
-    Logits<kHalf> x, d;
-    x.load(logit_row<kHalf>(a.logits, a.stride, e.row), a.vocab, min(seg, segs - 1), lane);
-    d.load(logit_row<kHalf>(a.draft, a.draft_stride, e.row), a.vocab, min(seg, segs - 1), lane);
-    const Rest rest(e);
+    const Rest<kHalf> rest(a, e);
+    RestLogits<kHalf> x;
+    x.load(rest, a.vocab, min(seg, segs - 1), lane);
     Exp2Table exp2;
     exp2.make<kBlk>(table, e.c);
     if (seg >= segs) return;
-    double sum[2] = {0., 0.};
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-        const double dx = (double)x.at(k) - (double)e.m, dd = (double)d.at(k) - (double)e.m_draft;
-        const double w = exp2(dx), w_draft = exp2(dd);
-        sum[k % 2] += rest.of(dx > exp2.least ? w : 0., dd > exp2.least ? w_draft : 0.);
-    }
-    const double all = wave_sum64(sum[0] + sum[1]);
-    if (lane == 0) work.rest[(size_t)seq * segs + seg] = all;
+    const double sum = x.sum(rest, exp2);
+    if (lane == 0) work.rest[(size_t)seq * segs + seg] = sum;
 }
 
 template <bool kHalf>
@@ -718,19 +787,11 @@ __global__ __launch_bounds__(kWalk) void verify_pick_kernel(VerifyDrafts a, int 
     const PathEnd e = work.ends[seq];
     if (!e.rest) return;
     const DraftRows rows = draft_rows(a.query_start, seq, a.rows, a.max_query);
-    const void* row = logit_row<kHalf>(a.logits, a.stride, e.row);
-    const void* draft_row = logit_row<kHalf>(a.draft, a.draft_stride, e.row);
     const float u = a.uniforms[rows.start];
-    const Rest rest(e);
+    const Rest<kHalf> rest(a, e);
     int next = pick(
         segs, u, [&](int j) { return work.rest[(size_t)seq * segs + j]; },
-        [&](int id, double (&w)[kRun]) {
-            float x[kRun], d[kRun];
-            load_run<kHalf>(row, id, a.vocab, x);
-            load_run<kHalf>(draft_row, id, a.vocab, d);
-#pragma unroll
-            for (int k = 0; k < kRun; ++k) w[k] = rest(x[k], d[k]);
-        });
+        [&](int id, double (&w)[kRun]) { rest.run(id, a.vocab, w); });
     if (next < 0) {   // nothing is left
         __syncthreads();
         const Segment* mine = work.segments + (size_t)e.row * segs;
@@ -740,7 +801,7 @@ __global__ __launch_bounds__(kWalk) void verify_pick_kernel(VerifyDrafts a, int 
         };
         next = pick(segs, u, value, [&](int id, double (&w)[kRun]) {
             float x[kRun];
-            load_run<kHalf>(row, id, a.vocab, x);
+            load_run<kHalf>(rest.row, id, a.vocab, x);
 #pragma unroll
             for (int k = 0; k < kRun; ++k) w[k] = weight(x[k], e.m, e.c);
         });
@@ -755,8 +816,9 @@ void launch_for(const VerifyDrafts& a, hipStream_t s) {
     const int segs = segments_of(a.vocab), blocks = (segs + kWaves - 1) / kWaves;
     launch_kernel_in_call(false, verify_sums_kernel<kHalf>, dim3(blocks, a.max_query * (a.draft ? 2 : 1), a.nseq),
                           dim3(kBlk), 0, s, a, segs);
-    launch_kernel_in_call(!a.draft, verify_walk_kernel<kHalf>, dim3(a.nseq), dim3(kWalk), 0, s, a, segs);
-    if (!a.draft) return;
+    const bool last = !a.draft || segs <= kAloneSegs;
+    launch_kernel_in_call(last, verify_walk_kernel<kHalf>, dim3(a.nseq), dim3(kWalk), 0, s, a, segs);
+    if (last) return;
     launch_kernel_in_call(false, verify_rest_kernel<kHalf>, dim3(blocks, a.nseq), dim3(kBlk), 0, s, a, segs);
     launch_kernel(verify_pick_kernel<kHalf>, dim3(a.nseq), dim3(kWalk), 0, s, a, segs);
 }
