@@ -215,8 +215,11 @@ __host__ __device__ inline Work work_of(const VerifyDrafts& a, int segs) {
     return w;
 }
 
+// 0: greedy.  An infinite one as the largest finite, at which finite logits weigh the
+// same and -inf still nothing.
 __device__ __forceinline__ float temperature(const VerifyDrafts& a, int seq) {
-    return a.temperatures ? a.temperatures[seq] : 1.f;
+    const float t = a.temperatures ? a.temperatures[seq] : 1.f;
+    return t > 0.f ? fminf(t, 0x1.fffffep127f) : 0.f;
 }
 constexpr double kLog2e = 1.4426950408889634074;
 
@@ -356,7 +359,9 @@ __device__ __forceinline__ Place find_place(int count, float u, V value) {
             if (!(total > 0.)) return {-1, 0., 0.};
             f.t = (double)unit(u) * total;
         }
-        uint64_t who = __builtin_amdgcn_ballot_w64(f.before + upto > f.t);
+        // (of those with a value: rounding does not order the sums, and the one of a lane
+        // without may exceed the one before it)
+        uint64_t who = __builtin_amdgcn_ballot_w64(v > 0. && f.before + upto > f.t);
         if (who == 0) {
             who = __builtin_amdgcn_ballot_w64(v > 0.);
             if (who == 0) return {-1, 0., 0.};

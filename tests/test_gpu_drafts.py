@@ -366,6 +366,58 @@ def test_temperatures_of_any_size(hip, heat):
         Step(hip, 22, [3, 3, 2], 2500, heat=heat, drafted=drafted).upload().launch().check()
 
 
+def test_an_infinite_temperature(hip):
+    """Every token that can come is as likely as the others, as at the largest
+    finite one (where a difference of logits of 20 is 2^-123 of a weight)."""
+    for drafted in (False, True):
+        for half in (False, True):
+            step = Step(hip, 30, [3, 3, 2], 2500, drafted=drafted, half=half)
+            for x in (step.logits, step.draft) if drafted else (step.logits,):
+                x[:, ::3] = -np.inf
+            step.heat[:] = np.inf
+            step.upload().launch()
+            step.heat[:] = np.finfo(np.float32).max
+            step.check()
+
+
+def test_running_sums_that_rounding_does_not_order(hip):
+    """Weights of e^-36.9 twice, 1, 0 and 1: the sum of the first three is 1 or its
+    successor, as they are added, and half of the total 1.  A segment without a
+    weight never has the token."""
+    step = Step(hip, 31, [1, 1], 5 * 2048)
+    step.logits[:] = -np.inf
+    step.logits[:, [5, 2048]] = -36.9
+    step.logits[:, [2 * 2048 + 7, 4 * 2048 + 9]] = 0
+    step.uniforms[:] = 0.5, 0
+    step.upload().launch()
+    after = step.d_next.download(np.int32, 2)
+    assert after[0] in (2 * 2048 + 7, 4 * 2048 + 9) and after[1] == 5
+
+
+def test_millions_of_tokens(hip):
+    """More than 64 * 64 segments; equal logits, whose sums are exact."""
+    vocab = 2 ** 23 + 70001
+    for drafted in (False, True):
+        step = Step(hip, 32, [2], 40, half=True)
+        step.vocab = step.stride = vocab
+        step.logits = np.full((2, vocab), 3, np.float16)
+        step.logits[:, ::5] = step.logits[:, 4500000:4700000] = -np.inf
+        step.draft = None
+        left = np.isfinite(step.logits[0])
+        if drafted:                  # half of what p has, each twice as likely: the rest is the other half
+            step.draft = step.logits.copy()
+            step.draft[:, np.flatnonzero(left)[1::2]] = -np.inf
+        step.tokens[1] = 10          # (10 is a multiple of 5: it cannot come)
+        for u in (0, 0.25, 0.4999999, 0.7, 1 - 2 ** -24):
+            step.uniforms[:] = u, 0.5
+            step.upload().launch()
+            ids = np.flatnonzero(left)[1::2] if drafted else np.flatnonzero(left)
+            want = ids[int(float(np.float32(u)) * len(ids))]
+            assert step.d_counts.download(np.int32, 1)[0] == 1
+            assert abs(int(np.searchsorted(ids, step.d_next.download(np.int32, 1)[0])) -
+                       int(np.searchsorted(ids, want))) <= (1 if drafted else 0)
+
+
 @pytest.mark.parametrize("scale", [1e4, 1e30, 3e38])
 def test_logits_of_any_size(hip, scale):
     for heat in (1.0, 0.0, 1e30):
