@@ -514,13 +514,20 @@ struct Rest {
 #pragma clang fp contract(off)   // equal p and q leave nothing
         return fmax(w * inv - w_draft * inv_draft, 0.);
     }
-    // of kRun ids from id on
-    __device__ void run(int id, int vocab, double (&w)[kRun]) const {
+    // of one id
+    __device__ double of(float x, float d, const Exp2Table& exp2) const {
+        const double dx = (double)x - (double)e.m, dd = (double)d - (double)e.m_draft;
+        const double w = exp2(dx), w_draft = exp2(dd);
+        return of(dx > exp2.least ? w : 0., dd > exp2.least ? w_draft : 0.);
+    }
+    // of kRun ids from id on: the same numbers as in their segment's sum, so that one which
+    // is above 0 has an id that is
+    __device__ void run(int id, int vocab, const Exp2Table& exp2, double (&w)[kRun]) const {
         float x[kRun], d[kRun];
         load_run<kHalf>(row, id, vocab, x);
         load_run<kHalf>(draft_row, id, vocab, d);
 #pragma unroll
-        for (int k = 0; k < kRun; ++k) w[k] = of(weight(x[k], e.m, e.c), weight(d[k], e.m_draft, e.c));
+        for (int k = 0; k < kRun; ++k) w[k] = of(x[k], d[k], exp2);
     }
 };
 // A segment of it, by one wave.
@@ -534,11 +541,7 @@ struct RestLogits {
     __device__ double sum(const Rest<kHalf>& r, const Exp2Table& exp2) const {
         double sum[2] = {0., 0.};
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-            const double dx = (double)x.at(k) - (double)r.e.m, dd = (double)d.at(k) - (double)r.e.m_draft;
-            const double w = exp2(dx), w_draft = exp2(dd);
-            sum[k % 2] += r.of(dx > exp2.least ? w : 0., dd > exp2.least ? w_draft : 0.);
-        }
+        for (int k = 0; k < kPer; ++k) sum[k % 2] += r.of(x.at(k), d.at(k), exp2);
         return wave_sum64(sum[0] + sum[1]);
     }
 };
@@ -698,7 +701,7 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerifyDrafts a, int 
             __syncthreads();
             const int next = pick(
                 segs, u0, [&](int j) { return rest_sum[j]; },
-                [&](int id, double (&w)[kRun]) { left.run(id, a.vocab, w); });
+                [&](int id, double (&w)[kRun]) { left.run(id, a.vocab, exp2, w); });
             if (next >= 0) {
                 if (tid == 0) a.next_tokens[seq] = next;
                 return;
@@ -787,16 +790,19 @@ __global__ __launch_bounds__(kBlk) void verify_rest_kernel(VerifyDrafts a, int s
 
 template <bool kHalf>
 __global__ __launch_bounds__(kWalk) void verify_pick_kernel(VerifyDrafts a, int segs) {
+    __shared__ double table[Exp2Table::kEntries];
     const int seq = blockIdx.x;
     const Work work = work_of(a, segs);
     const PathEnd e = work.ends[seq];
     if (!e.rest) return;
+    Exp2Table exp2;
+    exp2.make<kWalk>(table, e.c);
     const DraftRows rows = draft_rows(a.query_start, seq, a.rows, a.max_query);
     const float u = a.uniforms[rows.start];
     const Rest<kHalf> rest(a, e);
     int next = pick(
         segs, u, [&](int j) { return work.rest[(size_t)seq * segs + j]; },
-        [&](int id, double (&w)[kRun]) { rest.run(id, a.vocab, w); });
+        [&](int id, double (&w)[kRun]) { rest.run(id, a.vocab, exp2, w); });
     if (next < 0) {   // nothing is left
         __syncthreads();
         const Segment* mine = work.segments + (size_t)e.row * segs;
