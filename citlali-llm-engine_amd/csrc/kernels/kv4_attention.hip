@@ -139,7 +139,7 @@ __device__ __forceinline__ float score_factor(float a, float b, float scale_log2
 // sequences of 150 .. 1500, 52.6 MB, in 17.6.
 // ---------------------------------------------------------------------------
 template <int HD, int kCols, bool kTree>
-__global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 || (kTree && HD == 64) ? 3 : 2) void kv4_decode_kernel(
+__global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 || (kTree && HD == 64 && kCols == 3) ? 3 : 2) void kv4_decode_kernel(
     Kv4View c, Kv4Attention a, int chunk, int n_splits, float scale_log2) {
     using L = Kv4Layout<HD>;
     using Vec = std::conditional_t<HD == 128, u32x4, u32x2>;   // a lane's codes of 16 positions
@@ -292,6 +292,10 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 || (kTree && HD =
         uint32_t sees[kTree ? kCols : 1];   // of a tree's row, the tile's positions
 #pragma unroll
         for (int n = 0; n < kCols; ++n) {
+            if constexpr (kTree && kCols > 1) {   // (48 trees of 28 to 48 rows: 69.1 -> 66.1 us)
+                pw[n] = half8{};
+                if (16 * n >= rows) continue;   // none of the sequence's rows
+            }
             if (!whole) {
                 asm volatile("");   // a branch: most tiles skip it
                 if (kTree && tail)
@@ -923,6 +927,12 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
 // 30 / 59, 40 rows 26 / 54 against 32 / 67; built for 64 rows 37 / 82 against
 // 33 / 68).
 constexpr int kFewRows = 48;
+// Trees with heads of 64 go up to 80 rows (25 of 17 to 33 rows of 2 heads behind 176 to
+// 2500 positions: 23.5 us, on the prompt kernel, whose waves have 32 rows each, 29.5; 64
+// of 40 rows behind 2000 64 and 64; 100 of 64 rows and 600 positions 22 and 26).  Heads
+// of 128 spill at 64 rows: 34 us for 21 with one sequence, 108 for 80 with 64.
+constexpr int kFewTreeRows64 = 80;
+constexpr int few_rows(bool tree, int head_dim) { return tree && head_dim == 64 ? kFewTreeRows64 : kFewRows; }
 // Its chunks: whole turns of the four waves, as long as leaves one round of
 // resident workgroups (four, three or two per CU for 16, 32 or 48 rows), at
 // most 1024 positions (a lane per page) and at least 256 (16 sequences of 2000
@@ -957,17 +967,21 @@ struct Kv4Plan {
     bool few;
     int cols, tiles, chunk, n_splits;
 };
-Kv4Plan kv4_plan(bool tree, int max_context, int max_query, int nseq, int heads, int kv_heads) {
+Kv4Plan kv4_plan(bool tree, int max_context, int max_query, int nseq, int heads, int kv_heads, int head_dim) {
     Kv4Plan p{};
     const long long rows = (long long)max_query * (heads / kv_heads);
-    p.few = rows <= kFewRows;
+    p.few = rows <= few_rows(tree, head_dim);
     p.cols = p.few ? (int)(rows + 15) / 16 : 0;
     p.tiles = (int)((rows + kRowTile - 1) / kRowTile);
     auto whole = [](long long positions, int step) { return (int)((positions + step - 1) / step * step); };
     if (p.few) {
-        const int blocks = p.cols == 1 ? kFewBlocks : p.cols == 2 ? kFewBlocks * 3 / 4 : kFewBlocks / 2;
+        // (a tree's columns without rows cost little, so its grid counts on three per CU
+        // with heads of 64: 25 of 48 rows and 2500 positions 28.2 us, on two 31.7)
+        const int blocks = p.cols == 1                                  ? kFewBlocks
+                           : p.cols == 2 || (tree && head_dim == 64) ? kFewBlocks * 3 / 4
+                                                                        : kFewBlocks / 2;
         const long long share = ((long long)max_context * nseq * kv_heads + blocks - 1) / blocks;
-        p.chunk = max_context <= (p.cols == 1 ? kAlone : kAloneWide)
+        p.chunk = max_context <= (p.cols == 1 || p.cols > 3 ? kAlone : kAloneWide)
                       ? whole(max_context, kChunkStep)
                       : whole(std::max<long long>(kChunkLeast, std::min<long long>(kChunkMost, share)), kChunkStep);
     } else {
@@ -984,7 +998,7 @@ Kv4Plan kv4_plan(bool tree, int max_context, int max_query, int nseq, int heads,
 
 template <int HD, bool kTree>
 hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
-    const Kv4Plan p = kv4_plan(kTree, a.max_context, a.max_query, a.nseq, a.heads, c.kv_heads);
+    const Kv4Plan p = kv4_plan(kTree, a.max_context, a.max_query, a.nseq, a.heads, c.kv_heads, HD);
     const float scale_log2 = 1.44269504088896340736f / sqrtf((float)HD);
     const int group = a.heads / c.kv_heads;
     const bool last = p.n_splits == 1;
@@ -1008,7 +1022,7 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
     } else {
         const dim3 grid(c.kv_heads * a.nseq, p.n_splits);
         const int lds = kWaves * 16 * (HD + 4) * (int)sizeof(float);   // the merge; Q takes less
-        static_assert(kFewRows * HD * 2 <= kWaves * 16 * (HD + 4) * 4);
+        static_assert(few_rows(kTree, HD) * HD * 2 <= kWaves * 16 * (HD + 4) * 4);
         auto go = [&](auto kernel) {
             launch_kernel_in_call(last, kernel, grid, dim3(kBlk), lds, s, c, a, p.chunk, p.n_splits, scale_log2);
         };
@@ -1016,14 +1030,18 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
             go(kv4_decode_kernel<HD, 1, kTree>);
         else if (p.cols == 2)
             go(kv4_decode_kernel<HD, 2, kTree>);
-        else
+        else if (p.cols == 3)
             go(kv4_decode_kernel<HD, 3, kTree>);
+        if constexpr (few_rows(kTree, HD) > kFewRows) {
+            if (p.cols == 4) go(kv4_decode_kernel<HD, 4, kTree>);
+            if (p.cols == 5) go(kv4_decode_kernel<HD, 5, kTree>);
+        }
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || last) return e;
     // one wave covers 4 chunks a lane group at once; with more of them four waves share a head
     const long long units = (long long)a.max_query * a.heads;
-    const int tile_rows = p.few ? kFewRows : kRowTile;
+    const int tile_rows = p.few ? few_rows(kTree, HD) : kRowTile;
     if (p.n_splits <= 4 * kWave / (HD / 4) || (kTree && units * a.nseq > kMergeUnits))
         launch_kernel(kv4_merge_kernel<HD, 1, kTree>, dim3((unsigned)((units + kWaves - 1) / kWaves), a.nseq), dim3(kBlk), 0,
                       s, a, group, tile_rows, p.chunk, p.n_splits, scale_log2);
@@ -1037,7 +1055,7 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
 
 size_t kv4_attention_workspace(bool tree, int max_context, int max_query, int nseq, int tokens, int heads,
                                int kv_heads, int head_dim) {
-    const Kv4Plan p = kv4_plan(tree, max_context, max_query, nseq, heads, kv_heads);
+    const Kv4Plan p = kv4_plan(tree, max_context, max_query, nseq, heads, kv_heads, head_dim);
     if (p.n_splits == 1) return 0;
     return (size_t)tokens * heads * p.n_splits * (head_dim + 2) * sizeof(float);
 }

@@ -68,6 +68,25 @@ def test_trees(hip, heads, kv, lens, asked, hd, page):
     Trees(hip, 40, heads, kv, hd, page, lens, asked).upload().launch().check()
 
 
+@pytest.mark.parametrize("asked,group", [([25, 3, 17], 2), ([32, 9, 1], 2), ([33, 24, 25], 2), ([40, 16, 8], 2),
+                                         ([41, 40, 2], 2), ([16, 1, 4], 4), ([5, 2, 3], 16), ([80, 65, 17], 1),
+                                         ([10, 2, 8], 8)])
+def test_heads_of_64_have_up_to_80_rows_with_the_few(hip, asked, group):
+    """Sequences with some of the column tiles beside the widest; short, with the tree
+    across two chunks, and with slots whose values are NaN where a row is hidden."""
+    for page, lens in ((16, [300, 40, 18]), (32, [1040, 1025, 2300]), (128, [5000, 790, 64])):
+        Trees(hip, 60, 3 * group, 3, 64, page, lens, asked).upload().launch().check()
+    b = Trees(hip, 61, 2 * group, 2, 64, 16, [90, 70, 800], asked)
+    b.table[0, 1] = b.table[2, 3] = -1
+    b.table[1, 0] = b.cache.num_pages
+    b.upload().launch().check()
+    b = Trees(hip, 62, 2 * group, 2, 64, 32, [90, 70, 800], asked)
+    for s, see in enumerate(b.sees):
+        see[::3] = False                      # rows that see the prefix alone
+        b.lens[s] = max(len(see), b.lens[s])
+    b.upload().launch().check()
+
+
 @pytest.mark.parametrize("before", [0, 1, 15, 16, 31, 32, 33, 63, 64, 100, 127])
 @pytest.mark.parametrize("asked", [[9], [40], [100]])
 def test_trees_start_anywhere_in_a_tile(hip, before, asked):
@@ -150,7 +169,7 @@ def test_slots_past_the_end_may_hold_anything(hip, asked):
 
 @pytest.mark.parametrize("hd,page", [(128, 16), (64, 64)])
 @pytest.mark.parametrize("heads,asked", [(8, [4, 2, 3]), (8, [8, 1, 5]), (8, [12, 9, 10]), (8, [30, 9, 16]),
-                                         (4, [70, 9, 150])])
+                                         (4, [70, 9, 150]), (4, [40, 9, 26])])
 @pytest.mark.parametrize("keys", [False, True])
 def test_a_nan_is_kept_from_the_rows_that_do_not_see_it(hip, heads, asked, keys, hd, page):
     """Every third row of the tree has NaN values (and keys): the rows they are
