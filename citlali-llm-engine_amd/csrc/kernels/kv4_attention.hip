@@ -138,9 +138,11 @@ __device__ __forceinline__ float score_factor(float a, float b, float scale_log2
 // 20 rows, 24 sequences of 500 .. 6000, 101 MB, in 31.0; 16/8 heads of 64, 100
 // sequences of 150 .. 1500, 52.6 MB, in 17.6.
 // ---------------------------------------------------------------------------
-template <int HD, int kCols, bool kTree>
-__global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 || (kTree && HD == 64 && kCols == 3) ? 3 : 2) void kv4_decode_kernel(
-    Kv4View c, Kv4Attention a, int chunk, int n_splits, float scale_log2) {
+template <int HD, int kCols, bool kTree, int kWaves = 4>
+__global__ __launch_bounds__(kWaves * kWave, kWaves > 4 ? 2 : kCols == 1 ? 4
+                                             : kCols == 2 || (kTree && HD == 64 && kCols == 3) ? 3 : 2)
+void kv4_decode_kernel(Kv4View c, Kv4Attention a, int chunk, int n_splits, float scale_log2) {
+    constexpr int kBlk = kWaves * kWave;
     using L = Kv4Layout<HD>;
     using Vec = std::conditional_t<HD == 128, u32x4, u32x2>;   // a lane's codes of 16 positions
     constexpr int kSteps = HD / 32, kDims = HD / 16;   // MFMA steps of a score; dims (and O tiles) of a V lane
@@ -250,7 +252,7 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 || (kTree && HD =
     if constexpr (kTree && kQInLds) {
 #pragma unroll
         for (int n = 0; n < kCols; ++n)
-            if (kSteps == kWaves || wave / kSteps == (n & 1))
+            if (wave / kSteps == n % (kWaves / kSteps))
                 q_lds[(n * kSteps + wave % kSteps) * kWave + lane] = __builtin_bit_cast(half8, mine[n]);
     }
     if constexpr (kQInLds) lds_only_barrier();
@@ -261,7 +263,8 @@ __global__ __launch_bounds__(kBlk, kCols == 1 ? 4 : kCols == 2 || (kTree && HD =
     int t = c0 + 32 * wave;
 #pragma unroll
     for (int phase = kTree ? 0 : 1; phase < 2; ++phase)
-    for (const bool tail = kTree && phase == 1; t < (kTree && !tail ? min(c1, s.before() - 31) : c1); t += 32 * kWaves) {
+    for (const bool tail = kTree && phase == 1; t < (kTree && !tail ? min(c1, s.before() - 31) : c1);
+         t += 32 * kWaves) {
         const int there = (page_of(t) >= 0) | (page_of(t + 16) >= 0) << 1;
         const bool whole = there == 3 && t + 32 <= least;
         f32x4 sc[kCols][2];
@@ -963,9 +966,15 @@ constexpr int kTwoPartBlocks = 384, kTwoPartContext = 256;
 // wave a head from kMergeUnits heads on (180 rows of 40 heads in 15 parts: 12.1 us, by
 // four waves 18.5).
 constexpr int kTreeBlocks = 700, kMergeUnits = 2048;
+// Trees that one workgroup per CU serves have eight waves in each, so that a chunk takes
+// half the turns (32/8 heads, with four waves and with eight: 4 sequences of 8000
+// positions and 16 rows 20.1 and 15.7 us, 32 rows 29.0 and 18.8, 48 29.7 and 22.6; 16 of
+// 1000 with 32 19.0 and 15.5; one of 1000 with 16 10.6 and 10.2.  Two such workgroups
+// per CU: 16 of 2000 with 48 rows 31.6, 26.6 with four waves).
+constexpr int kWideWaves = 8, kWideBlocks = 256;
 struct Kv4Plan {
     bool few;
-    int cols, tiles, chunk, n_splits;
+    int cols, tiles, chunk, n_splits, waves;   // waves: of a workgroup with few rows
 };
 Kv4Plan kv4_plan(bool tree, int max_context, int max_query, int nseq, int heads, int kv_heads, int head_dim) {
     Kv4Plan p{};
@@ -977,9 +986,9 @@ Kv4Plan kv4_plan(bool tree, int max_context, int max_query, int nseq, int heads,
     if (p.few) {
         // (a tree's columns without rows cost little, so its grid counts on three per CU
         // with heads of 64: 25 of 48 rows and 2500 positions 28.2 us, on two 31.7)
-        const int blocks = p.cols == 1                                  ? kFewBlocks
+        const int blocks = p.cols == 1                               ? kFewBlocks
                            : p.cols == 2 || (tree && head_dim == 64) ? kFewBlocks * 3 / 4
-                                                                        : kFewBlocks / 2;
+                                                                     : kFewBlocks / 2;
         const long long share = ((long long)max_context * nseq * kv_heads + blocks - 1) / blocks;
         p.chunk = max_context <= (p.cols == 1 || p.cols > 3 ? kAlone : kAloneWide)
                       ? whole(max_context, kChunkStep)
@@ -991,6 +1000,16 @@ Kv4Plan kv4_plan(bool tree, int max_context, int max_query, int nseq, int heads,
             tree ? std::max(1ll, least(kTreeBlocks, kPromptChunk))
                  : std::max({1ll, least(kPromptBlocks, kPromptChunk), least(2 * kPromptBlocks, kPromptChunkFull)});
         p.chunk = whole((max_context + splits - 1) / splits, kTile);
+    }
+    p.waves = kWaves;
+    const long long units = (long long)kv_heads * nseq;
+    if (tree && p.few && units * ((max_context + kChunkMost - 1) / kChunkMost) <= kWideBlocks) {
+        p.waves = kWideWaves;
+        const int step = 32 * kWideWaves;
+        const long long share = (max_context * units + kWideBlocks - 1) / kWideBlocks;
+        const bool alone = max_context <= kAloneWide || (max_context <= kChunkMost && share > kChunkLeast);
+        p.chunk = whole(alone ? max_context : std::max<long long>(kChunkLeast, std::min<long long>(kChunkMost, share)),
+                        step);
     }
     p.n_splits = (max_context + p.chunk - 1) / p.chunk;
     return p;
@@ -1016,26 +1035,39 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
         } else {
             e = allow_lds<kv4_prompt_kernel<HD, 1, kTree>>(part);
             if (e != hipSuccess) return e;
-            launch_kernel_in_call(last, kv4_prompt_kernel<HD, 1, kTree>, grid, dim3(kBlk), part, s, c, a, p.chunk, p.n_splits,
-                                  scale_log2);
+            launch_kernel_in_call(last, kv4_prompt_kernel<HD, 1, kTree>, grid, dim3(kBlk), part, s, c, a, p.chunk,
+                                  p.n_splits, scale_log2);
         }
     } else {
         const dim3 grid(c.kv_heads * a.nseq, p.n_splits);
-        const int lds = kWaves * 16 * (HD + 4) * (int)sizeof(float);   // the merge; Q takes less
+        const int lds = p.waves * 16 * (HD + 4) * (int)sizeof(float);   // the merge; Q takes less
         static_assert(few_rows(kTree, HD) * HD * 2 <= kWaves * 16 * (HD + 4) * 4);
-        auto go = [&](auto kernel) {
-            launch_kernel_in_call(last, kernel, grid, dim3(kBlk), lds, s, c, a, p.chunk, p.n_splits, scale_log2);
+        auto go = [&](auto kernel, int waves) {
+            launch_kernel_in_call(last, kernel, grid, dim3(waves * kWave), lds, s, c, a, p.chunk, p.n_splits,
+                                  scale_log2);
         };
-        if (p.cols == 1)
-            go(kv4_decode_kernel<HD, 1, kTree>);
-        else if (p.cols == 2)
-            go(kv4_decode_kernel<HD, 2, kTree>);
-        else if (p.cols == 3)
-            go(kv4_decode_kernel<HD, 3, kTree>);
-        if constexpr (few_rows(kTree, HD) > kFewRows) {
-            if (p.cols == 4) go(kv4_decode_kernel<HD, 4, kTree>);
-            if (p.cols == 5) go(kv4_decode_kernel<HD, 5, kTree>);
-        }
+        auto with = [&](auto cols) {
+            if constexpr (16 * cols - 15 > few_rows(kTree, HD)) {
+                return hipErrorInvalidValue;   // (no plan has them)
+            } else {
+                if constexpr (kTree) {
+                    if (p.waves == kWideWaves) {
+                        constexpr auto kernel = kv4_decode_kernel<HD, cols, true, kWideWaves>;
+                        const hipError_t e = allow_lds<kernel>(lds);
+                        if (e == hipSuccess) go(kernel, kWideWaves);
+                        return e;
+                    }
+                }
+                go(kv4_decode_kernel<HD, cols, kTree>, kWaves);
+                return hipSuccess;
+            }
+        };
+        const hipError_t e = p.cols == 1   ? with(std::integral_constant<int, 1>{})
+                             : p.cols == 2 ? with(std::integral_constant<int, 2>{})
+                             : p.cols == 3 ? with(std::integral_constant<int, 3>{})
+                             : p.cols == 4 ? with(std::integral_constant<int, 4>{})
+                                           : with(std::integral_constant<int, 5>{});
+        if (e != hipSuccess) return e;
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || last) return e;
@@ -1043,8 +1075,8 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
     const long long units = (long long)a.max_query * a.heads;
     const int tile_rows = p.few ? few_rows(kTree, HD) : kRowTile;
     if (p.n_splits <= 4 * kWave / (HD / 4) || (kTree && units * a.nseq > kMergeUnits))
-        launch_kernel(kv4_merge_kernel<HD, 1, kTree>, dim3((unsigned)((units + kWaves - 1) / kWaves), a.nseq), dim3(kBlk), 0,
-                      s, a, group, tile_rows, p.chunk, p.n_splits, scale_log2);
+        launch_kernel(kv4_merge_kernel<HD, 1, kTree>, dim3((unsigned)((units + kWaves - 1) / kWaves), a.nseq),
+                      dim3(kBlk), 0, s, a, group, tile_rows, p.chunk, p.n_splits, scale_log2);
     else
         launch_kernel(kv4_merge_kernel<HD, kWaves, kTree>, dim3((unsigned)units, a.nseq), dim3(kBlk), 0, s, a, group,
                       tile_rows, p.chunk, p.n_splits, scale_log2);

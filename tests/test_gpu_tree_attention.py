@@ -87,6 +87,18 @@ def test_heads_of_64_have_up_to_80_rows_with_the_few(hip, asked, group):
     b.upload().launch().check()
 
 
+@pytest.mark.parametrize("hd,group,most", [(128, 2, 8), (128, 3, 10), (128, 4, 12), (128, 5, 16), (64, 2, 8), (64, 5, 6),
+                                           (64, 2, 24), (64, 2, 32), (64, 5, 16)])
+def test_more_workgroups_than_a_round(hip, hd, group, most):
+    """Many short sequences, and some beside one of many chunks, at each number of
+    column tiles and on the prompt kernel."""
+    rng = np.random.default_rng(most)
+    for seqs, kv, page, longest in ((90, 3, 16, 90), (20, 2, 32, 7000)):
+        asked = [most] + [int(x) for x in rng.integers(0, most + 1, seqs - 1)]
+        lens = [longest] + [n + int(rng.integers(0, 60)) for n in asked[1:]]
+        Trees(hip, 63, kv * group, kv, hd, page, lens, asked).upload().launch().check()
+
+
 @pytest.mark.parametrize("before", [0, 1, 15, 16, 31, 32, 33, 63, 64, 100, 127])
 @pytest.mark.parametrize("asked", [[9], [40], [100]])
 def test_trees_start_anywhere_in_a_tile(hip, before, asked):
