@@ -14,7 +14,9 @@ namespace {
 // ---------------------------------------------------------------------------
 // Masks and positions.  One workgroup per sequence, a thread per row, by
 // doubling: after step t a row's mask holds itself and the 2^t - 1 rows above it,
-// and `above` is the row 2^t up.
+// and `above` is the row 2^t up.  128 trees of 256 rows are 1 MB, written in 4 to 5 us,
+// eight rows' in 2 to 5: the launch and two round trips; a row by row walk up takes as
+// many LDS reads as the tree is deep.
 // ---------------------------------------------------------------------------
 constexpr int kNone = -1, kBad = -2;   // nothing above in the tree; a parent that is not an earlier row
 
@@ -61,6 +63,10 @@ __global__ __launch_bounds__(kMaxTree) void draft_tree_kernel(DraftTree a, int w
 // misplaced where the sums are off by more than u's distance to the next border,
 // of which a row has as many as tokens (151936 of them at an error of 2^-26, what
 // 32 bits give: 1 draw in 200).
+// Sums of segments of 2048 logits first, a wave each, then a workgroup per sequence for
+// all that is in turn: the path, and the draw of its token.
+// After the sums, five rows take 8 us, a chain of four with drafts 8.5, a tree of 40
+// 11.5: one round trip and one reduction after another.
 // ---------------------------------------------------------------------------
 constexpr int kBlk = 256, kWaves = kBlk / kWave;
 constexpr int kPer = 32, kSeg = kPer * kWave;   // logits of a lane, and of a wave: a segment
@@ -284,7 +290,12 @@ struct Logits {
     }
 };
 
-// Workgroup (4 segments, row, sequence), a segment a wave.
+// Workgroup (4 segments, row, sequence), a segment a wave; every logit is read once.
+// Bound by 64-bit instructions (ten a logit, beside the table's read), from some 150 MB
+// on by the reads too: rows of 151936, 14 trees of up to 40 in fp16, 131 MB, in 31 to 36
+// us, 40 chains of up to 6 and their drafts' in fp32, 200 MB, in 31 to 37; 150 chains of
+// up to 4 with drafts of 32003 in fp16, 47 MB, in 20.  By exp2_64 alone the first takes
+// 85.  Several segments a wave, the next one loaded ahead, are no faster.
 template <bool kHalf>
 __global__ __launch_bounds__(kBlk) void verify_sums_kernel(VerifyDrafts a, int segs) {
     __shared__ double table[Exp2Table::kEntries];
@@ -546,8 +557,8 @@ struct RestLogits {
     }
 };
 // Rows of up to kAloneSegs segments, two a wave: the workgroup that finds the path sums
-// what q leaves of them too (150 sequences of 32003 tokens: 12.3 us), without the two
-// launches that take longer rows' (14.7).
+// what q leaves of them too (150 sequences of 32003 tokens: 19.5 us in all), without the
+// two launches that take longer rows' (2.4 us more).
 constexpr int kAloneSegs = 2 * kWalkWaves;
 
 // ---------------------------------------------------------------------------
@@ -769,7 +780,8 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerifyDrafts a, int 
     if (tid == 0) a.next_tokens[seq] = next;
 }
 
-// Workgroup (4 segments, sequence): what q leaves of p where a draft was rejected.
+// Workgroup (4 segments, sequence): what q leaves of p where a draft was rejected.  40
+// sequences of 151936 tokens, 49 MB at most: 9 us, and 5 for the pick.
 template <bool kHalf>
 __global__ __launch_bounds__(kBlk) void verify_rest_kernel(VerifyDrafts a, int segs) {
     __shared__ double table[Exp2Table::kEntries];

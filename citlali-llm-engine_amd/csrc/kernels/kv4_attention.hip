@@ -112,8 +112,8 @@ __device__ __forceinline__ float score_factor(float a, float b, float scale_log2
 // Few rows: one workgroup per (chunk of positions, kv head, sequence) serves
 // every query of the sequence for every head of the kv head's group, at most
 // 16 kCols rows (row r: query r / group, head r % group), so the cache is read
-// once.  The four waves take tiles of 32 positions in turn, without LDS until
-// they merge:
+// once.  The waves, four or eight, take tiles of 32 positions in turn, without LDS
+// until they merge:
 //  * S^T[position][row] = K Q^T by v_mfma_f32_16x16x32_f16, 16 positions at a
 //    time: lane (col, grp) of the A operand holds position col's dims
 //    grp * HD/4 .. + HD/4 - 1, one 16-byte (head_dim 64: 8-byte) load of codes
@@ -137,6 +137,10 @@ __device__ __forceinline__ float score_factor(float a, float b, float scale_log2
 // positions, 403 MB, in 78 us (5.1 TB/s), 64 of 200 .. 4000, 174 MB, in 38.7 (4.5);
 // 20 rows, 24 sequences of 500 .. 6000, 101 MB, in 31.0; 16/8 heads of 64, 100
 // sequences of 150 .. 1500, 52.6 MB, in 17.6.
+// Of a tree (kTree): 48 sequences of 200 .. 4000, 28 to 48 rows of 32/8 heads of 128,
+// 154 MB, in 64 to 66; 25 of 176 .. 2500, 34 to 66 rows of 16/8 of 64, 22 MB, in 22.5:
+// the vector unit, busy for half of it, a chunk's start and end (5 us of 16) and CUs
+// with five chunks where others have four.
 // ---------------------------------------------------------------------------
 template <int HD, int kCols, bool kTree, int kWaves = 4>
 __global__ __launch_bounds__(kWaves * kWave, kWaves > 4 ? 2 : kCols == 1 ? 4
@@ -593,7 +597,7 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
     const int seq = seq_of(blockIdx.x / c.kv_heads, rest, a.nseq);
     const Kv4Seq<kTree> s = kv4_seq<kTree>(a, seq);
     int split, tile;
-    if constexpr (kTree) {   // every sequence's last chunk, the short one, last (304 -> 207 us, see below)
+    if constexpr (kTree) {   // every sequence's last chunk, the short one, last (304 -> 207 us, the case at kTreeBlocks)
         tile = rest % tiles;
         split = rest / tiles - (n_splits - kv4_chunks(s, chunk));
         if (split < 0) return;
@@ -961,8 +965,8 @@ constexpr int kTwoPartBlocks = 384, kTwoPartContext = 256;
 // Trees have few rows behind contexts of any length: the prompt kernel's grid is cut
 // finer than a prompt's, into about kTreeBlocks workgroups were all contexts the
 // longest (four sequences of 38 to 60 rows of 5 heads behind 22452 to 32000 positions:
-// kernel and merge 215 us, cut for one round of workgroups 263, into 1280 232; 25 of 17
-// to 33 rows of 2 heads of 64 behind 176 to 2500 37, 45 and 40).  The merge takes one
+// kernel and merge 208 us, cut for one round of workgroups 263, into 1280 229; 25 of up
+// to 64 rows of 4 heads of 128 behind 150 to 2500 44, 53 and 48).  The merge takes one
 // wave a head from kMergeUnits heads on (180 rows of 40 heads in 15 parts: 12.1 us, by
 // four waves 18.5).
 constexpr int kTreeBlocks = 700, kMergeUnits = 2048;
