@@ -15,8 +15,8 @@ namespace {
 // Masks and positions.  One workgroup per sequence, a thread per row, by
 // doubling: after step t a row's mask holds itself and the 2^t - 1 rows above it,
 // and `above` is the row 2^t up.  128 trees of 256 rows are 1 MB, written in 4 to 5 us,
-// eight rows' in 2 to 5: the launch and two round trips; a row by row walk up takes as
-// many LDS reads as the tree is deep.
+// eight rows' in 2: the launch and two round trips.  (A walk up the tree takes as many
+// LDS reads in a row as it is deep.)
 // ---------------------------------------------------------------------------
 constexpr int kNone = -1, kBad = -2;   // nothing above in the tree; a parent that is not an earlier row
 
@@ -291,11 +291,12 @@ struct Logits {
 };
 
 // Workgroup (4 segments, row, sequence), a segment a wave; every logit is read once.
-// Bound by 64-bit instructions (ten a logit, beside the table's read), from some 150 MB
-// on by the reads too: rows of 151936, 14 trees of up to 40 in fp16, 131 MB, in 31 to 36
-// us, 40 chains of up to 6 and their drafts' in fp32, 200 MB, in 31 to 37; 150 chains of
-// up to 4 with drafts of 32003 in fp16, 47 MB, in 20.  By exp2_64 alone the first takes
-// 85.  Several segments a wave, the next one loaded ahead, are no faster.
+// Bound by 64-bit instructions in fp16 (ten a logit, beside the table's read; the vector
+// unit is busy for 77%): 14 trees of up to 40 rows of 151936, 131 MB, in 31 to 33 us.  By
+// the reads in fp32: 40 chains of up to 6 and their drafts' logits, 200 MB, in 35 to 37
+// (5.4 TB/s).  150 chains of up to 4 with drafts of 32003 in fp16, 47 MB, in 20.  By
+// exp2_64 alone the first takes 85.  Several segments a wave, the next one loaded ahead,
+// are no faster.
 template <bool kHalf>
 __global__ __launch_bounds__(kBlk) void verify_sums_kernel(VerifyDrafts a, int segs) {
     __shared__ double table[Exp2Table::kEntries];
@@ -557,7 +558,7 @@ struct RestLogits {
     }
 };
 // Rows of up to kAloneSegs segments, two a wave: the workgroup that finds the path sums
-// what q leaves of them too (150 sequences of 32003 tokens: 19.5 us in all), without the
+// what q leaves of them too (150 sequences of 32003 tokens: 19 us in all), without the
 // two launches that take longer rows' (2.4 us more).
 constexpr int kAloneSegs = 2 * kWalkWaves;
 

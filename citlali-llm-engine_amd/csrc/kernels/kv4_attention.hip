@@ -565,6 +565,8 @@ __global__ __launch_bounds__(kBlk) void kv4_merge_kernel(Kv4Attention a, int gro
 // 578 us, 893 TFLOP/s (a large fp16 product: 1162), the matrix units busy for 36%
 // of it and the vector units for 46%; of 631 us of an early form the products
 // alone took 330, and 256 rows by eight waves as long as 128 by four.
+// Four trees of 190 to 300 rows behind 22452 .. 32000 positions, 40/8 heads (115 GFLOP):
+// 181 to 200 us, 570 to 630 TFLOP/s, with 78% of the row tiles' rows filled.
 // ---------------------------------------------------------------------------
 constexpr int kRowTile = 128, kTile = 64;   // rows of a workgroup; positions of a step
 constexpr int kPromptNotes = 10 * kWaves;   // words that a part's waves leave one another

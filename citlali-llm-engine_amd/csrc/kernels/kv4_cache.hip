@@ -332,10 +332,11 @@ __global__ __launch_bounds__(kBlk) void kv4_read_kernel(Kv4View c, const int32_t
 // codes or its params, for V a word of the four tokens' codes or params, gathered from
 // four places and stored at once.  Where the tokens come from and go to is looked up
 // for kAhead of them at a time, a thread a token.
-// Bound by HBM: 3500 of 8000 positions of 4 sequences, 8 heads of 128, in 12 caches (375
-// MB to read and write) in 114 us.  V's quads, of which nearly all have a position that
-// stays, are read whole, and K's lines of two: about 530 MB, 4.6 TB/s.  (A wave a token
-// with 2-byte pieces of V: 1227 us.  One turn's reads ahead instead of two: 118.)
+// Bound by HBM: 3500 of 8000 positions of 4 sequences, 8 heads of 128, in 12 caches, 187
+// MB to read and as many to write, in 114 to 122 us.  V's quads, of which nearly all have
+// a position that stays, are read whole, and K's lines of two: 272 MB read by the
+// counters, 3.8 to 4 TB/s in all.  (A wave a token with 2-byte pieces of V: 1227 us.  One
+// turn's reads ahead instead of two: 118 for 114.)
 // ---------------------------------------------------------------------------
 constexpr int kKeepWaves = 8, kAhead = 2048;
 template <int HD>
