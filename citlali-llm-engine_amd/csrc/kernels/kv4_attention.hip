@@ -569,14 +569,22 @@ __global__ __launch_bounds__(kBlk) void kv4_merge_kernel(Kv4Attention a, int gro
 // 181 to 200 us, 570 to 630 TFLOP/s, with 78% of the row tiles' rows filled.
 // ---------------------------------------------------------------------------
 constexpr int kRowTile = 128, kTile = 64;   // rows of a workgroup; positions of a step
+// Rows of a workgroup where a tree has no more (kPairs): a wave has half of the positions
+// of a step for 32 of them, and the halves join at the end (25 sequences of 32 to 64 rows
+// of heads of 128 behind 150 to 2500 positions 44.3 -> 39.5 us, 64 behind 200 to 2000 75.8
+// -> 63.2, 100 behind 100 to 600 48.8 -> 42.9; in tiles of 64, 300 rows take 255 us for
+// 200: the codes' way to fp16 is half of a step).
+constexpr int kPairTile = 64;
 constexpr int kPromptNotes = 10 * kWaves;   // words that a part's waves leave one another
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-template <int HD, int kParts, bool kTree>
+template <int HD, int kParts, bool kTree, bool kPairs = false>
 __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Attention a, int chunk,
                                                                       int n_splits, float scale_log2) {
     using L = Kv4Layout<HD>;
     using Vec = std::conditional_t<HD == 128, u32x4, u32x2>;
+    constexpr int kRows = kPairs ? kPairTile : kRowTile;
+    constexpr int kHalf = kPairs ? 1 : 2;              // a wave's positions of a step, by 32
     constexpr int kWords = HD / 32;                    // words of codes a thread has of a position (K) or of 4 (V)
     constexpr int kHalves = HD * kTile;                // of K (or V) in a buffer
     extern __shared__ __align__(16) float lds[];
@@ -594,12 +602,12 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
     // 88 us against 85 with one sequence's tiles after another's, but 29.5 against
     // 35.1 for two of 761, 43 against 50 for three pieces of 636 behind a prefix)
     const int kvh = blockIdx.x % c.kv_heads;
-    const int group = a.heads / c.kv_heads, tiles = (a.max_query * group + kRowTile - 1) / kRowTile;
+    const int group = a.heads / c.kv_heads, tiles = (a.max_query * group + kRows - 1) / kRows;
     const int rest = blockIdx.z * gridDim.y + blockIdx.y;
     const int seq = seq_of(blockIdx.x / c.kv_heads, rest, a.nseq);
     const Kv4Seq<kTree> s = kv4_seq<kTree>(a, seq);
     int split, tile;
-    if constexpr (kTree) {   // every sequence's last chunk, the short one, last (304 -> 207 us, the case at kTreeBlocks)
+    if constexpr (kTree) {   // every sequence's last chunk, the short one, last (kTreeBlocks' case: 304 -> 207 us)
         tile = rest % tiles;
         split = rest / tiles - (n_splits - kv4_chunks(s, chunk));
         if (split < 0) return;
@@ -607,9 +615,9 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
         split = rest % n_splits;
         tile = tiles - 1 - rest / n_splits;
     }
-    const int rows = min(s.n, a.max_query) * group, row0 = tile * kRowTile;
+    const int rows = min(s.n, a.max_query) * group, row0 = tile * kRows;
     if (tile < 0 || row0 >= rows) return;
-    const int most = max(0, s.see((min(rows, row0 + kRowTile) - 1) / group));
+    const int most = max(0, s.see((min(rows, row0 + kRows) - 1) / group));
     const int c0 = split * chunk, c1 = min(most, c0 + chunk);
     if (c0 >= most && split > 0) return;
     const int lane = threadIdx.x & (kWave - 1);
@@ -617,7 +625,8 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
     const int col = lane & 31, half = lane >> 5;
 
     // this lane's row of Q
-    const int r = row0 + 32 * wave + col;
+    const int row1 = row0 + 32 * (kPairs ? wave & 1 : wave), u0 = kPairs ? wave >> 1 : 0;   // the wave's, of both
+    const int r = row1 + col;
     const bool real = r < rows;
     const int i = real ? r / group : 0;
     const size_t head = (size_t)kvh * group + (real ? r - i * group : 0);
@@ -633,9 +642,9 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
         }
     }
     // positions that every / any row of the wave sees
-    const int r_last = min(rows - 1, row0 + 32 * wave + 31);
-    const int wave_least = r_last < row0 + 32 * wave + 31 ? 0 : min(s.all((row0 + 32 * wave) / group), c1);
-    const int wave_most = row0 + 32 * wave >= rows ? 0 : min(s.see(r_last / group), c1);
+    const int r_last = min(rows - 1, row1 + 31);
+    const int wave_least = r_last < row1 + 31 ? 0 : min(s.all((row1) / group), c1);
+    const int wave_most = row1 >= rows ? 0 : min(s.see(r_last / group), c1);
 
     const int least = min(s.all(row0 / group), c1);   // positions that every row of the workgroup sees
 
@@ -731,7 +740,7 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
     // kTail: of a tree, positions of its rows among the tile's
     auto process = [&](int t, int b, auto kTail) __attribute__((always_inline)) {
         hide(b ^ 1);
-        if (t >= wave_most) {   // uniform: no row of the wave sees the tile
+        if (t + 32 * u0 >= wave_most) {   // uniform: no row of the wave sees the tile
             store(b ^ 1);
             return;
         }
@@ -741,42 +750,46 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) there |= there_at[b * kWaves + w] << (2 * w);
         there = __builtin_amdgcn_readfirstlane(there);
-        const bool whole = (there & 0x55) == 0x55 && t + kTile <= wave_least;
+        constexpr int kThere = kPairs ? 0xf : 0xff;   // bits of the wave's positions
+        there = there >> 4 * u0 & kThere;
+        const bool whole = (there & 0x55) == (0x55 & kThere) && t + 32 * (u0 + kHalf) <= wave_least;
         __builtin_amdgcn_sched_barrier(0);
-        f32x16 sc[2];
+        f32x16 sc[kHalf];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < kHalf; ++u) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) sc[u][e] = 0.f;
 #pragma unroll
             for (int st = 0; st < HD / 16; ++st) {
-                const half8 k = *reinterpret_cast<const half8*>(kb + ((2 * st + half) * kTile + 32 * u + col) * 8);
+                const half8 k =
+                    *reinterpret_cast<const half8*>(kb + ((2 * st + half) * kTile + 32 * (u0 + u) + col) * 8);
                 sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[st], sc[u], 0, 0, 0);
             }
         }
         store(b ^ 1);   // the next tile's codes beside this one's products
 #pragma unroll
-        for (int n = 0; n < HD / 8; ++n) {   // an LDS read, a product, 8 vector instructions and a write at a time
+        // an LDS read, a product, 8 vector instructions and a write at a time (kPairs: twice the last two)
+        for (int n = 0; n < kHalf * HD / 16; ++n) {
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);
-            __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 16 / kHalf, 0);
+            __builtin_amdgcn_sched_group_barrier(0x200, 2 / kHalf, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
-        uint32_t sees[kTail ? 2 : 1];   // of a tree's row, the tile's positions
+        uint32_t sees[kTail ? kHalf : 1];   // of a tree's row, the wave's positions
         if (!whole) {
             if constexpr (kTail) {
                 const uint32_t* row = a.masks + (size_t)(s.start + i) * a.mask_words;
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
-                    sees[u] = real ? tree_bits(row, a.mask_words, t + 32 * u - s.before()) : 0u;
+                for (int u = 0; u < kHalf; ++u)
+                    sees[u] = real ? tree_bits(row, a.mask_words, t + 32 * (u0 + u) - s.before()) : 0u;
             }
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < kHalf; ++u)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int p = 32 * u + 8 * (e / 4) + 4 * half + e % 4;
-                    const bool seen = t + p < see && ((there >> (p >> 4) * 2) & 1) &&
+                    const bool seen = t + 32 * u0 + p < see && ((there >> (p >> 4) * 2) & 1) &&
                                       (!kTail || (sees[kTail ? u : 0] >> (p & 31) & 1));
                     sc[u][e] = seen ? sc[u][e] : -INFINITY;
                 }
@@ -787,11 +800,11 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
                 int first = INT_MAX;
                 bool meets = false;   // in a tree: the row sees one of them
 #pragma unroll 1
-                for (int w = 0; w < kWaves; ++w)
+                for (int w = 0; w < 2 * kHalf; ++w)
                     if ((there >> (2 * w)) & 2) {
-                        const int at = nan_at[(b * kWaves + w) * 4 + (HD == 128 ? 2 * y + half : y)];
+                        const int at = nan_at[(b * kWaves + 2 * u0 + w) * 4 + (HD == 128 ? 2 * y + half : y)];
                         if constexpr (kTail)
-                            meets |= ((w < 2 ? sees[0] : sees[1]) >> (16 * (w & 1)) & (uint32_t)at) != 0;
+                            meets |= ((w < 2 ? sees[0] : sees[kHalf - 1]) >> (16 * (w & 1)) & (uint32_t)at) != 0;
                         else if constexpr (kTree)
                             meets |= at != 0;
                         else
@@ -806,7 +819,7 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
         }
         float mt = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < kHalf; ++u)
 #pragma unroll
             for (int e = 0; e < 16; e += 2) mt = max3(mt, sc[u][e], sc[u][e + 1]);
         mt = max32(mt);
@@ -826,23 +839,24 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
         float off = fmaf(-ref, scale_log2, kShift - kSlack);
         if (__builtin_amdgcn_ballot_w64(fabsf(off) > kFar) != 0) {
             asm volatile("");   // a branch: most tiles skip it
-            sc[0] -= ref;
-            sc[1] -= ref;
+#pragma unroll
+            for (int u = 0; u < kHalf; ++u) sc[u] -= ref;
             off = kShift - kSlack;
         }
-        half8 pw[4];
+        half8 pw[2 * kHalf];
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < kHalf; ++u)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 pw[2 * u + e / 8][e % 8] = (_Float16)__builtin_amdgcn_exp2f(fmaf(sc[u][e], scale_log2, off));
 #pragma unroll
-        for (int st = 0; st < 4; ++st) l_run = add_weights(pw[st], l_run);
+        for (int st = 0; st < 2 * kHalf; ++st) l_run = add_weights(pw[st], l_run);
 #pragma unroll
-        for (int st = 0; st < 4; ++st)
+        for (int st = 0; st < 2 * kHalf; ++st)
 #pragma unroll
             for (int d = 0; d < HD / 32; ++d) {
-                const half8 v = *reinterpret_cast<const half8*>(vbuf + ((2 * st + half) * HD + 32 * d + col) * 8);
+                const half8 v = *reinterpret_cast<const half8*>(
+                    vbuf + ((2 * (2 * u0 + st) + half) * HD + 32 * d + col) * 8);
                 o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pw[st], o[d], 0, 0, 0);
             }
     };
@@ -868,19 +882,16 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
 
     // ---- out: O^T's rows back in dim order through LDS, a wave's rows at a time ----
     float l = sum32(l_run);
-    if constexpr (kParts == 2) {   // the second part's sums, lane by lane, through its own buffers
-        float* const sums = lds + 2 * kHalves + wave * (HD / 2) * kWave + lane;
-        float* const ml = reinterpret_cast<float*>(notes + 2 * kPromptNotes) + 2 * (wave * kWave + lane);
-        if (part == 1) {
+    // another wave's sums, lane by lane through LDS, join this one's
+    auto give = [&](float* sums, float* ml) {
 #pragma unroll
-            for (int d = 0; d < HD / 32; ++d)
+        for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) sums[(16 * d + e) * kWave] = o[d][e];
-            ml[0] = m_run;
-            ml[1] = l;
-        }
-        __syncthreads();
-        if (part == 1) return;
+            for (int e = 0; e < 16; ++e) sums[(16 * d + e) * kWave] = o[d][e];
+        ml[0] = m_run;
+        ml[1] = l;
+    };
+    auto take = [&](const float* sums, const float* ml) {
         const float m = fmaxf(m_run, ml[0]);
         const float f0 = score_factor(m_run, m, scale_log2), f1 = score_factor(ml[0], m, scale_log2);
         m_run = m;
@@ -889,10 +900,27 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
         for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[d][e] = o[d][e] * f0 + sums[(16 * d + e) * kWave] * f1;
+    };
+    if constexpr (kParts == 2) {   // the second part's, through its own buffers
+        float* const sums = lds + 2 * kHalves + wave * (HD / 2) * kWave + lane;
+        float* const ml = reinterpret_cast<float*>(notes + 2 * kPromptNotes) + 2 * (wave * kWave + lane);
+        if (part == 1) give(sums, ml);
+        __syncthreads();
+        if (part == 1) return;
+        take(sums, ml);
+    }
+    constexpr int kPitch = HD + 8;
+    if constexpr (kPairs) {   // the second half of the positions', behind the rows' buffers below
+        float* const sums = lds + 32 * kPitch + (wave & 1) * (HD / 2) * kWave + lane;
+        float* const ml = lds + 32 * kPitch + HD * kWave + 2 * ((wave & 1) * kWave + lane);
+        static_assert((32 * kPitch + HD * kWave + 4 * kWave) * 4 <= 4 * kHalves * 2);
+        if (u0 == 1) give(sums, ml);
+        __syncthreads();
+        if (u0 == 1) return;
+        take(sums, ml);
     }
     const bool alone = most <= chunk;
     if (alone) {
-        constexpr int kPitch = HD + 8;
         uint16_t* rowbuf = buf + wave * 32 * kPitch;
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
 #pragma unroll
@@ -904,7 +932,7 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
             }
         wave_lds_sync();
         for (int idx = lane; idx < 32 * (HD / 8); idx += kWave) {
-            const int rr = idx / (HD / 8), r1 = row0 + 32 * wave + rr, piece = idx % (HD / 8);
+            const int rr = idx / (HD / 8), r1 = row1 + rr, piece = idx % (HD / 8);
             if (r1 >= rows) break;
             const int i1 = r1 / group;
             *reinterpret_cast<u32x4*>(a.out + (size_t)(s.start + i1) * a.out_stride +
@@ -980,6 +1008,7 @@ constexpr int kTreeBlocks = 700, kMergeUnits = 2048;
 constexpr int kWideWaves = 8, kWideBlocks = 256;
 struct Kv4Plan {
     bool few;
+    bool pairs;                                // of the prompt kernel
     int cols, tiles, chunk, n_splits, waves;   // waves: of a workgroup with few rows
 };
 Kv4Plan kv4_plan(bool tree, int max_context, int max_query, int nseq, int heads, int kv_heads, int head_dim) {
@@ -987,6 +1016,7 @@ Kv4Plan kv4_plan(bool tree, int max_context, int max_query, int nseq, int heads,
     const long long rows = (long long)max_query * (heads / kv_heads);
     p.few = rows <= few_rows(tree, head_dim);
     p.cols = p.few ? (int)(rows + 15) / 16 : 0;
+    p.pairs = tree && head_dim == 128 && !p.few && rows <= kPairTile;   // (of 64, such rows are few)
     p.tiles = (int)((rows + kRowTile - 1) / kRowTile);
     auto whole = [](long long positions, int step) { return (int)((positions + step - 1) / step * step); };
     if (p.few) {
@@ -1031,19 +1061,26 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
         const int units = p.tiles * p.n_splits, y = std::min(units, 32768);   // at most 65535 in y
         const dim3 grid(c.kv_heads * a.nseq, y, (units + y - 1) / y);
         const int part = 4 * HD * kTile * (int)sizeof(uint16_t) + kPromptNotes * (int)sizeof(int);
+        const bool two = last && a.max_context > kTwoPartContext &&
+                         (long long)units * c.kv_heads * a.nseq <= kTwoPartBlocks;
+        const int lds = two ? 2 * part + 2 * kBlk * (int)sizeof(float) : part;
+        auto go = [&](auto pairs) {
+            auto with = [&](auto parts) {
+                constexpr auto kernel = kv4_prompt_kernel<HD, parts, kTree, pairs>;
+                const hipError_t e = allow_lds<kernel>(lds);
+                if (e == hipSuccess)
+                    launch_kernel_in_call(last, kernel, grid, dim3(parts * kBlk), lds, s, c, a, p.chunk, p.n_splits,
+                                          scale_log2);
+                return e;
+            };
+            return two ? with(std::integral_constant<int, 2>{}) : with(std::integral_constant<int, 1>{});
+        };
         hipError_t e;
-        if (last && a.max_context > kTwoPartContext && (long long)units * c.kv_heads * a.nseq <= kTwoPartBlocks) {
-            const int lds = 2 * part + 2 * kBlk * (int)sizeof(float);
-            e = allow_lds<kv4_prompt_kernel<HD, 2, kTree>>(lds);
-            if (e != hipSuccess) return e;
-            launch_kernel_in_call(last, kv4_prompt_kernel<HD, 2, kTree>, grid, dim3(2 * kBlk), lds, s, c, a, p.chunk,
-                                  p.n_splits, scale_log2);
-        } else {
-            e = allow_lds<kv4_prompt_kernel<HD, 1, kTree>>(part);
-            if (e != hipSuccess) return e;
-            launch_kernel_in_call(last, kv4_prompt_kernel<HD, 1, kTree>, grid, dim3(kBlk), part, s, c, a, p.chunk,
-                                  p.n_splits, scale_log2);
-        }
+        if constexpr (kTree && HD == 128)
+            e = p.pairs ? go(std::true_type{}) : go(std::false_type{});
+        else
+            e = go(std::false_type{});
+        if (e != hipSuccess) return e;
     } else {
         const dim3 grid(c.kv_heads * a.nseq, p.n_splits);
         const int lds = p.waves * 16 * (HD + 4) * (int)sizeof(float);   // the merge; Q takes less

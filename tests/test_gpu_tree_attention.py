@@ -87,8 +87,29 @@ def test_heads_of_64_have_up_to_80_rows_with_the_few(hip, asked, group):
     b.upload().launch().check()
 
 
-@pytest.mark.parametrize("hd,group,most", [(128, 2, 8), (128, 3, 10), (128, 4, 12), (128, 5, 16), (64, 2, 8), (64, 5, 6),
-                                           (64, 2, 24), (64, 2, 32), (64, 5, 16)])
+@pytest.mark.parametrize("asked,group", [([16, 3, 9], 4), ([13, 12, 1], 4), ([33, 16, 17], 1), ([64, 32, 31], 1),
+                                         ([32, 25, 8], 2), ([10, 9, 5], 5), ([8, 7, 1], 7)])
+def test_heads_of_128_have_up_to_64_rows_in_half_a_tile(hip, asked, group):
+    """One and two parts of the positions, chunks of them, sequences without pages in
+    places and rows that see the prefix alone; some waves without a row."""
+    for page, lens in ((16, [300, 80, 66]), (32, [100, 65, 190]), (64, [1040, 1025, 2300]), (256, [5000, 790, 64])):
+        Trees(hip, 64, 3 * group, 3, 128, page, lens, asked).upload().launch().check()
+    b = Trees(hip, 65, 2 * group, 2, 128, 16, [90, 70, 800], asked)
+    b.table[0, 1] = b.table[2, 3] = -1
+    b.table[1, 0] = b.cache.num_pages
+    b.upload().launch().check()
+    b = Trees(hip, 66, 2 * group, 2, 128, 32, [90, 70, 800], asked)
+    for see in b.sees:
+        see[::3] = False
+    b.upload().launch().check()
+    Trees(hip, 67, 2 * group, 2, 128, 16, [1, 0, 5], asked).upload().launch().check()   # more rows than positions
+    rng = np.random.default_rng(2)
+    many = [asked[0]] + [int(x) for x in rng.integers(0, asked[0] + 1, 69)]
+    Trees(hip, 68, 2 * group, 2, 128, 16, [n + int(rng.integers(0, 90)) for n in many], many).upload().launch().check()
+
+
+@pytest.mark.parametrize("hd,group,most", [(128, 2, 8), (128, 3, 10), (128, 4, 12), (128, 5, 16), (64, 2, 8),
+                                           (64, 5, 6), (64, 2, 24), (64, 2, 32), (64, 5, 16)])
 def test_more_workgroups_than_a_round(hip, hd, group, most):
     """Many short sequences, and some beside one of many chunks, at each number of
     column tiles and on the prompt kernel."""
@@ -181,7 +202,8 @@ def test_slots_past_the_end_may_hold_anything(hip, asked):
 
 @pytest.mark.parametrize("hd,page", [(128, 16), (64, 64)])
 @pytest.mark.parametrize("heads,asked", [(8, [4, 2, 3]), (8, [8, 1, 5]), (8, [12, 9, 10]), (8, [30, 9, 16]),
-                                         (4, [70, 9, 150]), (4, [40, 9, 26])])
+                                         (4, [70, 9, 150]), (4, [40, 9, 26]), (8, [16, 9, 13]),
+                                         (4, [32, 9, 17])])
 @pytest.mark.parametrize("keys", [False, True])
 def test_a_nan_is_kept_from_the_rows_that_do_not_see_it(hip, heads, asked, keys, hd, page):
     """Every third row of the tree has NaN values (and keys): the rows they are
