@@ -418,6 +418,24 @@ def test_millions_of_tokens(hip):
                        int(np.searchsorted(ids, want))) <= (1 if drafted else 0)
 
 
+@pytest.mark.parametrize("half", [False, True])
+def test_rows_past_four_gigabytes(hip, half):
+    """Rows 2 GiB apart."""
+    for drafted in (False, True):
+        step = Step(hip, 33, [2, 1], 5000, half=half, drafted=drafted).upload()
+        step.stride = (1 << 31) // step.type().itemsize
+
+        def spread(x):
+            d = hip.DeviceArray((len(x) - 1) * (1 << 31) + x[0].nbytes)
+            for r, row in enumerate(x):
+                d.upload(row, r << 31)
+            return d
+
+        step.d_logits = spread(step.logits)
+        step.d_draft = spread(step.draft) if drafted else None
+        step.launch().check()
+
+
 @pytest.mark.parametrize("scale", [1e4, 1e30, 3e38])
 def test_logits_of_any_size(hip, scale):
     for heat in (1.0, 0.0, 1e30):

@@ -147,6 +147,23 @@ def test_many_sequences(hip):
     Moves(hip, 8, 64, 16, 2, list(rng.integers(0, 40, 500)), kept, layers=3).upload().launch().check()
 
 
+def test_pages_past_four_gigabytes(hip):
+    """The same moves with pages whose byte offsets pass 32 bits."""
+    page, kv, hd = 256, 8, 128
+    b = Moves(hip, 10, hd, page, kv, [250, 5], [[1, 5, 6, 300, 301], [0, 2, 3]], layers=1, spare=0).upload()
+    want = b.launch().check()[0]
+    size = hip.device.kv4_page_bytes(page, kv, hd)
+    num = (1 << 32) // size + 9
+    pages = hip.DeviceArray(num * size)
+    for i in range(b.pages):
+        pages.upload(b.raw[0, i], (num - 1 - i) * size)
+    b.caches = hip.device.kv4_caches([hip.device.kv4_cache(pages, num, page, kv, hd)])
+    b.d[0] = hip.DeviceArray.from_numpy(np.where(b.table >= 0, num - 1 - b.table, -1).astype(np.int32))
+    b.launch()
+    for i in range(b.pages):
+        assert np.array_equal(pages.download(np.uint8, size, (num - 1 - i) * size).reshape(want[i].shape), want[i])
+
+
 def test_graphs(hip):
     """A captured call moves what the buffers say at each replay."""
     stream = hip.device.Stream()

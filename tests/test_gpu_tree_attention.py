@@ -272,6 +272,21 @@ def test_bounds_of_the_plan(hip):
     b.upload().launch().check()
 
 
+@pytest.mark.parametrize("asked", [[3], [16], [40]])
+def test_pages_past_four_gigabytes(hip, asked):
+    page, kv, hd = 256, 8, 128
+    b = Trees(hip, 69, 32, kv, hd, page, [400], asked, spare=0).upload()
+    size = hip.device.kv4_page_bytes(page, kv, hd)
+    num = (1 << 32) // size + 9
+    pages = hip.DeviceArray(num * size)
+    for i in range(b.cache.num_pages):
+        pages.upload(b.cache.raw[i], (num - 1 - i) * size)
+    want = b.launch().check()
+    b.view = hip.device.kv4_cache(pages, num, page, kv, hd)
+    b.d_table = hip.DeviceArray.from_numpy(np.where(b.table >= 0, num - 1 - b.table, -1).astype(np.int32))
+    assert np.array_equal(b.launch().check(), want)
+
+
 def test_one_row_each(hip):
     """No query_start: one row a sequence, and a mask that hides its own position."""
     b = Trees(hip, 56, 8, 2, 128, 16, [40, 1, 9], [1, 1, 1])
