@@ -996,7 +996,7 @@ constexpr int kTwoPartBlocks = 384, kTwoPartContext = 256;
 // finer than a prompt's, into about kTreeBlocks workgroups were all contexts the
 // longest (four sequences of 38 to 60 rows of 5 heads behind 22452 to 32000 positions:
 // kernel and merge 208 us, cut for one round of workgroups 263, into 1280 229; 25 of up
-// to 64 rows of 4 heads of 128 behind 150 to 2500 44, 53 and 48).  The merge takes one
+// to 64 rows of heads of 128 behind 150 to 2500 39.5, into 1024 45).  The merge takes one
 // wave a head from kMergeUnits heads on (180 rows of 40 heads in 15 parts: 12.1 us, by
 // four waves 18.5).
 constexpr int kTreeBlocks = 700, kMergeUnits = 2048;
