@@ -468,10 +468,10 @@ void kv4_decode_kernel(Kv4View c, Kv4Attention a, int chunk, int n_splits, float
 // one round trip behind the lengths.  Up to 8 chunks (head_dim 64: 16) it takes 3.2
 // to 4.7 us by one wave, by four 3.6 to 7.3; 32 chunks of 16 x 32 heads 4.7 by four,
 // 6.4 by one.
-template <int HD, int kTeam, bool kTree>
+template <int HD, int kTeam, bool kTree, int kBatch = 4>
 __global__ __launch_bounds__(kBlk) void kv4_merge_kernel(Kv4Attention a, int group, int tile_rows, int chunk,
                                                          int n_splits, float scale_log2) {
-    constexpr int kLanes = HD / 4, kTeams = kTeam * kWave / kLanes, kBatch = 4;
+    constexpr int kLanes = HD / 4, kTeams = kTeam * kWave / kLanes;
     __shared__ __align__(16) float lds[kTeam > 1 ? kTeam : 1][HD];
     const int seq = blockIdx.y, lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -1114,16 +1114,18 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || last) return e;
+    const dim3 one((unsigned)((units + kWaves - 1) / kWaves), a.nseq);   // a wave a head
+    auto merge = [&](auto kernel, dim3 grid) {
+        launch_kernel(kernel, grid, dim3(kBlk), 0, s, a, group, tile_rows, p.chunk, p.n_splits, scale_log2);
+        return hipGetLastError();
+    };
     // one wave covers 4 chunks a lane group at once; with more of them four waves share a head
-    const long long units = (long long)a.max_query * a.heads;
-    const int tile_rows = p.few ? few_rows(kTree, HD) : kRowTile;
+    if constexpr (kTree) {   // of few chunks, 2: none is read twice (48 x 384 heads of 4 chunks 9.6 -> 8.1 us)
+        if (p.n_splits <= 2 * kWave / (HD / 4)) return merge(kv4_merge_kernel<HD, 1, true, 2>, one);
+    }
     if (p.n_splits <= 4 * kWave / (HD / 4) || (kTree && units * a.nseq > kMergeUnits))
-        launch_kernel(kv4_merge_kernel<HD, 1, kTree>, dim3((unsigned)((units + kWaves - 1) / kWaves), a.nseq),
-                      dim3(kBlk), 0, s, a, group, tile_rows, p.chunk, p.n_splits, scale_log2);
-    else
-        launch_kernel(kv4_merge_kernel<HD, kWaves, kTree>, dim3((unsigned)units, a.nseq), dim3(kBlk), 0, s, a, group,
-                      tile_rows, p.chunk, p.n_splits, scale_log2);
-    return hipGetLastError();
+        return merge(kv4_merge_kernel<HD, 1, kTree>, one);
+    return merge(kv4_merge_kernel<HD, kWaves, kTree>, dim3((unsigned)units, a.nseq));
 }
 
 }  // namespace
