@@ -1114,6 +1114,8 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || last) return e;
+    const long long units = (long long)a.max_query * a.heads;
+    const int tile_rows = p.few ? few_rows(kTree, HD) : kRowTile;
     const dim3 one((unsigned)((units + kWaves - 1) / kWaves), a.nseq);   // a wave a head
     auto merge = [&](auto kernel, dim3 grid) {
         launch_kernel(kernel, grid, dim3(kBlk), 0, s, a, group, tile_rows, p.chunk, p.n_splits, scale_log2);
