@@ -569,21 +569,22 @@ __global__ __launch_bounds__(kBlk) void kv4_merge_kernel(Kv4Attention a, int gro
 // 181 to 200 us, 570 to 630 TFLOP/s, with 78% of the row tiles' rows filled.
 // ---------------------------------------------------------------------------
 constexpr int kRowTile = 128, kTile = 64;   // rows of a workgroup; positions of a step
-// Rows of a workgroup where a tree has no more (kPairs): a wave has half of the positions
-// of a step for 32 of them, and the halves join at the end (25 sequences of 32 to 64 rows
-// of heads of 128 behind 150 to 2500 positions 44.3 -> 39.5 us, 64 behind 200 to 2000 75.8
-// -> 63.2, 100 behind 100 to 600 48.8 -> 42.9; in tiles of 64, 300 rows take 255 us for
-// 200: the codes' way to fp16 is half of a step).
-constexpr int kPairTile = 64;
+// A row tile of a tree that has no more rows (kPairs): a wave has half of the positions of
+// a step for 32 of them, and the halves join at the end (heads of 128: 25 sequences of 32
+// to 64 rows behind 150 to 2500 positions 44.3 -> 39.2 us, 64 behind 200 to 2000 75.8 ->
+// 63.9, 25 of 80 to 160 rows 83.5 -> 69.3; in tiles of 64 throughout, 300 rows take 255 us
+// for 200: the codes' way to fp16 is half of a step).
+constexpr int kPairRows = 64;
 constexpr int kPromptNotes = 10 * kWaves;   // words that a part's waves leave one another
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-template <int HD, int kParts, bool kTree, bool kPairs = false>
-__global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Attention a, int chunk,
-                                                                      int n_splits, float scale_log2) {
+// Rows row0 .. of sequence seq's `rows`, against its positions c0 .. c1 - 1 (of `most`).
+template <int HD, int kParts, bool kTree, bool kPairs>
+__device__ __forceinline__ void kv4_prompt_tile(const Kv4View& c, const Kv4Attention& a, int chunk, int n_splits,
+                                                float scale_log2, const Kv4Seq<kTree>& s, int seq, int kvh, int group,
+                                                int split, int rows, int row0, int most, int c0, int c1) {
     using L = Kv4Layout<HD>;
     using Vec = std::conditional_t<HD == 128, u32x4, u32x2>;
-    constexpr int kRows = kPairs ? kPairTile : kRowTile;
     constexpr int kHalf = kPairs ? 1 : 2;              // a wave's positions of a step, by 32
     constexpr int kWords = HD / 32;                    // words of codes a thread has of a position (K) or of 4 (V)
     constexpr int kHalves = HD * kTile;                // of K (or V) in a buffer
@@ -595,31 +596,6 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
     int* const notes = reinterpret_cast<int*>(reinterpret_cast<uint16_t*>(lds) + kParts * 4 * kHalves);
     int* const there_at = notes + part * kPromptNotes;
     int* const nan_at = there_at + 2 * kWaves;                           // [2][4 waves][4 groups of dims]
-
-    // kv heads side by side, so that the workgroups of one meet in an XCD's L2
-    // where there are eight of them; row tiles with the most positions first,
-    // every sequence's before the next tile (6 prompts of 100 .. 2500 tokens:
-    // 88 us against 85 with one sequence's tiles after another's, but 29.5 against
-    // 35.1 for two of 761, 43 against 50 for three pieces of 636 behind a prefix)
-    const int kvh = blockIdx.x % c.kv_heads;
-    const int group = a.heads / c.kv_heads, tiles = (a.max_query * group + kRows - 1) / kRows;
-    const int rest = blockIdx.z * gridDim.y + blockIdx.y;
-    const int seq = seq_of(blockIdx.x / c.kv_heads, rest, a.nseq);
-    const Kv4Seq<kTree> s = kv4_seq<kTree>(a, seq);
-    int split, tile;
-    if constexpr (kTree) {   // every sequence's last chunk, the short one, last (kTreeBlocks' case: 304 -> 207 us)
-        tile = rest % tiles;
-        split = rest / tiles - (n_splits - kv4_chunks(s, chunk));
-        if (split < 0) return;
-    } else {
-        split = rest % n_splits;
-        tile = tiles - 1 - rest / n_splits;
-    }
-    const int rows = min(s.n, a.max_query) * group, row0 = tile * kRows;
-    if (tile < 0 || row0 >= rows) return;
-    const int most = max(0, s.see((min(rows, row0 + kRows) - 1) / group));
-    const int c0 = split * chunk, c1 = min(most, c0 + chunk);
-    if (c0 >= most && split > 0) return;
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) % kWaves;   // of the part
     const int col = lane & 31, half = lane >> 5;
@@ -957,6 +933,42 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
     }
 }
 
+template <int HD, int kParts, bool kTree>
+__global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c, Kv4Attention a, int chunk,
+                                                                      int n_splits, float scale_log2) {
+    // kv heads side by side, so that the workgroups of one meet in an XCD's L2
+    // where there are eight of them; row tiles with the most positions first,
+    // every sequence's before the next tile (6 prompts of 100 .. 2500 tokens:
+    // 88 us against 85 with one sequence's tiles after another's, but 29.5 against
+    // 35.1 for two of 761, 43 against 50 for three pieces of 636 behind a prefix)
+    const int kvh = blockIdx.x % c.kv_heads;
+    const int group = a.heads / c.kv_heads, tiles = (a.max_query * group + kRowTile - 1) / kRowTile;
+    const int rest = blockIdx.z * gridDim.y + blockIdx.y;
+    const int seq = seq_of(blockIdx.x / c.kv_heads, rest, a.nseq);
+    const Kv4Seq<kTree> s = kv4_seq<kTree>(a, seq);
+    int split, tile;
+    if constexpr (kTree) {   // every sequence's last chunk, the short one, last (kTreeBlocks' case: 304 -> 207 us)
+        tile = rest % tiles;
+        split = rest / tiles - (n_splits - kv4_chunks(s, chunk));
+        if (split < 0) return;
+    } else {
+        split = rest % n_splits;
+        tile = tiles - 1 - rest / n_splits;
+    }
+    const int rows = min(s.n, a.max_query) * group, row0 = tile * kRowTile;
+    if (tile < 0 || row0 >= rows) return;
+    const int most = max(0, s.see((min(rows, row0 + kRowTile) - 1) / group));
+    const int c0 = split * chunk, c1 = min(most, c0 + chunk);
+    if (c0 >= most && split > 0) return;
+    auto go = [&](auto pairs) __attribute__((always_inline)) {
+        kv4_prompt_tile<HD, kParts, kTree, pairs>(c, a, chunk, n_splits, scale_log2, s, seq, kvh, group, split, rows,
+                                                  row0, most, c0, c1);
+    };
+    if constexpr (kTree)
+        if (rows - row0 <= kPairRows) return go(std::true_type{});
+    go(std::false_type{});
+}
+
 // us below: 8 kv heads, head_dim 128, wall clock per call.
 // Which kernel: the few-row kernel up to 48 rows, where it beats the prompt
 // kernel from about 300 positions on and does not lose before (16 sequences of
@@ -1008,7 +1020,6 @@ constexpr int kTreeBlocks = 700, kMergeUnits = 2048;
 constexpr int kWideWaves = 8, kWideBlocks = 256;
 struct Kv4Plan {
     bool few;
-    bool pairs;                                // of the prompt kernel
     int cols, tiles, chunk, n_splits, waves;   // waves: of a workgroup with few rows
 };
 Kv4Plan kv4_plan(bool tree, int max_context, int max_query, int nseq, int heads, int kv_heads, int head_dim) {
@@ -1016,7 +1027,6 @@ Kv4Plan kv4_plan(bool tree, int max_context, int max_query, int nseq, int heads,
     const long long rows = (long long)max_query * (heads / kv_heads);
     p.few = rows <= few_rows(tree, head_dim);
     p.cols = p.few ? (int)(rows + 15) / 16 : 0;
-    p.pairs = tree && head_dim == 128 && !p.few && rows <= kPairTile;   // (of 64, such rows are few)
     p.tiles = (int)((rows + kRowTile - 1) / kRowTile);
     auto whole = [](long long positions, int step) { return (int)((positions + step - 1) / step * step); };
     if (p.few) {
@@ -1064,22 +1074,15 @@ hipError_t launch_for(const Kv4View& c, const Kv4Attention& a, hipStream_t s) {
         const bool two = last && a.max_context > kTwoPartContext &&
                          (long long)units * c.kv_heads * a.nseq <= kTwoPartBlocks;
         const int lds = two ? 2 * part + 2 * kBlk * (int)sizeof(float) : part;
-        auto go = [&](auto pairs) {
-            auto with = [&](auto parts) {
-                constexpr auto kernel = kv4_prompt_kernel<HD, parts, kTree, pairs>;
-                const hipError_t e = allow_lds<kernel>(lds);
-                if (e == hipSuccess)
-                    launch_kernel_in_call(last, kernel, grid, dim3(parts * kBlk), lds, s, c, a, p.chunk, p.n_splits,
-                                          scale_log2);
-                return e;
-            };
-            return two ? with(std::integral_constant<int, 2>{}) : with(std::integral_constant<int, 1>{});
+        auto with = [&](auto parts) {
+            constexpr auto kernel = kv4_prompt_kernel<HD, parts, kTree>;
+            const hipError_t e = allow_lds<kernel>(lds);
+            if (e == hipSuccess)
+                launch_kernel_in_call(last, kernel, grid, dim3(parts * kBlk), lds, s, c, a, p.chunk, p.n_splits,
+                                      scale_log2);
+            return e;
         };
-        hipError_t e;
-        if constexpr (kTree && HD == 128)
-            e = p.pairs ? go(std::true_type{}) : go(std::false_type{});
-        else
-            e = go(std::false_type{});
+        const hipError_t e = two ? with(std::integral_constant<int, 2>{}) : with(std::integral_constant<int, 1>{});
         if (e != hipSuccess) return e;
     } else {
         const dim3 grid(c.kv_heads * a.nseq, p.n_splits);
