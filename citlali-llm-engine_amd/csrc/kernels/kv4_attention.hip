@@ -976,10 +976,10 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
 // 30 / 59, 40 rows 26 / 54 against 32 / 67; built for 64 rows 37 / 82 against
 // 33 / 68).
 constexpr int kFewRows = 48;
-// Trees with heads of 64 go up to 80 rows (25 of 17 to 33 rows of 2 heads behind 176 to
-// 2500 positions: 23.5 us, on the prompt kernel, whose waves have 32 rows each, 29.5; 64
-// of 40 rows behind 2000 64 and 64; 100 of 64 rows and 600 positions 22 and 26).  Heads
-// of 128 spill at 64 rows: 34 us for 21 with one sequence, 108 for 80 with 64.
+// Trees with heads of 64 go up to 80 rows (few-row against prompt kernel: 25 of 17 to 33
+// rows of 2 heads behind 176 to 2500 positions 23.5 and 28.1, of up to 40 rows 31.3 and
+// 36.9, one of 16000 positions 20.3 and 23.0, but 64 behind 200 to 2000 59.6 and 52.7).
+// Heads of 128 spill at 64 rows: 34 us for 21 with one sequence, 108 for 80 with 64.
 constexpr int kFewTreeRows64 = 80;
 constexpr int few_rows(bool tree, int head_dim) { return tree && head_dim == 64 ? kFewTreeRows64 : kFewRows; }
 // Its chunks: whole turns of the four waves, as long as leaves one round of
