@@ -471,8 +471,9 @@ size_t citlali_hip_kv4_tree_attention_workspace_bytes(int max_context, int max_q
 /* Which drafted tokens stay, so that the tokens that come out are distributed as
  * if the model had drawn them one by one.  Row r's logits (element r * row_stride
  * on; gguf_type 0 = F32 or 1 = F16) are the model's after row r's token; p is
- * softmax(logits / temperatures[s]) (NULL: 1), or, where the temperature is not
- * above 0, 1 for the largest logit (the lowest id of equal ones).  uniforms has a
+ * softmax(logits / temperatures[s]) (NULL: 1; infinite: the tokens above -inf alike),
+ * or, where the temperature is not above 0 or NaN, 1 for the largest logit (the lowest
+ * id of equal ones).  uniforms has a
  * random number of [0, 1) for each row.
  *  - From row 0 on, the children of the current row are tried in order.  Child c,
  *    whose token is x, becomes the current row if u_c R < p(x), where R is 1 for a
