@@ -221,11 +221,11 @@ __host__ __device__ inline Work work_of(const VerifyDrafts& a, int segs) {
     return w;
 }
 
-// 0: greedy.  An infinite one as the largest finite, at which finite logits weigh the
-// same and -inf still nothing.
-__device__ __forceinline__ float temperature(const VerifyDrafts& a, int seq) {
+// 0: greedy.  An infinite one as 2^200, at which finite logits, 2^129 apart at most, all
+// weigh 1 (their exponents are below 2^-70) and -inf still nothing.
+__device__ __forceinline__ double temperature(const VerifyDrafts& a, int seq) {
     const float t = a.temperatures ? a.temperatures[seq] : 1.f;
-    return t > 0.f ? fminf(t, 0x1.fffffep127f) : 0.f;
+    return t > 0.f ? fmin((double)t, 0x1p200) : 0.;
 }
 constexpr double kLog2e = 1.4426950408889634074;
 
@@ -307,13 +307,13 @@ __global__ __launch_bounds__(kBlk) void verify_sums_kernel(VerifyDrafts a, int s
     if (i >= rows.n || (draft && i + 1 >= rows.n)) return;   // the last row's draft has no child
     const int lane = threadIdx.x & (kWave - 1);
     const int seg = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const float t = temperature(a, seq);
+    const double t = temperature(a, seq);
     const int r = rows.start + i;
     Logits<kHalf> x;
     x.load(draft ? logit_row<kHalf>(a.draft, a.draft_stride, r) : logit_row<kHalf>(a.logits, a.stride, r), a.vocab,
            min(seg, segs - 1), lane);
     Exp2Table exp2;
-    exp2.make<kBlk>(table, kLog2e / (double)t);
+    exp2.make<kBlk>(table, kLog2e / t);
     if (seg >= segs) return;
     float top = x.at(0);
 #pragma unroll
@@ -322,7 +322,7 @@ __global__ __launch_bounds__(kBlk) void verify_sums_kernel(VerifyDrafts a, int s
     top = wave_max(top);
     Segment out{0., bad ? NAN : top, 0};
     if (!bad && top > -INFINITY) {
-        if (t > 0.f) {
+        if (t > 0.) {
             double s[2] = {0., 0.};
 #pragma unroll
             for (int e = 0; e < kPer; ++e) s[e % 2] = exp2.add(s[e % 2], (double)x.at(e) - (double)top);
@@ -588,9 +588,9 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerifyDrafts a, int 
         }
         return;
     }
-    const float heat = temperature(a, seq);
-    const bool greedy = !(heat > 0.f);
-    const double c = greedy ? 0. : kLog2e / (double)heat;
+    const double heat = temperature(a, seq);
+    const bool greedy = !(heat > 0.);
+    const double c = greedy ? 0. : kLog2e / heat;
     const float u0 = a.uniforms[rows.start];
     // a row's draft and its logits, on their way beside the rows' sums
     int up = -1, x = -1;

@@ -497,3 +497,33 @@ def test_results_repeat(hip):
         probs = step.d_probs.download(np.uint32, step.rows)
         assert first is None or np.array_equal(first, probs)
         first = probs
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_an_infinite_temperature_over_masked_logits(hip, half):
+    """Logits of the type's lowest and largest value are as likely as the others.
+    Weights of 1, whose sums are exact: token floor(u n) of the n that can come."""
+    big = float(np.finfo(np.float16 if half else np.float32).max)
+    for vocab in (1000, 9001, 40000):
+        for drafted in (False, True):
+            step = Step(hip, 34, [1] * 9 + [2], vocab, drafted=drafted, half=half, heat=np.inf)
+            here = np.flatnonzero(np.arange(vocab) % 3 != 1)
+            for x in (step.logits, step.draft) if drafted else (step.logits,):
+                x[:, 2::3], x[:, 0::6] = -big, big
+                x[:, 1::3] = -np.inf
+            step.uniforms[:9] = 0, 0.1, 0.25, 1 / 3, 0.5, 0.6, 0.75, 0.9, 1 - 2 ** -24
+            step.tokens[10] = here[7]            # p = 1 / n: u = 1 / n is rejected, and what is left is all but it
+            step.uniforms[9:] = 0.3, 0.9
+            step.upload().launch()
+            after = step.d_next.download(np.int32, 10)
+            n = len(here)
+            assert after[:9].tolist() == [int(here[int(float(u) * n)]) for u in step.uniforms[:9]]
+            probs = step.d_probs.download(np.float32, step.rows)
+            assert abs(probs[10] * n - 1) <= 2 ** -24 + 1e-12
+            if drafted:                          # p = q: accepted
+                assert step.d_counts.download(np.int32, 10)[9] == 2
+                assert after[9] == here[int(float(step.uniforms[9]) * n)]
+            else:
+                rest = np.delete(here, 7)
+                assert step.d_counts.download(np.int32, 10)[9] == 1
+                assert after[9] == rest[int(float(step.uniforms[9]) * (n - 1))]
