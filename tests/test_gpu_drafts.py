@@ -527,3 +527,67 @@ def test_an_infinite_temperature_over_masked_logits(hip, half):
                 rest = np.delete(here, 7)
                 assert step.d_counts.download(np.int32, 10)[9] == 1
                 assert after[9] == rest[int(float(step.uniforms[9]) * (n - 1))]
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("vocab,ids", [(5000, (17, 18, 19)), (5000, (17, 2500, 4999)), (40000, (4100, 39999, 5))])
+def test_every_token_that_could_come_is_rejected(hip, half, vocab, ids):
+    """Three tokens that can come, weights 1, a = e^-16 and b = e^-31.125, all rejected
+    at u = 1 - 2^-24: nothing is left, and the token comes from p.  R is 1, a + b and
+    b of p, so u R is below what is left by 2^-24 of it.  Token 1: 1 - 2^-24 >= 1 -
+    1.1254e-7.  Token 2: b is 2.7e-7 of a, more than 2^-24.  Token 3: R is b and the
+    rounding of 1 / s, for R = 1 - 1 / s - a / s, 6.3e-17 or 2e-3 of b too much (s is
+    rounded up by a quarter of 2^-52 in every order of the three weights, 1 / s down)."""
+    w = np.exp(np.float64([0, -16, -31.125]))
+    assert (w[0] + w[1]) + w[2] == (w[0] + w[2]) + w[1] == w[0] + (w[1] + w[2])
+    step = Step(hip, 35, [4, 5, 4], vocab, tree=True, half=half)
+    step.parents = [[-1, 0, 0, 0], [-1, 0, 0, 0, 0], [-1, 0, 0, 0]]
+    step.logits[:] = -np.inf
+    step.logits[:, ids] = 0, -16, -31.125
+    step.tokens[[1, 2, 3, 5, 6, 7, 8, 10, 11, 12]] = (*ids, *ids, ids[0], *ids)
+    step.uniforms[:] = 1 - 2 ** -24
+    step.uniforms[[4, 9]] = 0.3, 0
+    got = step.upload().launch().check()
+    assert [path for path, _ in got] == [[0]] * 3
+    order = sorted(zip(ids, w))
+    assert got[2][1] == order[0][0] and got[1][1] == ids[0]
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("vocab", [5000, 32768, 32769, 151936])
+def test_drafts_that_leave_nothing(hip, vocab, half):
+    """p = q, and drafts that cannot come: rejected, and the token comes from p.  Rows
+    of up to 16 segments are finished by the workgroup that finds the path."""
+    step = Step(hip, 36, [2, 3, 2, 1], vocab, drafted=True, half=half, heat=[1, 0.6, 1.5, 1])
+    step.logits[:, [17, vocab - 1]] = -np.inf
+    step.draft[:] = step.logits
+    step.tokens[[1, 3, 6]] = 17, vocab - 1, -1
+    got = step.upload().launch().check()
+    assert [path for path, _ in got] == [[0]] * 4
+    for s in range(4):
+        row = step.start[s]
+        assert got[s][1] == tree_ref.draw(tree_ref.distribution(step.logits[row], step.heat[s]), step.uniforms[row])
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("vocab", [300, 5000, 151936])
+def test_a_wide_tree_of_rejected_drafts(hip, vocab, half):
+    """255 children of one row, with all but a fiftieth of p, each smaller than the
+    next and rejected at u = 1 - 2^-24 (R is at least a fiftieth more than its p): the
+    token comes from the others."""
+    step = Step(hip, 37, [256, 256], vocab, tree=True, half=half)
+    step.parents = [[-1] + [0] * 255] * 2
+    rng = np.random.default_rng(38)
+    step.logits[:] = rng.standard_normal(step.logits.shape)
+    for s, spread in enumerate((vocab, min(vocab, 290))):       # all over the row, and close together
+        ids = rng.permutation(spread)[:255]
+        x = step.logits[256 * s].astype(np.float64)
+        others = np.delete(np.exp(x), ids).sum()
+        part = np.linspace(0.5, 1.5, 255)
+        step.logits[256 * s, ids] = np.log(part / part.sum() * others * 49)
+        step.tokens[256 * s + 1:256 * s + 256] = ids[np.argsort(step.logits[256 * s, ids], kind="stable")]
+    step.uniforms[:] = 1 - 2 ** -24
+    step.uniforms[[0, 256]] = 0.37, 0.81
+    got = step.upload().launch().check()
+    for s, (path, token) in enumerate(got):
+        assert path == [0] and token not in step.tokens[256 * s + 1:256 * s + 256]
