@@ -70,6 +70,10 @@ __global__ __launch_bounds__(kMaxTree) void draft_tree_kernel(DraftTree a, int w
 // ---------------------------------------------------------------------------
 constexpr int kBlk = 256, kWaves = kBlk / kWave;
 constexpr int kPer = 32, kSeg = kPer * kWave;   // logits of a lane, and of a wave: a segment
+__device__ __forceinline__ int segment_of(int id) {   // below 0 for an id below 0
+    static_assert(kSeg == 1 << 11);
+    return id >> 11;
+}
 
 // 2^z, z <= 0 (0 from -1100 on).  2^f = 1 + f g(f), g by Chebyshev's interpolant of
 // degree 8 on [-1/2, 1/2]: 2^0 is 1, the rest off by 3.7e-14 at most.
@@ -730,24 +734,38 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerifyDrafts a, int 
             const Segment* mine = work.segments + ((size_t)rows.start + f) * segs;
             const int out = a.draft ? 0 : lost;   // rejected tokens, left out
             // What is left of their segments, a wave each: the sum less their weights, an
-            // error of 2^-43 of p in all; summed anew without them (some 10 us) where that
-            // counts, with less than a sixteenth of p left, or leaves hardly more than it.
+            // error of 2^-43 of p in all; summed anew without them where that counts, with
+            // less than a sixteenth of p left, or leaves hardly more than it.  A segment of
+            // several is summed for the first.  A call with 4, 60 or 255 children of one row
+            // of 151936 tokens, all rejected with a fiftieth of p left: 20, 157 and 443 us
+            // with tokens all over the row, 54 and 188 with the last two in one segment (by
+            // a sum for each token, every id against every token: 27, 916 and 13800).
             for (int g = wave; g < out; g += kWalkWaves) {
-                const int mark = __builtin_amdgcn_readfirstlane(gone[g]), seg = mark / kSeg;
-                if (mark < 0) continue;
+                const int seg = segment_of(__builtin_amdgcn_readfirstlane(gone[g]));
+                bool again = seg < 0;
+                for (int k = lane; k < g; k += kWave) again |= segment_of(gone[k]) == seg;
+                if (__builtin_amdgcn_ballot_w64(again) != 0) continue;
                 const Segment whole = mine[seg];
                 const double all = whole.sum * weight(whole.top, s.m, c);
                 double sum = all;
-                for (int k = 0; k < out; ++k) sum -= gone[k] >= 0 && gone[k] / kSeg == seg ? gone_p[k] * s.s : 0.;
+                if (end_left >= 0.0625)
+#pragma unroll 8
+                    for (int k = 0; k < out; ++k) sum -= segment_of(gone[k]) == seg ? gone_p[k] * s.s : 0.;
                 if (end_left < 0.0625 || !(sum >= all * 0x1p-40)) {
-                    const int id1 = min(a.vocab, (seg + 1) * kSeg);
+                    const int id0 = seg * kSeg, id1 = min(a.vocab, id0 + kSeg);
+                    uint32_t is_out = 0;   // which of the lane's ids, every 64th
+                    static_assert(kPer == 32);
+#pragma unroll 8
+                    for (int k = 0; k < out; ++k) {
+                        const int id = gone[k] - id0;
+                        is_out |= segment_of(id) == 0 && id % kWave == lane ? 1u << id / kWave : 0u;
+                    }
                     sum = 0.;
 #pragma unroll 4
-                    for (int id = seg * kSeg + lane; id < id1; id += kWave) {
-                        bool is_out = false;
-                        for (int k = 0; k < out; ++k) is_out |= gone[k] == id;
+                    for (int id = id0 + lane; id < id1; id += kWave) {
                         const double v = weight(logit<kHalf>(row, id), s.m, c);
-                        sum += is_out ? 0. : v;
+                        sum += is_out & 1u ? 0. : v;
+                        is_out >>= 1;
                     }
                     sum = wave_sum64(sum);
                 }
@@ -757,13 +775,16 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerifyDrafts a, int 
             auto draw = [&](int left_out) {
                 auto value = [&](int j) {
                     const Segment g = mine[j];
-                    double v = g.top > -INFINITY ? g.sum * weight(g.top, s.m, c) : 0.;
-                    for (int k = 0; k < left_out; ++k) v = gone[k] >= 0 && gone[k] / kSeg == j ? gone_sum[k] : v;
-                    return v;
+                    const double v = g.top > -INFINITY ? g.sum * weight(g.top, s.m, c) : 0.;
+                    int first = -1;   // of its rejected tokens
+#pragma unroll 8
+                    for (int k = left_out - 1; k >= 0; --k) first = segment_of(gone[k]) == j ? k : first;
+                    return first < 0 ? v : gone_sum[first];
                 };
                 return pick(segs, u0, value, [&](int id, double (&w)[kRun]) {
                     float l[kRun];
                     load_run<kHalf>(row, id, a.vocab, l);
+#pragma unroll 4
                     for (int k = 0; k < left_out; ++k)
 #pragma unroll
                         for (int e = 0; e < kRun; ++e) l[e] = gone[k] == id + e ? -INFINITY : l[e];
