@@ -328,3 +328,95 @@ def test_two_graphs_and_eager_calls(hip):
     finally:
         hip.device.set_stream(None)
         stream.close()
+
+
+# column tiles of the few rows' kernel, by eight waves and by four, and the prompt kernel
+KERNELS = [(8, 2, [300, 37, 5000], [3, 4, 2]), (8, 2, [700, 60], [8, 3]), (10, 2, [900, 33], [9, 7]),
+           (8, 2, [1500, 300], [14, 9]), (8, 2, [90, 300], [20, 9]), (16, 2, [900, 500], [20, 9]), (8, 8, [300], [200]),
+           (16, 8, [300] + [40] * 39, [5] * 40), (32, 8, [70] * 36, [8] * 36), (40, 8, [300] + [40] * 34, [9] * 35)]
+
+
+def _seen(b, s, i):
+    """Positions that row i of sequence s sees."""
+    before = int(b.lens[s]) - len(b.sees[s])
+    return np.concatenate((np.arange(before), before + np.flatnonzero(b.sees[s][i])))
+
+
+@pytest.mark.parametrize("hd,big", [(64, 3000.0), (128, 3000.0), (128, 40000.0)])
+@pytest.mark.parametrize("heads,kv,lens,asked", KERNELS)
+def test_scores_of_large_queries_and_keys(hip, heads, kv, lens, asked, hd, big):
+    """Finite queries and keys whose scores lie far beyond 2^20: a row whose
+    largest score leads the next by more than the scores' own rounding (2^-16
+    of their terms, both ways, and 30 for the exponential) is the value of that
+    position: half a step for the weight, half for the output."""
+    with np.errstate(over="ignore"):                         # infinities saturate
+        b = Trees(hip, 70, heads, kv, hd, 16, lens, asked, big=big)
+        b.q = np.clip(b.q.astype(np.float32) * big, -65504, 65504).astype(np.float16)
+    got = b.upload().launch().result().astype(np.float64)
+    assert np.isfinite(got).all()
+    tested = 0
+    for s in range(len(lens)):
+        for i in range(asked[s]):
+            p = _seen(b, s, i)
+            k, v = (x[b.table[s, p // 16], :, p % 16].astype(np.float64) for x in (b.cache.k, b.cache.v))
+            for h in range(heads):
+                q = b.q[b.start[s] + i, h].astype(np.float64)
+                kk = k[:, h // (heads // kv)]
+                x = kk @ q / np.sqrt(hd)
+                reach = (np.abs(kk) @ np.abs(q)).max() / np.sqrt(hd)
+                best = x.argmax()
+                if len(p) > 1 and np.delete(x, best).max() > x[best] - 2 * reach * 2.0 ** -16 - 30:
+                    continue
+                tested += 1
+                want = v[best, h // (heads // kv)]
+                assert (np.abs(got[b.start[s] + i, h] - want) <= np.abs(want) * 2.0 ** -10 + 2.0 ** -24).all()
+    assert tested >= 0.9 * heads * b.start[-1]
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("heads,kv,lens,asked", KERNELS)
+def test_scores_far_apart(hip, heads, kv, lens, asked, hd):
+    """Weights over the whole range of the exponential, and references that move
+    with the positions: keys that grow to their end, and that shrink."""
+    for turn in (1, -1):
+        b = Trees(hip, 71, heads, kv, hd, 16, lens, asked, big=12.0)
+        for s, n in enumerate(lens):                         # the row's largest keys last, or first
+            pages = b.table[s, :-(-n // 16)]
+            pages = pages[np.argsort(np.abs(b.cache.k[pages]).max((1, 2, 3)))][::turn]
+            b.table[s, :len(pages)] = pages
+        b.upload().launch().check()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("heads,kv,lens,asked", KERNELS)
+def test_infinite_queries(hip, hd, heads, kv, lens, asked):
+    """A query with infinities gives zeros where all its scores are -inf and NaN where
+    some are not; the other rows keep the bar of any row (to the bit they need not be
+    the same: a wave's rows share the choice of when their references move)."""
+    b = Trees(hip, 72, heads, kv, hd, 16, lens, asked)
+    want, spread, reach = b.expected()
+    other = np.ones(want.shape[:2], bool)
+    rows = [(0, 0, 1), (len(lens) - 1, asked[-1] - 1, heads - 1)]       # sequence, its row, head
+    for s, i, h in rows:
+        b.q[b.start[s] + i, h] = 0
+        b.q[b.start[s] + i, h, 5] = -np.inf
+        other[b.start[s] + i, h] = False
+    got = b.upload().launch().result().astype(np.float64)
+    for s, i, h in rows:
+        p = _seen(b, s, i)
+        k = b.cache.k[b.table[s, p // 16], h // (heads // kv), p % 16, 5].astype(np.float64)
+        out = got[b.start[s] + i, h]
+        # -inf times 0 is NaN too
+        assert np.isnan(out).all() if (k <= 0).any() else not out.any()
+    off = np.abs(got - want) - kv4_ref.tolerance(want, spread, reach)
+    assert (off[other] <= 0).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("heads,kv,lens,asked", KERNELS)
+def test_results_repeat(hip, hd, heads, kv, lens, asked):
+    """The same bits every time."""
+    b = Trees(hip, 73, heads, kv, hd, 16, lens, asked).upload()
+    first = b.launch().result().copy()
+    for _ in range(3):
+        assert np.array_equal(b.launch().result().view(np.uint16), first.view(np.uint16))
