@@ -299,7 +299,8 @@ struct Logits {
 // unit is busy for 77%): 14 trees of up to 40 rows of 151936, 131 MB, in 31 to 33 us.  By
 // the reads in fp32: 40 chains of up to 6 and their drafts' logits, 200 MB, in 35 to 37
 // (5.4 TB/s).  150 chains of up to 4 with drafts of 32003 in fp16, 47 MB, in 20.  By
-// exp2_64 alone the first takes 85.  Several segments a wave, the next one loaded ahead,
+// exp2_64 alone the first takes 85.  64 rows of 151936 to draw from: 11 in fp32, 9 in
+// fp16, in calls of 17.7 and 16.0.  Several segments a wave, the next one loaded ahead,
 // are no faster.
 template <bool kHalf>
 __global__ __launch_bounds__(kBlk) void verify_sums_kernel(VerifyDrafts a, int segs) {
@@ -563,7 +564,10 @@ struct RestLogits {
 };
 // Rows of up to kAloneSegs segments, two a wave: the workgroup that finds the path sums
 // what q leaves of them too (150 sequences of 32003 tokens: 19 us in all), without the
-// two launches that take longer rows' (2.4 us more).
+// two launches that take longer rows'.  Calls with every draft rejected, fp32, so and by
+// those launches: of 16000 tokens 1 sequence 17.1 / 18.7 us, 40 21.5 / 23.2, 150 30.3 /
+// 34.8; of 32003 150 43.8 / 47.2, 256 62.3 / 66.1, but few sequences leave CUs idle: 1
+// 22.1 / 18.5, 40 28.7 / 26.2.
 constexpr int kAloneSegs = 2 * kWalkWaves;
 
 // ---------------------------------------------------------------------------

@@ -118,29 +118,36 @@ __device__ __forceinline__ float score_factor(float a, float b, float scale_log2
 //    time: lane (col, grp) of the A operand holds position col's dims
 //    grp * HD/4 .. + HD/4 - 1, one 16-byte (head_dim 64: 8-byte) load of codes
 //    with one (d, m); Q, the B operand, is held in the same dim order (in LDS
-//    beyond 16 rows: that leaves registers for three waves per SIMD at 32).
+//    beyond 16 rows: that leaves registers for three waves per SIMD at 32).  Three of
+//    the tree's instances do not quite fit theirs: heads of 128 at 17 to 32 rows spill 36
+//    bytes a lane, 8 of them read again in every turn before V is asked for, at 16 rows
+//    8 and heads of 64 at 33 to 48 rows 16, outside the loop over the prefix.
 //  * online softmax down each column (row of Q): a lane has 8 of a tile's 32
 //    positions, the maximum takes two permlane swaps, the sum stays per lane
 //    until the end.
 //  * O^T[dim][row] += V^T P^T: the lanes' weights are the B operand as they
 //    stand (k index = grp 4 + i of the first 16 positions, then of the second),
 //    rounded to fp16 -- times 2^14, so that weights down to 2^-28 of the largest
-//    keep all their bits; their sum takes them so too.  V lies in groups of
+//    keep all their bits (of a tree's row times 2^10 to 2^14, as far as its reference
+//    lags behind the largest score: down to 2^-24); their sum takes them so too.  V lies in groups of
 //    four tokens, so lane (c, grp) loads the codes of its four positions and
 //    HD / 16 dims together, each word two positions' dims, and gets the A
 //    operand's pairs without a transposition.
 // Bound by the cache's bytes where contexts are long; else by the round trips of a
 // workgroup's start and by the unequal lengths of the one round of workgroups: the
 // vector unit (about 300 instructions a tile of 5 KB at head_dim 128, 215 a tile of
-// 2.5 KB at 64) is busy for half of the time in each case below but the first.
+// 2.5 KB at 64) is busy for half of the time in each causal case below but the first.
 // 32/8 heads of 128: 16 sequences of 4096 .. 32768
 // positions, 403 MB, in 78 us (5.1 TB/s), 64 of 200 .. 4000, 174 MB, in 38.7 (4.5);
 // 20 rows, 24 sequences of 500 .. 6000, 101 MB, in 31.0; 16/8 heads of 64, 100
 // sequences of 150 .. 1500, 52.6 MB, in 17.6.
 // Of a tree (kTree): 48 sequences of 200 .. 4000, 28 to 48 rows of 32/8 heads of 128,
-// 154 MB, in 64 to 66; 25 of 176 .. 2500, 34 to 66 rows of 16/8 of 64, 22 MB, in 22.5:
-// the vector unit, busy for half of it, a chunk's start and end (5 us of 16) and CUs
-// with five chunks where others have four.
+// 154 MB, in 63 to 66; 25 of 176 .. 2500, 34 to 66 rows of 16/8 of 64, 22 MB, in 22.7.
+// No unit is busy for half of it (vector units 43% and 33%, matrix units 14% and 9%): a
+// chunk's start and end, 5 us of 16 in the first, and CUs with five chunks where others
+// have four.  Chains of up to 8 as trees, 32 rows, and by the causal kernel: calls of 24
+// sequences of 200 .. 4000 36.3 and 35.9 us, of 64 69.7 and 68.1; of up to 4, 16 rows,
+// 24.7 and 24.8, 47.4 and 47.7.
 // ---------------------------------------------------------------------------
 template <int HD, int kCols, bool kTree, int kWaves = 4>
 __global__ __launch_bounds__(kWaves * kWave, kWaves > 4 ? 2 : kCols == 1 ? 4
@@ -976,9 +983,12 @@ __global__ __launch_bounds__(kParts * kBlk, 2) void kv4_prompt_kernel(Kv4View c,
 // 30 / 59, 40 rows 26 / 54 against 32 / 67; built for 64 rows 37 / 82 against
 // 33 / 68).
 constexpr int kFewRows = 48;
-// Trees with heads of 64 go up to 80 rows (few-row against prompt kernel: 25 of 17 to 33
-// rows of 2 heads behind 176 to 2500 positions 23.5 and 28.1, of up to 40 rows 31.3 and
-// 36.9, one of 16000 positions 20.3 and 23.0, but 64 behind 200 to 2000 59.6 and 52.7).
+// Trees with heads of 64 go up to 80 rows: few-row against prompt kernel, calls of 8 kv
+// heads, with up to 50, 66 and 80 rows of 2 heads: 25 sequences of 176 to 2500
+// positions 26.6 / 30.7, 34.9 / 36.9, 34.5 / 36.8; 100 of 150 to 1500 50.6 / 60.8, 60.6 /
+// 60.5, 68.2 / 74.8; one of 16000 17.4 / 18.4, 19.4 / 19.4, 19.8 / 19.9; but 64 of 200 to 2000 47.4 /
+// 47.1, 52.8 / 49.9, 59.8 / 57.9, and 8 of them 17.2 / 17.4, 20.3 / 19.3, 20.9 / 20.3: up
+// to 17% less, 6% more where the grid falls badly.
 // Heads of 128 spill at 64 rows: 34 us for 21 with one sequence, 108 for 80 with 64.
 constexpr int kFewTreeRows64 = 80;
 constexpr int few_rows(bool tree, int head_dim) { return tree && head_dim == 64 ? kFewTreeRows64 : kFewRows; }
