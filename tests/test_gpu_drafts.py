@@ -591,3 +591,32 @@ def test_a_wide_tree_of_rejected_drafts(hip, vocab, half):
     got = step.upload().launch().check()
     for s, (path, token) in enumerate(got):
         assert path == [0] and token not in step.tokens[256 * s + 1:256 * s + 256]
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_chains_of_256(hip, half):
+    """As long as a sequence can be: drafts of the model's own distribution are all
+    accepted, others are rejected somewhere."""
+    step = Step(hip, 39, [256, 200, 256], 3001, drafted=True, half=half)
+    step.draft[:456] = step.logits[:456]
+    got = step.upload().launch().check()
+    assert [len(path) for path, _ in got[:2]] == [256, 200] and len(got[2][0]) < 256
+
+
+def test_draft_rows_of_another_stride(hip):
+    for half in (False, True):
+        step = Step(hip, 40, [3, 4, 2], 5003, drafted=True, half=half).upload()
+        wide = np.full((step.rows, 5003 + 37), np.nan, step.type)
+        wide[:, :5003] = step.draft
+        step.d_draft = hip.DeviceArray.from_numpy(wide)
+        hip.device.verify_drafts(step.d_logits, "fp16" if half else "fp32", 5003, 5003, step.d_draft, 5003 + 37,
+                                 step.d_tokens, None, step.d_start, 3, step.rows, step.max_query, step.d_heat,
+                                 step.d_uniforms, step.d_paths, step.d_counts, step.d_next, step.d_probs, step.d_ws,
+                                 step.bytes)
+        step.check()
+
+
+def test_as_many_sequences_as_there_can_be(hip):
+    Step(hip, 41, [1] * 65535, 21).upload().launch().check()
+    Step(hip, 42, [2] * 65535, 9, drafted=True).upload().launch().check()
+    _check_tree(hip, [[-1, 0]] * 65535, [5] * 65535, 2)

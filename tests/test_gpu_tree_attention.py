@@ -420,3 +420,8 @@ def test_results_repeat(hip, hd, heads, kv, lens, asked):
     first = b.launch().result().copy()
     for _ in range(3):
         assert np.array_equal(b.launch().result().view(np.uint16), first.view(np.uint16))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_as_many_sequences_as_there_can_be(hip, hd):
+    Trees(hip, 74, 1, 1, hd, 16, [1 + s % 3 for s in range(65535)], [1] * 65535).upload().launch().check()
